@@ -38,7 +38,7 @@ typedef enum {
     KILN_ENOMEM = 4        /* workspace allocation failed or the given workspace is too small */
 } kiln_status;
 
-typedef enum { KILN_F32 = 0, KILN_F16 = 1 } kiln_dtype;
+typedef enum { KILN_F32 = 0, KILN_F16 = 1, KILN_BF16 = 2 } kiln_dtype; /* BF16: the entry points that name it */
 
 const char* kiln_attn_status_string(int status);
 const char* kiln_attn_last_error(void);
@@ -358,6 +358,78 @@ int kiln_dit_cross_attn_x16(void* out, void* out_neg, int out_dtype, int ldo, co
                             const uint16_t* const* kvp, const int* Lk, const int* npad, const uint16_t* kvp_neg,
                             int Lk_neg, int npad_neg, float nag_scale, float nag_tau, float nag_alpha, void* workspace,
                             size_t ws_bytes, kiln_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
+ * The attention section over an encoder's states: rotary positions, cross-attention, MXFP4 linear layers. Activations
+ * are [T, ld] rows as above, in KILN_F32, KILN_F16 or KILN_BF16 (cross-attention: the 16-bit types). Inference only, as
+ * all of this library; calls are stream-ordered, allocate nothing, never synchronize, and may be captured into a graph.
+ * Repeated calls give the same bits.
+ * ------------------------------------------------------------------------------------------ */
+
+/* How a model's rotary frequencies f_i = theta^(-2 i / rot), i < rot / 2, are stretched for contexts `factor` times the
+ * length `trained` that it was trained at:
+ *   NONE    f_i
+ *   LINEAR  f_i / factor                                             (position interpolation)
+ *   NTK     theta * factor^(rot / (rot - 2)) in theta's place         (rot > 2)
+ *   RAMP    between the two by frequency: with d(n) = rot ln(trained / (2 pi n)) / (2 ln theta) the pair that turns n times
+ *           over `trained`, and w_i = clamp((i - lo) / (hi - lo), 0, 1) between lo = max(floor d(fast), 0) and
+ *           hi = min(ceil d(slow), rot - 1): w f_i / factor + (1 - w) f_i; values scaled by 0.1 ln(factor) + 1  (YaRN)
+ *   BANDS   by the pair's own turns n_i = trained f_i / (2 pi): w = clamp((n_i - slow) / (fast - slow), 0, 1),
+ *           w f_i + (1 - w) f_i / factor
+ */
+typedef enum { KILN_ROPE_NONE = 0, KILN_ROPE_LINEAR = 1, KILN_ROPE_NTK = 2, KILN_ROPE_RAMP = 3, KILN_ROPE_BANDS = 4 } kiln_rope_scaling;
+
+/* Host code: freqs[rot / 2] (radians per position) and *mscale, the factor on rotated values (1 but for RAMP). factor >= 1;
+ * RAMP and BANDS need trained > 0 and 0 < slow < fast, RAMP theta > 1. */
+int kiln_rope_freqs(double* host_freqs, float* mscale, int rot, double theta, int scaling, double factor, double trained,
+                    double slow, double fast);
+
+/* Rotary positions of H heads of Dh per row: with a = p f_i for the row's position p, the pair (u, v) becomes
+ * mscale (u cos a - v sin a, v cos a + u sin a). Pairs are (i, i + rot/2) of the head, or (2i, 2i + 1) when interleaved;
+ * dimensions from rot on pass unchanged. rot even, 2 <= rot <= Dh <= 1024, H <= 65535. x, y [T, ld] in dtype (F32, F16,
+ * BF16; fp32 arithmetic, rounded once), any alignment (rows and halves of 16-byte multiples are fastest); y = x with
+ * ldy = ldx is in place, other overlaps are refused. pos [T] on the device, or NULL: pos0 + t. freqs [rot / 2] on the device
+ * (kiln_rope_freqs); the angle is taken in 64 bits, so far positions keep their phase. Negative positions turn back: the call
+ * with -pos undoes a rotation, and is its gradient. kiln_rope_half is the same rotation from given fp32 tables. */
+int kiln_rope(void* y, int ldy, const void* x, int ldx, int dtype, int T, int H, int Dh, int rot, int interleaved, const int32_t* pos,
+              int pos0, const double* freqs, float mscale, kiln_stream_t stream);
+
+/* Attention of B items of Tq queries to Tk encoder states of another length, Hq query heads on Hkv key heads (query head h
+ * reads key head h Hkv / Hq; Hq % Hkv == 0), Dh 64 or 128: out = softmax(scale Q K^T) V. q [Tq, ldq], k, v [Tk, ld*], out
+ * [Tq, ldo] per item in dtype (F16 or BF16), items bs* elements apart (0: all items share it, inputs only); 16-byte aligned
+ * rows and item strides (KILN_EUNSUPPORTED otherwise), ld <= 2^24. Item b's keys are the states below klen[b] (device [B],
+ * clamped to 0 .. Tk; NULL: all) whose byte in kmask (device, [Tk] per item, bsm bytes apart; NULL: all) is not 0; what the
+ * others hold does not matter, NaN included. A row without keys, or whose every score is -inf, gives zeros. Scores, maxima and
+ * sums are fp32, the weights are rounded to dtype for the product with V. workspace: kiln_cross_attn_workspace_bytes, for
+ * few rows against many keys, 16-byte aligned; NULL or a smaller one runs the call without splitting the keys over workgroups. */
+int kiln_cross_attn(void* out, int ldo, long long bso, const void* q, int ldq, long long bsq, const void* k, int ldk, long long bsk,
+                    const void* v, int ldv, long long bsv, int dtype, int B, int Tq, int Tk, int Hq, int Hkv, int Dh, float scale,
+                    const int32_t* klen, const uint8_t* kmask, long long bsm, void* workspace, size_t ws_bytes, kiln_stream_t stream);
+size_t kiln_cross_attn_workspace_bytes(int B, int Tq, int Tk, int Hq, int Hkv, int Dh);
+
+/* MXFP4: the values of a row in blocks of 32 neighbours. A block's scale byte s stands for 2^(s - 127), s - 127 being
+ * floor(log2(largest magnitude)) - 2 (not below -127); a value is a 4-bit code, bit 3 the sign and bits 0-2 one of 0, 0.5, 1,
+ * 1.5, 2, 3, 4, 6: the one nearest to it over the scale (ties to the even code, 6 above 5). A block with an infinity or a NaN
+ * has scale byte 255 and stands for NaNs. codes [rows, cols / 2], the even column in a byte's low half, scales
+ * [rows, cols / 32], both dense; codes 16-byte aligned. cols % 32 == 0 (KILN_EUNSUPPORTED otherwise). */
+int kiln_mxfp4_quantize(uint8_t* codes, uint8_t* scales, const void* x, int dtype, int ldx, int rows, int cols, kiln_stream_t stream);
+/* The values that codes and scales stand for (exact in F32 and BF16 down to their subnormals, rounded in F16 outside its range). */
+int kiln_mxfp4_dequantize(void* y, int dtype, int ldy, const uint8_t* codes, const uint8_t* scales, int rows, int cols,
+                          kiln_stream_t stream);
+
+/* kiln_linear16's layer with an MXFP4 weight and the rows of x quantised to MXFP4 within the call: y = epilogue(Q(x) W^T), on
+ * the scaled 4-bit matrix cores, products exact, sums fp32. x [T, cols] rows of ldx in dtype (F32, F16, BF16); epilogues as
+ * kiln_linear16 (kiln_epi: fp32 or fp16 y, GELU, gated residual), any rows, T, ldy >= rows and alignment (y rows of 4 elements'
+ * alignment are fastest), cols % 32 == 0. A LoRA pair is a kiln_linear16 call with KILN_EPI_F32, beta = 1 or KILN_EPI_RESID on
+ * the same y. wp: the weight's codes and scales in the product's layout, from kiln_linear_mxfp4_prepare_weight (which converts
+ * plain codes and scales, e.g. a checkpoint's or kiln_mxfp4_quantize's; 16-byte aligned). workspace:
+ * kiln_linear_mxfp4_workspace_bytes (the quantised rows; 0 for few rows), 16-byte aligned (KILN_ENOMEM if smaller). The order of
+ * a row's sum follows the sizes, as for kiln_linear16. */
+size_t kiln_linear_mxfp4_weight_bytes(int rows, int cols);
+int kiln_linear_mxfp4_prepare_weight(uint8_t* wp, const uint8_t* codes, const uint8_t* scales, int rows, int cols, kiln_stream_t stream);
+size_t kiln_linear_mxfp4_workspace_bytes(int T, int rows, int cols);
+int kiln_linear_mxfp4(void* y, int ldy, const void* x, int dtype, int ldx, int T, const uint8_t* wp, int rows, int cols, int epi,
+                      const float* gate, float beta, void* workspace, size_t ws_bytes, kiln_stream_t stream);
 
 #ifdef __cplusplus
 }

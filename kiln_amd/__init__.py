@@ -20,10 +20,12 @@ LIB_PATH = os.path.join(_HERE, "libkiln_attn.so")
 HEADER_PATH = os.path.join(os.path.dirname(_HERE), "include", "kiln_attn.h")
 
 KILN_OK, KILN_EINVAL, KILN_EUNSUPPORTED, KILN_EHIP, KILN_ENOMEM = 0, 1, 2, 3, 4
-KILN_F32, KILN_F16 = 0, 1
+KILN_F32, KILN_F16, KILN_BF16 = 0, 1, 2
 KILN_EPI_F32, KILN_EPI_F16, KILN_EPI_GELU16, KILN_EPI_RESID = 0, 1, 2, 3
+ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "ramp": 3, "bands": 4}
 
 _i, _ll, _f, _vp, _sz = ctypes.c_int, ctypes.c_longlong, ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t
+_d = ctypes.c_double
 
 # symbol -> (restype, argtypes)
 _SIGS = {
@@ -95,6 +97,17 @@ _SIGS = {
                                      _f, _f, _vp, _sz, _vp]),
     "kiln_cross_attn_nag": (_i, [_vp, _vp, _i, _i, _vp, _i, _i, _vp, _f, _i, _i, _i, _vp, _vp, _vp, _vp, _i, _i, _f,
                                  _f, _f, _vp]),
+    "kiln_rope_freqs": (_i, [_vp, _vp, _i, _d, _i, _d, _d, _d, _d]),
+    "kiln_rope": (_i, [_vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _vp, _i, _vp, _f, _vp]),
+    "kiln_cross_attn": (_i, [_vp, _i, _ll, _vp, _i, _ll, _vp, _i, _ll, _vp, _i, _ll, _i, _i, _i, _i, _i, _i, _i, _f, _vp,
+                             _vp, _ll, _vp, _sz, _vp]),
+    "kiln_cross_attn_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),
+    "kiln_mxfp4_quantize": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _vp]),
+    "kiln_mxfp4_dequantize": (_i, [_vp, _i, _i, _vp, _vp, _i, _i, _vp]),
+    "kiln_linear_mxfp4_weight_bytes": (_sz, [_i, _i]),
+    "kiln_linear_mxfp4_prepare_weight": (_i, [_vp, _vp, _vp, _i, _i, _vp]),
+    "kiln_linear_mxfp4_workspace_bytes": (_sz, [_i, _i, _i]),
+    "kiln_linear_mxfp4": (_i, [_vp, _i, _vp, _i, _i, _i, _vp, _i, _i, _i, _vp, _f, _vp, _sz, _vp]),
 }
 
 _LIB = None
@@ -585,3 +598,226 @@ def flow_ersde_step(x, den, old, oldd, noise, c, stream=None):
     _check(lib().kiln_flow_ersde_step(_ptr(x), _ptr(den), _ptr(old), _ptr(oldd), _ptr(noise), a, b, c2, inv2, c3, inv3,
                                       cn, stage, x.numel(), _stream(stream)))
     return x
+
+
+# ---------------------------------------------------------------------------------------------
+# the attention section over an encoder's states (no counterpart in the reference's op layer)
+# ---------------------------------------------------------------------------------------------
+_DT3 = {}
+
+
+def _dt3(t):
+    """fp32, fp16 or bf16 -> kiln_dtype."""
+    if not _DT3:
+        import torch
+        _DT3.update({torch.float32: KILN_F32, torch.float16: KILN_F16, torch.bfloat16: KILN_BF16})
+    if t.dtype not in _DT3:
+        raise TypeError(f"unsupported dtype {t.dtype}")
+    return _DT3[t.dtype]
+
+
+def _gpu(*ts):
+    """The device index shared by every tensor in ts (None skipped)."""
+    dev = None
+    for t in ts:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError(f"expected a tensor on the GPU, got one on {t.device}")
+        if dev is None:
+            dev = t.device.index
+        elif t.device.index != dev:
+            raise ValueError(f"tensors on different devices: {dev} and {t.device.index}")
+    return dev
+
+
+def _launch(fn, dev, stream, *args):
+    """fn(*args, stream) with device `dev` current, on the given stream or the device's current one."""
+    import torch
+    s = stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(dev)
+    if torch.cuda.current_device() == dev:
+        rc = fn(*args, s)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, s)
+    if rc != KILN_OK:
+        _check(rc)
+
+
+def _scratch(nbytes, dev, stream):
+    """Memory for one call on its stream: torch hands it out again only to work ordered behind that call."""
+    import torch
+    if stream is None:
+        return torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", dev))
+    with torch.cuda.stream(stream):
+        return torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", dev))
+
+
+def _rows_ld(t, what, cols=None):
+    """Row stride of a 2-D tensor whose rows are contiguous, have `cols` columns and do not repeat."""
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{what}: expected a 2-D tensor with contiguous rows, got shape {tuple(t.shape)} strides {t.stride()}")
+    if cols is not None and t.shape[1] != cols:
+        raise ValueError(f"{what}: expected {cols} columns, got {t.shape[1]}")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def rope_freqs(rot, theta=10000.0, scaling="none", factor=1.0, trained=0.0, slow=1.0, fast=None, device=None):
+    """Rotary frequencies of rot dimensions (float64 [rot / 2], radians per position) and the factor on rotated values;
+    scaling: none, linear, ntk, ramp or bands (kiln_rope_scaling in include/kiln_attn.h). fast defaults to 32 turns over
+    the trained length (ramp) or 4 (bands)."""
+    import torch
+    if scaling not in ROPE_SCALINGS:
+        raise ValueError(f"rope_freqs: scaling {scaling!r}, expected one of {sorted(ROPE_SCALINGS)}")
+    fast = (4.0 if scaling == "bands" else 32.0) if fast is None else fast
+    freqs, mscale = torch.empty(max(rot, 2) // 2, dtype=torch.float64), ctypes.c_float()
+    _check(lib().kiln_rope_freqs(_ptr(freqs), ctypes.byref(mscale), rot, theta, ROPE_SCALINGS[scaling], factor, trained, slow, fast))
+    return freqs if device is None else freqs.to(device), mscale.value
+
+
+def rope(y, x, H, Dh, freqs, pos=None, pos0=0, interleaved=False, mscale=1.0, stream=None):
+    """Rotary positions (kiln_rope) of the H heads of Dh in the rows of x [T, H*Dh], into y (y = x: in place); the first
+    2 * freqs.numel() dimensions of a head turn. pos: int32 [T], or None for pos0, pos0 + 1, .."""
+    import torch
+    dev = _gpu(y, x, freqs, pos)
+    T = x.shape[0]
+    ldx, ldy = _rows_ld(x, "rope: x", H * Dh), _rows_ld(y, "rope: y", H * Dh)
+    if y.shape[0] != T or y.dtype != x.dtype:
+        raise ValueError(f"rope: y {tuple(y.shape)} {y.dtype} does not match x {tuple(x.shape)} {x.dtype}")
+    if freqs.dtype != torch.float64 or not freqs.is_contiguous():
+        raise ValueError("rope: freqs must be a contiguous float64 tensor (rope_freqs)")
+    if pos is not None and (pos.dtype != torch.int32 or pos.numel() != T or not pos.is_contiguous()):
+        raise ValueError(f"rope: pos must be a contiguous int32 tensor of {T} positions")
+    _launch(lib().kiln_rope, dev, stream, y.data_ptr(), ldy, x.data_ptr(), ldx, _dt3(x), T, H, Dh, 2 * freqs.numel(),
+            int(bool(interleaved)), None if pos is None else pos.data_ptr(), pos0, freqs.data_ptr(), mscale)
+    return y
+
+
+def cross_attn_workspace_bytes(B, Tq, Tk, Hq, Hkv, Dh):
+    return lib().kiln_cross_attn_workspace_bytes(B, Tq, Tk, Hq, Hkv, Dh)
+
+
+def cross_attn(out, q, k, v, Hq, Hkv=None, scale=None, klen=None, kmask=None, workspace=None, stream=None):
+    """Attention of q [B, Tq, Hq*Dh] to the encoder states k, v [B, Tk, Hkv*Dh] (kiln_cross_attn), out like q; fp16 or bf16,
+    Dh 64 or 128. klen: int32 [B] keys per item; kmask: bool or uint8 [B, Tk], 0 where a key is left out. scale defaults to
+    Dh^-0.5. workspace: cross_attn_workspace_bytes; None takes one for the call."""
+    import torch
+    dev = _gpu(out, q, k, v, klen, kmask, workspace)
+    Hkv = Hq if Hkv is None else Hkv
+    for n, t in (("out", out), ("q", q), ("k", k), ("v", v)):
+        if t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1):
+            raise ValueError(f"cross_attn: {n} must be [B, T, heads*Dh] with contiguous rows")
+        if t.dtype != q.dtype:
+            raise ValueError(f"cross_attn: {n} is {t.dtype}, q is {q.dtype}")
+    B, Tq, W = q.shape
+    Tk = k.shape[1]
+    if Hq <= 0 or Hkv <= 0 or Hq % Hkv or W % Hq:
+        raise ValueError(f"cross_attn: {W} columns, {Hq} query heads on {Hkv} key heads")
+    Dh = W // Hq
+    if out.shape != q.shape or k.shape != (B, Tk, Hkv * Dh) or v.shape != k.shape:
+        raise ValueError(f"cross_attn: shapes out {tuple(out.shape)} q {tuple(q.shape)} k {tuple(k.shape)} v {tuple(v.shape)}")
+    if klen is not None and (klen.dtype != torch.int32 or klen.numel() != B or not klen.is_contiguous()):
+        raise ValueError(f"cross_attn: klen must be a contiguous int32 tensor of {B} lengths")
+    if kmask is not None and (kmask.dtype not in (torch.bool, torch.uint8) or kmask.shape != (B, Tk) or (Tk > 1 and kmask.stride(1) != 1)):
+        raise ValueError(f"cross_attn: kmask must be a bool or uint8 tensor [{B}, {Tk}] with contiguous rows")
+    if workspace is None:
+        n = lib().kiln_cross_attn_workspace_bytes(B, Tq, Tk, Hq, Hkv, Dh)
+        if n:
+            workspace = _scratch(n, dev, stream)
+    elif not workspace.is_contiguous():
+        raise ValueError("cross_attn: workspace must be contiguous")
+    _launch(lib().kiln_cross_attn, dev, stream, out.data_ptr(), out.stride(1), out.stride(0), q.data_ptr(), q.stride(1), q.stride(0),
+            k.data_ptr(), k.stride(1), k.stride(0), v.data_ptr(), v.stride(1), v.stride(0), _dt3(q), B, Tq, Tk, Hq, Hkv, Dh,
+            Dh ** -0.5 if scale is None else scale, None if klen is None else klen.data_ptr(),
+            None if kmask is None else kmask.data_ptr(), 0 if kmask is None else kmask.stride(0),
+            None if workspace is None else workspace.data_ptr(),
+            0 if workspace is None else workspace.numel() * workspace.element_size())
+    return out
+
+
+def _mx_plain(codes, scales, rows, cols, what):
+    import torch
+    for n, t, shape in (("codes", codes, (rows, cols // 2)), ("scales", scales, (rows, cols // 32))):
+        if t.dtype != torch.uint8 or tuple(t.shape) != shape or not t.is_contiguous():
+            raise ValueError(f"{what}: {n} must be a contiguous uint8 tensor {list(shape)}, got {t.dtype} {list(t.shape)}")
+
+
+def mxfp4_quantize(x, codes=None, scales=None, stream=None):
+    """x [rows, cols] (fp32, fp16 or bf16, cols % 32 == 0) to MXFP4 (kiln_mxfp4_quantize): uint8 codes [rows, cols / 2] and
+    scales [rows, cols / 32]."""
+    import torch
+    ldx = _rows_ld(x, "mxfp4_quantize: x")
+    rows, cols = x.shape
+    dev = _gpu(x, codes, scales)
+    if codes is None or scales is None:
+        if codes is not None or scales is not None:
+            raise ValueError("mxfp4_quantize: codes and scales go together")
+        with torch.cuda.stream(stream):
+            codes = torch.empty(rows, cols // 2, dtype=torch.uint8, device=x.device)
+            scales = torch.empty(rows, cols // 32, dtype=torch.uint8, device=x.device)
+    _mx_plain(codes, scales, rows, cols, "mxfp4_quantize")
+    _launch(lib().kiln_mxfp4_quantize, dev, stream, codes.data_ptr(), scales.data_ptr(), x.data_ptr(), _dt3(x), ldx, rows, cols)
+    return codes, scales
+
+
+def mxfp4_dequantize(y, codes, scales, stream=None):
+    """The values of MXFP4 codes and scales (kiln_mxfp4_dequantize) into y [rows, cols]."""
+    ldy = _rows_ld(y, "mxfp4_dequantize: y")
+    rows, cols = y.shape
+    _mx_plain(codes, scales, rows, cols, "mxfp4_dequantize")
+    _launch(lib().kiln_mxfp4_dequantize, _gpu(y, codes, scales), stream, y.data_ptr(), _dt3(y), ldy, codes.data_ptr(), scales.data_ptr(),
+            rows, cols)
+    return y
+
+
+class Mxfp4Weight:
+    """A linear_mxfp4 weight: codes and scales in the product's layout (kiln_linear_mxfp4_prepare_weight)."""
+
+    def __init__(self, buf, rows, cols):
+        self.buf, self.shape = buf, (rows, cols)
+
+
+def linear_mxfp4_weight(w, scales=None, stream=None):
+    """A weight for linear_mxfp4: from w [rows, cols] (fp32, fp16 or bf16, quantised here), or from its MXFP4 codes
+    [rows, cols / 2] and scales [rows, cols / 32] (uint8)."""
+    if scales is None:
+        w, scales = mxfp4_quantize(w, stream=stream)
+    if w.dim() != 2:
+        raise ValueError("linear_mxfp4_weight: expected 2-D codes")
+    rows, cols = w.shape[0], 2 * w.shape[1]
+    dev = _gpu(w, scales)
+    _mx_plain(w, scales, rows, cols, "linear_mxfp4_weight")
+    buf = _scratch(lib().kiln_linear_mxfp4_weight_bytes(rows, cols), dev, stream)
+    _launch(lib().kiln_linear_mxfp4_prepare_weight, dev, stream, buf.data_ptr(), w.data_ptr(), scales.data_ptr(), rows, cols)
+    return Mxfp4Weight(buf, rows, cols)
+
+
+def linear_mxfp4_workspace_bytes(T, rows, cols):
+    return lib().kiln_linear_mxfp4_workspace_bytes(T, rows, cols)
+
+
+def linear_mxfp4(y, x, w, epi=KILN_EPI_F32, gate=None, beta=0.0, workspace=None, stream=None):
+    """linear16's layer with an MXFP4 weight (kiln_linear_mxfp4): y [T, rows] = epilogue(Q(x) w^T), x [T, cols] fp32, fp16 or
+    bf16, w an Mxfp4Weight, y fp32 (F32, RESID) or fp16 (F16, GELU16). workspace: linear_mxfp4_workspace_bytes; None takes
+    one for the call."""
+    import torch
+    rows, cols = w.shape
+    dev = _gpu(y, x, w.buf, gate, workspace)
+    ldx, ldy = _rows_ld(x, "linear_mxfp4: x", cols), _rows_ld(y, "linear_mxfp4: y", rows)
+    T = x.shape[0]
+    if y.shape[0] != T:
+        raise ValueError(f"linear_mxfp4: y has {y.shape[0]} rows, x {T}")
+    if y.dtype != (torch.float32 if epi in (KILN_EPI_F32, KILN_EPI_RESID) else torch.float16):
+        raise ValueError(f"linear_mxfp4: y is {y.dtype} with epilogue {epi}")
+    if gate is not None and (gate.dtype != torch.float32 or gate.numel() != rows or not gate.is_contiguous()):
+        raise ValueError(f"linear_mxfp4: gate must be a contiguous float32 tensor of {rows}")
+    if workspace is None:
+        n = lib().kiln_linear_mxfp4_workspace_bytes(T, rows, cols)
+        if n:
+            workspace = _scratch(n, dev, stream)
+    elif not workspace.is_contiguous():
+        raise ValueError("linear_mxfp4: workspace must be contiguous")
+    _launch(lib().kiln_linear_mxfp4, dev, stream, y.data_ptr(), ldy, x.data_ptr(), _dt3(x), ldx, T, w.buf.data_ptr(), rows, cols, epi,
+            None if gate is None else gate.data_ptr(), beta, None if workspace is None else workspace.data_ptr(),
+            0 if workspace is None else workspace.numel() * workspace.element_size())
+    return y

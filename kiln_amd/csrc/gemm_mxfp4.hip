@@ -1,0 +1,312 @@
+// The MXFP4 linear layer (kiln_linear_mxfp4): y = epilogue(Q(x) Wq^T) with v_mfma_scale_f32_16x16x128_f8f6f4, both operands
+// 4-bit codes with a scale per 32 values (mxfp4.hpp). Products of codes and powers of two are exact; sums are fp32.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "gemm16.hpp"
+#include "mxfp4.hpp"
+
+namespace kiln {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+typedef __attribute__((address_space(3))) uint32_t lds_u32;
+
+struct MxGemmParams {
+    const uint8_t* xc;  // x in the operand layout (the tiled form)
+    const uint8_t* xs;
+    const void* x;      // x as it is (the few-row form, which quantises it itself)
+    size_t ldx;
+    const uint8_t* wc;
+    const uint8_t* ws;
+    int T, N, K, kbs;
+    void* y;
+    size_t ldy;
+    const float* gate;
+    float beta;
+    int vec;            // rows and base of y take 4-element stores
+    int tiles_m, tiles_n, total, per;
+};
+
+// A and B blocks' scale bytes are selected from a register of four: J, I are constants
+template <int J, int I>
+__device__ __forceinline__ floatx4 mx_mfma(u32x4 a, uint32_t sa, u32x4 b, uint32_t sb, floatx4 c) {
+    const i32x8 A = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
+    const i32x8 B = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, c, 4, 4, J, (int)sa, I, (int)sb);  // 4: E2M1
+}
+__device__ __forceinline__ floatx4 mx_mfma_at(int j, int i, u32x4 a, uint32_t sa, u32x4 b, uint32_t sb, floatx4 c) {
+    switch (j * 4 + i) {  // j and i are constants once the loops around are unrolled
+#define MX_CASE(J, I) case J * 4 + I: return mx_mfma<J, I>(a, sa, b, sb, c);
+#define MX_ROW(J) MX_CASE(J, 0) MX_CASE(J, 1) MX_CASE(J, 2) MX_CASE(J, 3)
+        MX_ROW(0) MX_ROW(1) MX_ROW(2) MX_ROW(3)
+#undef MX_ROW
+#undef MX_CASE
+    }
+    return c;
+}
+
+// columns n .. n + 3 of row m
+template <int EPI>
+__device__ __forceinline__ void mx_store(const MxGemmParams& p, int m, int n, floatx4 v) {
+    if (m >= p.T || n >= p.N) return;
+    constexpr bool F32 = EPI == KILN_EPI_F32 || EPI == KILN_EPI_RESID;
+    if constexpr (EPI == KILN_EPI_GELU16)
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = gelu_erf(v[e]);
+    const size_t off = (size_t)m * p.ldy + n;
+    if (p.vec && n + 4 <= p.N) {
+        if constexpr (F32) {
+            float* dst = static_cast<float*>(p.y) + off;
+            if (EPI == KILN_EPI_RESID || p.beta != 0.f) {
+                const floatx4 o = *reinterpret_cast<const floatx4*>(dst);
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    v[e] = EPI == KILN_EPI_RESID ? o[e] + (p.gate ? p.gate[n + e] : 1.f) * v[e] : v[e] + p.beta * o[e];
+            }
+            *reinterpret_cast<floatx4*>(dst) = v;
+        } else {
+            *reinterpret_cast<half4*>(static_cast<_Float16*>(p.y) + off) =
+                half4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        if (n + e >= p.N) break;
+        if constexpr (F32) {
+            float* dst = static_cast<float*>(p.y) + off + e;
+            if constexpr (EPI == KILN_EPI_RESID) *dst += (p.gate ? p.gate[n + e] : 1.f) * v[e];
+            else *dst = p.beta != 0.f ? v[e] + p.beta * *dst : v[e];
+        } else {
+            static_cast<_Float16*>(p.y)[off + e] = (_Float16)v[e];
+        }
+    }
+}
+
+// ---- few rows: a workgroup takes 16 weight rows and every row of x ----
+//
+// Eight waves share out the k blocks; each quantises its part of x in registers (a lane of the operand layout holds exactly
+// one block of 32) and reads its units of the weight, 1 KB each, straight from memory. The waves' sums meet in LDS.
+// Bound by the weight's bytes and, at these sizes, by the launch: one launch, no workspace.
+constexpr int FEW_WAVES = 8;
+template <class E, int EPI, int MB, bool VEC>
+__global__ __launch_bounds__(FEW_WAVES * 64) void k_mx_few(const MxGemmParams p) {
+    __shared__ floatx4 red[FEW_WAVES][MB][64];
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int nb = blockIdx.x, r = lane & 15;
+    floatx4 acc[MB];
+#pragma unroll
+    for (int mb = 0; mb < MB; mb++) acc[mb] = floatx4{0.f, 0.f, 0.f, 0.f};
+    const uint8_t* wc = p.wc + (size_t)nb * p.kbs * MX_UNIT + lane * 16;
+    const uint8_t* wsc = p.ws + (size_t)(nb >> 2) * p.kbs * MX_SUNIT + lane * 4 + (nb & 3);
+    const E* x = static_cast<const E*>(p.x);
+    for (int kb = wv; kb < p.kbs; kb += FEW_WAVES) {
+        const u32x4 w = *reinterpret_cast<const u32x4*>(wc + (size_t)kb * MX_UNIT);
+        const uint32_t sw = wsc[(size_t)kb * MX_SUNIT];
+        const int k = kb * 128 + 32 * (lane >> 4);
+        MxVals<E, MXB> v[MB];
+#pragma unroll
+        for (int mb = 0; mb < MB; mb++) {
+            const bool in = mb * 16 + r < p.T && k < p.K;
+            const E* src = x + (in ? (mb * 16 + r) * p.ldx + k : 0);
+            if constexpr (VEC) v[mb].load(src);
+            else v[mb].load_any(src, in ? MXB : 0);
+        }
+#pragma unroll
+        for (int mb = 0; mb < MB; mb++) {
+            uint32_t s;
+            u32x4 c = mx_block<E>(v[mb], s);
+            if (!(mb * 16 + r < p.T && k < p.K)) c = u32x4{0, 0, 0, 0}, s = 0;
+            acc[mb] = mx_mfma<0, 0>(w, sw, c, s, acc[mb]);
+        }
+    }
+#pragma unroll
+    for (int mb = 0; mb < MB; mb++) red[wv][mb][lane] = acc[mb];
+    __syncthreads();
+    if (wv < MB) {
+        floatx4 t = red[0][wv][lane];
+#pragma unroll
+        for (int w = 1; w < FEW_WAVES; w++) t += red[w][wv][lane];
+        mx_store<EPI>(p, wv * 16 + r, nb * 16 + 4 * (lane >> 4), t);
+    }
+}
+
+// ---- tiles ----
+//
+// WN x WM waves of 16 NB x 16 MB blocks. A stage of the LDS ring holds one k block of 128: the tile's units of W and of x
+// (1 KB each) and their scales, all by LDS DMA in the operand layout, so that every operand read is 1 KB without conflicts.
+template <int WN_, int WM_, int NB_, int MB_, int NST_, int WGS_>
+struct MxCfg {
+    static constexpr int WN = WN_, WM = WM_, NB = NB_, MB = MB_, NST = NST_, WGS = WGS_, WAVES = WN * WM, THREADS = WAVES * 64;
+    static constexpr int BN = WN * NB * 16, BM = WM * MB * 16;
+    static constexpr int UN = BN / 16, UM = BM / 16, SN = (BN + 63) / 64, SM = (BM + 63) / 64;
+    static constexpr int CODE_DMA = (UN + UM) / WAVES, SCALE_DMA = (SN + SM + WAVES - 1) / WAVES, DPS = CODE_DMA + SCALE_DMA;
+    static constexpr int SC_OFF = (UN + UM) * MX_UNIT, STAGE = SC_OFF + (SN + SM) * MX_SUNIT, LDS = NST * STAGE;
+    static_assert((UN + UM) % WAVES == 0 && NB % 4 == 0 && MB % 4 == 0 && LDS * WGS <= 160 * 1024, "tile");
+};
+
+template <int EPI, class C>
+__global__ __launch_bounds__(C::THREADS, C::WAVES * C::WGS / 4) void k_mx_gemm(const MxGemmParams p) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds8[];
+    constexpr int NB = C::NB, MB = C::MB;
+    // blocks go round the 8 XCDs: each takes a contiguous range of tiles, in groups of row tiles that share W in its L2
+    const int ti = (int)(blockIdx.x & 7) * p.per + (int)(blockIdx.x >> 3);
+    if (ti >= p.total) return;
+    int tm, tn;
+    raster_tile(ti, 4, p.tiles_m, p.tiles_n, tm, tn);
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wn = wv % C::WN, wm = wv / C::WN;
+    const int nrb = (p.N + 63) / 64 * 4, mrb = (p.T + 63) / 64 * 4;  // row blocks that exist
+
+    // DMA pieces of this wave: units wv, wv + WAVES, .. of the stage (W's first), then the scale units; row blocks past the
+    // matrix re-read its last one (their results are not stored)
+    typedef __attribute__((address_space(3))) void* lds_p;
+    const uint8_t* src[C::CODE_DMA];
+#pragma unroll
+    for (int i = 0; i < C::CODE_DMA; i++) {
+        const int u = wv + i * C::WAVES;
+        src[i] = u < C::UN ? p.wc + (size_t)min(tn * C::UN + u, nrb - 1) * p.kbs * MX_UNIT
+                           : p.xc + (size_t)min(tm * C::UM + u - C::UN, mrb - 1) * p.kbs * MX_UNIT;
+    }
+    const uint8_t* ssrc[C::SCALE_DMA];
+    int sdst[C::SCALE_DMA];
+#pragma unroll
+    for (int i = 0; i < C::SCALE_DMA; i++) {
+        const int u = (wv + i * C::WAVES) % (C::SN + C::SM);  // a wave without one copies another's again
+        sdst[i] = C::SC_OFF + u * MX_SUNIT;
+        ssrc[i] = u < C::SN ? p.ws + (size_t)min(tn * C::BN / 64 + u, nrb / 4 - 1) * p.kbs * MX_SUNIT
+                            : p.xs + (size_t)min(tm * C::BM / 64 + u - C::SN, mrb / 4 - 1) * p.kbs * MX_SUNIT;
+    }
+    auto dma = [&](int kb, int stage) {
+        uint8_t* base = lds8 + stage * C::STAGE;
+#pragma unroll
+        for (int i = 0; i < C::CODE_DMA; i++)
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src[i] + (size_t)kb * MX_UNIT + lane * 16),
+                                             (lds_p)(base + (wv + i * C::WAVES) * MX_UNIT), 16, 0, 0);
+#pragma unroll
+        for (int i = 0; i < C::SCALE_DMA; i++)
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(ssrc[i] + (size_t)kb * MX_SUNIT + lane * 4),
+                                             (lds_p)(base + sdst[i]), 4, 0, 0);
+    };
+
+    const uint32_t lds_base = (uint32_t)(size_t)(__attribute__((address_space(3))) uint8_t*)lds8;
+    floatx4 acc[NB][MB];
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+        for (int mb = 0; mb < MB; mb++) acc[nb][mb] = floatx4{0.f, 0.f, 0.f, 0.f};
+
+#pragma unroll
+    for (int s = 0; s < C::NST - 1; s++) dma(min(s, p.kbs - 1), s);
+    int stage = 0;
+    for (int kb = 0; kb < p.kbs; kb++) {
+        // stage kb landed in every wave, and every wave is done with the stage before it, which is refilled (past the end
+        // with the last block again: the count of loads in flight stays the same)
+        wait_vmcnt<(C::NST - 2) * C::DPS>();
+        __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        dma(min(kb + C::NST - 1, p.kbs - 1), stage == 0 ? C::NST - 1 : stage - 1);
+        const uint32_t sb = lds_base + stage * C::STAGE;
+        u32x4 fw[NB], fx[MB];
+        uint32_t sw[NB / 4], sx[MB / 4];
+        const uint32_t wa = sb + wn * NB * MX_UNIT + lane * 16, xa = sb + (C::UN + wm * MB) * MX_UNIT + lane * 16;
+        const uint32_t sa = sb + C::SC_OFF + lane * 4;
+#pragma unroll
+        for (int i = 0; i < NB / 4; i++) sw[i] = *reinterpret_cast<const lds_u32*>((size_t)(sa + (wn * NB / 4 + i) * MX_SUNIT));
+#pragma unroll
+        for (int i = 0; i < MB / 4; i++) sx[i] = *reinterpret_cast<const lds_u32*>((size_t)(sa + (C::SN + wm * MB / 4 + i) * MX_SUNIT));
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++) fw[nb] = *reinterpret_cast<const lds_u32x4*>((size_t)(wa + nb * MX_UNIT));
+#pragma unroll
+        for (int mb = 0; mb < MB; mb++) fx[mb] = *reinterpret_cast<const lds_u32x4*>((size_t)(xa + mb * MX_UNIT));
+#pragma unroll
+        for (int mb = 0; mb < MB; mb++)
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++)
+                acc[nb][mb] = mx_mfma_at(nb & 3, mb & 3, fw[nb], sw[nb / 4], fx[mb], sx[mb / 4], acc[nb][mb]);
+        __builtin_amdgcn_sched_barrier(0);
+        stage = stage == C::NST - 1 ? 0 : stage + 1;
+    }
+    wait_vmcnt<0>();  // no copy into LDS outlives the workgroup
+    const int g = lane >> 4, rl = lane & 15;
+#pragma unroll
+    for (int mb = 0; mb < MB; mb++)
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++)
+            mx_store<EPI>(p, tm * C::BM + (wm * MB + mb) * 16 + rl, tn * C::BN + (wn * NB + nb) * 16 + 4 * g, acc[nb][mb]);
+}
+
+using MxBig = MxCfg<4, 2, 4, 8, 4, 1>;    // 256 x 256 (n x m), 8 waves, 136 KB
+using MxMid = MxCfg<2, 2, 4, 4, 4, 2>;    // 128 x 128, 4 waves, 68 KB
+
+template <int EPI, class C>
+static hipError_t mx_tiles(MxGemmParams p, hipStream_t s) {
+    p.tiles_m = (p.T + C::BM - 1) / C::BM;
+    p.tiles_n = (p.N + C::BN - 1) / C::BN;
+    p.total = p.tiles_m * p.tiles_n;
+    p.per = (p.total + 7) / 8;
+    hipLaunchKernelGGL((k_mx_gemm<EPI, C>), dim3(p.per * 8), dim3(C::THREADS), C::LDS, s, p);
+    return hipGetLastError();
+}
+template <class E, int EPI>
+static hipError_t mx_few(const MxGemmParams& p, hipStream_t s) {
+    const bool vec = ((uintptr_t)p.x & 15) == 0 && (p.T == 1 || p.ldx * sizeof(E) % 16 == 0);
+    const int mb = p.T <= 16 ? 1 : p.T <= 32 ? 2 : 4;
+    auto pick = [&]() {
+        if (mb == 1) return vec ? k_mx_few<E, EPI, 1, true> : k_mx_few<E, EPI, 1, false>;
+        if (mb == 2) return vec ? k_mx_few<E, EPI, 2, true> : k_mx_few<E, EPI, 2, false>;
+        return vec ? k_mx_few<E, EPI, 4, true> : k_mx_few<E, EPI, 4, false>;
+    };
+    hipLaunchKernelGGL(pick(), dim3((p.N + 15) / 16), dim3(FEW_WAVES * 64), 0, s, p);
+    return hipGetLastError();
+}
+
+constexpr int FEW_ROWS = 64;
+size_t linear_mx_workspace(int T, int rows, int cols) {
+    return T <= FEW_ROWS ? 0 : mx_code_bytes(T, cols) + mx_scale_bytes(T, cols);
+}
+
+template <int EPI>
+static hipError_t linear_mx_epi(MxGemmParams p, DT dt, uint8_t* ws, hipStream_t s) {
+    if (p.T <= FEW_ROWS) {
+        if (dt == DT::F32) return mx_few<float, EPI>(p, s);
+        if (dt == DT::F16) return mx_few<_Float16, EPI>(p, s);
+        return mx_few<__bf16, EPI>(p, s);
+    }
+    if (hipError_t e = launch_mx_quantize_pack(ws, p.x, dt, p.ldx, p.T, p.K, s)) return e;
+    p.xc = ws;
+    p.xs = ws + mx_code_bytes(p.T, p.K);
+    const long big = (long)((p.T + 255) / 256) * ((p.N + 255) / 256);
+    if (big >= cu_count()) return mx_tiles<EPI, MxBig>(p, s);
+    return mx_tiles<EPI, MxMid>(p, s);
+}
+
+hipError_t launch_linear_mx(void* y, size_t ldy, const void* x, DT dt, size_t ldx, int T, const uint8_t* wp, int rows, int cols, int epi,
+                            const float* gate, float beta, uint8_t* ws, hipStream_t s) {
+    MxGemmParams p{};
+    p.x = x;
+    p.ldx = ldx;
+    p.wc = wp;
+    p.ws = wp + mx_code_bytes(rows, cols);
+    p.T = T;
+    p.N = rows;
+    p.K = cols;
+    p.kbs = mx_kb(cols);
+    p.y = y;
+    p.ldy = ldy;
+    p.gate = gate;
+    p.beta = beta;
+    const int e4 = epi == KILN_EPI_F32 || epi == KILN_EPI_RESID ? 16 : 8;
+    p.vec = ((uintptr_t)y & (e4 - 1)) == 0 && (T == 1 || ldy % 4 == 0);
+    switch (epi) {
+        case KILN_EPI_F32: return linear_mx_epi<KILN_EPI_F32>(p, dt, ws, s);
+        case KILN_EPI_F16: return linear_mx_epi<KILN_EPI_F16>(p, dt, ws, s);
+        case KILN_EPI_GELU16: return linear_mx_epi<KILN_EPI_GELU16>(p, dt, ws, s);
+        default: return linear_mx_epi<KILN_EPI_RESID>(p, dt, ws, s);
+    }
+}
+
+}  // namespace kiln

@@ -7,7 +7,7 @@
 
 namespace kiln {
 
-enum class DT { F32 = 0, F16 = 1 };
+enum class DT { F32 = 0, F16 = 1, BF16 = 2 };
 
 int cu_count();  // CUs of the current device (256 without one)
 
@@ -139,6 +139,41 @@ hipError_t launch_crop(float* dst, const float* src, int Hs, int Ws, int Hd, int
 hipError_t launch_fill_uniform_bf16(uint16_t* p, size_t n, uint64_t seed, float lo, float hi, hipStream_t st);
 hipError_t launch_zero_rows(void* out, size_t ld_bytes, size_t row_bytes, int rows, hipStream_t s);
 hipError_t launch_flow_euler_den(float* x, const float* den, float s, float sn, size_t n, hipStream_t st);
+
+// rotary positions (rope.hip): in place when y == x; row strides in elements
+hipError_t launch_rope(void* y, size_t ldy, const void* x, size_t ldx, DT dt, int T, int H, int Dh, int rot, bool inter,
+                       const int* pos, int pos0, const double* freqs, float mscale, hipStream_t s);
+// MXFP4 (mxfp4.hip, layouts in mxfp4.hpp): cols % 32 == 0; _pack forms write the operand layout, codes then scales
+hipError_t launch_mx_quantize(uint8_t* codes, uint8_t* scales, const void* x, DT dt, size_t ldx, int rows, int cols, hipStream_t s);
+hipError_t launch_mx_dequantize(void* y, DT dt, size_t ldy, const uint8_t* codes, const uint8_t* scales, int rows, int cols,
+                                hipStream_t s);
+hipError_t launch_mx_pack(uint8_t* op, const uint8_t* codes, const uint8_t* scales, int rows, int cols, hipStream_t s);
+hipError_t launch_mx_quantize_pack(uint8_t* op, const void* x, DT dt, size_t ldx, int rows, int cols, hipStream_t s);
+// the MXFP4 linear layer (gemm_mxfp4.hip); ws: linear_mx_workspace bytes
+size_t linear_mx_workspace(int T, int rows, int cols);
+hipError_t launch_linear_mx(void* y, size_t ldy, const void* x, DT dt, size_t ldx, int T, const uint8_t* wp, int rows, int cols, int epi,
+                            const float* gate, float beta, uint8_t* ws, hipStream_t s);
+
+// attention of B x Tq queries to Tk states (cross_attn.hip); strides in elements, F16 or BF16; ws smaller than
+// cross_attn_workspace (or null): the keys are not split over workgroups
+struct CrossLaunch {
+    void* out;
+    const void* q;
+    const void* k;
+    const void* v;
+    size_t ldo, ldq, ldk, ldv;
+    long long bso, bsq, bsk, bsv;
+    DT dt;
+    int B, Tq, Tk, Hq, Hkv, Dh;
+    float scale;
+    const int* klen;       // [B] on the device, or null
+    const uint8_t* kmask;  // [Tk] per item (stride bsm), or null
+    long long bsm;
+    void* ws;
+    size_t ws_bytes;
+};
+size_t cross_attn_workspace(int B, int Tq, int Tk, int Hq, int Hkv, int Dh);
+hipError_t launch_cross_attn(const CrossLaunch& c, hipStream_t s);
 
 // torch.manual_seed(seed); torch.randn(n) on the host (host_rng.cpp); false if n < 16
 bool host_torch_randn(float* out, uint64_t seed, size_t n);

@@ -1,0 +1,178 @@
+// MXFP4 quantisation, its inverse, and the operand layout of the MXFP4 product (mxfp4.hpp). All bound by memory.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "mxfp4.hpp"
+
+namespace kiln {
+
+__device__ __forceinline__ uint32_t quad_umax(uint32_t v) {  // over the four lanes of a quad
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, false));
+    return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, false));
+}
+
+// x [rows, cols] to codes [rows, cols / 2] (even column in the low half) and scales [rows, cols / 32]. Four lanes take a
+// block of 32, eight values each: loads of 16 or 32 contiguous bytes per lane, 4-byte stores of codes.
+template <class E, bool VEC>
+__global__ __launch_bounds__(256) void k_mx_quantize(uint8_t* codes, uint8_t* scales, const E* x, size_t ldx, int rows, int cols) {
+    const size_t n = (size_t)rows * (cols / 8);
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
+        const size_t r = i / (cols / 8);
+        const int c = (int)(i - r * (cols / 8)) * 8;
+        MxVals<E, 8> v;
+        if constexpr (VEC) v.load(x + r * ldx + c);
+        else v.load_any(x + r * ldx + c, 8);
+        const uint32_t s = mx_scale(quad_umax(v.top()));
+        *reinterpret_cast<uint32_t*>(codes + i * 4) = s == 255 ? 0u : v.codes8(0, mx_scale_f32(s));
+        if ((threadIdx.x & 3) == 0) scales[i >> 2] = (uint8_t)s;
+    }
+}
+
+// eight values of a code word times 2^(s - 127), exact in fp32 (and in bf16 and fp16 within their ranges)
+template <class E>
+__device__ __forceinline__ void mx_values8(uint32_t c, uint32_t s, E (&o)[8]) {
+    const float sc = s == 255 ? __uint_as_float(0x7fc00000u) : mx_scale_f32(s);
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        // magnitude bits eem: 0.5 m for ee = 0, else 2^(ee - 1) (1 + m / 2): as fp32 bits, with ee = 0 an exact half
+        const uint32_t m = (c >> (4 * i)) & 7;
+        const float a = m < 2 ? 0.5f * (float)m : __uint_as_float(((m >> 1) + 126) << 23 | (m & 1) << 22);
+        o[i] = (E)(__uint_as_float(__float_as_uint(a) | (c >> (4 * i) & 8) << 28) * sc);
+    }
+}
+template <class E, bool VEC>
+__global__ __launch_bounds__(256) void k_mx_dequantize(E* y, size_t ldy, const uint8_t* codes, const uint8_t* scales, int rows, int cols) {
+    const size_t n = (size_t)rows * (cols / 8);
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
+        const size_t r = i / (cols / 8);
+        const int c = (int)(i - r * (cols / 8)) * 8;
+        E o[8];
+        mx_values8(*reinterpret_cast<const uint32_t*>(codes + i * 4), scales[i >> 2], o);
+        E* dst = y + r * ldy + c;
+        if constexpr (VEC) {
+            typedef E V __attribute__((ext_vector_type(16 / sizeof(E))));
+#pragma unroll
+            for (int j = 0; j < 8; j += 16 / (int)sizeof(E)) {
+                V v;
+#pragma unroll
+                for (int e = 0; e < 16 / (int)sizeof(E); e++) v[e] = o[j + e];
+                *reinterpret_cast<V*>(dst + j) = v;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) dst[j] = o[j];
+        }
+    }
+}
+
+// codes and scales (row-major) to the operand layout, one wave per (64 rows, k block of 128); the padding is written too
+__global__ __launch_bounds__(256) void k_mx_pack(uint8_t* oc, uint8_t* os, const uint8_t* codes, const uint8_t* scales, int rows,
+                                                 int cols, int kbs, size_t units) {
+    const size_t u = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (u >= units) return;
+    const int lane = threadIdx.x & 63, kb = (int)(u % kbs), k = kb * 128 + 32 * (lane >> 4);
+    const size_t rg = u / kbs;
+    uint32_t sc = 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const size_t r = rg * 64 + 16 * j + (lane & 15);
+        u32x4 c = {0, 0, 0, 0};
+        if (r < (size_t)rows && k < cols) {
+            c = *reinterpret_cast<const u32x4*>(codes + r * (cols / 2) + k / 2);
+            sc |= (uint32_t)scales[r * (cols / 32) + k / 32] << (8 * j);
+        }
+        *reinterpret_cast<u32x4*>(oc + ((rg * 4 + j) * kbs + kb) * MX_UNIT + lane * 16) = c;
+    }
+    *reinterpret_cast<uint32_t*>(os + (rg * kbs + kb) * MX_SUNIT + lane * 4) = sc;
+}
+
+// the rows of an activation straight to the operand layout: a lane holds a whole block of 32
+template <class E, bool VEC>
+__global__ __launch_bounds__(256) void k_mx_quantize_pack(uint8_t* oc, uint8_t* os, const E* x, size_t ldx, int rows, int cols, int kbs,
+                                                          size_t units) {
+    const size_t u = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (u >= units) return;
+    const int lane = threadIdx.x & 63, kb = (int)(u % kbs), k = kb * 128 + 32 * (lane >> 4);
+    const size_t rg = u / kbs;
+    MxVals<E, MXB> v[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const size_t r = rg * 64 + 16 * j + (lane & 15);
+        const bool in = r < (size_t)rows && k < cols;
+        const E* src = x + (in ? r * ldx + k : 0);
+        if constexpr (VEC) v[j].load(src);
+        else v[j].load_any(src, in ? MXB : 0);
+    }
+    uint32_t sc = 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const bool in = rg * 64 + 16 * j + (lane & 15) < (size_t)rows && k < cols;
+        uint32_t s;
+        u32x4 c = mx_block<E>(v[j], s);
+        if (!in) c = u32x4{0, 0, 0, 0}, s = 0;
+        sc |= s << (8 * j);
+        *reinterpret_cast<u32x4*>(oc + ((rg * 4 + j) * kbs + kb) * MX_UNIT + lane * 16) = c;
+    }
+    *reinterpret_cast<uint32_t*>(os + (rg * kbs + kb) * MX_SUNIT + lane * 4) = sc;
+}
+
+static unsigned grid_of(size_t n) { return (unsigned)std::min<size_t>((n + 255) / 256, (size_t)cu_count() * 32); }
+
+template <class E>
+static hipError_t quantize_of(uint8_t* codes, uint8_t* scales, const void* x, size_t ldx, int rows, int cols, bool vec, hipStream_t s) {
+    const size_t n = (size_t)rows * (cols / 8);
+    auto kern = vec ? k_mx_quantize<E, true> : k_mx_quantize<E, false>;
+    hipLaunchKernelGGL(kern, dim3(grid_of(n)), dim3(256), 0, s, codes, scales, static_cast<const E*>(x), ldx, rows, cols);
+    return hipGetLastError();
+}
+template <class E>
+static hipError_t dequantize_of(void* y, size_t ldy, const uint8_t* codes, const uint8_t* scales, int rows, int cols, bool vec,
+                                hipStream_t s) {
+    const size_t n = (size_t)rows * (cols / 8);
+    auto kern = vec ? k_mx_dequantize<E, true> : k_mx_dequantize<E, false>;
+    hipLaunchKernelGGL(kern, dim3(grid_of(n)), dim3(256), 0, s, static_cast<E*>(y), ldy, codes, scales, rows, cols);
+    return hipGetLastError();
+}
+template <class E>
+static hipError_t quantize_pack_of(uint8_t* op, const void* x, size_t ldx, int rows, int cols, bool vec, hipStream_t s) {
+    const int kbs = mx_kb(cols);
+    const size_t units = (size_t)((rows + 63) / 64) * kbs;
+    auto kern = vec ? k_mx_quantize_pack<E, true> : k_mx_quantize_pack<E, false>;
+    hipLaunchKernelGGL(kern, dim3((unsigned)((units + 3) / 4)), dim3(256), 0, s, op, op + mx_code_bytes(rows, cols),
+                       static_cast<const E*>(x), ldx, rows, cols, kbs, units);
+    return hipGetLastError();
+}
+// 16-byte loads of the rows
+static bool rows16(const void* p, size_t ld, DT dt, int rows) {
+    return ((uintptr_t)p & 15) == 0 && (rows == 1 || ld * (dt == DT::F32 ? 4 : 2) % 16 == 0);
+}
+
+hipError_t launch_mx_quantize(uint8_t* codes, uint8_t* scales, const void* x, DT dt, size_t ldx, int rows, int cols, hipStream_t s) {
+    const bool vec = rows16(x, ldx, dt, rows);
+    if (dt == DT::F32) return quantize_of<float>(codes, scales, x, ldx, rows, cols, vec, s);
+    if (dt == DT::F16) return quantize_of<_Float16>(codes, scales, x, ldx, rows, cols, vec, s);
+    return quantize_of<__bf16>(codes, scales, x, ldx, rows, cols, vec, s);
+}
+hipError_t launch_mx_dequantize(void* y, DT dt, size_t ldy, const uint8_t* codes, const uint8_t* scales, int rows, int cols,
+                                hipStream_t s) {
+    const bool vec = rows16(y, ldy, dt, rows);
+    if (dt == DT::F32) return dequantize_of<float>(y, ldy, codes, scales, rows, cols, vec, s);
+    if (dt == DT::F16) return dequantize_of<_Float16>(y, ldy, codes, scales, rows, cols, vec, s);
+    return dequantize_of<__bf16>(y, ldy, codes, scales, rows, cols, vec, s);
+}
+hipError_t launch_mx_pack(uint8_t* op, const uint8_t* codes, const uint8_t* scales, int rows, int cols, hipStream_t s) {
+    const int kbs = mx_kb(cols);
+    const size_t units = (size_t)((rows + 63) / 64) * kbs;
+    hipLaunchKernelGGL(k_mx_pack, dim3((unsigned)((units + 3) / 4)), dim3(256), 0, s, op, op + mx_code_bytes(rows, cols), codes, scales,
+                       rows, cols, kbs, units);
+    return hipGetLastError();
+}
+hipError_t launch_mx_quantize_pack(uint8_t* op, const void* x, DT dt, size_t ldx, int rows, int cols, hipStream_t s) {
+    const bool vec = rows16(x, ldx, dt, rows);
+    if (dt == DT::F32) return quantize_pack_of<float>(op, x, ldx, rows, cols, vec, s);
+    if (dt == DT::F16) return quantize_pack_of<_Float16>(op, x, ldx, rows, cols, vec, s);
+    return quantize_pack_of<__bf16>(op, x, ldx, rows, cols, vec, s);
+}
+
+}  // namespace kiln
