@@ -87,34 +87,36 @@ __global__ __launch_bounds__(256) void k_mx_pack(uint8_t* oc, uint8_t* os, const
     *reinterpret_cast<uint32_t*>(os + (rg * kbs + kb) * MX_SUNIT + lane * 4) = sc;
 }
 
-// the rows of an activation straight to the operand layout: a lane holds a whole block of 32
+// The rows of an activation straight to the operand layout: a workgroup takes 64 rows x 128 columns (four units of codes, one
+// of scales). Four lanes share a block, so a load covers 256-byte pieces (fp16) of four rows, four loads in flight; the codes
+// meet in LDS and leave as whole units. (A lane per block reads the same lines four times over: 6912 x 2048 fp16 10.7 us.)
 template <class E, bool VEC>
-__global__ __launch_bounds__(256) void k_mx_quantize_pack(uint8_t* oc, uint8_t* os, const E* x, size_t ldx, int rows, int cols, int kbs,
-                                                          size_t units) {
-    const size_t u = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (u >= units) return;
-    const int lane = threadIdx.x & 63, kb = (int)(u % kbs), k = kb * 128 + 32 * (lane >> 4);
-    const size_t rg = u / kbs;
-    MxVals<E, MXB> v[4];
+__global__ __launch_bounds__(256) void k_mx_quantize_pack(uint8_t* oc, uint8_t* os, const E* x, size_t ldx, int rows, int cols, int kbs) {
+    __shared__ __attribute__((aligned(16))) uint32_t lc[4][64][4];  // [row block][operand lane][8 codes]
+    __shared__ __attribute__((aligned(16))) uint8_t ls[64][4];                                   // [operand lane][row block]
+    const int kb = blockIdx.x % kbs, q = threadIdx.x & 15, k = kb * 128 + 8 * q;
+    const size_t rg = blockIdx.x / kbs;
+    MxVals<E, 8> v[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        const size_t r = rg * 64 + 16 * j + (lane & 15);
+        const size_t r = rg * 64 + 16 * j + (threadIdx.x >> 4);
         const bool in = r < (size_t)rows && k < cols;
         const E* src = x + (in ? r * ldx + k : 0);
         if constexpr (VEC) v[j].load(src);
-        else v[j].load_any(src, in ? MXB : 0);
+        else v[j].load_any(src, in ? 8 : 0);
     }
-    uint32_t sc = 0;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        const bool in = rg * 64 + 16 * j + (lane & 15) < (size_t)rows && k < cols;
-        uint32_t s;
-        u32x4 c = mx_block<E>(v[j], s);
-        if (!in) c = u32x4{0, 0, 0, 0}, s = 0;
-        sc |= s << (8 * j);
-        *reinterpret_cast<u32x4*>(oc + ((rg * 4 + j) * kbs + kb) * MX_UNIT + lane * 16) = c;
+        const int rl = threadIdx.x >> 4, lane = rl + 16 * (q >> 2);
+        const bool in = rg * 64 + 16 * j + rl < (size_t)rows && k < cols;
+        const uint32_t s = mx_scale(quad_umax(v[j].top()));
+        lc[j][lane][q & 3] = in && s != 255 ? v[j].codes8(0, mx_scale_f32(s)) : 0u;
+        if ((q & 3) == 0) ls[lane][j] = in ? (uint8_t)s : 0;
     }
-    *reinterpret_cast<uint32_t*>(os + (rg * kbs + kb) * MX_SUNIT + lane * 4) = sc;
+    __syncthreads();
+    const int j = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    *reinterpret_cast<u32x4*>(oc + ((rg * 4 + j) * kbs + kb) * MX_UNIT + lane * 16) = *reinterpret_cast<const u32x4*>(lc[j][lane]);
+    if (j == 0) *reinterpret_cast<uint32_t*>(os + (rg * kbs + kb) * MX_SUNIT + lane * 4) = *reinterpret_cast<const uint32_t*>(ls[lane]);
 }
 
 static unsigned grid_of(size_t n) { return (unsigned)std::min<size_t>((n + 255) / 256, (size_t)cu_count() * 32); }
@@ -137,10 +139,9 @@ static hipError_t dequantize_of(void* y, size_t ldy, const uint8_t* codes, const
 template <class E>
 static hipError_t quantize_pack_of(uint8_t* op, const void* x, size_t ldx, int rows, int cols, bool vec, hipStream_t s) {
     const int kbs = mx_kb(cols);
-    const size_t units = (size_t)((rows + 63) / 64) * kbs;
     auto kern = vec ? k_mx_quantize_pack<E, true> : k_mx_quantize_pack<E, false>;
-    hipLaunchKernelGGL(kern, dim3((unsigned)((units + 3) / 4)), dim3(256), 0, s, op, op + mx_code_bytes(rows, cols),
-                       static_cast<const E*>(x), ldx, rows, cols, kbs, units);
+    hipLaunchKernelGGL(kern, dim3((unsigned)(((size_t)rows + 63) / 64 * kbs)), dim3(256), 0, s, op, op + mx_code_bytes(rows, cols),
+                       static_cast<const E*>(x), ldx, rows, cols, kbs);
     return hipGetLastError();
 }
 // 16-byte loads of the rows
