@@ -603,7 +603,8 @@ def flow_ersde_step(x, den, old, oldd, noise, c, stream=None):
 # ---------------------------------------------------------------------------------------------
 # the attention section over an encoder's states (no counterpart in the reference's op layer)
 # ---------------------------------------------------------------------------------------------
-_DT3 = {}
+_DT3 = {}  # torch dtype -> kiln_dtype, filled at the first use (torch is imported there)
+_NOW = []  # torch's current device and current stream of a device, as plain functions: these calls take microseconds
 
 
 def _dt3(t):
@@ -611,36 +612,37 @@ def _dt3(t):
     if not _DT3:
         import torch
         _DT3.update({torch.float32: KILN_F32, torch.float16: KILN_F16, torch.bfloat16: KILN_BF16})
-    if t.dtype not in _DT3:
+    d = _DT3.get(t.dtype)
+    if d is None:
         raise TypeError(f"unsupported dtype {t.dtype}")
-    return _DT3[t.dtype]
+    return d
 
 
-def _gpu(*ts):
-    """The device index shared by every tensor in ts (None skipped)."""
-    dev = None
-    for t in ts:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise ValueError(f"expected a tensor on the GPU, got one on {t.device}")
-        if dev is None:
-            dev = t.device.index
-        elif t.device.index != dev:
-            raise ValueError(f"tensors on different devices: {dev} and {t.device.index}")
+def _gpu(t, *others):
+    """The device index of t, which every other tensor (None skipped) shares."""
+    dev = t.get_device()
+    if dev < 0:
+        raise ValueError(f"expected a tensor on the GPU, got one on {t.device}")
+    for o in others:
+        if o is not None and o.get_device() != dev:
+            raise ValueError(f"tensors on different devices: {t.device} and {o.device}")
     return dev
 
 
 def _launch(fn, dev, stream, *args):
     """fn(*args, stream) with device `dev` current, on the given stream or the device's current one."""
-    import torch
-    s = stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(dev)
-    if torch.cuda.current_device() == dev:
+    if not _NOW:
+        import torch
+        torch.cuda.init()
+        _NOW.extend((torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream))
+    s = stream.cuda_stream if stream is not None else _NOW[1](dev)
+    if _NOW[0]() == dev:
         rc = fn(*args, s)
     else:
+        import torch
         with torch.cuda.device(dev):
             rc = fn(*args, s)
-    if rc != KILN_OK:
+    if rc:
         _check(rc)
 
 
@@ -653,13 +655,20 @@ def _scratch(nbytes, dev, stream):
         return torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", dev))
 
 
-def _rows_ld(t, what, cols=None):
-    """Row stride of a 2-D tensor whose rows are contiguous, have `cols` columns and do not repeat."""
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise ValueError(f"{what}: expected a 2-D tensor with contiguous rows, got shape {tuple(t.shape)} strides {t.stride()}")
-    if cols is not None and t.shape[1] != cols:
-        raise ValueError(f"{what}: expected {cols} columns, got {t.shape[1]}")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _nbytes(workspace, what):
+    if workspace is None:
+        return 0
+    if not workspace.is_contiguous():
+        raise ValueError(f"{what}: workspace must be contiguous")
+    return workspace.numel() * workspace.element_size()
+
+
+def _rows_ld(t, what):
+    """Row stride of a 2-D tensor whose rows are contiguous (its columns, where there is one row)."""
+    st = t.stride()
+    if len(st) != 2 or (st[1] != 1 and t.shape[1] > 1):
+        raise ValueError(f"{what}: expected a 2-D tensor with contiguous rows, got shape {tuple(t.shape)} strides {st}")
+    return st[0] if t.shape[0] > 1 else t.shape[1]
 
 
 def rope_freqs(rot, theta=10000.0, scaling="none", factor=1.0, trained=0.0, slow=1.0, fast=None, device=None):
@@ -678,18 +687,17 @@ def rope_freqs(rot, theta=10000.0, scaling="none", factor=1.0, trained=0.0, slow
 def rope(y, x, H, Dh, freqs, pos=None, pos0=0, interleaved=False, mscale=1.0, stream=None):
     """Rotary positions (kiln_rope) of the H heads of Dh in the rows of x [T, H*Dh], into y (y = x: in place); the first
     2 * freqs.numel() dimensions of a head turn. pos: int32 [T], or None for pos0, pos0 + 1, .."""
-    import torch
-    dev = _gpu(y, x, freqs, pos)
-    T = x.shape[0]
-    ldx, ldy = _rows_ld(x, "rope: x", H * Dh), _rows_ld(y, "rope: y", H * Dh)
-    if y.shape[0] != T or y.dtype != x.dtype:
-        raise ValueError(f"rope: y {tuple(y.shape)} {y.dtype} does not match x {tuple(x.shape)} {x.dtype}")
-    if freqs.dtype != torch.float64 or not freqs.is_contiguous():
+    dev = _gpu(x, y, freqs, pos)
+    ldx, ldy = _rows_ld(x, "rope: x"), _rows_ld(y, "rope: y")
+    T, W = x.shape
+    if W != H * Dh or y.shape != x.shape or y.dtype != x.dtype:
+        raise ValueError(f"rope: x {tuple(x.shape)} {x.dtype}, y {tuple(y.shape)} {y.dtype} for {H} heads of {Dh}")
+    if freqs.element_size() != 8 or not freqs.is_floating_point() or not freqs.is_contiguous():
         raise ValueError("rope: freqs must be a contiguous float64 tensor (rope_freqs)")
-    if pos is not None and (pos.dtype != torch.int32 or pos.numel() != T or not pos.is_contiguous()):
+    if pos is not None and (pos.element_size() != 4 or pos.is_floating_point() or pos.numel() != T or not pos.is_contiguous()):
         raise ValueError(f"rope: pos must be a contiguous int32 tensor of {T} positions")
-    _launch(lib().kiln_rope, dev, stream, y.data_ptr(), ldy, x.data_ptr(), ldx, _dt3(x), T, H, Dh, 2 * freqs.numel(),
-            int(bool(interleaved)), None if pos is None else pos.data_ptr(), pos0, freqs.data_ptr(), mscale)
+    _launch((_LIB or lib()).kiln_rope, dev, stream, y.data_ptr(), ldy, x.data_ptr(), ldx, _dt3(x), T, H, Dh, 2 * freqs.numel(),
+            1 if interleaved else 0, pos.data_ptr() if pos is not None else None, pos0, freqs.data_ptr(), mscale)
     return y
 
 
@@ -701,14 +709,13 @@ def cross_attn(out, q, k, v, Hq, Hkv=None, scale=None, klen=None, kmask=None, wo
     """Attention of q [B, Tq, Hq*Dh] to the encoder states k, v [B, Tk, Hkv*Dh] (kiln_cross_attn), out like q; fp16 or bf16,
     Dh 64 or 128. klen: int32 [B] keys per item; kmask: bool or uint8 [B, Tk], 0 where a key is left out. scale defaults to
     Dh^-0.5. workspace: cross_attn_workspace_bytes; None takes one for the call."""
-    import torch
-    dev = _gpu(out, q, k, v, klen, kmask, workspace)
+    dev = _gpu(q, out, k, v, klen, kmask, workspace)
     Hkv = Hq if Hkv is None else Hkv
-    for n, t in (("out", out), ("q", q), ("k", k), ("v", v)):
-        if t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1):
-            raise ValueError(f"cross_attn: {n} must be [B, T, heads*Dh] with contiguous rows")
-        if t.dtype != q.dtype:
-            raise ValueError(f"cross_attn: {n} is {t.dtype}, q is {q.dtype}")
+    so, sq, sk, sv = out.stride(), q.stride(), k.stride(), v.stride()
+    if not len(so) == len(sq) == len(sk) == len(sv) == 3 or not so[2] == sq[2] == sk[2] == sv[2] == 1:
+        raise ValueError("cross_attn: out, q, k and v must be [B, T, heads*Dh] with contiguous rows")
+    if not out.dtype == q.dtype == k.dtype == v.dtype:
+        raise ValueError(f"cross_attn: out is {out.dtype}, q {q.dtype}, k {k.dtype}, v {v.dtype}")
     B, Tq, W = q.shape
     Tk = k.shape[1]
     if Hq <= 0 or Hkv <= 0 or Hq % Hkv or W % Hq:
@@ -716,57 +723,55 @@ def cross_attn(out, q, k, v, Hq, Hkv=None, scale=None, klen=None, kmask=None, wo
     Dh = W // Hq
     if out.shape != q.shape or k.shape != (B, Tk, Hkv * Dh) or v.shape != k.shape:
         raise ValueError(f"cross_attn: shapes out {tuple(out.shape)} q {tuple(q.shape)} k {tuple(k.shape)} v {tuple(v.shape)}")
-    if klen is not None and (klen.dtype != torch.int32 or klen.numel() != B or not klen.is_contiguous()):
+    if klen is not None and (klen.element_size() != 4 or klen.is_floating_point() or klen.numel() != B or not klen.is_contiguous()):
         raise ValueError(f"cross_attn: klen must be a contiguous int32 tensor of {B} lengths")
-    if kmask is not None and (kmask.dtype not in (torch.bool, torch.uint8) or kmask.shape != (B, Tk) or (Tk > 1 and kmask.stride(1) != 1)):
-        raise ValueError(f"cross_attn: kmask must be a bool or uint8 tensor [{B}, {Tk}] with contiguous rows")
+    if kmask is not None:
+        sm = kmask.stride()
+        if kmask.element_size() != 1 or kmask.shape != (B, Tk) or (sm[1] != 1 and Tk > 1):
+            raise ValueError(f"cross_attn: kmask must be a bool or uint8 tensor [{B}, {Tk}] with contiguous rows")
+    L = _LIB or lib()
     if workspace is None:
-        n = lib().kiln_cross_attn_workspace_bytes(B, Tq, Tk, Hq, Hkv, Dh)
+        n = L.kiln_cross_attn_workspace_bytes(B, Tq, Tk, Hq, Hkv, Dh)
         if n:
             workspace = _scratch(n, dev, stream)
-    elif not workspace.is_contiguous():
-        raise ValueError("cross_attn: workspace must be contiguous")
-    _launch(lib().kiln_cross_attn, dev, stream, out.data_ptr(), out.stride(1), out.stride(0), q.data_ptr(), q.stride(1), q.stride(0),
-            k.data_ptr(), k.stride(1), k.stride(0), v.data_ptr(), v.stride(1), v.stride(0), _dt3(q), B, Tq, Tk, Hq, Hkv, Dh,
-            Dh ** -0.5 if scale is None else scale, None if klen is None else klen.data_ptr(),
-            None if kmask is None else kmask.data_ptr(), 0 if kmask is None else kmask.stride(0),
-            None if workspace is None else workspace.data_ptr(),
-            0 if workspace is None else workspace.numel() * workspace.element_size())
+    _launch(L.kiln_cross_attn, dev, stream, out.data_ptr(), so[1], so[0], q.data_ptr(), sq[1], sq[0], k.data_ptr(), sk[1], sk[0],
+            v.data_ptr(), sv[1], sv[0], _dt3(q), B, Tq, Tk, Hq, Hkv, Dh, Dh ** -0.5 if scale is None else scale,
+            klen.data_ptr() if klen is not None else None, kmask.data_ptr() if kmask is not None else None,
+            sm[0] if kmask is not None else 0, workspace.data_ptr() if workspace is not None else None,
+            _nbytes(workspace, "cross_attn"))
     return out
 
 
 def _mx_plain(codes, scales, rows, cols, what):
-    import torch
-    for n, t, shape in (("codes", codes, (rows, cols // 2)), ("scales", scales, (rows, cols // 32))):
-        if t.dtype != torch.uint8 or tuple(t.shape) != shape or not t.is_contiguous():
-            raise ValueError(f"{what}: {n} must be a contiguous uint8 tensor {list(shape)}, got {t.dtype} {list(t.shape)}")
+    if codes.shape != (rows, cols // 2) or scales.shape != (rows, cols // 32) or codes.element_size() != 1 or \
+            scales.element_size() != 1 or not codes.is_contiguous() or not scales.is_contiguous():
+        raise ValueError(f"{what}: codes and scales must be contiguous uint8 tensors {[rows, cols // 2]} and {[rows, cols // 32]}, got "
+                         f"{codes.dtype} {list(codes.shape)} and {scales.dtype} {list(scales.shape)}")
 
 
 def mxfp4_quantize(x, codes=None, scales=None, stream=None):
     """x [rows, cols] (fp32, fp16 or bf16, cols % 32 == 0) to MXFP4 (kiln_mxfp4_quantize): uint8 codes [rows, cols / 2] and
     scales [rows, cols / 32]."""
-    import torch
-    ldx = _rows_ld(x, "mxfp4_quantize: x")
+    dev, ldx = _gpu(x, codes, scales), _rows_ld(x, "mxfp4_quantize: x")
     rows, cols = x.shape
-    dev = _gpu(x, codes, scales)
     if codes is None or scales is None:
         if codes is not None or scales is not None:
             raise ValueError("mxfp4_quantize: codes and scales go together")
+        import torch
         with torch.cuda.stream(stream):
             codes = torch.empty(rows, cols // 2, dtype=torch.uint8, device=x.device)
             scales = torch.empty(rows, cols // 32, dtype=torch.uint8, device=x.device)
     _mx_plain(codes, scales, rows, cols, "mxfp4_quantize")
-    _launch(lib().kiln_mxfp4_quantize, dev, stream, codes.data_ptr(), scales.data_ptr(), x.data_ptr(), _dt3(x), ldx, rows, cols)
+    _launch((_LIB or lib()).kiln_mxfp4_quantize, dev, stream, codes.data_ptr(), scales.data_ptr(), x.data_ptr(), _dt3(x), ldx, rows, cols)
     return codes, scales
 
 
 def mxfp4_dequantize(y, codes, scales, stream=None):
     """The values of MXFP4 codes and scales (kiln_mxfp4_dequantize) into y [rows, cols]."""
-    ldy = _rows_ld(y, "mxfp4_dequantize: y")
+    dev, ldy = _gpu(y, codes, scales), _rows_ld(y, "mxfp4_dequantize: y")
     rows, cols = y.shape
     _mx_plain(codes, scales, rows, cols, "mxfp4_dequantize")
-    _launch(lib().kiln_mxfp4_dequantize, _gpu(y, codes, scales), stream, y.data_ptr(), _dt3(y), ldy, codes.data_ptr(), scales.data_ptr(),
-            rows, cols)
+    _launch((_LIB or lib()).kiln_mxfp4_dequantize, dev, stream, y.data_ptr(), _dt3(y), ldy, codes.data_ptr(), scales.data_ptr(), rows, cols)
     return y
 
 
@@ -800,24 +805,22 @@ def linear_mxfp4(y, x, w, epi=KILN_EPI_F32, gate=None, beta=0.0, workspace=None,
     """linear16's layer with an MXFP4 weight (kiln_linear_mxfp4): y [T, rows] = epilogue(Q(x) w^T), x [T, cols] fp32, fp16 or
     bf16, w an Mxfp4Weight, y fp32 (F32, RESID) or fp16 (F16, GELU16). workspace: linear_mxfp4_workspace_bytes; None takes
     one for the call."""
-    import torch
+    dev = _gpu(x, y, w.buf, gate, workspace)
+    ldx, ldy = _rows_ld(x, "linear_mxfp4: x"), _rows_ld(y, "linear_mxfp4: y")
     rows, cols = w.shape
-    dev = _gpu(y, x, w.buf, gate, workspace)
-    ldx, ldy = _rows_ld(x, "linear_mxfp4: x", cols), _rows_ld(y, "linear_mxfp4: y", rows)
     T = x.shape[0]
-    if y.shape[0] != T:
-        raise ValueError(f"linear_mxfp4: y has {y.shape[0]} rows, x {T}")
-    if y.dtype != (torch.float32 if epi in (KILN_EPI_F32, KILN_EPI_RESID) else torch.float16):
+    if x.shape[1] != cols or y.shape != (T, rows):
+        raise ValueError(f"linear_mxfp4: x {tuple(x.shape)}, y {tuple(y.shape)} for a weight [{rows}, {cols}]")
+    if _dt3(y) != (KILN_F32 if epi in (KILN_EPI_F32, KILN_EPI_RESID) else KILN_F16):
         raise ValueError(f"linear_mxfp4: y is {y.dtype} with epilogue {epi}")
-    if gate is not None and (gate.dtype != torch.float32 or gate.numel() != rows or not gate.is_contiguous()):
+    if gate is not None and (_dt3(gate) != KILN_F32 or gate.numel() != rows or not gate.is_contiguous()):
         raise ValueError(f"linear_mxfp4: gate must be a contiguous float32 tensor of {rows}")
+    L = _LIB or lib()
     if workspace is None:
-        n = lib().kiln_linear_mxfp4_workspace_bytes(T, rows, cols)
+        n = L.kiln_linear_mxfp4_workspace_bytes(T, rows, cols)
         if n:
             workspace = _scratch(n, dev, stream)
-    elif not workspace.is_contiguous():
-        raise ValueError("linear_mxfp4: workspace must be contiguous")
-    _launch(lib().kiln_linear_mxfp4, dev, stream, y.data_ptr(), ldy, x.data_ptr(), _dt3(x), ldx, T, w.buf.data_ptr(), rows, cols, epi,
-            None if gate is None else gate.data_ptr(), beta, None if workspace is None else workspace.data_ptr(),
-            0 if workspace is None else workspace.numel() * workspace.element_size())
+    _launch(L.kiln_linear_mxfp4, dev, stream, y.data_ptr(), ldy, x.data_ptr(), _dt3(x), ldx, T, w.buf.data_ptr(), rows, cols, epi,
+            gate.data_ptr() if gate is not None else None, beta, workspace.data_ptr() if workspace is not None else None,
+            _nbytes(workspace, "linear_mxfp4"))
     return y
