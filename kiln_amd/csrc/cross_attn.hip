@@ -38,7 +38,8 @@ struct CrossParams {
     long long bsm;
     float sc;  // scale log2(e)
     int rows;                       // Tq G
-    int rtiles, ksplit, total, per;  // row tiles, key ranges of one, work items, items per XCD
+    int rtiles, ksplit, ct;         // row tiles, key ranges of one (ct tiles each), ..
+    int total, per;                 // .. work items, items per XCD
     float* part;                    // ksplit > 1: partial results [item][row of the tile][DH], then [item][row](m, l)
 };
 
@@ -77,32 +78,40 @@ template <int N>
 __device__ __forceinline__ void x_wait_vmcnt() {
     __builtin_amdgcn_s_waitcnt((N & 0xF) | (0x7 << 4) | (0xF << 8) | ((N >> 4) << 14));
 }
-// position of 16-byte chunk c of key row r: K is read 16 keys x one chunk at a time (eight neighbouring keys take eight
-// positions), V four keys x a pair of chunks at a time (four neighbouring keys take four pairs)
-__device__ __forceinline__ int k_swz(int c, int r) { return c ^ (r & 7); }
-__device__ __forceinline__ int v_swz(int c, int r) { return c ^ (((r & 3) << 1) | ((r >> 2) & 1)); }
+// Position of 16-byte chunk c of key row r in its LDS row. K is read 16 keys x one chunk at a time, V eight keys x a pair of
+// chunks: either way 256 bytes that lie in all 64 banks, for rows of 256 bytes (Dh 128) and of 128.
+template <int DH>
+__device__ __forceinline__ int k_swz(int c, int r) {
+    return DH == 128 ? c ^ (r & 15) : c ^ ((r >> 1) & 7);
+}
+template <int DH>
+__device__ __forceinline__ int v_swz(int c, int r) {
+    return DH == 128 ? c ^ ((r & 7) << 1) : c ^ (((r >> 1) & 3) << 1);
+}
 
-// QB 16-row blocks per wave; KW = 1: four waves with rows of their own share the tiles; KW = 4: four waves with the same
-// rows, each with a quarter of the keys and tiles of its own, whose results meet in LDS
-template <class E, int DH, int QB, int KW>
+// A workgroup's geometry: NW waves of 16 QB rows. SHARED: the waves have rows of their own and share a ring of NS tiles.
+// Otherwise every wave has the same rows, a ring and a share of the keys of its own; the results of four meet in LDS.
+template <int DH_, int QB_, int NW_, bool SHARED_, int NS_>
 struct XCfg {
-    static constexpr int RW = 16 * QB, RT = RW * 4 / KW;              // rows of a wave, of the workgroup
-    static constexpr int PC = DH / 8;                                 // 16-byte chunks of a row
-    static constexpr int TILE = XKT * DH * 2, STAGE = 2 * TILE;       // K tile, V tile
-    static constexpr int NS = KW == 4 ? 2 : 4;                        // stages of a ring
-    static constexpr int THREADS_PER_RING = 256 / KW;
-    static constexpr int DMA = XKT * PC / THREADS_PER_RING;           // 16-byte pieces per thread, for K and for V each
-    static constexpr int RING = NS * STAGE;
-    static constexpr int BITS = 4 * 32 * 4;                           // each wave's mask windows: 2 x 16 words
-    static constexpr int MERGE = KW == 4 ? 4 * RW * (DH + 2) * 4 : 0; // the waves' results
-    static constexpr int LDS = (RING * KW > MERGE ? RING * KW : MERGE) + BITS;
+    static constexpr int DH = DH_, QB = QB_, NW = NW_, NS = NS_;
+    static constexpr bool SHARED = SHARED_;
+    static constexpr int THREADS = 64 * NW, RW = 16 * QB, RT = SHARED ? RW * NW : RW;  // rows of a wave, of the workgroup
+    static constexpr int PC = DH / 8;                                  // 16-byte chunks of a row
+    static constexpr int TILE = XKT * DH * 2, STAGE = 2 * TILE;        // K tile, V tile
+    static constexpr int RTHREADS = SHARED ? THREADS : 64;             // threads that fill a ring
+    static constexpr int DMA = XKT * PC / RTHREADS;                    // 16-byte pieces per thread, for K and for V each
+    static constexpr int RING = NS * STAGE, RINGS = SHARED ? RING : RING * NW;
+    static constexpr int BITS = NW * 32 * 4;                           // each wave's mask windows: 2 x 16 words
+    static constexpr int MERGE = !SHARED && NW > 1 ? NW * RW * (DH + 2) * 4 : 0;
+    static constexpr int LDS = (RINGS > MERGE ? RINGS : MERGE) + BITS;
+    static constexpr int WAVES = LDS <= 40 * 1024 ? 4 : LDS <= 80 * 1024 || NW == 1 ? 2 : 1;  // per SIMD that registers have to allow
 };
 
-template <class E, int DH, int QB, int KW>
-__global__ __launch_bounds__(256) void k_cross_attn(const CrossParams p) {
+template <class E, class C, bool MASK>
+__global__ __launch_bounds__(C::THREADS, C::WAVES) void k_cross_attn(const CrossParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)  // the host pass drops a kernel template whose target builtins it cannot check
-    using C = XCfg<E, DH, QB, KW>;
     using M = XMma<E>;
+    constexpr int DH = C::DH, QB = C::QB;
     extern __shared__ __attribute__((aligned(16))) uint8_t xlds[];
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, c16 = lane & 15;
@@ -114,15 +123,16 @@ __global__ __launch_bounds__(256) void k_cross_attn(const CrossParams p) {
     const int L = p.klen ? max(0, min(p.klen[b], p.Tk)) : p.Tk;
     const int nt = (L + XKT - 1) / XKT;
     // this workgroup's tiles, this wave's tiles
-    const int g0 = (int)((long long)nt * ks / p.ksplit), g1 = (int)((long long)nt * (ks + 1) / p.ksplit);
-    const int t0 = KW == 1 ? g0 : g0 + (g1 - g0) * wv / 4, t1 = KW == 1 ? g1 : g0 + (g1 - g0) * (wv + 1) / 4;
-    const uint8_t* mask = p.kmask ? p.kmask + (long long)b * p.bsm : nullptr;
+    const int g0 = ks * p.ct, g1 = min(nt, g0 + p.ct);
+    if (p.ksplit > 1 && g0 >= g1) return;  // the merge leaves ranges past the item's keys out
+    const int t0 = C::SHARED ? g0 : g0 + max(g1 - g0, 0) * wv / C::NW, t1 = C::SHARED ? g1 : g0 + max(g1 - g0, 0) * (wv + 1) / C::NW;
 
-    uint8_t* ring = xlds + (KW == 4 ? wv * C::RING : 0);
+    uint8_t* ring = xlds + (C::SHARED ? 0 : wv * C::RING);
     const uint32_t lds_base = (uint32_t)(size_t)(__attribute__((address_space(3))) uint8_t*)ring;
+    const uint8_t* mask = MASK ? p.kmask + (long long)b * p.bsm : nullptr;
     uint32_t* bits = reinterpret_cast<uint32_t*>(xlds + C::LDS - C::BITS) + wv * 32;
 
-    // The keys of tile j as bits. With a mask: windows of 16 tiles (512 keys) in LDS, two of them, each wave its own.
+    // The keys of tile j < t1 as bits. With a mask: windows of 16 tiles (512 keys) in LDS, two of them, each wave its own.
     auto fill_window = [&](int w) {  // window w of this wave's tiles: tiles t0 + 16 w ..
 #pragma unroll
         for (int i = 0; i < 8; i++) {
@@ -133,49 +143,56 @@ __global__ __launch_bounds__(256) void k_cross_attn(const CrossParams p) {
         __builtin_amdgcn_wave_barrier();
     };
     auto tile_bits = [&](int j) -> uint32_t {
-        if (j >= t1) return 0u;
-        if (mask) return __builtin_amdgcn_readfirstlane(bits[(j - t0) & 31]);
+        if constexpr (MASK) return __builtin_amdgcn_readfirstlane(bits[(j - t0) & 31]);
         const int left = L - j * XKT;
         return left >= XKT ? ~0u : (1u << left) - 1u;
     };
 
-    // DMA of tile j: a thread's pieces are chunks of fixed rows; a masked row's offset is beyond every range
-    const int tr = KW == 4 ? lane : (int)threadIdx.x;
-    const uint8_t* kb = static_cast<const uint8_t*>(p.k) + ((long long)b * p.bsk + (long long)hk * DH) * 2;
-    const uint8_t* vb = static_cast<const uint8_t*>(p.v) + ((long long)b * p.bsv + (long long)hk * DH) * 2;
+    // DMA of the tiles in turn: a thread's pieces are chunks of fixed rows of a tile; the descriptor's range ends with the
+    // item's last row (empty past the last tile), and a masked row's offset is beyond every range
+    const int tr = C::SHARED ? (int)threadIdx.x : lane;
+    const uint32_t ldk2 = (uint32_t)p.ldk * 2, ldv2 = (uint32_t)p.ldv * 2;
+    const uint8_t* kp = static_cast<const uint8_t*>(p.k) + ((long long)b * p.bsk + (long long)hk * DH) * 2 + (long long)t0 * XKT * ldk2;
+    const uint8_t* vp = static_cast<const uint8_t*>(p.v) + ((long long)b * p.bsv + (long long)hk * DH) * 2 + (long long)t0 * XKT * ldv2;
+    int dma_j = t0, into = 0;  // the next tile to copy, its stage
     uint32_t ko[C::DMA], vo[C::DMA];
     int prow[C::DMA];
 #pragma unroll
     for (int i = 0; i < C::DMA; i++) {
-        const int pc = i * C::THREADS_PER_RING + tr, r = pc / C::PC, c = pc % C::PC;
+        const int pc = i * C::RTHREADS + tr, r = pc / C::PC, c = pc % C::PC;
         prow[i] = r;
-        ko[i] = (uint32_t)(r * p.ldk * 2 + k_swz(c, r) * 16);
-        vo[i] = (uint32_t)(r * p.ldv * 2 + v_swz(c, r) * 16);
+        ko[i] = r * ldk2 + k_swz<DH>(c, r) * 16;
+        vo[i] = r * ldv2 + v_swz<DH>(c, r) * 16;
     }
-    auto dma = [&](int j, int stage) {
-        if (mask && j < t1 && ((j - t0) & 15) == 0) fill_window((j - t0) >> 4);
-        const int left = j < t1 ? min(XKT, L - j * XKT) : 0;
-        const long long row0 = (long long)j * XKT;
+    auto dma = [&]() {
+        uint32_t m = ~0u;
+        const int left = dma_j < t1 ? min(XKT, L - dma_j * XKT) : 0;
+        if constexpr (MASK) {
+            if (left > 0) {
+                if (((dma_j - t0) & 15) == 0) fill_window((dma_j - t0) >> 4);
+                m = tile_bits(dma_j);
+            }
+        }
         const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
-            const_cast<uint8_t*>(kb + (j < t1 ? row0 * (long long)p.ldk * 2 : 0)), (short)0,
-            left > 0 ? (int)((left - 1) * p.ldk * 2 + DH * 2) : 0, 0x00020000 /* raw */);
+            const_cast<uint8_t*>(kp), (short)0, left > 0 ? (int)((left - 1) * ldk2 + DH * 2) : 0, 0x00020000 /* raw */);
         const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
-            const_cast<uint8_t*>(vb + (j < t1 ? row0 * (long long)p.ldv * 2 : 0)), (short)0,
-            left > 0 ? (int)((left - 1) * p.ldv * 2 + DH * 2) : 0, 0x00020000);
-        uint8_t* dst = ring + stage * C::STAGE + (KW == 4 ? 0 : wv * 1024);
-        const uint32_t m = mask ? tile_bits(j) : ~0u;
+            const_cast<uint8_t*>(vp), (short)0, left > 0 ? (int)((left - 1) * ldv2 + DH * 2) : 0, 0x00020000);
+        uint8_t* dst = ring + into * C::STAGE + (C::SHARED ? wv * 1024 : 0);
 #pragma unroll
         for (int i = 0; i < C::DMA; i++)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_ptr)(dst + i * C::THREADS_PER_RING * 16), 16,
-                                                     m >> prow[i] & 1 ? ko[i] : 0x7ffffff0u, 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_ptr)(dst + i * C::RTHREADS * 16), 16,
+                                                     !MASK || (m >> prow[i] & 1) ? ko[i] : 0x7ffffff0u, 0, 0, 0);
 #pragma unroll
         for (int i = 0; i < C::DMA; i++)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_ptr)(dst + C::TILE + i * C::THREADS_PER_RING * 16), 16,
-                                                     m >> prow[i] & 1 ? vo[i] : 0x7ffffff0u, 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_ptr)(dst + C::TILE + i * C::RTHREADS * 16), 16,
+                                                     !MASK || (m >> prow[i] & 1) ? vo[i] : 0x7ffffff0u, 0, 0, 0);
+        if (dma_j + 1 < t1) kp += (size_t)XKT * ldk2, vp += (size_t)XKT * ldv2;
+        dma_j++;
+        into = into == C::NS - 1 ? 0 : into + 1;
     };
 
     // Q: the B operands of S^T, lane (row c16, chunk 4 cc + g); rows past the last read row 0 and are not stored
-    const int row0 = rt * C::RT + (KW == 4 ? 0 : wv * C::RW);
+    const int row0 = rt * C::RT + (C::SHARED ? wv * C::RW : 0);
     u32x4 qf[QB][DH / 32];
 #pragma unroll
     for (int qb = 0; qb < QB; qb++) {
@@ -185,43 +202,50 @@ __global__ __launch_bounds__(256) void k_cross_attn(const CrossParams p) {
         for (int cc = 0; cc < DH / 32; cc++) qf[qb][cc] = *reinterpret_cast<const u32x4*>(src + 64 * cc);
     }
 
-    floatx4 o[DH / 16][QB];
-    float m[QB], mn[QB], l[QB];  // running maximum; its negative as subtracted (0 while the maximum is -inf); this lane's sum
+    floatx4 o[DH / 16][QB], l[QB];  // l: every register of a lane holds its row's sum (P^T times ones)
+    float m[QB], mn[QB];            // running maximum; its negative as subtracted (0 while the maximum is -inf)
 #pragma unroll
     for (int qb = 0; qb < QB; qb++) {
         m[qb] = -INFINITY;
         mn[qb] = 0.f;
-        l[qb] = 0.f;
+        l[qb] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int db = 0; db < DH / 16; db++) o[db][qb] = floatx4{0.f, 0.f, 0.f, 0.f};
     }
+    const uint32_t one2 = M::pack(1.f, 1.f);
+    const u32x4 ones = {one2, one2, one2, one2};
+    // operand addresses within a stage: the chunk's permutation depends on the row's low bits only, the same for rows 16 apart
+    uint32_t kaddr[DH / 32], vaddr[DH / 16];
+#pragma unroll
+    for (int cc = 0; cc < DH / 32; cc++) kaddr[cc] = lds_base + c16 * DH * 2 + k_swz<DH>(4 * cc + g, c16) * 16;
+    // V: keys 16 jh + 4 g .. + 3 of dimension 16 db + c16, from the rows and 8-byte pieces that the 16 lanes name
+    const int vr = 4 * g + (c16 >> 2);
+#pragma unroll
+    for (int db = 0; db < DH / 16; db++)
+        vaddr[db] = lds_base + C::TILE + vr * DH * 2 + v_swz<DH>(2 * db + ((c16 & 3) >> 1), vr) * 16 + (c16 & 1) * 8;
 
 #pragma unroll
-    for (int s = 0; s < C::NS - 1; s++) dma(t0 + s, s);
-    int stage = 0;
+    for (int s = 0; s < C::NS - 1; s++) dma();
+    uint32_t st = 0;  // the stage's offset
     for (int j = t0; j < t1; j++) {
         // tile j landed (past the last tile the copies go on with empty ranges, which keeps the count); every wave that
         // shares the ring is done with tile j - 1, whose stage is refilled
         x_wait_vmcnt<(C::NS - 2) * 2 * C::DMA>();
         __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
-        if constexpr (KW == 1) __builtin_amdgcn_s_barrier();
+        if constexpr (C::SHARED) __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
-        if constexpr (C::NS > 2) dma(j + C::NS - 1, stage == 0 ? C::NS - 1 : stage - 1);
-        else dma(j + 1, stage ^ 1);
-        const uint32_t bt = tile_bits(j);
-        const uint32_t ka = lds_base + stage * C::STAGE, va = ka + C::TILE;
+        dma();
         floatx4 s[2][QB];
 #pragma unroll
-        for (int kk = 0; kk < 2; kk++) {
-            const int r = 16 * kk + c16;
+        for (int kk = 0; kk < 2; kk++)
 #pragma unroll
             for (int cc = 0; cc < DH / 32; cc++) {
-                const u32x4 kf = *reinterpret_cast<const lds_x4*>((size_t)(ka + r * DH * 2 + k_swz(4 * cc + g, r) * 16));
+                const u32x4 kf = *reinterpret_cast<const lds_x4*>((size_t)(kaddr[cc] + st + kk * 16 * DH * 2));
 #pragma unroll
                 for (int qb = 0; qb < QB; qb++)
                     s[kk][qb] = M::mul(kf, qf[qb][cc], cc == 0 ? floatx4{0.f, 0.f, 0.f, 0.f} : s[kk][qb]);
             }
-        }
+        const uint32_t bt = tile_bits(j);
         if (bt != ~0u) {
 #pragma unroll
             for (int kk = 0; kk < 2; kk++)
@@ -237,79 +261,70 @@ __global__ __launch_bounds__(256) void k_cross_attn(const CrossParams p) {
         for (int qb = 0; qb < QB; qb++) {
             float t = fmaxf(s[0][qb][0], s[1][qb][0]);
 #pragma unroll
-            for (int i = 1; i < 4; i++) t = fmaxf(t, fmaxf(s[0][qb][i], s[1][qb][i]));
+            for (int i = 1; i < 4; i++) t = fmaxf(fmaxf(t, s[0][qb][i]), s[1][qb][i]);
             top[qb] = t * p.sc;
             moves |= top[qb] > m[qb] + XRESCALE;  // from -inf: any score that is not
         }
         if (__any(moves)) {
 #pragma unroll
             for (int qb = 0; qb < QB; qb++) {
-                const float t = quad_max(top[qb]);
-                if (t > m[qb]) {
-                    const float f = __builtin_amdgcn_exp2f(m[qb] - t);
-                    m[qb] = t;
-                    mn[qb] = -t;
-                    l[qb] *= f;
+                const float t = fmaxf(m[qb], quad_max(top[qb]));
+                const float f = t > m[qb] ? __builtin_amdgcn_exp2f(m[qb] - t) : 1.f;
+                m[qb] = t;
+                mn[qb] = t == -INFINITY ? 0.f : -t;
+                l[qb] *= f;
 #pragma unroll
-                    for (int db = 0; db < DH / 16; db++) o[db][qb] *= f;
-                }
+                for (int db = 0; db < DH / 16; db++) o[db][qb] *= f;
             }
         }
         u32x4 pf[QB];
 #pragma unroll
-        for (int qb = 0; qb < QB; qb++) {
-            float e[8];
+        for (int qb = 0; qb < QB; qb++)
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                e[i] = __builtin_amdgcn_exp2f(fmaf(s[i / 4][qb][i % 4], p.sc, mn[qb]));
-                l[qb] += e[i];
-            }
+            for (int i = 0; i < 4; i++)
+                pf[qb][i] = M::pack(__builtin_amdgcn_exp2f(fmaf(s[i / 2][qb][2 * i % 4], p.sc, mn[qb])),
+                                    __builtin_amdgcn_exp2f(fmaf(s[i / 2][qb][2 * i % 4 + 1], p.sc, mn[qb])));
 #pragma unroll
-            for (int i = 0; i < 4; i++) pf[qb][i] = M::pack(e[2 * i], e[2 * i + 1]);
-        }
+        for (int qb = 0; qb < QB; qb++) l[qb] = M::mul(ones, pf[qb], l[qb]);
 #pragma unroll
         for (int db = 0; db < DH / 16; db++) {
-            // lane: keys 16 jh + 4 g .. + 3 of dimension 16 db + c16, from the rows and 8-byte pieces the 16 lanes name
-            const int r = 4 * g + (c16 >> 2), c = 2 * db + ((c16 & 3) >> 1), h8 = (c16 & 1) * 8;
-            const s4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v*)(size_t)(va + r * DH * 2 + v_swz(c, r) * 16 + h8));
-            const s4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v*)(size_t)(va + (r + 16) * DH * 2 + v_swz(c, r + 16) * 16 + h8));
-            const u32x2 a = __builtin_bit_cast(u32x2, lo), d = __builtin_bit_cast(u32x2, hi);
+            const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v*)(size_t)(vaddr[db] + st)));
+            const u32x2 d = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v*)(size_t)(vaddr[db] + st + 16 * DH * 2)));
             const u32x4 vf = {a[0], a[1], d[0], d[1]};
 #pragma unroll
             for (int qb = 0; qb < QB; qb++) o[db][qb] = M::mul(vf, pf[qb], o[db][qb]);
         }
-        stage = stage == C::NS - 1 ? 0 : stage + 1;
+        st = st == (C::NS - 1) * C::STAGE ? 0 : st + C::STAGE;
     }
     x_wait_vmcnt<0>();  // no copy into LDS outlives its ring
 
-#pragma unroll
-    for (int qb = 0; qb < QB; qb++) l[qb] = quad_sum(l[qb]);
-
-    if constexpr (KW == 1) {
+    auto store4 = [&](int r, int d, float a0, float a1, float a2, float a3) {
+        const int t = r / p.G, h = hk * p.G + r % p.G;
+        uint8_t* dst = static_cast<uint8_t*>(p.o) + ((long long)b * p.bso + (long long)t * p.ldo + (long long)h * DH + d) * 2;
+        *reinterpret_cast<u32x2*>(dst) = u32x2{M::pack(a0, a1), M::pack(a2, a3)};
+    };
+    if constexpr (C::SHARED || C::NW == 1) {
 #pragma unroll
         for (int qb = 0; qb < QB; qb++) {
             const int r = row0 + 16 * qb + c16;
             if (r >= p.rows) continue;
             if (p.ksplit > 1) {
-                const size_t at = (size_t)item * C::RT + (wv * C::RW + 16 * qb + c16);
+                const size_t at = (size_t)item * C::RT + (r - rt * C::RT);
 #pragma unroll
                 for (int db = 0; db < DH / 16; db++) *reinterpret_cast<floatx4*>(p.part + at * DH + 16 * db + 4 * g) = o[db][qb];
-                if (g == 0) *reinterpret_cast<float2*>(p.part + (size_t)p.total * C::RT * DH + at * 2) = make_float2(m[qb], l[qb]);
+                if (g == 0) *reinterpret_cast<float2*>(p.part + (size_t)p.total * C::RT * DH + at * 2) = make_float2(m[qb], l[qb][0]);
                 continue;
             }
-            const float inv = l[qb] > 0.f || l[qb] != l[qb] ? 1.f / l[qb] : 0.f;  // no key: zeros
-            const int t = r / p.G, h = hk * p.G + r % p.G;
-            uint8_t* dst = static_cast<uint8_t*>(p.o) + ((long long)b * p.bso + (long long)t * p.ldo + (long long)h * DH + 4 * g) * 2;
+            const float inv = l[qb][0] > 0.f || l[qb][0] != l[qb][0] ? 1.f / l[qb][0] : 0.f;  // no key: zeros
 #pragma unroll
             for (int db = 0; db < DH / 16; db++)
-                *reinterpret_cast<u32x2*>(dst + 32 * db) =
-                    u32x2{M::pack(o[db][qb][0] * inv, o[db][qb][1] * inv), M::pack(o[db][qb][2] * inv, o[db][qb][3] * inv)};
+                store4(r, 16 * db + 4 * g, o[db][qb][0] * inv, o[db][qb][1] * inv, o[db][qb][2] * inv, o[db][qb][3] * inv);
         }
     } else {
-        // the four waves' results of the same 16 QB rows
+        // the waves' results of the same 16 QB rows
         __syncthreads();
         float* ro = reinterpret_cast<float*>(xlds);
-        float* rml = ro + 4 * C::RW * DH;
+        float* rml = ro + C::NW * C::RW * DH;
 #pragma unroll
         for (int qb = 0; qb < QB; qb++) {
 #pragma unroll
@@ -317,112 +332,133 @@ __global__ __launch_bounds__(256) void k_cross_attn(const CrossParams p) {
                 *reinterpret_cast<floatx4*>(ro + (wv * C::RW + 16 * qb + c16) * DH + 16 * db + 4 * g) = o[db][qb];
             if (g == 0) {
                 rml[(wv * C::RW + 16 * qb + c16) * 2] = m[qb];
-                rml[(wv * C::RW + 16 * qb + c16) * 2 + 1] = l[qb];
+                rml[(wv * C::RW + 16 * qb + c16) * 2 + 1] = l[qb][0];
             }
         }
         __syncthreads();
-        for (int i = threadIdx.x; i < C::RW * DH / 4; i += 256) {
+        for (int i = threadIdx.x; i < C::RW * DH / 4; i += C::THREADS) {
             const int rl = i / (DH / 4), d = (i % (DH / 4)) * 4, r = row0 + rl;
             if (r >= p.rows) break;  // rows ascend with i
             float mm = -INFINITY, ll = 0.f;
 #pragma unroll
-            for (int w = 0; w < 4; w++) mm = fmaxf(mm, rml[(w * C::RW + rl) * 2]);
+            for (int w = 0; w < C::NW; w++) mm = fmaxf(mm, rml[(w * C::RW + rl) * 2]);
             const float me = mm == -INFINITY ? 0.f : mm;
             floatx4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int w = 0; w < 4; w++) {
+            for (int w = 0; w < C::NW; w++) {
                 const float f = __builtin_amdgcn_exp2f(rml[(w * C::RW + rl) * 2] - me);
                 ll += f * rml[(w * C::RW + rl) * 2 + 1];
                 acc += f * *reinterpret_cast<const floatx4*>(ro + (w * C::RW + rl) * DH + d);
             }
-            if (p.ksplit > 1) {
-                const size_t at = (size_t)item * C::RT + rl;
-                *reinterpret_cast<floatx4*>(p.part + at * DH + d) = acc;
-                if (d == 0) *reinterpret_cast<float2*>(p.part + (size_t)p.total * C::RT * DH + at * 2) = make_float2(mm, ll);
-                continue;
-            }
             const float inv = ll > 0.f || ll != ll ? 1.f / ll : 0.f;
-            const int t = r / p.G, h = hk * p.G + r % p.G;
-            uint8_t* dst = static_cast<uint8_t*>(p.o) + ((long long)b * p.bso + (long long)t * p.ldo + (long long)h * DH + d) * 2;
-            *reinterpret_cast<u32x2*>(dst) = u32x2{M::pack(acc[0] * inv, acc[1] * inv), M::pack(acc[2] * inv, acc[3] * inv)};
+            store4(r, d, acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
         }
     }
 #endif
 }
 
-// the key ranges of each row joined, in the ranges' order: DH / 4 lanes to a row
+// The key ranges of a row joined, in the ranges' order: a workgroup per row. Its first threads hold the ranges' maxima and sums
+// (at most 256), then DH / 4 threads a group take every 4 GR / DH th range.
 template <class E, int DH>
 __global__ __launch_bounds__(256) void k_cross_merge(const CrossParams p, int RT) {
-    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x, n = (size_t)p.B * p.Hkv * p.rows * (DH / 4);
-    if (i >= n) return;
-    const int d = (int)(i % (DH / 4)) * 4;
-    const size_t rr = i / (DH / 4), bh = rr / p.rows;
+    constexpr int GR = 256 / (DH / 4);
+    __shared__ float fac[256], red[8];
+    __shared__ floatx4 acc_s[GR][DH / 4];
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    const size_t rr = blockIdx.x, bh = rr / p.rows;
     const int r = (int)(rr - bh * p.rows), rt = r / RT, rl = r - rt * RT, hk = (int)(bh % p.Hkv), b = (int)(bh / p.Hkv);
+    const int L = p.klen ? max(0, min(p.klen[b], p.Tk)) : p.Tk;
+    const int n = ((L + XKT - 1) / XKT + p.ct - 1) / p.ct;  // the item's ranges
     const float* ml = p.part + (size_t)p.total * RT * DH;
     const size_t at0 = ((bh * p.ksplit) * p.rtiles + rt) * RT + rl, step = (size_t)p.rtiles * RT;
-    float mm = -INFINITY, ll = 0.f;
-    for (int k = 0; k < p.ksplit; k++) mm = fmaxf(mm, ml[(at0 + k * step) * 2]);
-    const float me = mm == -INFINITY ? 0.f : mm;
+    float2 e = make_float2(-INFINITY, 0.f);
+    if (tid < n) e = *reinterpret_cast<const float2*>(ml + (at0 + tid * step) * 2);
+    float mm = e.x;
+#pragma unroll
+    for (int i = 32; i; i >>= 1) mm = fmaxf(mm, __shfl_xor(mm, i, 64));
+    if (lane == 0) red[wv] = mm;
+    __syncthreads();
+    mm = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    const float f = __builtin_amdgcn_exp2f(e.x - (mm == -INFINITY ? 0.f : mm));
+    fac[tid] = f;
+    float ll = f * e.y;
+#pragma unroll
+    for (int i = 32; i; i >>= 1) ll += __shfl_xor(ll, i, 64);
+    if (lane == 0) red[4 + wv] = ll;
+    __syncthreads();
+    ll = (red[4] + red[5]) + (red[6] + red[7]);
+    const int gr = tid / (DH / 4), d = tid % (DH / 4);
     floatx4 acc = {0.f, 0.f, 0.f, 0.f};
-    for (int k = 0; k < p.ksplit; k++) {
-        const float2 e = *reinterpret_cast<const float2*>(ml + (at0 + k * step) * 2);
-        const float f = __builtin_amdgcn_exp2f(e.x - me);
-        ll += f * e.y;
-        acc += f * *reinterpret_cast<const floatx4*>(p.part + (at0 + k * step) * DH + d);
-    }
+#pragma unroll 4
+    for (int k = gr; k < n; k += GR) acc += fac[k] * *reinterpret_cast<const floatx4*>(p.part + (at0 + k * step) * DH + 4 * d);
+    acc_s[gr][d] = acc;
+    __syncthreads();
+    if (tid >= DH / 4) return;
+#pragma unroll
+    for (int i = 1; i < GR; i++) acc += acc_s[i][d];
     const float inv = ll > 0.f || ll != ll ? 1.f / ll : 0.f;
     const int t = r / p.G, h = hk * p.G + r % p.G;
-    uint8_t* dst = static_cast<uint8_t*>(p.o) + ((long long)b * p.bso + (long long)t * p.ldo + (long long)h * DH + d) * 2;
+    uint8_t* dst = static_cast<uint8_t*>(p.o) + ((long long)b * p.bso + (long long)t * p.ldo + (long long)h * DH + 4 * d) * 2;
     *reinterpret_cast<u32x2*>(dst) =
         u32x2{XMma<E>::pack(acc[0] * inv, acc[1] * inv), XMma<E>::pack(acc[2] * inv, acc[3] * inv)};
 }
 
-// The form of a call: rows and key ranges per workgroup.
+// The form of a call. ONE: a wave alone has 16 rows and a range of the keys; FOUR: four waves with the same 16 rows split the
+// keys; S16, S32: four waves of 16 or 32 rows share the keys.
+enum XKind { X_ONE, X_FOUR, X_S16, X_S32 };
 struct XForm {
-    int qb, kw, rt, ksplit;
+    XKind kind;
+    int rt, ksplit, ct;  // rows of a workgroup, key ranges, tiles of a range
 };
-static XForm cross_form(int B, int Tq, int Tk, int Hq, int Hkv, int Dh) {
-    const long rows = (long)Tq * (Hq / Hkv), heads = (long)B * Hkv, cus = cu_count(), tiles = (Tk + XKT - 1) / XKT;
+static XForm cross_form(int B, int Tq, int Tk, int Hq, int Hkv, bool split) {
+    const long rows = (long)Tq * (Hq / Hkv), heads = (long)B * Hkv, cus = cu_count(), tiles = std::max(1, (Tk + XKT - 1) / XKT);
+    const auto ranges = [&](XKind k, int rt, long ct) {
+        ct = std::max(ct, (tiles + 255) / 256);  // the merge takes 256 ranges
+        const long n = split ? (tiles + ct - 1) / ct : 1;
+        return XForm{k, rt, (int)n, (int)(n == 1 ? tiles : ct)};
+    };
     if (rows <= 16) {
-        // one row block: the waves split the keys, and ranges of at least 8 tiles (2 per wave) fill the chip
-        const long ks = std::min<long>({(2 * cus + heads - 1) / heads, tiles / 8, 256});
-        return {1, 4, 16, (int)std::max<long>(1, ks)};
+        if (heads >= 2 * cus) return {X_ONE, 16, 1, (int)tiles};
+        if (tiles <= 32 || !split) return {X_FOUR, 16, 1, (int)tiles};
+        return ranges(X_ONE, 16, std::max<long>(4, tiles * heads / (4 * cus)));
     }
-    const int qb = rows * heads >= 128 * cus ? 2 : 1, rt = 64 * qb;
-    const long units = (rows + rt - 1) / rt * heads;
-    const long ks = units >= cus ? 1 : std::min<long>({2 * cus / units, tiles / 8, 256});
-    return {qb, 1, rt, (int)std::max<long>(1, ks)};
+    const long u32 = (rows + 127) / 128 * heads, u16 = (rows + 63) / 64 * heads;
+    if (u32 >= cus) return {X_S32, 128, 1, (int)tiles};
+    if (u16 >= cus || tiles < 16) return {X_S16, 64, 1, (int)tiles};
+    return ranges(X_S16, 64, std::max<long>(8, tiles * u16 / (2 * cus)));
 }
 size_t cross_attn_workspace(int B, int Tq, int Tk, int Hq, int Hkv, int Dh) {
-    const XForm f = cross_form(B, Tq, Tk, Hq, Hkv, Dh);
+    const XForm f = cross_form(B, Tq, Tk, Hq, Hkv, true);
     if (f.ksplit == 1) return 0;
     const size_t rtiles = ((size_t)Tq * (Hq / Hkv) + f.rt - 1) / f.rt;
     return (size_t)B * Hkv * f.ksplit * rtiles * f.rt * (Dh + 2) * sizeof(float);
 }
 
-template <class E, int DH, int QB, int KW>
+template <class E, class C>
 static hipError_t cross_launch(CrossParams p, hipStream_t s) {
-    using C = XCfg<E, DH, QB, KW>;
     p.rtiles = (p.rows + C::RT - 1) / C::RT;
     p.total = p.B * p.Hkv * p.ksplit * p.rtiles;
     p.per = (p.total + 7) / 8;
-    hipLaunchKernelGGL((k_cross_attn<E, DH, QB, KW>), dim3(p.per * 8), dim3(256), C::LDS, s, p);
+    auto kern = p.kmask ? k_cross_attn<E, C, true> : k_cross_attn<E, C, false>;
+    hipLaunchKernelGGL(kern, dim3(p.per * 8), dim3(C::THREADS), C::LDS, s, p);
     if (hipError_t e = hipGetLastError()) return e;
     if (p.ksplit == 1) return hipSuccess;
-    const size_t n = (size_t)p.B * p.Hkv * p.rows * (DH / 4);
-    hipLaunchKernelGGL((k_cross_merge<E, DH>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, p, C::RT);
+    hipLaunchKernelGGL((k_cross_merge<E, C::DH>), dim3((unsigned)((size_t)p.B * p.Hkv * p.rows)), dim3(256), 0, s, p, C::RT);
     return hipGetLastError();
 }
 template <class E, int DH>
-static hipError_t cross_of(const CrossParams& p, const XForm& f, hipStream_t s) {
-    if (f.kw == 4) return cross_launch<E, DH, 1, 4>(p, s);
-    if (f.qb == 1) return cross_launch<E, DH, 1, 1>(p, s);
-    return cross_launch<E, DH, 2, 1>(p, s);
+static hipError_t cross_of(const CrossParams& p, XKind k, hipStream_t s) {
+    switch (k) {
+        case X_ONE: return cross_launch<E, XCfg<DH, 1, 1, false, 3>>(p, s);
+        case X_FOUR: return cross_launch<E, XCfg<DH, 1, 4, false, 2>>(p, s);
+        case X_S16: return cross_launch<E, XCfg<DH, 1, 4, true, 4>>(p, s);
+        default: return cross_launch<E, XCfg<DH, 2, 4, true, 4>>(p, s);
+    }
 }
 
 hipError_t launch_cross_attn(const CrossLaunch& c, hipStream_t s) {
-    XForm f = cross_form(c.B, c.Tq, c.Tk, c.Hq, c.Hkv, c.Dh);
-    if (c.ws_bytes < cross_attn_workspace(c.B, c.Tq, c.Tk, c.Hq, c.Hkv, c.Dh) || !c.ws) f.ksplit = 1;
+    const bool split = c.ws && c.ws_bytes >= cross_attn_workspace(c.B, c.Tq, c.Tk, c.Hq, c.Hkv, c.Dh);
+    const XForm f = cross_form(c.B, c.Tq, c.Tk, c.Hq, c.Hkv, split);
     CrossParams p{};
     p.q = c.q;
     p.k = c.k;
@@ -447,9 +483,10 @@ hipError_t launch_cross_attn(const CrossLaunch& c, hipStream_t s) {
     p.sc = c.scale * LOG2E;
     p.rows = c.Tq * p.G;
     p.ksplit = f.ksplit;
+    p.ct = f.ct;
     p.part = static_cast<float*>(c.ws);
-    if (c.dt == DT::F16) return c.Dh == 64 ? cross_of<_Float16, 64>(p, f, s) : cross_of<_Float16, 128>(p, f, s);
-    return c.Dh == 64 ? cross_of<__bf16, 64>(p, f, s) : cross_of<__bf16, 128>(p, f, s);
+    if (c.dt == DT::F16) return c.Dh == 64 ? cross_of<_Float16, 64>(p, f.kind, s) : cross_of<_Float16, 128>(p, f.kind, s);
+    return c.Dh == 64 ? cross_of<__bf16, 64>(p, f.kind, s) : cross_of<__bf16, 128>(p, f.kind, s);
 }
 
 }  // namespace kiln
