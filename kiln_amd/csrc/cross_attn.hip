@@ -7,8 +7,8 @@
 // S^T accumulators holds eight of a 32-key tile's keys for one row, which is the B operand of the second product as it
 // is, if V's keys come in the same order: two transposing LDS reads per 16 dimensions.
 //
-// Keys come in tiles of 32: K and V rows go to LDS by buffer DMA, 16 bytes a lane, and the 16-byte chunks of a row lie
-// permuted (k_swz, v_swz) so that both kinds of read spread over the banks; the permutation is on the global side. Rows past
+// Keys come in tiles of 32: K and V rows go to LDS by buffer DMA, 16 bytes a lane, the chunks of a row permuted (k_swz, v_swz) so
+// that both kinds of operand read lie in all banks. Rows past
 // the length or masked out lie outside the descriptor's range and arrive as zeros, whatever they hold: their scores are set
 // to -inf by the tile's bit mask, and 0 times an infinity or a NaN never happens.
 //
@@ -79,7 +79,8 @@ __device__ __forceinline__ void x_wait_vmcnt() {
     __builtin_amdgcn_s_waitcnt((N & 0xF) | (0x7 << 4) | (0xF << 8) | ((N >> 4) << 14));
 }
 // Position of 16-byte chunk c of key row r in its LDS row. K is read 16 keys x one chunk at a time, V eight keys x a pair of
-// chunks: either way 256 bytes that lie in all 64 banks, for rows of 256 bytes (Dh 128) and of 128.
+// chunks: either way 256 bytes that lie in all 64 banks, for rows of 256 bytes (Dh 128) and of 128. The permutation is on the
+// side of the copies' sources, where it costs nothing (rows in order and padded blocks instead: the same time, more conflicts).
 template <int DH>
 __device__ __forceinline__ int k_swz(int c, int r) {
     return DH == 128 ? c ^ (r & 15) : c ^ ((r >> 1) & 7);
@@ -104,7 +105,7 @@ struct XCfg {
     static constexpr int BITS = NW * 32 * 4;                           // each wave's mask windows: 2 x 16 words
     static constexpr int MERGE = !SHARED && NW > 1 ? NW * RW * (DH + 2) * 4 : 0;
     static constexpr int LDS = (RINGS > MERGE ? RINGS : MERGE) + BITS;
-    static constexpr int WAVES = LDS <= 40 * 1024 ? 4 : LDS <= 80 * 1024 || NW == 1 ? 2 : 1;  // per SIMD that registers have to allow
+    static constexpr int WAVES = QB == 1 && LDS <= 40 * 1024 ? 4 : LDS <= 80 * 1024 || NW == 1 || NW == 8 ? 2 : 1;  // per SIMD that registers have to allow
 };
 
 template <class E, class C, bool MASK>
@@ -116,6 +117,7 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_cross_attn(const Cross
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, c16 = lane & 15;
     // blocks go round the 8 XCDs: each takes a contiguous range of items, so that the row tiles of a key head share its L2
+    // (the key heads of a row tile side by side instead: B = 2, 4096 x 4096, 16 heads of 128 295 -> 314 us)
     const int item = (int)(blockIdx.x & 7) * p.per + (int)(blockIdx.x >> 3);
     if (item >= p.total) return;
     const int rt = item % p.rtiles, ks = item / p.rtiles % p.ksplit, bh = item / p.rtiles / p.ksplit;
@@ -148,48 +150,48 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_cross_attn(const Cross
         return left >= XKT ? ~0u : (1u << left) - 1u;
     };
 
-    // DMA of the tiles in turn: a thread's pieces are chunks of fixed rows of a tile; the descriptor's range ends with the
-    // item's last row (empty past the last tile), and a masked row's offset is beyond every range
-    const int tr = C::SHARED ? (int)threadIdx.x : lane;
-    const uint32_t ldk2 = (uint32_t)p.ldk * 2, ldv2 = (uint32_t)p.ldv * 2;
-    const uint8_t* kp = static_cast<const uint8_t*>(p.k) + ((long long)b * p.bsk + (long long)hk * DH) * 2 + (long long)t0 * XKT * ldk2;
-    const uint8_t* vp = static_cast<const uint8_t*>(p.v) + ((long long)b * p.bsv + (long long)hk * DH) * 2 + (long long)t0 * XKT * ldv2;
-    int dma_j = t0, into = 0;  // the next tile to copy, its stage
-    uint32_t ko[C::DMA], vo[C::DMA];
+    // DMA of the tiles' K and V in turn: a thread's pieces are chunks of fixed rows of a tile; the descriptor's range ends with
+    // the item's last row (empty past the last tile), and a masked row's offset is beyond every range
+    struct Stream {
+        const uint8_t* src;     // the next tile to copy
+        uint32_t ld2;           // bytes from row to row
+        int j;                  // its index
+        uint32_t off[C::DMA];
+    } kst, vst;
+    kst.ld2 = (uint32_t)p.ldk * 2;
+    vst.ld2 = (uint32_t)p.ldv * 2;
+    kst.src = static_cast<const uint8_t*>(p.k) + ((long long)b * p.bsk + (long long)hk * DH) * 2 + (long long)t0 * XKT * kst.ld2;
+    vst.src = static_cast<const uint8_t*>(p.v) + ((long long)b * p.bsv + (long long)hk * DH) * 2 + (long long)t0 * XKT * vst.ld2;
+    kst.j = vst.j = t0;
     int prow[C::DMA];
 #pragma unroll
     for (int i = 0; i < C::DMA; i++) {
-        const int pc = i * C::RTHREADS + tr, r = pc / C::PC, c = pc % C::PC;
+        const int pc = i * C::RTHREADS + (C::SHARED ? (int)threadIdx.x : lane), r = pc / C::PC, c = pc % C::PC;
         prow[i] = r;
-        ko[i] = r * ldk2 + k_swz<DH>(c, r) * 16;
-        vo[i] = r * ldv2 + v_swz<DH>(c, r) * 16;
+        kst.off[i] = r * kst.ld2 + k_swz<DH>(c, r) * 16;
+        vst.off[i] = r * vst.ld2 + v_swz<DH>(c, r) * 16;
     }
-    auto dma = [&]() {
+    auto copy = [&](Stream& t, uint32_t at, bool first) {  // first: the stream that comes to a tile first, and reads its mask
         uint32_t m = ~0u;
-        const int left = dma_j < t1 ? min(XKT, L - dma_j * XKT) : 0;
+        const int left = t.j < t1 ? min(XKT, L - t.j * XKT) : 0;
         if constexpr (MASK) {
             if (left > 0) {
-                if (((dma_j - t0) & 15) == 0) fill_window((dma_j - t0) >> 4);
-                m = tile_bits(dma_j);
+                if (first && ((t.j - t0) & 15) == 0) fill_window((t.j - t0) >> 4);
+                m = tile_bits(t.j);
             }
         }
-        const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
-            const_cast<uint8_t*>(kp), (short)0, left > 0 ? (int)((left - 1) * ldk2 + DH * 2) : 0, 0x00020000 /* raw */);
-        const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
-            const_cast<uint8_t*>(vp), (short)0, left > 0 ? (int)((left - 1) * ldv2 + DH * 2) : 0, 0x00020000);
-        uint8_t* dst = ring + into * C::STAGE + (C::SHARED ? wv * 1024 : 0);
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<uint8_t*>(t.src), (short)0, left > 0 ? (int)((left - 1) * t.ld2 + DH * 2) : 0, 0x00020000 /* raw */);
+        uint8_t* dst = ring + at + (C::SHARED ? wv * 1024 : 0);
 #pragma unroll
         for (int i = 0; i < C::DMA; i++)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_ptr)(dst + i * C::RTHREADS * 16), 16,
-                                                     !MASK || (m >> prow[i] & 1) ? ko[i] : 0x7ffffff0u, 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < C::DMA; i++)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_ptr)(dst + C::TILE + i * C::RTHREADS * 16), 16,
-                                                     !MASK || (m >> prow[i] & 1) ? vo[i] : 0x7ffffff0u, 0, 0, 0);
-        if (dma_j + 1 < t1) kp += (size_t)XKT * ldk2, vp += (size_t)XKT * ldv2;
-        dma_j++;
-        into = into == C::NS - 1 ? 0 : into + 1;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(dst + i * C::RTHREADS * 16), 16,
+                                                     !MASK || (m >> prow[i] & 1) ? t.off[i] : 0x7ffffff0u, 0, 0, 0);
+        if (t.j + 1 < t1) t.src += (size_t)XKT * t.ld2;
+        t.j++;
     };
+    auto copy_k = [&](int stage) { copy(kst, stage * C::STAGE, true); };
+    auto copy_v = [&](int stage) { copy(vst, stage * C::STAGE + C::TILE, false); };
 
     // Q: the B operands of S^T, lane (row c16, chunk 4 cc + g); rows past the last read row 0 and are not stored
     const int row0 = rt * C::RT + (C::SHARED ? wv * C::RW : 0);
@@ -214,7 +216,7 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_cross_attn(const Cross
     }
     const uint32_t one2 = M::pack(1.f, 1.f);
     const u32x4 ones = {one2, one2, one2, one2};
-    // operand addresses within a stage: the chunk's permutation depends on the row's low bits only, the same for rows 16 apart
+    // operand addresses within a stage; the chunks' permutation is the same for rows 16 apart
     uint32_t kaddr[DH / 32], vaddr[DH / 16];
 #pragma unroll
     for (int cc = 0; cc < DH / 32; cc++) kaddr[cc] = lds_base + c16 * DH * 2 + k_swz<DH>(4 * cc + g, c16) * 16;
@@ -224,77 +226,178 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_cross_attn(const Cross
     for (int db = 0; db < DH / 16; db++)
         vaddr[db] = lds_base + C::TILE + vr * DH * 2 + v_swz<DH>(2 * db + ((c16 & 3) >> 1), vr) * 16 + (c16 & 1) * 8;
 
-#pragma unroll
-    for (int s = 0; s < C::NS - 1; s++) dma();
-    uint32_t st = 0;  // the stage's offset
-    for (int j = t0; j < t1; j++) {
-        // tile j landed (past the last tile the copies go on with empty ranges, which keeps the count); every wave that
-        // shares the ring is done with tile j - 1, whose stage is refilled
-        x_wait_vmcnt<(C::NS - 2) * 2 * C::DMA>();
-        __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
-        if constexpr (C::SHARED) __builtin_amdgcn_s_barrier();
-        __builtin_amdgcn_sched_barrier(0);
-        dma();
-        floatx4 s[2][QB];
+    // pieces of a tile's work
+    auto read_k = [&](uint32_t st, u32x4 (&kf)[2][DH / 32]) {
 #pragma unroll
         for (int kk = 0; kk < 2; kk++)
 #pragma unroll
-            for (int cc = 0; cc < DH / 32; cc++) {
-                const u32x4 kf = *reinterpret_cast<const lds_x4*>((size_t)(kaddr[cc] + st + kk * 16 * DH * 2));
+            for (int cc = 0; cc < DH / 32; cc++)
+                kf[kk][cc] = *reinterpret_cast<const lds_x4*>((size_t)(kaddr[cc] + st + kk * 16 * DH * 2));
+    };
+    auto read_v = [&](uint32_t st, int db) {
+        const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v*)(size_t)(vaddr[db] + st)));
+        const u32x2 d = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v*)(size_t)(vaddr[db] + st + 16 * DH * 2)));
+        return u32x4{a[0], a[1], d[0], d[1]};
+    };
+    auto scores = [&](const u32x4 (&kf)[2][DH / 32], floatx4 (&s)[2][QB]) {
 #pragma unroll
-                for (int qb = 0; qb < QB; qb++)
-                    s[kk][qb] = M::mul(kf, qf[qb][cc], cc == 0 ? floatx4{0.f, 0.f, 0.f, 0.f} : s[kk][qb]);
-            }
-        const uint32_t bt = tile_bits(j);
-        if (bt != ~0u) {
+        for (int cc = 0; cc < DH / 32; cc++)
 #pragma unroll
             for (int kk = 0; kk < 2; kk++)
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    if (!(bt >> (16 * kk + 4 * g + i) & 1))
+                for (int qb = 0; qb < QB; qb++)
+                    s[kk][qb] = M::mul(kf[kk][cc], qf[qb][cc], cc == 0 ? floatx4{0.f, 0.f, 0.f, 0.f} : s[kk][qb]);
+    };
+    auto hide = [&](int j, floatx4 (&s)[2][QB]) {
+        const uint32_t bt = tile_bits(j);
+        if (bt == ~0u) return;
 #pragma unroll
-                        for (int qb = 0; qb < QB; qb++) s[kk][qb][i] = -INFINITY;
-        }
-        float top[QB];
-        bool moves = false;
+        for (int kk = 0; kk < 2; kk++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (!(bt >> (16 * kk + 4 * g + i) & 1))
+#pragma unroll
+                    for (int qb = 0; qb < QB; qb++) s[kk][qb][i] = -INFINITY;
+    };
+    auto largest = [&](const floatx4 (&s)[2][QB], float (&top)[QB]) {
 #pragma unroll
         for (int qb = 0; qb < QB; qb++) {
             float t = fmaxf(s[0][qb][0], s[1][qb][0]);
 #pragma unroll
             for (int i = 1; i < 4; i++) t = fmaxf(fmaxf(t, s[0][qb][i]), s[1][qb][i]);
             top[qb] = t * p.sc;
-            moves |= top[qb] > m[qb] + XRESCALE;  // from -inf: any score that is not
         }
-        if (__any(moves)) {
+    };
+    auto rescale = [&](const float (&top)[QB]) {
+        bool moves = false;
 #pragma unroll
-            for (int qb = 0; qb < QB; qb++) {
-                const float t = fmaxf(m[qb], quad_max(top[qb]));
-                const float f = t > m[qb] ? __builtin_amdgcn_exp2f(m[qb] - t) : 1.f;
-                m[qb] = t;
-                mn[qb] = t == -INFINITY ? 0.f : -t;
-                l[qb] *= f;
+        for (int qb = 0; qb < QB; qb++) moves |= top[qb] > m[qb] + XRESCALE;  // from -inf: any score that is not
+        if (!__any(moves)) return;
 #pragma unroll
-                for (int db = 0; db < DH / 16; db++) o[db][qb] *= f;
-            }
+        for (int qb = 0; qb < QB; qb++) {
+            const float t = fmaxf(m[qb], quad_max(top[qb]));
+            const float f = t > m[qb] ? __builtin_amdgcn_exp2f(m[qb] - t) : 1.f;
+            m[qb] = t;
+            mn[qb] = t == -INFINITY ? 0.f : -t;
+            l[qb] *= f;
+#pragma unroll
+            for (int db = 0; db < DH / 16; db++) o[db][qb] *= f;
         }
-        u32x4 pf[QB];
+    };
+    auto weights = [&](const floatx4 (&s)[2][QB], u32x4 (&pf)[QB]) {
 #pragma unroll
         for (int qb = 0; qb < QB; qb++)
 #pragma unroll
             for (int i = 0; i < 4; i++)
                 pf[qb][i] = M::pack(__builtin_amdgcn_exp2f(fmaf(s[i / 2][qb][2 * i % 4], p.sc, mn[qb])),
                                     __builtin_amdgcn_exp2f(fmaf(s[i / 2][qb][2 * i % 4 + 1], p.sc, mn[qb])));
+    };
+
+    if constexpr (C::SHARED) {
+        // The scores of tile j + 1 are computed between the exponentials of tile j, and its maxima between tile j's products
+        // with V, so that matrix and vector work overlap within a wave. K of tile j + 1 and V of tile j landed (past the last
+        // tile the copies go on with empty ranges, which keeps the count); every wave is done with K of tile j and V of tile
+        // j - 1, whose places take K of tile j + NS and V of tile j + NS - 1. Stages are constants: the reads' offsets too.
+        constexpr int NS = C::NS;
+        static_assert(NS % 2 == 0, "the scores' two sets go with the stages");
+        floatx4 s[2][2][QB];
+        float top[QB];
+        u32x4 kf[2][DH / 32], vf[DH / 16], pf[QB];
+        copy_k(0);
 #pragma unroll
-        for (int qb = 0; qb < QB; qb++) l[qb] = M::mul(ones, pf[qb], l[qb]);
-#pragma unroll
-        for (int db = 0; db < DH / 16; db++) {
-            const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v*)(size_t)(vaddr[db] + st)));
-            const u32x2 d = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v*)(size_t)(vaddr[db] + st + 16 * DH * 2)));
-            const u32x4 vf = {a[0], a[1], d[0], d[1]};
-#pragma unroll
-            for (int qb = 0; qb < QB; qb++) o[db][qb] = M::mul(vf, pf[qb], o[db][qb]);
+        for (int i = 1; i < NS; i++) {
+            copy_k(i);
+            copy_v(i - 1);
         }
-        st = st == (C::NS - 1) * C::STAGE ? 0 : st + C::STAGE;
+        x_wait_vmcnt<2 * (NS - 1) * C::DMA>();
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        if (t0 < t1) {
+            read_k(0, kf);
+            scores(kf, s[0]);
+            hide(t0, s[0]);
+            largest(s[0], top);
+        }
+        auto step = [&](int j, auto parity, auto st) {  // st: the stage of tile j, a constant or not
+            constexpr int cur = decltype(parity)::value;
+            x_wait_vmcnt<2 * (NS - 2) * C::DMA>();
+            __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+            copy_k(st);
+            copy_v((st + NS - 1) % NS);
+            read_k((st + 1) % NS * C::STAGE, kf);
+#pragma unroll
+            for (int db = 0; db < DH / 16; db++) vf[db] = read_v(st * C::STAGE, db);
+            rescale(top);
+            __builtin_amdgcn_sched_barrier(0);
+            weights(s[cur], pf);
+            scores(kf, s[cur ^ 1]);
+            __builtin_amdgcn_sched_barrier(0);
+            if (j + 1 < t1) hide(j + 1, s[cur ^ 1]);
+#pragma unroll
+            for (int qb = 0; qb < QB; qb++) l[qb] = M::mul(ones, pf[qb], l[qb]);
+#pragma unroll
+            for (int db = 0; db < DH / 16; db++)
+#pragma unroll
+                for (int qb = 0; qb < QB; qb++) o[db][qb] = M::mul(vf[db], pf[qb], o[db][qb]);
+            largest(s[cur ^ 1], top);
+        };
+        using P0 = std::integral_constant<int, 0>;
+        using P1 = std::integral_constant<int, 1>;
+        if constexpr (QB == 1) {  // the compiler spills 16-row waves' registers in the loop of four
+            for (int j = t0, st = 0; j < t1; j += 2, st = (st + 2) % NS) {
+                step(j, P0{}, st);
+                if (j + 1 >= t1) break;
+                step(j + 1, P1{}, st + 1);
+            }
+        } else {
+            static_assert(NS == 4, "the loop names its stages");
+            for (int j = t0; j < t1; j += 4) {
+                step(j, P0{}, P0{});
+                if (j + 1 >= t1) break;
+                step(j + 1, P1{}, P1{});
+                if (j + 2 >= t1) break;
+                step(j + 2, P0{}, std::integral_constant<int, 2>{});
+                if (j + 3 >= t1) break;
+                step(j + 3, P1{}, std::integral_constant<int, 3>{});
+            }
+        }
+    } else {
+        int stage = 0;
+        auto next = [](int i) { return i == C::NS - 1 ? 0 : i + 1; };
+#pragma unroll
+        for (int i = 0; i < C::NS - 1; i++) {
+            copy_k(i);
+            copy_v(i);
+        }
+        for (int j = t0; j < t1; j++) {
+            x_wait_vmcnt<(C::NS - 2) * 2 * C::DMA>();
+            __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): this wave is done with tile j - 1, whose stage is refilled
+            __builtin_amdgcn_sched_barrier(0);
+            const int into = stage == 0 ? C::NS - 1 : stage - 1;
+            copy_k(into);
+            copy_v(into);
+            const uint32_t st = stage * C::STAGE;
+            floatx4 s[2][QB];
+            float top[QB];
+            u32x4 kf[2][DH / 32], pf[QB];
+            read_k(st, kf);
+            scores(kf, s);
+            hide(j, s);
+            largest(s, top);
+            rescale(top);
+            weights(s, pf);
+#pragma unroll
+            for (int qb = 0; qb < QB; qb++) l[qb] = M::mul(ones, pf[qb], l[qb]);
+#pragma unroll
+            for (int db = 0; db < DH / 16; db++) {
+                const u32x4 vf = read_v(st, db);
+#pragma unroll
+                for (int qb = 0; qb < QB; qb++) o[db][qb] = M::mul(vf, pf[qb], o[db][qb]);
+            }
+            stage = next(stage);
+        }
     }
     x_wait_vmcnt<0>();  // no copy into LDS outlives its ring
 
@@ -304,21 +407,41 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_cross_attn(const Cross
         *reinterpret_cast<u32x2*>(dst) = u32x2{M::pack(a0, a1), M::pack(a2, a3)};
     };
     if constexpr (C::SHARED || C::NW == 1) {
+        if (p.ksplit > 1) {
 #pragma unroll
-        for (int qb = 0; qb < QB; qb++) {
-            const int r = row0 + 16 * qb + c16;
-            if (r >= p.rows) continue;
-            if (p.ksplit > 1) {
+            for (int qb = 0; qb < QB; qb++) {
+                const int r = row0 + 16 * qb + c16;
+                if (r >= p.rows) continue;
                 const size_t at = (size_t)item * C::RT + (r - rt * C::RT);
 #pragma unroll
                 for (int db = 0; db < DH / 16; db++) *reinterpret_cast<floatx4*>(p.part + at * DH + 16 * db + 4 * g) = o[db][qb];
                 if (g == 0) *reinterpret_cast<float2*>(p.part + (size_t)p.total * C::RT * DH + at * 2) = make_float2(m[qb], l[qb][0]);
-                continue;
             }
+            return;
+        }
+        // rows leave through LDS, whole and 16 bytes a lane (8-byte pieces of 16 rows per store: 10 of 57 us in the same case);
+        // a row's chunks lie permuted by its number
+        static_assert(C::RW * DH * 2 * C::NW <= C::RINGS, "the waves' rows fit in the rings");
+        uint8_t* stg = xlds + wv * C::RW * DH * 2;
+        if constexpr (C::SHARED) __builtin_amdgcn_s_barrier();  // every wave is done with the ring, and its copies landed
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int qb = 0; qb < QB; qb++) {
+            const int r = 16 * qb + c16;
             const float inv = l[qb][0] > 0.f || l[qb][0] != l[qb][0] ? 1.f / l[qb][0] : 0.f;  // no key: zeros
 #pragma unroll
             for (int db = 0; db < DH / 16; db++)
-                store4(r, 16 * db + 4 * g, o[db][qb][0] * inv, o[db][qb][1] * inv, o[db][qb][2] * inv, o[db][qb][3] * inv);
+                *reinterpret_cast<u32x2*>(stg + r * DH * 2 + ((2 * db + (g >> 1)) ^ (r & (C::PC - 1))) * 16 + (g & 1) * 8) =
+                    u32x2{M::pack(o[db][qb][0] * inv, o[db][qb][1] * inv), M::pack(o[db][qb][2] * inv, o[db][qb][3] * inv)};
+        }
+        __builtin_amdgcn_wave_barrier();  // a wave's LDS operations keep their order
+#pragma unroll
+        for (int i = 0; i < C::RW * C::PC / 64; i++) {
+            const int rl = (i * 64 + lane) / C::PC, c = lane % C::PC, r = row0 + rl;
+            const u32x4 v = *reinterpret_cast<const u32x4*>(stg + rl * DH * 2 + (c ^ (rl & (C::PC - 1))) * 16);
+            if (r >= p.rows) continue;
+            const int t = r / p.G, h = hk * p.G + r % p.G;
+            *reinterpret_cast<u32x4*>(static_cast<uint8_t*>(p.o) + ((long long)b * p.bso + (long long)t * p.ldo + (long long)h * DH + c * 8) * 2) = v;
         }
     } else {
         // the waves' results of the same 16 QB rows
@@ -404,13 +527,13 @@ __global__ __launch_bounds__(256) void k_cross_merge(const CrossParams p, int RT
 }
 
 // The form of a call. ONE: a wave alone has 16 rows and a range of the keys; FOUR: four waves with the same 16 rows split the
-// keys; S16, S32: four waves of 16 or 32 rows share the keys.
-enum XKind { X_ONE, X_FOUR, X_S16, X_S32 };
+// keys; S16, S32, S64: four waves of 16, 32 or 64 rows share the keys.
+enum XKind { X_ONE, X_FOUR, X_S16, X_S32, X_S64 };
 struct XForm {
     XKind kind;
     int rt, ksplit, ct;  // rows of a workgroup, key ranges, tiles of a range
 };
-static XForm cross_form(int B, int Tq, int Tk, int Hq, int Hkv, bool split) {
+static XForm cross_form(int B, int Tq, int Tk, int Hq, int Hkv, int Dh, bool split) {
     const long rows = (long)Tq * (Hq / Hkv), heads = (long)B * Hkv, cus = cu_count(), tiles = std::max(1, (Tk + XKT - 1) / XKT);
     const auto ranges = [&](XKind k, int rt, long ct) {
         ct = std::max(ct, (tiles + 255) / 256);  // the merge takes 256 ranges
@@ -423,12 +546,13 @@ static XForm cross_form(int B, int Tq, int Tk, int Hq, int Hkv, bool split) {
         return ranges(X_ONE, 16, std::max<long>(4, tiles * heads / (4 * cus)));
     }
     const long u32 = (rows + 127) / 128 * heads, u16 = (rows + 63) / 64 * heads;
+    if (Dh == 64 && tiles >= 8 && (rows + 255) / 256 * heads >= cus) return {X_S64, 256, 1, (int)tiles};
     if (u32 >= cus) return {X_S32, 128, 1, (int)tiles};
     if (u16 >= cus || tiles < 16) return {X_S16, 64, 1, (int)tiles};
     return ranges(X_S16, 64, std::max<long>(8, tiles * u16 / (2 * cus)));
 }
 size_t cross_attn_workspace(int B, int Tq, int Tk, int Hq, int Hkv, int Dh) {
-    const XForm f = cross_form(B, Tq, Tk, Hq, Hkv, true);
+    const XForm f = cross_form(B, Tq, Tk, Hq, Hkv, Dh, true);
     if (f.ksplit == 1) return 0;
     const size_t rtiles = ((size_t)Tq * (Hq / Hkv) + f.rt - 1) / f.rt;
     return (size_t)B * Hkv * f.ksplit * rtiles * f.rt * (Dh + 2) * sizeof(float);
@@ -452,13 +576,14 @@ static hipError_t cross_of(const CrossParams& p, XKind k, hipStream_t s) {
         case X_ONE: return cross_launch<E, XCfg<DH, 1, 1, false, 3>>(p, s);
         case X_FOUR: return cross_launch<E, XCfg<DH, 1, 4, false, 2>>(p, s);
         case X_S16: return cross_launch<E, XCfg<DH, 1, 4, true, 4>>(p, s);
-        default: return cross_launch<E, XCfg<DH, 2, 4, true, 4>>(p, s);
+        case X_S32: return cross_launch<E, XCfg<DH, 2, 4, true, 4>>(p, s);
+        default: return cross_launch<E, XCfg<64, 4, 4, true, 4>>(p, s);
     }
 }
 
 hipError_t launch_cross_attn(const CrossLaunch& c, hipStream_t s) {
     const bool split = c.ws && c.ws_bytes >= cross_attn_workspace(c.B, c.Tq, c.Tk, c.Hq, c.Hkv, c.Dh);
-    const XForm f = cross_form(c.B, c.Tq, c.Tk, c.Hq, c.Hkv, split);
+    const XForm f = cross_form(c.B, c.Tq, c.Tk, c.Hq, c.Hkv, c.Dh, split);
     CrossParams p{};
     p.q = c.q;
     p.k = c.k;
