@@ -541,13 +541,20 @@ static XForm cross_form(int B, int Tq, int Tk, int Hq, int Hkv, int Dh, bool spl
         return XForm{k, rt, (int)n, (int)(n == 1 ? tiles : ct)};
     };
     if (rows <= 16) {
+        // One row block, bound by the keys' bytes: single waves of 32 KB of LDS, five a CU, with ranges that fill the chip three
+        // times over (a shorter item's ranges past its length end at once), at least 4 tiles each. Few keys in four waves of
+        // one workgroup need no merge. In us, four waves / ranges: 1 x 3000, 20 heads of 128 24.8 / 11.6; 1 x 2048, 16 of 64
+        // 10.4 / 10.3; 4 x 512, 16 of 128 8.4 / 10.6; 64 x 100, 16 of 128 (1024 heads) 21.5 / 11.5 in one range.
         if (heads >= 2 * cus) return {X_ONE, 16, 1, (int)tiles};
-        if (tiles <= 32 || !split) return {X_FOUR, 16, 1, (int)tiles};
-        return ranges(X_ONE, 16, std::max<long>(4, tiles * heads / (4 * cus)));
+        if (!split || (tiles <= 32 && heads <= cus)) return {X_FOUR, 16, 1, (int)tiles};
+        return ranges(X_ONE, 16, std::max<long>(4, (tiles * heads + 3 * cus - 1) / (3 * cus)));
     }
-    const long u32 = (rows + 127) / 128 * heads, u16 = (rows + 63) / 64 * heads;
-    if (Dh == 64 && tiles >= 8 && (rows + 255) / 256 * heads >= cus) return {X_S64, 256, 1, (int)tiles};
-    if (u32 >= cus) return {X_S32, 128, 1, (int)tiles};
+    // More rows per wave read LDS less often per product, but two workgroups per CU have to come of them. In us, 16 / 32 / 64 rows:
+    // 2 x 4096 x 512, 10 heads of 64 26.7 / 23.1 / 27.7, 16 heads - / 32.1 / 29.9; 2 x 4096 x 77, 16 of 128 28.7 / 23.9;
+    // 1 x 2048 x 2048, 16 of 128 (256 workgroups of 128 rows) 54.1 / 58.2; 2 x 1024 x 77, 20 of 64 8.4 / 10.2.
+    const long u64 = (rows + 255) / 256 * heads, u32 = (rows + 127) / 128 * heads, u16 = (rows + 63) / 64 * heads;
+    if (Dh == 64 && tiles >= 8 && u64 >= 2 * cus) return {X_S64, 256, 1, (int)tiles};
+    if (u32 >= 2 * cus) return {X_S32, 128, 1, (int)tiles};
     if (u16 >= cus || tiles < 16) return {X_S16, 64, 1, (int)tiles};
     return ranges(X_S16, 64, std::max<long>(8, tiles * u16 / (2 * cus)));
 }
@@ -573,7 +580,7 @@ static hipError_t cross_launch(CrossParams p, hipStream_t s) {
 template <class E, int DH>
 static hipError_t cross_of(const CrossParams& p, XKind k, hipStream_t s) {
     switch (k) {
-        case X_ONE: return cross_launch<E, XCfg<DH, 1, 1, false, 3>>(p, s);
+        case X_ONE: return cross_launch<E, XCfg<DH, 1, 1, false, 2>>(p, s);
         case X_FOUR: return cross_launch<E, XCfg<DH, 1, 4, false, 2>>(p, s);
         case X_S16: return cross_launch<E, XCfg<DH, 1, 4, true, 4>>(p, s);
         case X_S32: return cross_launch<E, XCfg<DH, 2, 4, true, 4>>(p, s);
