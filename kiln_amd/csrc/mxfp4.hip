@@ -2,6 +2,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "mxfp4.hpp"
 
@@ -12,44 +13,64 @@ __device__ __forceinline__ uint32_t quad_umax(uint32_t v) {  // over the four la
     return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, false));
 }
 
+// Eight neighbours are a unit: n = rows * cols / 8 of them, row by row. The place of unit i in rows of stride ld: dense rows need no
+// row number, others a 32-bit division (64-bit ones took a third of the kernels' time)
+template <bool DENSE>
+__device__ __forceinline__ size_t mx_place(size_t i, size_t n, uint32_t per_row, size_t ld) {
+    if constexpr (DENSE) return i * 8;
+    const size_t r = n >> 32 ? i / per_row : (uint32_t)i / per_row;
+    return r * ld + (i - r * per_row) * 8;
+}
+
 // x [rows, cols] to codes [rows, cols / 2] (even column in the low half) and scales [rows, cols / 32]. Four lanes take a
 // block of 32, eight values each: loads of 16 or 32 contiguous bytes per lane, 4-byte stores of codes.
-template <class E, bool VEC>
-__global__ __launch_bounds__(256) void k_mx_quantize(uint8_t* codes, uint8_t* scales, const E* x, size_t ldx, int rows, int cols) {
-    const size_t n = (size_t)rows * (cols / 8);
+template <class E, bool VEC, bool DENSE>
+__global__ __launch_bounds__(256) void k_mx_quantize(uint8_t* codes, uint8_t* scales, const E* x, size_t ldx, size_t n, uint32_t per_row) {
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
-        const size_t r = i / (cols / 8);
-        const int c = (int)(i - r * (cols / 8)) * 8;
+        const E* src = x + mx_place<DENSE>(i, n, per_row, ldx);
         MxVals<E, 8> v;
-        if constexpr (VEC) v.load(x + r * ldx + c);
-        else v.load_any(x + r * ldx + c, 8);
+        if constexpr (VEC) v.load(src);
+        else v.load_any(src, 8);
         const uint32_t s = mx_scale(quad_umax(v.top()));
         *reinterpret_cast<uint32_t*>(codes + i * 4) = s == 255 ? 0u : v.codes8(0, mx_scale_f32(s));
         if ((threadIdx.x & 3) == 0) scales[i >> 2] = (uint8_t)s;
     }
 }
 
-// eight values of a code word times 2^(s - 127), exact in fp32 (and in bf16 and fp16 within their ranges)
+// The eight values of a code word times the scale, by the conversion instructions: exact in fp32 and bf16 (fp16 rounds outside
+// its range). The scale NaN is put in by hand.
 template <class E>
 __device__ __forceinline__ void mx_values8(uint32_t c, uint32_t s, E (&o)[8]) {
-    const float sc = s == 255 ? __uint_as_float(0x7fc00000u) : mx_scale_f32(s);
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        // magnitude bits eem: 0.5 m for ee = 0, else 2^(ee - 1) (1 + m / 2): as fp32 bits, with ee = 0 an exact half
-        const uint32_t m = (c >> (4 * i)) & 7;
-        const float a = m < 2 ? 0.5f * (float)m : __uint_as_float(((m >> 1) + 126) << 23 | (m & 1) << 22);
-        o[i] = (E)(__uint_as_float(__float_as_uint(a) | (c >> (4 * i) & 8) << 28) * sc);
+    const float sc = mx_scale_f32(s);
+    auto two = [&](auto pair, int i) {
+        const bool nan = s == 255;
+        o[2 * i] = nan ? (E)__uint_as_float(0x7fc00000u) : (E)pair[0];
+        o[2 * i + 1] = nan ? (E)__uint_as_float(0x7fc00000u) : (E)pair[1];
+    };
+    if constexpr (sizeof(E) == 4) {
+        two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, sc, 0), 0);
+        two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, sc, 1), 1);
+        two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, sc, 2), 2);
+        two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, sc, 3), 3);
+    } else if constexpr (std::is_same<E, _Float16>::value) {
+        two(__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, sc, 0), 0);
+        two(__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, sc, 1), 1);
+        two(__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, sc, 2), 2);
+        two(__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, sc, 3), 3);
+    } else {
+        two(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, sc, 0), 0);
+        two(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, sc, 1), 1);
+        two(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, sc, 2), 2);
+        two(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, sc, 3), 3);
     }
 }
-template <class E, bool VEC>
-__global__ __launch_bounds__(256) void k_mx_dequantize(E* y, size_t ldy, const uint8_t* codes, const uint8_t* scales, int rows, int cols) {
-    const size_t n = (size_t)rows * (cols / 8);
+template <class E, bool VEC, bool DENSE>
+__global__ __launch_bounds__(256) void k_mx_dequantize(E* y, size_t ldy, const uint8_t* codes, const uint8_t* scales, size_t n,
+                                                       uint32_t per_row) {
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
-        const size_t r = i / (cols / 8);
-        const int c = (int)(i - r * (cols / 8)) * 8;
         E o[8];
         mx_values8(*reinterpret_cast<const uint32_t*>(codes + i * 4), scales[i >> 2], o);
-        E* dst = y + r * ldy + c;
+        E* dst = y + mx_place<DENSE>(i, n, per_row, ldy);
         if constexpr (VEC) {
             typedef E V __attribute__((ext_vector_type(16 / sizeof(E))));
 #pragma unroll
@@ -124,16 +145,20 @@ static unsigned grid_of(size_t n) { return (unsigned)std::min<size_t>((n + 255) 
 template <class E>
 static hipError_t quantize_of(uint8_t* codes, uint8_t* scales, const void* x, size_t ldx, int rows, int cols, bool vec, hipStream_t s) {
     const size_t n = (size_t)rows * (cols / 8);
-    auto kern = vec ? k_mx_quantize<E, true> : k_mx_quantize<E, false>;
-    hipLaunchKernelGGL(kern, dim3(grid_of(n)), dim3(256), 0, s, codes, scales, static_cast<const E*>(x), ldx, rows, cols);
+    const bool dense = rows == 1 || ldx == (size_t)cols;
+    auto kern = vec ? (dense ? k_mx_quantize<E, true, true> : k_mx_quantize<E, true, false>)
+                    : (dense ? k_mx_quantize<E, false, true> : k_mx_quantize<E, false, false>);
+    hipLaunchKernelGGL(kern, dim3(grid_of(n)), dim3(256), 0, s, codes, scales, static_cast<const E*>(x), ldx, n, (uint32_t)(cols / 8));
     return hipGetLastError();
 }
 template <class E>
 static hipError_t dequantize_of(void* y, size_t ldy, const uint8_t* codes, const uint8_t* scales, int rows, int cols, bool vec,
                                 hipStream_t s) {
     const size_t n = (size_t)rows * (cols / 8);
-    auto kern = vec ? k_mx_dequantize<E, true> : k_mx_dequantize<E, false>;
-    hipLaunchKernelGGL(kern, dim3(grid_of(n)), dim3(256), 0, s, static_cast<E*>(y), ldy, codes, scales, rows, cols);
+    const bool dense = rows == 1 || ldy == (size_t)cols;
+    auto kern = vec ? (dense ? k_mx_dequantize<E, true, true> : k_mx_dequantize<E, true, false>)
+                    : (dense ? k_mx_dequantize<E, false, true> : k_mx_dequantize<E, false, false>);
+    hipLaunchKernelGGL(kern, dim3(grid_of(n)), dim3(256), 0, s, static_cast<E*>(y), ldy, codes, scales, n, (uint32_t)(cols / 8));
     return hipGetLastError();
 }
 template <class E>
