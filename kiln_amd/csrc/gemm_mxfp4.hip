@@ -2,6 +2,8 @@
 // 4-bit codes with a scale per 32 values (mxfp4.hpp). Products of codes and powers of two are exact; sums are fp32.
 #include <hip/hip_runtime.h>
 
+#include <math.h>
+
 #include <algorithm>
 
 #include "gemm16.hpp"
@@ -120,24 +122,48 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void k_mx_few(const MxGemmParams p)
     const uint8_t* wc = p.wc + (size_t)nb * p.kbs * MX_UNIT + lane * 16;
     const uint8_t* wsc = p.ws + (size_t)(nb >> 2) * p.kbs * MX_SUNIT + lane * 4 + (nb & 3);
     const E* x = static_cast<const E*>(p.x);
-    for (int kb = wv; kb < p.kbs; kb += FEW_WAVES) {
-        const u32x4 w = *reinterpret_cast<const u32x4*>(wc + (size_t)kb * MX_UNIT);
-        const uint32_t sw = wsc[(size_t)kb * MX_SUNIT];
-        const int k = kb * 128 + 32 * (lane >> 4);
+    struct Ops {
+        u32x4 w;
+        uint32_t sw;
         MxVals<E, MXB> v[MB];
+    };
+    auto inside = [&](int mb, int kb) { return mb * 16 + r < p.T && kb * 128 + 32 * (lane >> 4) < p.K; };
+    auto load = [&](Ops& o, int kb) {
+        kb = min(kb, p.kbs - 1);
+        o.w = *reinterpret_cast<const u32x4*>(wc + (size_t)kb * MX_UNIT);
+        o.sw = wsc[(size_t)kb * MX_SUNIT];
 #pragma unroll
         for (int mb = 0; mb < MB; mb++) {
-            const bool in = mb * 16 + r < p.T && k < p.K;
-            const E* src = x + (in ? (mb * 16 + r) * p.ldx + k : 0);
-            if constexpr (VEC) v[mb].load(src);
-            else v[mb].load_any(src, in ? MXB : 0);
+            const bool in = inside(mb, kb);
+            const E* src = x + (in ? (mb * 16 + r) * p.ldx + kb * 128 + 32 * (lane >> 4) : 0);
+            if constexpr (VEC) o.v[mb].load(src);
+            else o.v[mb].load_any(src, in ? MXB : 0);
         }
+    };
+    auto mul = [&](const Ops& o, int kb) {
 #pragma unroll
         for (int mb = 0; mb < MB; mb++) {
             uint32_t s;
-            u32x4 c = mx_block<E>(v[mb], s);
-            if (!(mb * 16 + r < p.T && k < p.K)) c = u32x4{0, 0, 0, 0}, s = 0;
-            acc[mb] = mx_mfma<0, 0>(w, sw, c, s, acc[mb]);
+            u32x4 c = mx_block<E>(o.v[mb], s);
+            if (!inside(mb, kb)) c = u32x4{0, 0, 0, 0}, s = 0;
+            acc[mb] = mx_mfma<0, 0>(o.w, o.sw, c, s, acc[mb]);
+        }
+    };
+    if constexpr (MB * sizeof(E) <= 4) {  // two k blocks in flight, where the registers hold them
+        Ops o[2];
+        load(o[0], wv);
+        load(o[1], wv + FEW_WAVES);
+        for (int kb = wv; kb < p.kbs; kb += 2 * FEW_WAVES) {
+            mul(o[0], kb);
+            load(o[0], kb + 2 * FEW_WAVES);
+            if (kb + FEW_WAVES < p.kbs) mul(o[1], kb + FEW_WAVES);
+            load(o[1], kb + 3 * FEW_WAVES);
+        }
+    } else {
+        for (int kb = wv; kb < p.kbs; kb += FEW_WAVES) {
+            Ops o;
+            load(o, kb);
+            mul(o, kb);
         }
     }
 #pragma unroll
@@ -149,6 +175,79 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void k_mx_few(const MxGemmParams p)
         for (int w = 1; w < FEW_WAVES; w++) t += red[w][wv][lane];
         mx_store<EPI>(p, wv * 16 + r, nb * 16 + 4 * (lane >> 4), t);
     }
+}
+
+// ---- small products: operands from the quantised rows straight into registers ----
+//
+// A workgroup takes 16 NB weight rows x 16 MB rows of x; its eight waves share out the k blocks, each reading whole 1 KB units
+// of both operands (from L2) two k blocks ahead of their products, and meet in LDS. No ring to fill: what bounds it at these sizes
+// is the latency of a few loads, then L2's rate.
+constexpr int THIN_WAVES = 8;
+template <int EPI, int NB, int MB>
+__global__ __launch_bounds__(THIN_WAVES * 64, 2) void k_mx_thin(const MxGemmParams p) {
+    extern __shared__ __attribute__((aligned(16))) floatx4 thin_red[];  // [wave][block][lane]
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int ti = (int)(blockIdx.x & 7) * p.per + (int)(blockIdx.x >> 3);  // an XCD's range: the row tiles of a W tile together
+    if (ti >= p.total) return;
+    const int tm = ti % p.tiles_m, tn = ti / p.tiles_m, nb0 = tn * NB, mb0 = tm * MB;
+    const uint8_t* wc = p.wc + (size_t)nb0 * p.kbs * MX_UNIT + lane * 16;
+    const uint8_t* xc = p.xc + (size_t)mb0 * p.kbs * MX_UNIT + lane * 16;
+    const uint8_t* wsc = p.ws + (size_t)(nb0 >> 2) * p.kbs * MX_SUNIT + lane * 4;
+    const uint8_t* xsc = p.xs + (size_t)(mb0 >> 2) * p.kbs * MX_SUNIT + lane * 4;
+    const int wsh = 8 * (nb0 & 3), xsh = 8 * (mb0 & 3);  // the tile's first block's byte of a scale unit
+    struct Ops {
+        u32x4 w[NB], x[MB];
+        uint32_t sw, sx;
+    } ops[2];
+    auto load = [&](Ops& o, int kb) {
+        kb = min(kb, p.kbs - 1);
+#pragma unroll
+        for (int i = 0; i < NB; i++) o.w[i] = *reinterpret_cast<const u32x4*>(wc + ((size_t)i * p.kbs + kb) * MX_UNIT);
+#pragma unroll
+        for (int i = 0; i < MB; i++) o.x[i] = *reinterpret_cast<const u32x4*>(xc + ((size_t)i * p.kbs + kb) * MX_UNIT);
+        o.sw = *reinterpret_cast<const uint32_t*>(wsc + (size_t)kb * MX_SUNIT);
+        o.sx = *reinterpret_cast<const uint32_t*>(xsc + (size_t)kb * MX_SUNIT);
+    };
+    floatx4 acc[NB][MB];
+#pragma unroll
+    for (int i = 0; i < NB; i++)
+#pragma unroll
+        for (int j = 0; j < MB; j++) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+    auto mul = [&](const Ops& o) {
+        const uint32_t sw = o.sw >> wsh, sx = o.sx >> xsh;
+#pragma unroll
+        for (int i = 0; i < NB; i++)
+#pragma unroll
+            for (int j = 0; j < MB; j++) acc[i][j] = mx_mfma_at(i, j, o.w[i], sw, o.x[j], sx, acc[i][j]);
+    };
+    load(ops[0], wv);
+    load(ops[1], wv + THIN_WAVES);
+    for (int kb = wv; kb < p.kbs; kb += 2 * THIN_WAVES) {
+        mul(ops[0]);
+        load(ops[0], kb + 2 * THIN_WAVES);
+        if (kb + THIN_WAVES < p.kbs) mul(ops[1]);
+        load(ops[1], kb + 3 * THIN_WAVES);
+    }
+#pragma unroll
+    for (int i = 0; i < NB; i++)
+#pragma unroll
+        for (int j = 0; j < MB; j++) thin_red[(wv * NB * MB + i * MB + j) * 64 + lane] = acc[i][j];
+    __syncthreads();
+    for (int b = wv; b < NB * MB; b += THIN_WAVES) {
+        floatx4 t = thin_red[b * 64 + lane];
+#pragma unroll
+        for (int w = 1; w < THIN_WAVES; w++) t += thin_red[(w * NB * MB + b) * 64 + lane];
+        mx_store<EPI>(p, (mb0 + b % MB) * 16 + (lane & 15), (nb0 + b / MB) * 16 + 4 * (lane >> 4), t);
+    }
+}
+template <int EPI, int NB, int MB>
+static hipError_t mx_thin(MxGemmParams p, hipStream_t s) {
+    p.tiles_m = (p.T + 16 * MB - 1) / (16 * MB);
+    p.tiles_n = (p.N + 16 * NB - 1) / (16 * NB);
+    p.total = p.tiles_m * p.tiles_n;
+    p.per = (p.total + 7) / 8;
+    hipLaunchKernelGGL((k_mx_thin<EPI, NB, MB>), dim3(p.per * 8), dim3(THIN_WAVES * 64), THIN_WAVES * NB * MB * 1024, s, p);
+    return hipGetLastError();
 }
 
 // ---- tiles ----
@@ -371,14 +470,38 @@ static hipError_t mx_few(const MxGemmParams& p, hipStream_t s) {
     return hipGetLastError();
 }
 
-constexpr int FEW_ROWS = 64;
+// The form of a product.
+enum MxKind { MX_FEW, MX_THIN22, MX_THIN44, MX_MID, MX_BIG };
+// Few rows quantise in the product, one launch: as long as 16 of them, or little of x, is quantised anew in each workgroup (fp16
+// out, the whole call among others, against the next best form: 2048 x 2048, T = 32 7.6 / 8.5 us, T = 64 10.5 / 8.3;
+// 2048 x 8192, T = 8 7.6 / 8.2, T = 17 12.5 / 8.6; 1024 x 1024, T = 64 6.8 / 8.4).
+static bool mx_few_rows(int T, int N, int K) {
+    const int mb = (T + 15) / 16, groups = std::max(1, (N + 15) / 16 / cu_count());
+    return T <= 64 && (mb == 1 || (long)(mb > 2 ? 4 : mb) * mx_kb(K) * groups <= 32);
+}
+// Modelled time of the other forms' product kernel in us: workgroups that follow each other on a CU, each with a fixed cost and one
+// per k block, and what the tiles in flight take from each other. Fitted to T = 17 .. 6912 x {1024 x 1024, 2048 x 2048,
+// 8192 x 2048, 2048 x 8192}; where two forms meet they measured within 5% (8192 x 2048, T = 128 8.7 and T = 200 12.2 with 64 x 64,
+// 10.6 and 10.5 with 128 x 128 tiles; T = 1537 28.5 with 128 x 128, 25.9 with 256 x 256).
+static MxKind mx_choose(int T, int N, int K) {
+    if (mx_few_rows(T, N, K)) return MX_FEW;
+    const double cus = cu_count(), kb = mx_kb(K);
+    auto tiles = [&](int bn, int bm) { return (double)((N + bn - 1) / bn) * ((T + bm - 1) / bm); };
+    const double t22 = tiles(32, 32), t44 = tiles(64, 64), tm = tiles(128, 128), tb = tiles(256, 256);
+    const double cost[4] = {0.8 + 0.01 * kb + 0.056 * kb * t22 / cus,
+                            ceil(t44 / cus) * (1.2 + 0.045 * kb) + 0.125 * kb * t44 / cus,
+                            1.9 * std::max(1.0, tm / cus) + kb * (0.155 + 0.22 * tm / cus),
+                            ceil(tb / cus) * (5.0 + 0.55 * kb) + 0.35 * kb * tb / cus};
+    return (MxKind)(MX_THIN22 + (std::min_element(cost, cost + 4) - cost));
+}
 size_t linear_mx_workspace(int T, int rows, int cols) {
-    return T <= FEW_ROWS ? 0 : mx_code_bytes(T, cols) + mx_scale_bytes(T, cols);
+    return mx_few_rows(T, rows, cols) ? 0 : mx_code_bytes(T, cols) + mx_scale_bytes(T, cols);
 }
 
 template <int EPI>
 static hipError_t linear_mx_epi(MxGemmParams p, DT dt, uint8_t* ws, hipStream_t s) {
-    if (p.T <= FEW_ROWS) {
+    const MxKind kind = mx_choose(p.T, p.N, p.K);
+    if (kind == MX_FEW) {
         if (dt == DT::F32) return mx_few<float, EPI>(p, s);
         if (dt == DT::F16) return mx_few<_Float16, EPI>(p, s);
         return mx_few<__bf16, EPI>(p, s);
@@ -386,9 +509,12 @@ static hipError_t linear_mx_epi(MxGemmParams p, DT dt, uint8_t* ws, hipStream_t 
     if (hipError_t e = launch_mx_quantize_pack(ws, p.x, dt, p.ldx, p.T, p.K, s)) return e;
     p.xc = ws;
     p.xs = ws + mx_code_bytes(p.T, p.K);
-    const long big = (long)((p.T + 255) / 256) * ((p.N + 255) / 256);
-    if (big >= cu_count()) return mx_tiles<EPI, MxBig>(p, s);
-    return mx_tiles<EPI, MxMid>(p, s);
+    switch (kind) {
+        case MX_THIN22: return mx_thin<EPI, 2, 2>(p, s);
+        case MX_THIN44: return mx_thin<EPI, 4, 4>(p, s);
+        case MX_MID: return mx_tiles<EPI, MxMid>(p, s);
+        default: return mx_tiles<EPI, MxBig>(p, s);
+    }
 }
 
 hipError_t launch_linear_mx(void* y, size_t ldy, const void* x, DT dt, size_t ldx, int T, const uint8_t* wp, int rows, int cols, int epi,
