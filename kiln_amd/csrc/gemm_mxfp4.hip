@@ -119,8 +119,9 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void k_mx_few(const MxGemmParams p)
     floatx4 acc[MB];
 #pragma unroll
     for (int mb = 0; mb < MB; mb++) acc[mb] = floatx4{0.f, 0.f, 0.f, 0.f};
-    const uint8_t* wc = p.wc + (size_t)nb * p.kbs * MX_UNIT + lane * 16;
-    const uint8_t* wsc = p.ws + (size_t)(nb >> 2) * p.kbs * MX_SUNIT + lane * 4 + (nb & 3);
+    const uint8_t* wc = p.wc + (size_t)nb * MX_UNIT + lane * 16;
+    const uint8_t* wsc = p.ws + (size_t)(nb >> 2) * MX_SUNIT + lane * 4 + (nb & 3);
+    const size_t rgs = mx_rg(p.N);
     const E* x = static_cast<const E*>(p.x);
     struct Ops {
         u32x4 w;
@@ -130,8 +131,8 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void k_mx_few(const MxGemmParams p)
     auto inside = [&](int mb, int kb) { return mb * 16 + r < p.T && kb * 128 + 32 * (lane >> 4) < p.K; };
     auto load = [&](Ops& o, int kb) {
         kb = min(kb, p.kbs - 1);
-        o.w = *reinterpret_cast<const u32x4*>(wc + (size_t)kb * MX_UNIT);
-        o.sw = wsc[(size_t)kb * MX_SUNIT];
+        o.w = *reinterpret_cast<const u32x4*>(wc + kb * rgs * 4 * MX_UNIT);
+        o.sw = wsc[kb * rgs * MX_SUNIT];
 #pragma unroll
         for (int mb = 0; mb < MB; mb++) {
             const bool in = inside(mb, kb);
@@ -190,10 +191,11 @@ __global__ __launch_bounds__(THIN_WAVES * 64, 2) void k_mx_thin(const MxGemmPara
     const int ti = (int)(blockIdx.x & 7) * p.per + (int)(blockIdx.x >> 3);  // an XCD's range: the row tiles of a W tile together
     if (ti >= p.total) return;
     const int tm = ti % p.tiles_m, tn = ti / p.tiles_m, nb0 = tn * NB, mb0 = tm * MB;
-    const uint8_t* wc = p.wc + (size_t)nb0 * p.kbs * MX_UNIT + lane * 16;
-    const uint8_t* xc = p.xc + (size_t)mb0 * p.kbs * MX_UNIT + lane * 16;
-    const uint8_t* wsc = p.ws + (size_t)(nb0 >> 2) * p.kbs * MX_SUNIT + lane * 4;
-    const uint8_t* xsc = p.xs + (size_t)(mb0 >> 2) * p.kbs * MX_SUNIT + lane * 4;
+    const uint8_t* wc = p.wc + (size_t)nb0 * MX_UNIT + lane * 16;
+    const uint8_t* xc = p.xc + (size_t)mb0 * MX_UNIT + lane * 16;
+    const uint8_t* wsc = p.ws + (size_t)(nb0 >> 2) * MX_SUNIT + lane * 4;
+    const uint8_t* xsc = p.xs + (size_t)(mb0 >> 2) * MX_SUNIT + lane * 4;
+    const size_t wrg = mx_rg(p.N), xrg = mx_rg(p.T);
     const int wsh = 8 * (nb0 & 3), xsh = 8 * (mb0 & 3);  // the tile's first block's byte of a scale unit
     struct Ops {
         u32x4 w[NB], x[MB];
@@ -202,11 +204,11 @@ __global__ __launch_bounds__(THIN_WAVES * 64, 2) void k_mx_thin(const MxGemmPara
     auto load = [&](Ops& o, int kb) {
         kb = min(kb, p.kbs - 1);
 #pragma unroll
-        for (int i = 0; i < NB; i++) o.w[i] = *reinterpret_cast<const u32x4*>(wc + ((size_t)i * p.kbs + kb) * MX_UNIT);
+        for (int i = 0; i < NB; i++) o.w[i] = *reinterpret_cast<const u32x4*>(wc + (kb * wrg * 4 + i) * MX_UNIT);
 #pragma unroll
-        for (int i = 0; i < MB; i++) o.x[i] = *reinterpret_cast<const u32x4*>(xc + ((size_t)i * p.kbs + kb) * MX_UNIT);
-        o.sw = *reinterpret_cast<const uint32_t*>(wsc + (size_t)kb * MX_SUNIT);
-        o.sx = *reinterpret_cast<const uint32_t*>(xsc + (size_t)kb * MX_SUNIT);
+        for (int i = 0; i < MB; i++) o.x[i] = *reinterpret_cast<const u32x4*>(xc + (kb * xrg * 4 + i) * MX_UNIT);
+        o.sw = *reinterpret_cast<const uint32_t*>(wsc + kb * wrg * MX_SUNIT);
+        o.sx = *reinterpret_cast<const uint32_t*>(xsc + kb * xrg * MX_SUNIT);
     };
     floatx4 acc[NB][MB];
 #pragma unroll
@@ -254,64 +256,73 @@ static hipError_t mx_thin(MxGemmParams p, hipStream_t s) {
 //
 // WN x WM waves of 16 NB x 16 MB blocks. A stage of the LDS ring holds one k block of 128: the tile's units of W and of x
 // (1 KB each) and their scales, all by LDS DMA in the operand layout, so that every operand read is 1 KB without conflicts.
-template <int WN_, int WM_, int NB_, int MB_, int NST_, int WGS_>
+// KG groups of such waves with a ring each take every KG th k block; their sums meet in LDS, in the groups' order.
+template <int WN_, int WM_, int NB_, int MB_, int KG_, int NST_, int WGS_>
 struct MxCfg {
-    static constexpr int WN = WN_, WM = WM_, NB = NB_, MB = MB_, NST = NST_, WGS = WGS_, WAVES = WN * WM, THREADS = WAVES * 64;
+    static constexpr int WN = WN_, WM = WM_, NB = NB_, MB = MB_, KG = KG_, NST = NST_, WGS = WGS_, WAVES = WN * WM;
+    static constexpr int THREADS = WAVES * KG * 64;
     static constexpr int BN = WN * NB * 16, BM = WM * MB * 16;
     static constexpr int UN = BN / 16, UM = BM / 16, SN = (BN + 63) / 64, SM = (BM + 63) / 64;
     static constexpr int CODE_DMA = (UN + UM) / WAVES, SCALE_DMA = (SN + SM + WAVES - 1) / WAVES, DPS = CODE_DMA + SCALE_DMA;
-    static constexpr int SC_OFF = (UN + UM) * MX_UNIT, STAGE = SC_OFF + (SN + SM) * MX_SUNIT, LDS = NST * STAGE;
+    static constexpr int SC_OFF = (UN + UM) * MX_UNIT, STAGE = SC_OFF + (SN + SM) * MX_SUNIT, RING = NST * STAGE, LDS = KG * RING;
     static_assert((UN + UM) % WAVES == 0 && NB % 4 == 0 && MB % 4 == 0 && LDS * WGS <= 160 * 1024, "tile");
 };
 
 template <int EPI, class C>
-__global__ __launch_bounds__(C::THREADS, C::WAVES * C::WGS / 4) void k_mx_gemm(const MxGemmParams p) {
+__global__ __launch_bounds__(C::THREADS, C::WAVES * C::KG * C::WGS / 4) void k_mx_gemm(const MxGemmParams p) {
 #ifdef __HIP_DEVICE_COMPILE__  // the host pass only needs the kernel's handle
     extern __shared__ __attribute__((aligned(16))) uint8_t lds8[];
-    constexpr int NB = C::NB, MB = C::MB;
+    constexpr int NB = C::NB, MB = C::MB, KG = C::KG;
     // blocks go round the 8 XCDs: each takes a contiguous range of tiles, in groups of row tiles that share W in its L2
     const int ti = (int)(blockIdx.x & 7) * p.per + (int)(blockIdx.x >> 3);
     if (ti >= p.total) return;
     int tm, tn;
     raster_tile(ti, 4, p.tiles_m, p.tiles_n, tm, tn);
-    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wn = wv % C::WN, wm = wv / C::WN;
-    const int nrb = (p.N + 63) / 64 * 4, mrb = (p.T + 63) / 64 * 4;  // row blocks that exist
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int kg = wave / C::WAVES, wv = wave % C::WAVES, wn = wv % C::WN, wm = wv / C::WN;
+    const int steps = (p.kbs + KG - 1) / KG;  // the group's k blocks: kg, kg + KG, .. (a last one past the end is not multiplied)
+    uint8_t* ring = lds8 + kg * C::RING;
+    const int wrg = mx_rg(p.N), xrg = mx_rg(p.T);  // row groups that exist
 
     // DMA pieces of this wave: units wv, wv + WAVES, .. of the stage (W's first), then the scale units; row blocks past the
     // matrix re-read its last one (their results are not stored)
     typedef __attribute__((address_space(3))) void* lds_p;
     const uint8_t* src[C::CODE_DMA];
+    uint32_t kstep[C::CODE_DMA];  // units from a k block to the next
 #pragma unroll
     for (int i = 0; i < C::CODE_DMA; i++) {
         const int u = wv + i * C::WAVES;
-        src[i] = u < C::UN ? p.wc + (size_t)min(tn * C::UN + u, nrb - 1) * p.kbs * MX_UNIT
-                           : p.xc + (size_t)min(tm * C::UM + u - C::UN, mrb - 1) * p.kbs * MX_UNIT;
+        src[i] = (u < C::UN ? p.wc + (size_t)min(tn * C::UN + u, 4 * wrg - 1) * MX_UNIT
+                            : p.xc + (size_t)min(tm * C::UM + u - C::UN, 4 * xrg - 1) * MX_UNIT) + lane * 16;
+        kstep[i] = 4 * (u < C::UN ? wrg : xrg);
     }
     const uint8_t* ssrc[C::SCALE_DMA];
+    uint32_t skstep[C::SCALE_DMA];
     int sdst[C::SCALE_DMA];
 #pragma unroll
     for (int i = 0; i < C::SCALE_DMA; i++) {
         const int u = (wv + i * C::WAVES) % (C::SN + C::SM);  // a wave without one copies another's again
         sdst[i] = C::SC_OFF + u * MX_SUNIT;
-        ssrc[i] = u < C::SN ? p.ws + (size_t)min(tn * C::BN / 64 + u, nrb / 4 - 1) * p.kbs * MX_SUNIT
-                            : p.xs + (size_t)min(tm * C::BM / 64 + u - C::SN, mrb / 4 - 1) * p.kbs * MX_SUNIT;
+        ssrc[i] = (u < C::SN ? p.ws + (size_t)min(tn * C::BN / 64 + u, wrg - 1) * MX_SUNIT
+                             : p.xs + (size_t)min(tm * C::BM / 64 + u - C::SN, xrg - 1) * MX_SUNIT) + lane * 4;
+        skstep[i] = u < C::SN ? wrg : xrg;
     }
-    auto dma_piece = [&](int i, int kb, int stage) {
-        uint8_t* base = lds8 + stage * C::STAGE;
+    typedef const __attribute__((address_space(1))) void* glb_p;
+    auto dma_piece = [&](int i, int step, int stage) {
+        const size_t kb = min(step * KG + kg, p.kbs - 1);
+        uint8_t* base = ring + stage * C::STAGE;
         if (i < C::CODE_DMA)
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src[i] + (size_t)kb * MX_UNIT + lane * 16),
-                                             (lds_p)(base + (wv + i * C::WAVES) * MX_UNIT), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((glb_p)(src[i] + kb * kstep[i] * MX_UNIT), (lds_p)(base + (wv + i * C::WAVES) * MX_UNIT), 16, 0, 0);
         else if (i < C::DPS)
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(ssrc[i - C::CODE_DMA] + (size_t)kb * MX_SUNIT + lane * 4),
+            __builtin_amdgcn_global_load_lds((glb_p)(ssrc[i - C::CODE_DMA] + kb * skstep[i - C::CODE_DMA] * MX_SUNIT),
                                              (lds_p)(base + sdst[i - C::CODE_DMA]), 4, 0, 0);
     };
-    auto dma = [&](int kb, int stage) {
+    auto dma = [&](int step, int stage) {
 #pragma unroll
-        for (int i = 0; i < C::DPS; i++) dma_piece(i, kb, stage);
+        for (int i = 0; i < C::DPS; i++) dma_piece(i, step, stage);
     };
 
-    const uint32_t lds_base = (uint32_t)(size_t)(__attribute__((address_space(3))) uint8_t*)lds8;
+    const uint32_t lds_base = (uint32_t)(size_t)(__attribute__((address_space(3))) uint8_t*)ring;
     floatx4 acc[NB][MB];
 #pragma unroll
     for (int nb = 0; nb < NB; nb++)
@@ -334,57 +345,77 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES * C::WGS / 4) void k_mx_gemm(c
     auto read_x = [&](int mb, uint32_t st) { fx[mb] = *reinterpret_cast<const lds_u32x4*>((size_t)(xa + st + mb * MX_UNIT)); };
 
 #pragma unroll
-    for (int s = 0; s < C::NST - 1; s++) dma(min(s, p.kbs - 1), s);
+    for (int s = 0; s < C::NST - 1; s++) dma(s, s);
     wait_vmcnt<(C::NST - 2) * C::DPS>();
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
     read_w(0, 0);
 #pragma unroll
     for (int mb = 0; mb < MB; mb++) read_x(mb, 0);
-    int next = 1;  // the stage of block kb + 1
-    // Block kb: its operands are in registers. Block kb + 1 landed in every wave; the stage of block kb - 1, whose reads every
-    // wave finished before its products of kb - 1, is refilled (past the end with the last block again: the count of loads
-    // in flight stays the same). The operands of kb + 1 are read between the products of kb, x's into the registers that are done.
-    auto step = [&](int kb, auto tag) {
+    int next = 1;  // the stage of step i + 1
+    // Step i: its operands are in registers. Those of step i + 1 landed in every wave; the stage of step i - 1, whose reads every
+    // wave finished before its products of i - 1, is refilled (past the end with the last block again: the count of loads
+    // in flight stays the same). The operands of i + 1 are read between the products of i, x's into the registers that are done.
+    auto step = [&](int i, auto tag) {
         constexpr int cur = decltype(tag)::value;
         wait_vmcnt<(C::NST - 3) * C::DPS>();
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
-        const int dk = min(kb + C::NST - 1, p.kbs - 1), ds = next >= 2 ? next - 2 : next - 2 + C::NST;
+        const bool real = KG == 1 || i * KG + kg < p.kbs;
+        const int ds = next >= 2 ? next - 2 : next - 2 + C::NST;
         const uint32_t st = next * C::STAGE;
 #pragma unroll
         for (int mb = 0; mb < MB; mb++) {
+            if (real)
 #pragma unroll
-            for (int nb = 0; nb < NB; nb++)
-                acc[nb][mb] = mx_mfma_at(nb & 3, mb & 3, fw[cur][nb], sw[cur][nb / 4], fx[mb], sx[cur][mb / 4], acc[nb][mb]);
+                for (int nb = 0; nb < NB; nb++)
+                    acc[nb][mb] = mx_mfma_at(nb & 3, mb & 3, fw[cur][nb], sw[cur][nb / 4], fx[mb], sx[cur][mb / 4], acc[nb][mb]);
             __builtin_amdgcn_sched_barrier(0);
             read_x(mb, st);
             if (mb == 0) {
 #pragma unroll
-                for (int i = 0; i < NB / 4; i++) sw[cur ^ 1][i] = *reinterpret_cast<const lds_u32*>((size_t)(swa + st + i * MX_SUNIT));
+                for (int u = 0; u < NB / 4; u++) sw[cur ^ 1][u] = *reinterpret_cast<const lds_u32*>((size_t)(swa + st + u * MX_SUNIT));
 #pragma unroll
-                for (int i = 0; i < MB / 4; i++) sx[cur ^ 1][i] = *reinterpret_cast<const lds_u32*>((size_t)(sxa + st + i * MX_SUNIT));
+                for (int u = 0; u < MB / 4; u++) sx[cur ^ 1][u] = *reinterpret_cast<const lds_u32*>((size_t)(sxa + st + u * MX_SUNIT));
             }
             if (mb < MB / 2) {
 #pragma unroll
-                for (int i = 0; i < 2 * NB / MB; i++) {
-                    const int nb = mb * (2 * NB / MB) + i;
+                for (int n = 0; n < 2 * NB / MB; n++) {
+                    const int nb = mb * (2 * NB / MB) + n;
                     fw[cur ^ 1][nb] = *reinterpret_cast<const lds_u32x4*>((size_t)(wa + st + nb * MX_UNIT));
                 }
             }
 #pragma unroll
-            for (int i = 0; i < (C::DPS + MB - 1) / MB; i++) dma_piece(mb * ((C::DPS + MB - 1) / MB) + i, dk, ds);
+            for (int n = 0; n < (C::DPS + MB - 1) / MB; n++) dma_piece(mb * ((C::DPS + MB - 1) / MB) + n, i + C::NST - 1, ds);
             __builtin_amdgcn_sched_barrier(0);
         }
         next = next == C::NST - 1 ? 0 : next + 1;
     };
-    int kb = 0;
-    for (; kb + 2 <= p.kbs; kb += 2) {
-        step(kb, std::integral_constant<int, 0>{});
-        step(kb + 1, std::integral_constant<int, 1>{});
+    int i = 0;
+    for (; i + 2 <= steps; i += 2) {
+        step(i, std::integral_constant<int, 0>{});
+        step(i + 1, std::integral_constant<int, 1>{});
     }
-    if (kb < p.kbs) step(kb, std::integral_constant<int, 0>{});
+    if (i < steps) step(i, std::integral_constant<int, 0>{});
     wait_vmcnt<0>();  // no copy into LDS outlives the ring
+    if constexpr (KG > 1) {
+        floatx4* red = reinterpret_cast<floatx4*>(lds8);  // [group - 1][wave][block][lane]
+        static_assert((KG - 1) * C::WAVES * NB * MB * 1024 <= C::LDS, "the groups' sums fit in the rings");
+        __syncthreads();  // every wave is done with the rings
+        if (kg)
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                for (int mb = 0; mb < MB; mb++) red[((((kg - 1) * C::WAVES + wv) * NB + nb) * MB + mb) * 64 + lane] = acc[nb][mb];
+        __syncthreads();
+        if (kg) return;
+#pragma unroll
+        for (int k = 0; k < KG - 1; k++)
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                for (int mb = 0; mb < MB; mb++) acc[nb][mb] += red[(((k * C::WAVES + wv) * NB + nb) * MB + mb) * 64 + lane];
+    }
     const int g = lane >> 4, rl = lane & 15;
     const int m0 = tm * C::BM + wm * MB * 16, n0 = tn * C::BN + wn * NB * 16;
     if (p.vec < 2) {
@@ -401,7 +432,7 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES * C::WGS / 4) void k_mx_gemm(c
     static_assert(RB * 16 * CH * 16 * C::WAVES <= C::LDS, "the waves' regions fit in the ring");
     uint8_t* stg = lds8 + wv * (RB * 16 * CH * 16);
     __builtin_amdgcn_s_waitcnt(0xC07F);
-    __builtin_amdgcn_s_barrier();  // every wave is done with the ring
+    __builtin_amdgcn_s_barrier();  // every wave (of the last group) is done with the ring, or with the sums in it
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int h = 0; h < MB / RB; h++) {
@@ -445,8 +476,9 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES * C::WGS / 4) void k_mx_gemm(c
 #endif
 }
 
-using MxBig = MxCfg<4, 2, 4, 8, 4, 1>;    // 256 x 256 (n x m), 8 waves, 136 KB
-using MxMid = MxCfg<2, 2, 4, 4, 4, 2>;    // 128 x 128, 4 waves, 68 KB
+using MxBig = MxCfg<4, 2, 4, 8, 1, 4, 1>;    // 256 x 256 (n x m), 8 waves, 136 KB
+using MxMid = MxCfg<2, 2, 4, 4, 1, 4, 2>;    // 128 x 128, 4 waves, 68 KB
+using MxMidK = MxCfg<2, 2, 4, 4, 2, 4, 1>;   // 128 x 128, two groups of 4 waves, 136 KB
 
 template <int EPI, class C>
 static hipError_t mx_tiles(MxGemmParams p, hipStream_t s) {
@@ -471,7 +503,7 @@ static hipError_t mx_few(const MxGemmParams& p, hipStream_t s) {
 }
 
 // The form of a product.
-enum MxKind { MX_FEW, MX_THIN22, MX_THIN44, MX_MID, MX_BIG };
+enum MxKind { MX_FEW, MX_THIN22, MX_THIN44, MX_MID, MX_BIG, MX_MIDK };
 // Few rows quantise in the product, one launch: as long as 16 of them, or little of x, is quantised anew in each workgroup (fp16
 // out, the whole call among others, against the next best form: 2048 x 2048, T = 32 7.6 / 8.5 us, T = 64 10.5 / 8.3;
 // 2048 x 8192, T = 8 7.6 / 8.2, T = 17 12.5 / 8.6; 1024 x 1024, T = 64 6.8 / 8.4).
@@ -513,6 +545,7 @@ static hipError_t linear_mx_epi(MxGemmParams p, DT dt, uint8_t* ws, hipStream_t 
         case MX_THIN22: return mx_thin<EPI, 2, 2>(p, s);
         case MX_THIN44: return mx_thin<EPI, 4, 4>(p, s);
         case MX_MID: return mx_tiles<EPI, MxMid>(p, s);
+        case MX_MIDK: return mx_tiles<EPI, MxMidK>(p, s);
         default: return mx_tiles<EPI, MxBig>(p, s);
     }
 }

@@ -89,11 +89,11 @@ __global__ __launch_bounds__(256) void k_mx_dequantize(E* y, size_t ldy, const u
 
 // codes and scales (row-major) to the operand layout, one wave per (64 rows, k block of 128); the padding is written too
 __global__ __launch_bounds__(256) void k_mx_pack(uint8_t* oc, uint8_t* os, const uint8_t* codes, const uint8_t* scales, int rows,
-                                                 int cols, int kbs, size_t units) {
+                                                 int cols, size_t units) {
     const size_t u = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (u >= units) return;
-    const int lane = threadIdx.x & 63, kb = (int)(u % kbs), k = kb * 128 + 32 * (lane >> 4);
-    const size_t rg = u / kbs;
+    const size_t rgs = mx_rg(rows), rg = u % rgs, kb = u / rgs;
+    const int lane = threadIdx.x & 63, k = (int)kb * 128 + 32 * (lane >> 4);
     uint32_t sc = 0;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -103,9 +103,9 @@ __global__ __launch_bounds__(256) void k_mx_pack(uint8_t* oc, uint8_t* os, const
             c = *reinterpret_cast<const u32x4*>(codes + r * (cols / 2) + k / 2);
             sc |= (uint32_t)scales[r * (cols / 32) + k / 32] << (8 * j);
         }
-        *reinterpret_cast<u32x4*>(oc + ((rg * 4 + j) * kbs + kb) * MX_UNIT + lane * 16) = c;
+        *reinterpret_cast<u32x4*>(oc + ((kb * rgs + rg) * 4 + j) * MX_UNIT + lane * 16) = c;
     }
-    *reinterpret_cast<uint32_t*>(os + (rg * kbs + kb) * MX_SUNIT + lane * 4) = sc;
+    *reinterpret_cast<uint32_t*>(os + (kb * rgs + rg) * MX_SUNIT + lane * 4) = sc;
 }
 
 // The rows of an activation straight to the operand layout: a workgroup takes 64 rows x 128 columns (four units of codes, one
@@ -115,8 +115,8 @@ template <class E, bool VEC>
 __global__ __launch_bounds__(256) void k_mx_quantize_pack(uint8_t* oc, uint8_t* os, const E* x, size_t ldx, int rows, int cols, int kbs) {
     __shared__ __attribute__((aligned(16))) uint32_t lc[4][64][4];  // [row block][operand lane][8 codes]
     __shared__ __attribute__((aligned(16))) uint8_t ls[64][4];                                   // [operand lane][row block]
-    const int kb = blockIdx.x % kbs, q = threadIdx.x & 15, k = kb * 128 + 8 * q;
-    const size_t rg = blockIdx.x / kbs;
+    const size_t rgs = mx_rg(rows), rg = blockIdx.x / kbs, kb = blockIdx.x % kbs;
+    const int q = threadIdx.x & 15, k = (int)kb * 128 + 8 * q;
     MxVals<E, 8> v[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -136,8 +136,8 @@ __global__ __launch_bounds__(256) void k_mx_quantize_pack(uint8_t* oc, uint8_t* 
     }
     __syncthreads();
     const int j = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    *reinterpret_cast<u32x4*>(oc + ((rg * 4 + j) * kbs + kb) * MX_UNIT + lane * 16) = *reinterpret_cast<const u32x4*>(lc[j][lane]);
-    if (j == 0) *reinterpret_cast<uint32_t*>(os + (rg * kbs + kb) * MX_SUNIT + lane * 4) = *reinterpret_cast<const uint32_t*>(ls[lane]);
+    *reinterpret_cast<u32x4*>(oc + ((kb * rgs + rg) * 4 + j) * MX_UNIT + lane * 16) = *reinterpret_cast<const u32x4*>(lc[j][lane]);
+    if (j == 0) *reinterpret_cast<uint32_t*>(os + (kb * rgs + rg) * MX_SUNIT + lane * 4) = *reinterpret_cast<const uint32_t*>(ls[lane]);
 }
 
 static unsigned grid_of(size_t n) { return (unsigned)std::min<size_t>((n + 255) / 256, (size_t)cu_count() * 32); }
@@ -188,10 +188,9 @@ hipError_t launch_mx_dequantize(void* y, DT dt, size_t ldy, const uint8_t* codes
     return dequantize_of<__bf16>(y, ldy, codes, scales, rows, cols, vec, s);
 }
 hipError_t launch_mx_pack(uint8_t* op, const uint8_t* codes, const uint8_t* scales, int rows, int cols, hipStream_t s) {
-    const int kbs = mx_kb(cols);
-    const size_t units = (size_t)((rows + 63) / 64) * kbs;
+    const size_t units = (size_t)mx_rg(rows) * mx_kb(cols);
     hipLaunchKernelGGL(k_mx_pack, dim3((unsigned)((units + 3) / 4)), dim3(256), 0, s, op, op + mx_code_bytes(rows, cols), codes, scales,
-                       rows, cols, kbs, units);
+                       rows, cols, units);
     return hipGetLastError();
 }
 hipError_t launch_mx_quantize_pack(uint8_t* op, const void* x, DT dt, size_t ldx, int rows, int cols, hipStream_t s) {

@@ -3,9 +3,11 @@
 //
 // Operand layout of a [rows, cols] matrix, as the scaled matrix instruction of 16 x 16 x 128 reads it (lane l: row l % 16,
 // k block of 32 l / 16):
-//   codes   [rows / 16][KB][lane 64][16 bytes]   unit (row block, k block of 128): 1 KB, in the instruction's lane order
-//   scales  [rows / 64][KB][lane 64][4 bytes]    byte j: row block 4 (row / 64) + j
-// with rows padded to 64 and KB = ceil(cols / 128). Codes and scales of the padding are 0, so it adds nothing.
+//   codes   [KB][rows / 16][lane 64][16 bytes]   unit (k block of 128, row block): 1 KB, in the instruction's lane order
+//   scales  [KB][rows / 64][lane 64][4 bytes]    byte j: row block 4 (row / 64) + j
+// with rows padded to 64 and KB = ceil(cols / 128). Codes and scales of the padding are 0, so it adds nothing. The k block comes
+// first: workgroups of a product are at about the same k block, and its row blocks side by side lie in all of an L2's channels
+// (with the row block first they were KB kilobytes apart, often in the same few).
 #pragma once
 #include "common.hpp"
 #include "internal.hpp"
@@ -16,6 +18,7 @@ constexpr int MXB = 32;           // values that share a scale
 constexpr int MX_UNIT = 1024;     // bytes of a unit of codes
 constexpr int MX_SUNIT = 256;     // bytes of a unit of scales (64 rows)
 __host__ __device__ inline int mx_kb(int cols) { return (cols + 127) / 128; }
+__host__ __device__ inline int mx_rg(int rows) { return (rows + 63) / 64; }  // groups of 64 rows
 __host__ __device__ inline size_t mx_code_bytes(int rows, int cols) { return (size_t)((rows + 63) / 64) * 4 * mx_kb(cols) * MX_UNIT; }
 __host__ __device__ inline size_t mx_scale_bytes(int rows, int cols) { return (size_t)((rows + 63) / 64) * mx_kb(cols) * MX_SUNIT; }
 
