@@ -70,7 +70,7 @@ int kiln_attn_workspace_release(void);
  * engine/src/kernels.cu:14-58, gpu.h:92-99). While enabled, every entry point records a hipEvent pair
  * on its stream under its category: attention (all attention entry points and the K/V prepare),
  * gemm_tc16 (linear16 and the projections of the fused DiT sections), gemm_fp32, matvec, norm,
- * layernorm, rope, nag, eltwise, w->f16. Not for use under HIP graph capture.
+ * layernorm, rope, nag, eltwise, w->f16, gemm_mxfp4, mxfp4. Not for use under HIP graph capture.
  * ------------------------------------------------------------------------------------------ */
 /* on != 0 starts a new profile (clears the previous one); 0 stops recording. */
 int kiln_prof_enable(int on);

@@ -11,6 +11,7 @@
 
 #include <stdexcept>
 #include <string>
+#include <vector>
 
 #include "../../include/kiln_attn.h"
 
@@ -216,6 +217,91 @@ inline void dit_cross_attention(uint16_t* out, uint16_t* out_neg, int ldo, const
                               n ? n->kv(block) : nullptr, n ? n->real() : 0, n ? n->npad() : 0, nag.scale, nag.tau,
                               nag.alpha, (kiln_stream_t)stream_ref()),
           "cross-attention");
+}
+
+// ---- the attention section over an encoder's states: rotary positions, cross-attention, MXFP4 linear layers ----
+
+// Rotary frequencies and the factor on rotated values, on the host and on the device (kiln_rope_freqs).
+class RopeFreqs {
+   public:
+    explicit RopeFreqs(int rot, double theta = 10000.0, kiln_rope_scaling scaling = KILN_ROPE_NONE, double factor = 1.0,
+                       double trained = 0.0, double slow = 1.0, double fast = 32.0)
+        : rot_(rot), host_(rot > 0 ? rot / 2 : 0) {
+        check(kiln_rope_freqs(host_.data(), &mscale_, rot, theta, scaling, factor, trained, slow, fast), "rope_freqs");
+        if (hipMalloc(&dev_, host_.size() * sizeof(double)) != hipSuccess) throw std::runtime_error("RopeFreqs: hipMalloc failed");
+        if (hipMemcpy(dev_, host_.data(), host_.size() * sizeof(double), hipMemcpyHostToDevice) != hipSuccess) {
+            (void)hipFree(dev_);
+            throw std::runtime_error("RopeFreqs: hipMemcpy failed");
+        }
+    }
+    ~RopeFreqs() { (void)hipFree(dev_); }
+    RopeFreqs(const RopeFreqs&) = delete;
+    RopeFreqs& operator=(const RopeFreqs&) = delete;
+    const double* data() const { return dev_; }
+    const double* host() const { return host_.data(); }
+    int rot() const { return rot_; }
+    float mscale() const { return mscale_; }
+
+   private:
+    int rot_;
+    std::vector<double> host_;
+    double* dev_ = nullptr;
+    float mscale_ = 1.f;
+};
+
+// H heads of Dh per row of x [T, ldx] turn to y [T, ldy] (y = x: in place); pos [T] on the device, or null: pos0 + t.
+inline void rope(void* y, int ldy, const void* x, int ldx, int dtype, int T, int H, int Dh, const RopeFreqs& f, bool interleaved,
+                 const int32_t* pos, int pos0 = 0) {
+    check(kiln_rope(y, ldy, x, ldx, dtype, T, H, Dh, f.rot(), interleaved ? 1 : 0, pos, pos0, f.data(), f.mscale(),
+                    (kiln_stream_t)stream_ref()),
+          "rope");
+}
+
+// B items of Tq queries against Tk encoder states, items one after the other (kiln_cross_attn with item strides T * ld).
+inline void cross_attn(void* out, int ldo, const void* q, int ldq, const void* k, int ldk, const void* v, int ldv, int dtype, int B,
+                       int Tq, int Tk, int Hq, int Hkv, int Dh, float scale, const int32_t* klen = nullptr,
+                       const uint8_t* kmask = nullptr, void* workspace = nullptr, size_t ws_bytes = 0) {
+    check(kiln_cross_attn(out, ldo, (long long)Tq * ldo, q, ldq, (long long)Tq * ldq, k, ldk, (long long)Tk * ldk, v, ldv,
+                          (long long)Tk * ldv, dtype, B, Tq, Tk, Hq, Hkv, Dh, scale, klen, kmask, Tk, workspace, ws_bytes,
+                          (kiln_stream_t)stream_ref()),
+          "cross_attn");
+}
+
+// A linear_mxfp4 weight, owning its device buffer: from plain MXFP4 codes [rows, cols / 2] and scales [rows, cols / 32].
+class Mxfp4Weight {
+   public:
+    Mxfp4Weight(const uint8_t* codes, const uint8_t* scales, int rows, int cols) : rows_(rows), cols_(cols) {
+        const size_t n = kiln_linear_mxfp4_weight_bytes(rows, cols);
+        if (!n || hipMalloc(&p_, n) != hipSuccess) throw std::runtime_error("kiln: MXFP4 weight allocation failed");
+        const int rc = kiln_linear_mxfp4_prepare_weight(p_, codes, scales, rows, cols, (kiln_stream_t)stream_ref());
+        if (rc != KILN_OK) (void)hipFree(p_);
+        check(rc, "linear_mxfp4_prepare_weight");
+    }
+    ~Mxfp4Weight() { (void)hipFree(p_); }
+    Mxfp4Weight(const Mxfp4Weight&) = delete;
+    Mxfp4Weight& operator=(const Mxfp4Weight&) = delete;
+    const uint8_t* data() const { return p_; }
+    int rows() const { return rows_; }
+    int cols() const { return cols_; }
+
+   private:
+    uint8_t* p_ = nullptr;
+    int rows_, cols_;
+};
+
+inline void mxfp4_quantize(uint8_t* codes, uint8_t* scales, const void* x, int dtype, int ldx, int rows, int cols) {
+    check(kiln_mxfp4_quantize(codes, scales, x, dtype, ldx, rows, cols, (kiln_stream_t)stream_ref()), "mxfp4_quantize");
+}
+inline void mxfp4_dequantize(void* y, int dtype, int ldy, const uint8_t* codes, const uint8_t* scales, int rows, int cols) {
+    check(kiln_mxfp4_dequantize(y, dtype, ldy, codes, scales, rows, cols, (kiln_stream_t)stream_ref()), "mxfp4_dequantize");
+}
+// y [T, ldy] (fp32 for F32/Resid, fp16 for F16/Gelu16) from x [T, W.cols()] rows of ldx, workspace
+// kiln_linear_mxfp4_workspace_bytes(T, W.rows(), W.cols()).
+inline void linear_mxfp4(void* y, int ldy, const void* x, int dtype, int ldx, int T, const Mxfp4Weight& W, Epi16 epi,
+                         const float* gate = nullptr, float beta = 0.f, void* workspace = nullptr, size_t ws_bytes = 0) {
+    check(kiln_linear_mxfp4(y, ldy, x, dtype, ldx, T, W.data(), W.rows(), W.cols(), (int)epi, gate, beta, workspace, ws_bytes,
+                            (kiln_stream_t)stream_ref()),
+          "linear_mxfp4");
 }
 
 }  // namespace kiln
