@@ -663,12 +663,12 @@ def _nbytes(workspace, what):
     return workspace.numel() * workspace.element_size()
 
 
-def _rows_ld(t, what):
-    """Row stride of a 2-D tensor whose rows are contiguous (its columns, where there is one row)."""
-    st = t.stride()
-    if len(st) != 2 or (st[1] != 1 and t.shape[1] > 1):
-        raise ValueError(f"{what}: expected a 2-D tensor with contiguous rows, got shape {tuple(t.shape)} strides {st}")
-    return st[0] if t.shape[0] > 1 else t.shape[1]
+def _rows(t, what):
+    """Shape and row stride of a 2-D tensor whose rows are contiguous (the stride of one row is its columns)."""
+    shape, st = t.shape, t.stride()
+    if len(st) != 2 or (st[1] != 1 and shape[1] > 1):
+        raise ValueError(f"{what}: expected a 2-D tensor with contiguous rows, got shape {tuple(shape)} strides {st}")
+    return shape, st[0] if shape[0] > 1 else shape[1]
 
 
 def rope_freqs(rot, theta=10000.0, scaling="none", factor=1.0, trained=0.0, slow=1.0, fast=None, device=None):
@@ -688,9 +688,10 @@ def rope(y, x, H, Dh, freqs, pos=None, pos0=0, interleaved=False, mscale=1.0, st
     """Rotary positions (kiln_rope) of the H heads of Dh in the rows of x [T, H*Dh], into y (y = x: in place); the first
     2 * freqs.numel() dimensions of a head turn. pos: int32 [T], or None for pos0, pos0 + 1, .."""
     dev = _gpu(x, y, freqs, pos)
-    ldx, ldy = _rows_ld(x, "rope: x"), _rows_ld(y, "rope: y")
-    T, W = x.shape
-    if W != H * Dh or y.shape != x.shape or y.dtype != x.dtype:
+    shape, ldx = _rows(x, "rope: x")
+    shape_y, ldy = _rows(y, "rope: y")
+    T, W = shape
+    if W != H * Dh or shape_y != shape or y.dtype is not x.dtype:
         raise ValueError(f"rope: x {tuple(x.shape)} {x.dtype}, y {tuple(y.shape)} {y.dtype} for {H} heads of {Dh}")
     if freqs.element_size() != 8 or not freqs.is_floating_point() or not freqs.is_contiguous():
         raise ValueError("rope: freqs must be a contiguous float64 tensor (rope_freqs)")
@@ -752,8 +753,7 @@ def _mx_plain(codes, scales, rows, cols, what):
 def mxfp4_quantize(x, codes=None, scales=None, stream=None):
     """x [rows, cols] (fp32, fp16 or bf16, cols % 32 == 0) to MXFP4 (kiln_mxfp4_quantize): uint8 codes [rows, cols / 2] and
     scales [rows, cols / 32]."""
-    dev, ldx = _gpu(x, codes, scales), _rows_ld(x, "mxfp4_quantize: x")
-    rows, cols = x.shape
+    dev, (rows, cols), ldx = _gpu(x, codes, scales), *_rows(x, "mxfp4_quantize: x")
     if codes is None or scales is None:
         if codes is not None or scales is not None:
             raise ValueError("mxfp4_quantize: codes and scales go together")
@@ -768,8 +768,7 @@ def mxfp4_quantize(x, codes=None, scales=None, stream=None):
 
 def mxfp4_dequantize(y, codes, scales, stream=None):
     """The values of MXFP4 codes and scales (kiln_mxfp4_dequantize) into y [rows, cols]."""
-    dev, ldy = _gpu(y, codes, scales), _rows_ld(y, "mxfp4_dequantize: y")
-    rows, cols = y.shape
+    dev, (rows, cols), ldy = _gpu(y, codes, scales), *_rows(y, "mxfp4_dequantize: y")
     _mx_plain(codes, scales, rows, cols, "mxfp4_dequantize")
     _launch((_LIB or lib()).kiln_mxfp4_dequantize, dev, stream, y.data_ptr(), _dt3(y), ldy, codes.data_ptr(), scales.data_ptr(), rows, cols)
     return y
@@ -806,10 +805,10 @@ def linear_mxfp4(y, x, w, epi=KILN_EPI_F32, gate=None, beta=0.0, workspace=None,
     bf16, w an Mxfp4Weight, y fp32 (F32, RESID) or fp16 (F16, GELU16). workspace: linear_mxfp4_workspace_bytes; None takes
     one for the call."""
     dev = _gpu(x, y, w.buf, gate, workspace)
-    ldx, ldy = _rows_ld(x, "linear_mxfp4: x"), _rows_ld(y, "linear_mxfp4: y")
     rows, cols = w.shape
-    T = x.shape[0]
-    if x.shape[1] != cols or y.shape != (T, rows):
+    (T, width), ldx = _rows(x, "linear_mxfp4: x")
+    shape_y, ldy = _rows(y, "linear_mxfp4: y")
+    if width != cols or shape_y != (T, rows):
         raise ValueError(f"linear_mxfp4: x {tuple(x.shape)}, y {tuple(y.shape)} for a weight [{rows}, {cols}]")
     if _dt3(y) != (KILN_F32 if epi in (KILN_EPI_F32, KILN_EPI_RESID) else KILN_F16):
         raise ValueError(f"linear_mxfp4: y is {y.dtype} with epilogue {epi}")

@@ -2,6 +2,7 @@
 // layers. Argument checks and dispatch; declarations and contracts: include/kiln_attn.h.
 #include <hip/hip_runtime.h>
 #include <math.h>
+#include <stdlib.h>
 
 #include <algorithm>
 
@@ -110,7 +111,7 @@ int kiln_cross_attn(void* out, int ldo, long long bso, const void* q, int ldq, l
     if (!B || !Tq) return KILN_OK;
     if (!out || !q || (Tk && (!k || !v))) return fail(KILN_EINVAL, "cross_attn: null pointer");
     const long long G = Hq / Hkv, rows = Tq * G;
-    if (rows > MAX_ROWS || Tk > MAX_ROWS || (rows / 16 + 1) * B * Hkv > MAX_ROWS / 256)
+    if (rows > MAX_ROWS || Tk > MAX_ROWS || (rows / 16 + 1) * B * Hkv > MAX_ROWS)
         return fail(KILN_EUNSUPPORTED, "cross_attn: too many rows or keys (B=%d Tq=%d Tk=%d)", B, Tq, Tk);
     const struct {
         const char* name;
@@ -120,11 +121,11 @@ int kiln_cross_attn(void* out, int ldo, long long bso, const void* q, int ldq, l
     } ten[4] = {{"out", out, ldo, Tq, Hq, bso}, {"q", q, ldq, Tq, Hq, bsq}, {"k", k, ldk, Tk, Hkv, bsk}, {"v", v, ldv, Tk, Hkv, bsv}};
     for (const auto& t : ten) {
         if (!ld_ok(t.ld, (long long)t.H * Dh, t.T)) return fail(KILN_EINVAL, "cross_attn: %s row stride %d", t.name, t.ld);
-        if (!aligned(t.p, 16) || (t.T > 1 && t.ld % 8) || (B > 1 && t.bs % 8) || t.ld > (1 << 24))
+        if (!aligned(t.p, 16) || (t.T > 1 && t.ld % 8) || (B > 1 && t.bs % 8) || (t.T > 1 && t.ld > (1 << 24)))
             return fail(KILN_EUNSUPPORTED, "cross_attn: %s rows not 16-byte aligned, or more than 2^24 elements apart", t.name);
     }
     if (!aligned(klen, 4)) return fail(KILN_EUNSUPPORTED, "cross_attn: klen not aligned");
-    if (B > 1 && std::llabs(bso) < (long long)Hq * Dh) return fail(KILN_EINVAL, "cross_attn: items' outputs overlap (bso %lld)", bso);
+    if (B > 1 && llabs(bso) < (long long)Hq * Dh) return fail(KILN_EINVAL, "cross_attn: items' outputs overlap (bso %lld)", bso);
     if (workspace && !aligned(workspace, 16)) return fail(KILN_EUNSUPPORTED, "cross_attn: workspace not 16-byte aligned");
     kiln::CrossLaunch c{};
     c.out = out;

@@ -163,6 +163,13 @@ def test_nonfinite_states_propagate(gpu):
     assert torch.equal(torch.isnan(out), want)
 
 
+def test_strides_of_single_rows(gpu):
+    """One query and one state: their row strides mean nothing, however large or odd."""
+    q, k, v = make(2, 1, 1, 2, 2, 64, torch.float16)
+    odd = lambda t: t.as_strided(t.shape, (t.stride(0), (1 << 30) + 3, 1))  # noqa: E731
+    assert torch.equal(ka.cross_attn(torch.empty_like(q), odd(q), odd(k), odd(v), 2), v)
+
+
 def test_no_keys_at_all(gpu):
     q = torch.randn(2, 3, 128, device=DEV).half()
     k = torch.empty(2, 0, 128, device=DEV, dtype=torch.float16)
