@@ -105,7 +105,7 @@ struct XCfg {
     static constexpr int BITS = NW * 32 * 4;                           // each wave's mask windows: 2 x 16 words
     static constexpr int MERGE = !SHARED && NW > 1 ? NW * RW * (DH + 2) * 4 : 0;
     static constexpr int LDS = (RINGS > MERGE ? RINGS : MERGE) + BITS;
-    static constexpr int WAVES = QB == 1 && LDS <= 40 * 1024 ? 4 : LDS <= 80 * 1024 || NW == 1 || NW == 8 ? 2 : 1;  // per SIMD that registers have to allow
+    static constexpr int WAVES = QB == 1 && NW > 1 && LDS <= 40 * 1024 ? 4 : LDS <= 80 * 1024 || NW == 1 || NW == 8 ? 2 : 1;  // per SIMD that registers have to allow
 };
 
 template <class E, class C, bool MASK>
@@ -135,11 +135,14 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_cross_attn(const Cross
     uint32_t* bits = reinterpret_cast<uint32_t*>(xlds + C::LDS - C::BITS) + wv * 32;
 
     // The keys of tile j < t1 as bits. With a mask: windows of 16 tiles (512 keys) in LDS, two of them, each wave its own.
-    auto fill_window = [&](int w) {  // window w of this wave's tiles: tiles t0 + 16 w ..
+    auto fill_window = [&](int w) {  // window w of this wave's tiles: tiles t0 + 16 w .., at least one key
+        const long long key0 = (long long)(t0 + 16 * w) * XKT + lane;
+        uint8_t byte[8];  // all loads before the first is looked at
+#pragma unroll
+        for (int i = 0; i < 8; i++) byte[i] = mask[min(key0 + 64 * i, (long long)L - 1)];
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const long long key = (long long)(t0 + 16 * w) * XKT + 64 * i + lane;
-            const unsigned long long m = __ballot(key < L && mask[key < L ? key : 0] != 0);
+            const unsigned long long m = __ballot((byte[i] != 0) & (key0 + 64 * i < L));
             if (lane == i) *reinterpret_cast<unsigned long long*>(bits + (w & 1) * 16 + 2 * i) = m;
         }
         __builtin_amdgcn_wave_barrier();
@@ -151,7 +154,7 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_cross_attn(const Cross
     };
 
     // DMA of the tiles' K and V in turn: a thread's pieces are chunks of fixed rows of a tile; the descriptor's range ends with
-    // the item's last row (empty past the last tile), and a masked row's offset is beyond every range
+    // the item's last row (empty past the last tile), and a masked V row's offset is beyond every range
     struct Stream {
         const uint8_t* src;     // the next tile to copy
         uint32_t ld2;           // bytes from row to row
@@ -171,12 +174,15 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_cross_attn(const Cross
         kst.off[i] = r * kst.ld2 + k_swz<DH>(c, r) * 16;
         vst.off[i] = r * vst.ld2 + v_swz<DH>(c, r) * 16;
     }
-    auto copy = [&](Stream& t, uint32_t at, bool first) {  // first: the stream that comes to a tile first, and reads its mask
+    // V's copies leave masked rows out; K's need not: a masked key's score is replaced, whatever it came to. So the first K tiles
+    // are under way while the mask is read.
+    auto copy = [&](Stream& t, uint32_t at, auto masked) {
+        constexpr bool M_ = decltype(masked)::value;
         uint32_t m = ~0u;
         const int left = t.j < t1 ? min(XKT, L - t.j * XKT) : 0;
-        if constexpr (MASK) {
+        if constexpr (M_) {
             if (left > 0) {
-                if (first && ((t.j - t0) & 15) == 0) fill_window((t.j - t0) >> 4);
+                if (((t.j - t0) & 15) == 0) fill_window((t.j - t0) >> 4);
                 m = tile_bits(t.j);
             }
         }
@@ -186,12 +192,12 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_cross_attn(const Cross
 #pragma unroll
         for (int i = 0; i < C::DMA; i++)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(dst + i * C::RTHREADS * 16), 16,
-                                                     !MASK || (m >> prow[i] & 1) ? t.off[i] : 0x7ffffff0u, 0, 0, 0);
+                                                     !M_ || (m >> prow[i] & 1) ? t.off[i] : 0x7ffffff0u, 0, 0, 0);
         if (t.j + 1 < t1) t.src += (size_t)XKT * t.ld2;
         t.j++;
     };
-    auto copy_k = [&](int stage) { copy(kst, stage * C::STAGE, true); };
-    auto copy_v = [&](int stage) { copy(vst, stage * C::STAGE + C::TILE, false); };
+    auto copy_k = [&](int stage) { copy(kst, stage * C::STAGE, std::false_type{}); };
+    auto copy_v = [&](int stage) { copy(vst, stage * C::STAGE + C::TILE, std::integral_constant<bool, MASK>{}); };
 
     // Q: the B operands of S^T, lane (row c16, chunk 4 cc + g); rows past the last read row 0 and are not stored
     const int row0 = rt * C::RT + (C::SHARED ? wv * C::RW : 0);
@@ -494,6 +500,12 @@ __global__ __launch_bounds__(256) void k_cross_merge(const CrossParams p, int RT
     const int n = ((L + XKT - 1) / XKT + p.ct - 1) / p.ct;  // the item's ranges
     const float* ml = p.part + (size_t)p.total * RT * DH;
     const size_t at0 = ((bh * p.ksplit) * p.rtiles + rt) * RT + rl, step = (size_t)p.rtiles * RT;
+    const int gr = tid / (DH / 4), d = tid % (DH / 4);
+    const float* src = p.part + at0 * DH + 4 * d;
+    floatx4 ahead[4];  // a group's first ranges, under way while the factors are found
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        ahead[i] = gr + i * GR < n ? *reinterpret_cast<const floatx4*>(src + (gr + i * GR) * step * DH) : floatx4{0.f, 0.f, 0.f, 0.f};
     float2 e = make_float2(-INFINITY, 0.f);
     if (tid < n) e = *reinterpret_cast<const float2*>(ml + (at0 + tid * step) * 2);
     float mm = e.x;
@@ -510,10 +522,12 @@ __global__ __launch_bounds__(256) void k_cross_merge(const CrossParams p, int RT
     if (lane == 0) red[4 + wv] = ll;
     __syncthreads();
     ll = (red[4] + red[5]) + (red[6] + red[7]);
-    const int gr = tid / (DH / 4), d = tid % (DH / 4);
     floatx4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (gr + i * GR < n) acc += fac[gr + i * GR] * ahead[i];
 #pragma unroll 4
-    for (int k = gr; k < n; k += GR) acc += fac[k] * *reinterpret_cast<const floatx4*>(p.part + (at0 + k * step) * DH + 4 * d);
+    for (int k = gr + 4 * GR; k < n; k += GR) acc += fac[k] * *reinterpret_cast<const floatx4*>(src + k * step * DH);
     acc_s[gr][d] = acc;
     __syncthreads();
     if (tid >= DH / 4) return;
