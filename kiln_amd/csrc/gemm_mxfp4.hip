@@ -256,32 +256,28 @@ static hipError_t mx_thin(MxGemmParams p, hipStream_t s) {
 //
 // WN x WM waves of 16 NB x 16 MB blocks. A stage of the LDS ring holds one k block of 128: the tile's units of W and of x
 // (1 KB each) and their scales, all by LDS DMA in the operand layout, so that every operand read is 1 KB without conflicts.
-// KG groups of such waves with a ring each take every KG th k block; their sums meet in LDS, in the groups' order.
-template <int WN_, int WM_, int NB_, int MB_, int KG_, int NST_, int WGS_>
+template <int WN_, int WM_, int NB_, int MB_, int NST_, int WGS_>
 struct MxCfg {
-    static constexpr int WN = WN_, WM = WM_, NB = NB_, MB = MB_, KG = KG_, NST = NST_, WGS = WGS_, WAVES = WN * WM;
-    static constexpr int THREADS = WAVES * KG * 64;
+    static constexpr int WN = WN_, WM = WM_, NB = NB_, MB = MB_, NST = NST_, WGS = WGS_, WAVES = WN * WM, THREADS = WAVES * 64;
     static constexpr int BN = WN * NB * 16, BM = WM * MB * 16;
     static constexpr int UN = BN / 16, UM = BM / 16, SN = (BN + 63) / 64, SM = (BM + 63) / 64;
     static constexpr int CODE_DMA = (UN + UM) / WAVES, SCALE_DMA = (SN + SM + WAVES - 1) / WAVES, DPS = CODE_DMA + SCALE_DMA;
-    static constexpr int SC_OFF = (UN + UM) * MX_UNIT, STAGE = SC_OFF + (SN + SM) * MX_SUNIT, RING = NST * STAGE, LDS = KG * RING;
+    static constexpr int SC_OFF = (UN + UM) * MX_UNIT, STAGE = SC_OFF + (SN + SM) * MX_SUNIT, LDS = NST * STAGE;
     static_assert((UN + UM) % WAVES == 0 && NB % 4 == 0 && MB % 4 == 0 && LDS * WGS <= 160 * 1024, "tile");
 };
 
 template <int EPI, class C>
-__global__ __launch_bounds__(C::THREADS, C::WAVES * C::KG * C::WGS / 4) void k_mx_gemm(const MxGemmParams p) {
+__global__ __launch_bounds__(C::THREADS, C::WAVES * C::WGS / 4) void k_mx_gemm(const MxGemmParams p) {
 #ifdef __HIP_DEVICE_COMPILE__  // the host pass only needs the kernel's handle
     extern __shared__ __attribute__((aligned(16))) uint8_t lds8[];
-    constexpr int NB = C::NB, MB = C::MB, KG = C::KG;
+    constexpr int NB = C::NB, MB = C::MB;
     // blocks go round the 8 XCDs: each takes a contiguous range of tiles, in groups of row tiles that share W in its L2
     const int ti = (int)(blockIdx.x & 7) * p.per + (int)(blockIdx.x >> 3);
     if (ti >= p.total) return;
     int tm, tn;
     raster_tile(ti, 4, p.tiles_m, p.tiles_n, tm, tn);
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int kg = wave / C::WAVES, wv = wave % C::WAVES, wn = wv % C::WN, wm = wv / C::WN;
-    const int steps = (p.kbs + KG - 1) / KG;  // the group's k blocks: kg, kg + KG, .. (a last one past the end is not multiplied)
-    uint8_t* ring = lds8 + kg * C::RING;
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wn = wv % C::WN, wm = wv / C::WN;
     const int wrg = mx_rg(p.N), xrg = mx_rg(p.T);  // row groups that exist
 
     // DMA pieces of this wave: units wv, wv + WAVES, .. of the stage (W's first), then the scale units; row blocks past the
@@ -309,8 +305,8 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES * C::KG * C::WGS / 4) void k_m
     }
     typedef const __attribute__((address_space(1))) void* glb_p;
     auto dma_piece = [&](int i, int step, int stage) {
-        const size_t kb = min(step * KG + kg, p.kbs - 1);
-        uint8_t* base = ring + stage * C::STAGE;
+        const size_t kb = min(step, p.kbs - 1);
+        uint8_t* base = lds8 + stage * C::STAGE;
         if (i < C::CODE_DMA)
             __builtin_amdgcn_global_load_lds((glb_p)(src[i] + kb * kstep[i] * MX_UNIT), (lds_p)(base + (wv + i * C::WAVES) * MX_UNIT), 16, 0, 0);
         else if (i < C::DPS)
@@ -322,7 +318,7 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES * C::KG * C::WGS / 4) void k_m
         for (int i = 0; i < C::DPS; i++) dma_piece(i, step, stage);
     };
 
-    const uint32_t lds_base = (uint32_t)(size_t)(__attribute__((address_space(3))) uint8_t*)ring;
+    const uint32_t lds_base = (uint32_t)(size_t)(__attribute__((address_space(3))) uint8_t*)lds8;
     floatx4 acc[NB][MB];
 #pragma unroll
     for (int nb = 0; nb < NB; nb++)
@@ -361,15 +357,13 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES * C::KG * C::WGS / 4) void k_m
         wait_vmcnt<(C::NST - 3) * C::DPS>();
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
-        const bool real = KG == 1 || i * KG + kg < p.kbs;
         const int ds = next >= 2 ? next - 2 : next - 2 + C::NST;
         const uint32_t st = next * C::STAGE;
 #pragma unroll
         for (int mb = 0; mb < MB; mb++) {
-            if (real)
 #pragma unroll
-                for (int nb = 0; nb < NB; nb++)
-                    acc[nb][mb] = mx_mfma_at(nb & 3, mb & 3, fw[cur][nb], sw[cur][nb / 4], fx[mb], sx[cur][mb / 4], acc[nb][mb]);
+            for (int nb = 0; nb < NB; nb++)
+                acc[nb][mb] = mx_mfma_at(nb & 3, mb & 3, fw[cur][nb], sw[cur][nb / 4], fx[mb], sx[cur][mb / 4], acc[nb][mb]);
             __builtin_amdgcn_sched_barrier(0);
             read_x(mb, st);
             if (mb == 0) {
@@ -392,30 +386,12 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES * C::KG * C::WGS / 4) void k_m
         next = next == C::NST - 1 ? 0 : next + 1;
     };
     int i = 0;
-    for (; i + 2 <= steps; i += 2) {
+    for (; i + 2 <= p.kbs; i += 2) {
         step(i, std::integral_constant<int, 0>{});
         step(i + 1, std::integral_constant<int, 1>{});
     }
-    if (i < steps) step(i, std::integral_constant<int, 0>{});
+    if (i < p.kbs) step(i, std::integral_constant<int, 0>{});
     wait_vmcnt<0>();  // no copy into LDS outlives the ring
-    if constexpr (KG > 1) {
-        floatx4* red = reinterpret_cast<floatx4*>(lds8);  // [group - 1][wave][block][lane]
-        static_assert((KG - 1) * C::WAVES * NB * MB * 1024 <= C::LDS, "the groups' sums fit in the rings");
-        __syncthreads();  // every wave is done with the rings
-        if (kg)
-#pragma unroll
-            for (int nb = 0; nb < NB; nb++)
-#pragma unroll
-                for (int mb = 0; mb < MB; mb++) red[((((kg - 1) * C::WAVES + wv) * NB + nb) * MB + mb) * 64 + lane] = acc[nb][mb];
-        __syncthreads();
-        if (kg) return;
-#pragma unroll
-        for (int k = 0; k < KG - 1; k++)
-#pragma unroll
-            for (int nb = 0; nb < NB; nb++)
-#pragma unroll
-                for (int mb = 0; mb < MB; mb++) acc[nb][mb] += red[(((k * C::WAVES + wv) * NB + nb) * MB + mb) * 64 + lane];
-    }
     const int g = lane >> 4, rl = lane & 15;
     const int m0 = tm * C::BM + wm * MB * 16, n0 = tn * C::BN + wn * NB * 16;
     if (p.vec < 2) {
@@ -432,7 +408,7 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES * C::KG * C::WGS / 4) void k_m
     static_assert(RB * 16 * CH * 16 * C::WAVES <= C::LDS, "the waves' regions fit in the ring");
     uint8_t* stg = lds8 + wv * (RB * 16 * CH * 16);
     __builtin_amdgcn_s_waitcnt(0xC07F);
-    __builtin_amdgcn_s_barrier();  // every wave (of the last group) is done with the ring, or with the sums in it
+    __builtin_amdgcn_s_barrier();  // every wave is done with the ring
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int h = 0; h < MB / RB; h++) {
@@ -476,9 +452,8 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES * C::KG * C::WGS / 4) void k_m
 #endif
 }
 
-using MxBig = MxCfg<4, 2, 4, 8, 1, 4, 1>;    // 256 x 256 (n x m), 8 waves, 136 KB
-using MxMid = MxCfg<2, 2, 4, 4, 1, 4, 2>;    // 128 x 128, 4 waves, 68 KB
-using MxMidK = MxCfg<2, 2, 4, 4, 2, 4, 1>;   // 128 x 128, two groups of 4 waves, 136 KB
+using MxBig = MxCfg<4, 2, 4, 8, 4, 1>;  // 256 x 256 (n x m), 8 waves, 136 KB
+using MxMid = MxCfg<2, 2, 4, 4, 4, 2>;  // 128 x 128, 4 waves, 68 KB
 
 template <int EPI, class C>
 static hipError_t mx_tiles(MxGemmParams p, hipStream_t s) {
@@ -503,7 +478,7 @@ static hipError_t mx_few(const MxGemmParams& p, hipStream_t s) {
 }
 
 // The form of a product.
-enum MxKind { MX_FEW, MX_THIN22, MX_THIN44, MX_MID, MX_BIG, MX_MIDK };
+enum MxKind { MX_FEW, MX_THIN22, MX_THIN44, MX_MID, MX_BIG };
 // Few rows quantise in the product, one launch: as long as 16 of them, or little of x, is quantised anew in each workgroup (fp16
 // out, the whole call among others, against the next best form: 2048 x 2048, T = 32 7.6 / 8.5 us, T = 64 10.5 / 8.3;
 // 2048 x 8192, T = 8 7.6 / 8.2, T = 17 12.5 / 8.6; 1024 x 1024, T = 64 6.8 / 8.4).
@@ -545,7 +520,6 @@ static hipError_t linear_mx_epi(MxGemmParams p, DT dt, uint8_t* ws, hipStream_t 
         case MX_THIN22: return mx_thin<EPI, 2, 2>(p, s);
         case MX_THIN44: return mx_thin<EPI, 4, 4>(p, s);
         case MX_MID: return mx_tiles<EPI, MxMid>(p, s);
-        case MX_MIDK: return mx_tiles<EPI, MxMidK>(p, s);
         default: return mx_tiles<EPI, MxBig>(p, s);
     }
 }
