@@ -53,7 +53,7 @@ __device__ __forceinline__ floatx4 mx_mfma_at(int j, int i, u32x4 a, uint32_t sa
 // polynomial of degree 7 with the least largest error on [0, 6] (2^-18.2 of Phi; below 2^-17 with fp32's roundings), decreasing
 // beyond, where |v| Phi(-|v|) < 2^-27 is nothing to fp16. Relative to GELU itself the error is no larger (Phi(-z) <= 1/2), a
 // hundredth of the fp16 rounding that follows. 10 operations and one exp against erfc's 17, a reciprocal and an exp: the GELU
-// of 6912 x 8192 outputs, which nothing overlaps, takes 21 us instead of 40. -inf gives 0, inf inf, NaN NaN.
+// of 6912 x 8192 outputs takes some 24 us instead of 40. -inf gives 0, inf inf, NaN NaN.
 __device__ __forceinline__ float mx_gelu(float v) {
     const float z = fabsf(v);
     float q = -1.83525563e-6f;
@@ -109,7 +109,8 @@ __device__ __forceinline__ void mx_store(const MxGemmParams& p, int m, int n, fl
 //
 // Eight waves share out the k blocks; each quantises its part of x in registers (a lane of the operand layout holds exactly
 // one block of 32) and reads its units of the weight, 1 KB each, straight from memory. The waves' sums meet in LDS.
-// Bound by the weight's bytes and, at these sizes, by the launch: one launch, no workspace.
+// Bound by the latency of two dependent loads and the launch: one launch, no workspace. 1 row x 8192 x 2048 with GELU, 9 MB, in 5.4 us
+// (an empty launch is 2.2, the bytes 1.7).
 constexpr int FEW_WAVES = 8;
 template <class E, int EPI, int MB, bool VEC>
 __global__ __launch_bounds__(FEW_WAVES * 64) void k_mx_few(const MxGemmParams p) {
@@ -182,7 +183,7 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void k_mx_few(const MxGemmParams p)
 //
 // A workgroup takes 16 NB weight rows x 16 MB rows of x; its eight waves share out the k blocks, each reading whole 1 KB units
 // of both operands (from L2) two k blocks ahead of their products, and meet in LDS. No ring to fill: what bounds it at these sizes
-// is the latency of a few loads, then L2's rate.
+// is the latency of a few loads, then L2's rate. 64 x 2048 x 8192 in 9.7 us with its quantise pass (128 x 128 tiles: 21.3).
 constexpr int THIN_WAVES = 8;
 template <int EPI, int NB, int MB>
 __global__ __launch_bounds__(THIN_WAVES * 64, 2) void k_mx_thin(const MxGemmParams p) {
@@ -256,6 +257,14 @@ static hipError_t mx_thin(MxGemmParams p, hipStream_t s) {
 //
 // WN x WM waves of 16 NB x 16 MB blocks. A stage of the LDS ring holds one k block of 128: the tile's units of W and of x
 // (1 KB each) and their scales, all by LDS DMA in the operand layout, so that every operand read is 1 KB without conflicts.
+//
+// 256 x 256 (8 waves of 64 x 128): 8192^3 in 282 us with its quantise pass (25), 4.3 PFLOP/s; the matrix instructions alone, random operands
+// in registers, reach 6.9 on this chip (2.4 GHz gives way to 1.7 under the power limit, 9.3 on zeros), so that whatever else costs
+// energy costs time: three 1 KB operand reads per 8 products (four waves of 128 x 128 would need two, but their registers spill
+// into moves: 40% slower), the GELU, the stores. 6912 x 8192 x 2048 takes 76 us, with GELU 98. Two workgroups of 128 x 256 per CU
+// (one's epilogue beside the other's products, in step or staggered) measured the same.
+// 128 x 128 (4 waves of 64 x 64): bound by what a CU takes in, 57 GB/s while its lines come from beyond the L2, whatever the ring's
+// depth (4 to 9 stages) or the number of waves: 0.3 us for the 17 KB of a k block. 1537 x 2048 x 2048 in 10.4 us, fp32 out 12.3.
 template <int WN_, int WM_, int NB_, int MB_, int NST_, int WGS_>
 struct MxCfg {
     static constexpr int WN = WN_, WM = WM_, NB = NB_, MB = MB_, NST = NST_, WGS = WGS_, WAVES = WN * WM, THREADS = WAVES * 64;
@@ -284,16 +293,16 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES * C::WGS / 4) void k_mx_gemm(c
     // matrix re-read its last one (their results are not stored)
     typedef __attribute__((address_space(3))) void* lds_p;
     const uint8_t* src[C::CODE_DMA];
-    uint32_t kstep[C::CODE_DMA];  // units from a k block to the next
+    size_t kstep[C::CODE_DMA];  // bytes from a k block to the next
 #pragma unroll
     for (int i = 0; i < C::CODE_DMA; i++) {
         const int u = wv + i * C::WAVES;
         src[i] = (u < C::UN ? p.wc + (size_t)min(tn * C::UN + u, 4 * wrg - 1) * MX_UNIT
                             : p.xc + (size_t)min(tm * C::UM + u - C::UN, 4 * xrg - 1) * MX_UNIT) + lane * 16;
-        kstep[i] = 4 * (u < C::UN ? wrg : xrg);
+        kstep[i] = (size_t)4 * MX_UNIT * (u < C::UN ? wrg : xrg);
     }
     const uint8_t* ssrc[C::SCALE_DMA];
-    uint32_t skstep[C::SCALE_DMA];
+    size_t skstep[C::SCALE_DMA];
     int sdst[C::SCALE_DMA];
 #pragma unroll
     for (int i = 0; i < C::SCALE_DMA; i++) {
@@ -301,21 +310,23 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES * C::WGS / 4) void k_mx_gemm(c
         sdst[i] = C::SC_OFF + u * MX_SUNIT;
         ssrc[i] = (u < C::SN ? p.ws + (size_t)min(tn * C::BN / 64 + u, wrg - 1) * MX_SUNIT
                              : p.xs + (size_t)min(tm * C::BM / 64 + u - C::SN, xrg - 1) * MX_SUNIT) + lane * 4;
-        skstep[i] = u < C::SN ? wrg : xrg;
+        skstep[i] = (size_t)MX_SUNIT * (u < C::SN ? wrg : xrg);
     }
     typedef const __attribute__((address_space(1))) void* glb_p;
-    auto dma_piece = [&](int i, int step, int stage) {
-        const size_t kb = min(step, p.kbs - 1);
+    // piece i of the next k block to copy (`more`: there is one after it; past the end the last one again)
+    auto dma_piece = [&](int i, bool more, int stage) {
         uint8_t* base = lds8 + stage * C::STAGE;
-        if (i < C::CODE_DMA)
-            __builtin_amdgcn_global_load_lds((glb_p)(src[i] + kb * kstep[i] * MX_UNIT), (lds_p)(base + (wv + i * C::WAVES) * MX_UNIT), 16, 0, 0);
-        else if (i < C::DPS)
-            __builtin_amdgcn_global_load_lds((glb_p)(ssrc[i - C::CODE_DMA] + kb * skstep[i - C::CODE_DMA] * MX_SUNIT),
-                                             (lds_p)(base + sdst[i - C::CODE_DMA]), 4, 0, 0);
+        if (i < C::CODE_DMA) {
+            __builtin_amdgcn_global_load_lds((glb_p)src[i], (lds_p)(base + (wv + i * C::WAVES) * MX_UNIT), 16, 0, 0);
+            src[i] += more ? kstep[i] : 0;
+        } else if (i < C::DPS) {
+            __builtin_amdgcn_global_load_lds((glb_p)ssrc[i - C::CODE_DMA], (lds_p)(base + sdst[i - C::CODE_DMA]), 4, 0, 0);
+            ssrc[i - C::CODE_DMA] += more ? skstep[i - C::CODE_DMA] : 0;
+        }
     };
     auto dma = [&](int step, int stage) {
 #pragma unroll
-        for (int i = 0; i < C::DPS; i++) dma_piece(i, step, stage);
+        for (int i = 0; i < C::DPS; i++) dma_piece(i, step + 1 < p.kbs, stage);
     };
 
     const uint32_t lds_base = (uint32_t)(size_t)(__attribute__((address_space(3))) uint8_t*)lds8;
@@ -325,7 +336,8 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES * C::WGS / 4) void k_mx_gemm(c
 #pragma unroll
         for (int mb = 0; mb < MB; mb++) acc[nb][mb] = floatx4{0.f, 0.f, 0.f, 0.f};
 
-    u32x4 fw[2][NB], fx[MB];
+    constexpr int XB = MB <= 4 ? 2 : 1;  // x's operands double where the registers hold them, read ahead like W's
+    u32x4 fw[2][NB], fx[XB][MB];
     uint32_t sw[2][NB / 4], sx[2][MB / 4];
     const uint32_t wa = lds_base + wn * NB * MX_UNIT + lane * 16, xa = lds_base + (C::UN + wm * MB) * MX_UNIT + lane * 16;
     const uint32_t swa = lds_base + C::SC_OFF + wn * NB / 4 * MX_SUNIT + lane * 4;
@@ -338,7 +350,7 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES * C::WGS / 4) void k_mx_gemm(c
 #pragma unroll
         for (int i = 0; i < MB / 4; i++) sx[b][i] = *reinterpret_cast<const lds_u32*>((size_t)(sxa + st + i * MX_SUNIT));
     };
-    auto read_x = [&](int mb, uint32_t st) { fx[mb] = *reinterpret_cast<const lds_u32x4*>((size_t)(xa + st + mb * MX_UNIT)); };
+    auto read_x = [&](int b, int mb, uint32_t st) { fx[b & (XB - 1)][mb] = *reinterpret_cast<const lds_u32x4*>((size_t)(xa + st + mb * MX_UNIT)); };
 
 #pragma unroll
     for (int s = 0; s < C::NST - 1; s++) dma(s, s);
@@ -347,11 +359,11 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES * C::WGS / 4) void k_mx_gemm(c
     __builtin_amdgcn_sched_barrier(0);
     read_w(0, 0);
 #pragma unroll
-    for (int mb = 0; mb < MB; mb++) read_x(mb, 0);
+    for (int mb = 0; mb < MB; mb++) read_x(0, mb, 0);
     int next = 1;  // the stage of step i + 1
     // Step i: its operands are in registers. Those of step i + 1 landed in every wave; the stage of step i - 1, whose reads every
     // wave finished before its products of i - 1, is refilled (past the end with the last block again: the count of loads
-    // in flight stays the same). The operands of i + 1 are read between the products of i, x's into the registers that are done.
+    // in flight stays the same). The operands of i + 1 are read between the products of i.
     auto step = [&](int i, auto tag) {
         constexpr int cur = decltype(tag)::value;
         wait_vmcnt<(C::NST - 3) * C::DPS>();
@@ -363,9 +375,13 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES * C::WGS / 4) void k_mx_gemm(c
         for (int mb = 0; mb < MB; mb++) {
 #pragma unroll
             for (int nb = 0; nb < NB; nb++)
-                acc[nb][mb] = mx_mfma_at(nb & 3, mb & 3, fw[cur][nb], sw[cur][nb / 4], fx[mb], sx[cur][mb / 4], acc[nb][mb]);
+                acc[nb][mb] = mx_mfma_at(nb & 3, mb & 3, fw[cur][nb], sw[cur][nb / 4], fx[cur & (XB - 1)][mb], sx[cur][mb / 4], acc[nb][mb]);
             __builtin_amdgcn_sched_barrier(0);
-            read_x(mb, st);
+            if (XB == 1) read_x(0, mb, st);
+            else if (mb < MB / 2) {
+                read_x(cur ^ 1, 2 * mb, st);
+                read_x(cur ^ 1, 2 * mb + 1, st);
+            }
             if (mb == 0) {
 #pragma unroll
                 for (int u = 0; u < NB / 4; u++) sw[cur ^ 1][u] = *reinterpret_cast<const lds_u32*>((size_t)(swa + st + u * MX_SUNIT));
@@ -380,7 +396,7 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES * C::WGS / 4) void k_mx_gemm(c
                 }
             }
 #pragma unroll
-            for (int n = 0; n < (C::DPS + MB - 1) / MB; n++) dma_piece(mb * ((C::DPS + MB - 1) / MB) + n, i + C::NST - 1, ds);
+            for (int n = 0; n < (C::DPS + MB - 1) / MB; n++) dma_piece(mb * ((C::DPS + MB - 1) / MB) + n, i + C::NST < p.kbs, ds);
             __builtin_amdgcn_sched_barrier(0);
         }
         next = next == C::NST - 1 ? 0 : next + 1;
@@ -495,7 +511,7 @@ static MxKind mx_choose(int T, int N, int K) {
     const double cus = cu_count(), kb = mx_kb(K);
     auto tiles = [&](int bn, int bm) { return (double)((N + bn - 1) / bn) * ((T + bm - 1) / bm); };
     const double t22 = tiles(32, 32), t44 = tiles(64, 64), tm = tiles(128, 128), tb = tiles(256, 256);
-    const double cost[4] = {0.8 + 0.01 * kb + 0.056 * kb * t22 / cus,
+    const double cost[4] = {0.8 + 0.01 * kb + (0.25 + 0.05 * kb) * t22 / cus,
                             ceil(t44 / cus) * (1.2 + 0.045 * kb) + 0.125 * kb * t44 / cus,
                             1.9 * std::max(1.0, tm / cus) + kb * (0.155 + 0.22 * tm / cus),
                             ceil(tb / cus) * (5.0 + 0.55 * kb) + 0.35 * kb * tb / cus};
