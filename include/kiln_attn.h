@@ -406,6 +406,9 @@ int kiln_cross_attn(void* out, int ldo, long long bso, const void* q, int ldq, l
                     const void* v, int ldv, long long bsv, int dtype, int B, int Tq, int Tk, int Hq, int Hkv, int Dh, float scale,
                     const int32_t* klen, const uint8_t* kmask, long long bsm, void* workspace, size_t ws_bytes, kiln_stream_t stream);
 size_t kiln_cross_attn_workspace_bytes(int B, int Tq, int Tk, int Hq, int Hkv, int Dh);
+/* Which form a call with that workspace runs, for tests and profiles: query rows (Tq Hq / Hkv) of a workgroup << 16 | waves that split
+ * the keys within it << 8 | whether the keys are split over workgroups; 0 for sizes that the call refuses. */
+int kiln_cross_attn_form(int B, int Tq, int Tk, int Hq, int Hkv, int Dh);
 
 /* MXFP4: the values of a row in blocks of 32 neighbours. A block's scale byte s stands for 2^(s - 127), s - 127 being
  * floor(log2(largest magnitude)) - 2 (not below -127); a value is a 4-bit code, bit 3 the sign and bits 0-2 one of 0, 0.5, 1,
@@ -428,6 +431,9 @@ int kiln_mxfp4_dequantize(void* y, int dtype, int ldy, const uint8_t* codes, con
 size_t kiln_linear_mxfp4_weight_bytes(int rows, int cols);
 int kiln_linear_mxfp4_prepare_weight(uint8_t* wp, const uint8_t* codes, const uint8_t* scales, int rows, int cols, kiln_stream_t stream);
 size_t kiln_linear_mxfp4_workspace_bytes(int T, int rows, int cols);
+/* Which tile a call of these sizes runs on, for tests and profiles (weight rows << 16 | rows of x; 16 weight rows: the form that
+ * quantises x itself); 0 for sizes that the call refuses. */
+int kiln_linear_mxfp4_tile(int T, int rows, int cols);
 int kiln_linear_mxfp4(void* y, int ldy, const void* x, int dtype, int ldx, int T, const uint8_t* wp, int rows, int cols, int epi,
                       const float* gate, float beta, void* workspace, size_t ws_bytes, kiln_stream_t stream);
 

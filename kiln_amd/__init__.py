@@ -102,6 +102,8 @@ _SIGS = {
     "kiln_cross_attn": (_i, [_vp, _i, _ll, _vp, _i, _ll, _vp, _i, _ll, _vp, _i, _ll, _i, _i, _i, _i, _i, _i, _i, _f, _vp,
                              _vp, _ll, _vp, _sz, _vp]),
     "kiln_cross_attn_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),
+    "kiln_cross_attn_form": (_i, [_i, _i, _i, _i, _i, _i]),
+    "kiln_linear_mxfp4_tile": (_i, [_i, _i, _i]),
     "kiln_mxfp4_quantize": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _vp]),
     "kiln_mxfp4_dequantize": (_i, [_vp, _i, _i, _vp, _vp, _i, _i, _vp]),
     "kiln_linear_mxfp4_weight_bytes": (_sz, [_i, _i]),
@@ -706,6 +708,13 @@ def cross_attn_workspace_bytes(B, Tq, Tk, Hq, Hkv, Dh):
     return lib().kiln_cross_attn_workspace_bytes(B, Tq, Tk, Hq, Hkv, Dh)
 
 
+def cross_attn_form(B, Tq, Tk, Hq, Hkv, Dh):
+    """The form that cross_attn runs these sizes on: query rows of a workgroup, its waves that split the keys, and whether
+    the keys are split over workgroups."""
+    f = lib().kiln_cross_attn_form(B, Tq, Tk, Hq, Hkv, Dh)
+    return f >> 16, f >> 8 & 0xff, bool(f & 1)
+
+
 def cross_attn(out, q, k, v, Hq, Hkv=None, scale=None, klen=None, kmask=None, workspace=None, stream=None):
     """Attention of q [B, Tq, Hq*Dh] to the encoder states k, v [B, Tk, Hkv*Dh] (kiln_cross_attn), out like q; fp16 or bf16,
     Dh 64 or 128. klen: int32 [B] keys per item; kmask: bool or uint8 [B, Tk], 0 where a key is left out. scale defaults to
@@ -798,6 +807,12 @@ def linear_mxfp4_weight(w, scales=None, stream=None):
 
 def linear_mxfp4_workspace_bytes(T, rows, cols):
     return lib().kiln_linear_mxfp4_workspace_bytes(T, rows, cols)
+
+
+def linear_mxfp4_tile(T, rows, cols):
+    """The tile (weight rows, rows of x) that linear_mxfp4 runs these sizes on; 16 weight rows: the form that quantises x itself."""
+    t = lib().kiln_linear_mxfp4_tile(T, rows, cols)
+    return t >> 16, t & 0xffff
 
 
 def linear_mxfp4(y, x, w, epi=KILN_EPI_F32, gate=None, beta=0.0, workspace=None, stream=None):

@@ -99,6 +99,12 @@ size_t kiln_cross_attn_workspace_bytes(int B, int Tq, int Tk, int Hq, int Hkv, i
     return kiln::cross_attn_workspace(B, Tq, Tk, Hq, Hkv, Dh);
 }
 
+int kiln_cross_attn_form(int B, int Tq, int Tk, int Hq, int Hkv, int Dh) {
+    if (B <= 0 || Tq <= 0 || Tk < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || (Dh != 64 && Dh != 128)) return 0;
+    if (Tk > MAX_ROWS || (long long)Tq * (Hq / Hkv) > MAX_ROWS) return 0;
+    return kiln::cross_attn_form(B, Tq, Tk, Hq, Hkv, Dh);
+}
+
 int kiln_cross_attn(void* out, int ldo, long long bso, const void* q, int ldq, long long bsq, const void* k, int ldk, long long bsk,
                     const void* v, int ldv, long long bsv, int dtype, int B, int Tq, int Tk, int Hq, int Hkv, int Dh, float scale,
                     const int32_t* klen, const uint8_t* kmask, long long bsm, void* workspace, size_t ws_bytes, kiln_stream_t stream) {
@@ -205,6 +211,11 @@ int kiln_linear_mxfp4_prepare_weight(uint8_t* wp, const uint8_t* codes, const ui
 size_t kiln_linear_mxfp4_workspace_bytes(int T, int rows, int cols) {
     if (T <= 0 || !kiln_linear_mxfp4_weight_bytes(rows, cols) || T > MAX_ROWS) return 0;
     return kiln::linear_mx_workspace(T, rows, cols);
+}
+
+int kiln_linear_mxfp4_tile(int T, int rows, int cols) {
+    if (T <= 0 || !kiln_linear_mxfp4_weight_bytes(rows, cols) || T > MAX_ROWS) return 0;
+    return kiln::linear_mx_tile(T, rows, cols);
 }
 
 int kiln_linear_mxfp4(void* y, int ldy, const void* x, int dtype, int ldx, int T, const uint8_t* wp, int rows, int cols, int epi,

@@ -521,6 +521,16 @@ size_t linear_mx_workspace(int T, int rows, int cols) {
     return mx_few_rows(T, rows, cols) ? 0 : mx_code_bytes(T, cols) + mx_scale_bytes(T, cols);
 }
 
+int linear_mx_tile(int T, int rows, int cols) {
+    switch (mx_choose(T, rows, cols)) {
+        case MX_FEW: return 16 << 16 | (T <= 16 ? 16 : T <= 32 ? 32 : 64);
+        case MX_THIN22: return 32 << 16 | 32;
+        case MX_THIN44: return 64 << 16 | 64;
+        case MX_MID: return MxMid::BN << 16 | MxMid::BM;
+        default: return MxBig::BN << 16 | MxBig::BM;
+    }
+}
+
 template <int EPI>
 static hipError_t linear_mx_epi(MxGemmParams p, DT dt, uint8_t* ws, hipStream_t s) {
     const MxKind kind = mx_choose(p.T, p.N, p.K);

@@ -151,6 +151,7 @@ hipError_t launch_mx_pack(uint8_t* op, const uint8_t* codes, const uint8_t* scal
 hipError_t launch_mx_quantize_pack(uint8_t* op, const void* x, DT dt, size_t ldx, int rows, int cols, hipStream_t s);
 // the MXFP4 linear layer (gemm_mxfp4.hip); ws: linear_mx_workspace bytes
 size_t linear_mx_workspace(int T, int rows, int cols);
+int linear_mx_tile(int T, int rows, int cols);  // weight rows << 16 | rows of x
 hipError_t launch_linear_mx(void* y, size_t ldy, const void* x, DT dt, size_t ldx, int T, const uint8_t* wp, int rows, int cols, int epi,
                             const float* gate, float beta, uint8_t* ws, hipStream_t s);
 
@@ -173,6 +174,7 @@ struct CrossLaunch {
     size_t ws_bytes;
 };
 size_t cross_attn_workspace(int B, int Tq, int Tk, int Hq, int Hkv, int Dh);
+int cross_attn_form(int B, int Tq, int Tk, int Hq, int Hkv, int Dh);  // rows << 16 | waves along the keys << 8 | split
 hipError_t launch_cross_attn(const CrossLaunch& c, hipStream_t s);
 
 // torch.manual_seed(seed); torch.randn(n) on the host (host_rng.cpp); false if n < 16

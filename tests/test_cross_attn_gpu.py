@@ -63,8 +63,18 @@ def make(B, Tq, Tk, Hq, Hkv, Dh, dt, seed=0):
 
 SHAPES = [  # B, Tq, Tk, Hq, Hkv, Dh
     (1, 1, 1, 1, 1, 64), (1, 1, 33, 16, 16, 128), (3, 1, 300, 16, 4, 64), (2, 3, 65, 20, 4, 128), (8, 1, 5000, 16, 4, 128), (1, 1, 9001, 2, 1, 64),
+    (1, 20, 2500, 2, 2, 64),
     (1, 16, 2049, 4, 4, 128), (1, 17, 31, 2, 2, 64), (1, 17, 4000, 2, 2, 128), (2, 65, 96, 10, 10, 64), (1, 200, 1111, 8, 8, 64), (1, 512, 120, 16, 16, 64),
-    (1, 130, 1000, 12, 1, 128), (2, 700, 77, 10, 10, 64), (2, 2048, 77, 10, 10, 128), (2, 1025, 130, 32, 8, 64), (1, 4097, 40, 16, 16, 128)]
+    (1, 130, 1000, 12, 1, 128), (2, 700, 77, 10, 10, 64), (2, 2048, 77, 10, 10, 128), (2, 1025, 130, 32, 8, 64), (1, 4097, 40, 16, 16, 128),
+    (2, 4097, 300, 16, 16, 64), (64, 1, 70, 16, 16, 64), (40, 2, 200, 16, 16, 128)]
+
+
+def test_shapes_reach_every_form(gpu):
+    """16 rows: one wave alone, on a range of the keys or on all of them, or four waves that split them; 64, 128 and (heads of 64) 256
+    rows, 64 also on ranges of the keys."""
+    forms = {(d, ka.cross_attn_form(*s)) for s in SHAPES for d in (s[5],)}
+    want = {(16, 1, False), (16, 1, True), (16, 4, False), (64, 1, False), (64, 1, True), (128, 1, False)}
+    assert forms == {(d, f) for d in (64, 128) for f in want} | {(64, (256, 1, False))}
 
 
 @pytest.mark.parametrize("B,Tq,Tk,Hq,Hkv,Dh", SHAPES)

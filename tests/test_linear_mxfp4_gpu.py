@@ -54,9 +54,19 @@ def out_of(epi, T, N):
     return torch.full((T, N), float("nan"), device=DEV, dtype=torch.float32 if epi in ("f32", "resid") else torch.float16)
 
 
-@pytest.mark.parametrize("T,N,K", [(1, 16, 32), (1, 1, 32), (1, 2048, 2048), (2, 33, 64), (16, 128, 160), (17, 100, 96), (32, 2048, 8192), (33, 65, 1024),
+SIZES = [(1, 16, 32), (1, 1, 32), (1, 2048, 2048), (2, 33, 64), (16, 128, 160), (17, 100, 96), (32, 2048, 8192), (33, 65, 1024),
                                    (64, 257, 128), (65, 257, 128), (65, 1, 32), (128, 128, 2048), (129, 130, 288), (300, 2048, 1024), (1537, 256, 512),
-                                   (2048, 2048, 256), (257, 8192, 2048), (4100, 4100, 96)])
+                                   (2048, 2048, 256), (257, 8192, 2048), (4100, 4100, 96), (2047, 8190, 640), (2048, 8192, 96)]
+EPI_SIZES = [(1, 48, 64), (20, 130, 96), (50, 1024, 1024), (64, 2048, 1024), (70, 2048, 4096), (200, 129, 2048), (1000, 2048, 1024), (4352, 4352, 64),
+             (300, 2048, 1024), (2047, 8190, 640)]
+
+
+@pytest.mark.parametrize("sizes", [SIZES, EPI_SIZES])
+def test_sizes_reach_every_tile(gpu, sizes):
+    assert {ka.linear_mxfp4_tile(*s) for s in sizes} == {(16, 16), (16, 32), (16, 64), (32, 32), (64, 64), (128, 128), (256, 256)}
+
+
+@pytest.mark.parametrize("T,N,K", SIZES)
 @pytest.mark.parametrize("dt", [torch.float32, torch.float16, torch.bfloat16])
 def test_sizes(gpu, T, N, K, dt):
     x, w = make(T, N, K, dt)
@@ -66,7 +76,7 @@ def test_sizes(gpu, T, N, K, dt):
     assert torch.equal(y, ka.linear_mxfp4(out_of("f32", T, N), x, W))
 
 
-@pytest.mark.parametrize("T,N,K", [(1, 48, 64), (20, 130, 96), (64, 2048, 1024), (200, 129, 2048), (1000, 2048, 1024), (4352, 4352, 64)])
+@pytest.mark.parametrize("T,N,K", EPI_SIZES)
 @pytest.mark.parametrize("epi", list(EPI))
 def test_epilogues(gpu, T, N, K, epi):
     x, w = make(T, N, K, torch.float16, 5)

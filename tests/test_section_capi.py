@@ -172,3 +172,10 @@ def test_python_checks():
     with pytest.raises(ValueError, match="GPU"):
         ka.mxfp4_quantize(x)
     assert ctypes.sizeof(ctypes.c_double) == 8
+
+
+def test_forms_of_refused_sizes(L):
+    assert L.kiln_cross_attn_form(0, 1, 1, 1, 1, 64) == 0 and L.kiln_cross_attn_form(1, 1, 1, 3, 2, 64) == 0
+    assert L.kiln_cross_attn_form(1, 1, 1, 1, 1, 96) == 0 and L.kiln_cross_attn_form(1, 1, (1 << 30) + 1, 1, 1, 64) == 0
+    assert L.kiln_linear_mxfp4_tile(0, 64, 64) == 0 and L.kiln_linear_mxfp4_tile(64, 64, 40) == 0
+    assert ka.linear_mxfp4_tile(1, 64, 64) == (16, 16)
