@@ -386,7 +386,7 @@ int kiln_rope_freqs(double* host_freqs, float* mscale, int rot, double theta, in
 
 /* Rotary positions of H heads of Dh per row: with a = p f_i for the row's position p, the pair (u, v) becomes
  * mscale (u cos a - v sin a, v cos a + u sin a). Pairs are (i, i + rot/2) of the head, or (2i, 2i + 1) when interleaved;
- * dimensions from rot on pass unchanged. rot even, 2 <= rot <= Dh <= 1024, H <= 65535. x, y [T, ld] in dtype (F32, F16,
+ * dimensions from rot on pass unchanged. rot even, 2 <= rot <= Dh <= 1024, H <= 65535, T <= 2^30. x, y [T, ld] in dtype (F32, F16,
  * BF16; fp32 arithmetic, rounded once), any alignment (rows and halves of 16-byte multiples are fastest); y = x with
  * ldy = ldx is in place, other overlaps are refused. pos [T] on the device, or NULL: pos0 + t. freqs [rot / 2] on the device
  * (kiln_rope_freqs); the angle is taken in 64 bits, so far positions keep their phase. Negative positions turn back: the call
@@ -396,7 +396,8 @@ int kiln_rope(void* y, int ldy, const void* x, int ldx, int dtype, int T, int H,
 
 /* Attention of B items of Tq queries to Tk encoder states of another length, Hq query heads on Hkv key heads (query head h
  * reads key head h Hkv / Hq; Hq % Hkv == 0), Dh 64 or 128: out = softmax(scale Q K^T) V. q [Tq, ldq], k, v [Tk, ld*], out
- * [Tq, ldo] per item in dtype (F16 or BF16), items bs* elements apart (0: all items share it, inputs only); 16-byte aligned
+ * [Tq, ldo] per item in dtype (F16 or BF16), items bs* elements apart (0: all items share it, inputs only; items' outputs
+ * one behind the other, or side by side in rows of all of them, and apart from the inputs); 16-byte aligned
  * rows and item strides (KILN_EUNSUPPORTED otherwise), ld <= 2^24. Item b's keys are the states below klen[b] (device [B],
  * clamped to 0 .. Tk; NULL: all) whose byte in kmask (device, [Tk] per item, bsm bytes apart; NULL: all) is not 0; what the
  * others hold does not matter, NaN included. A row without keys, or whose every score is -inf, gives zeros. Scores, maxima and

@@ -80,7 +80,8 @@ int kiln_rope(void* y, int ldy, const void* x, int ldx, int dtype, int T, int H,
     if (!dtype_ok(dtype)) return fail(KILN_EINVAL, "rope: dtype %d", dtype);
     if (T < 0 || H <= 0 || Dh <= 0 || rot < 2 || rot % 2 || rot > Dh)
         return fail(KILN_EINVAL, "rope: bad sizes T=%d H=%d Dh=%d rot=%d", T, H, Dh, rot);
-    if (Dh > 1024 || H > 65535) return fail(KILN_EUNSUPPORTED, "rope: Dh=%d above 1024 or H=%d above 65535", Dh, H);
+    if (Dh > 1024 || H > 65535 || T > MAX_ROWS)
+        return fail(KILN_EUNSUPPORTED, "rope: Dh=%d above 1024, H=%d above 65535 or T=%d above 2^30", Dh, H, T);
     if (!T) return KILN_OK;
     if (!x || !y || !freqs) return fail(KILN_EINVAL, "rope: null pointer");
     const long long W = (long long)H * Dh;
@@ -131,7 +132,10 @@ int kiln_cross_attn(void* out, int ldo, long long bso, const void* q, int ldq, l
             return fail(KILN_EUNSUPPORTED, "cross_attn: %s rows not 16-byte aligned, or more than 2^24 elements apart", t.name);
     }
     if (!aligned(klen, 4)) return fail(KILN_EUNSUPPORTED, "cross_attn: klen not aligned");
-    if (B > 1 && llabs(bso) < (long long)Hq * Dh) return fail(KILN_EINVAL, "cross_attn: items' outputs overlap (bso %lld)", bso);
+    // items' outputs one behind the other, or side by side in rows that hold them all
+    const long long W = (long long)Hq * Dh, abso = bso < 0 ? -bso : bso;
+    if (B > 1 && abso < (Tq - 1) * (long long)ldo + W && (abso < W || ldo < (B - 1) * abso + W))
+        return fail(KILN_EINVAL, "cross_attn: items' outputs overlap (bso %lld, ldo %d)", bso, ldo);
     if (workspace && !aligned(workspace, 16)) return fail(KILN_EUNSUPPORTED, "cross_attn: workspace not 16-byte aligned");
     kiln::CrossLaunch c{};
     c.out = out;
@@ -140,8 +144,8 @@ int kiln_cross_attn(void* out, int ldo, long long bso, const void* q, int ldq, l
     c.v = v;
     c.ldo = (size_t)(Tq == 1 ? 0 : ldo);
     c.ldq = (size_t)(Tq == 1 ? 0 : ldq);
-    c.ldk = (size_t)(Tk <= 1 ? Hkv * Dh : ldk);
-    c.ldv = (size_t)(Tk <= 1 ? Hkv * Dh : ldv);
+    c.ldk = (size_t)(Tk <= 1 ? Dh : ldk);
+    c.ldv = (size_t)(Tk <= 1 ? Dh : ldv);
     c.bso = bso;
     c.bsq = bsq;
     c.bsk = bsk;

@@ -13,8 +13,10 @@
 // never happens.
 //
 // Softmax in one pass: running maximum m and sum l per row in fp32, in units of log2. The maximum moves (and O and l are
-// rescaled) only when a tile's exceeds it by more than 8, so P <= 2^8 and most tiles need no exchange between lanes. P is
-// rounded to the inputs' type, half a step of it (2^-11 fp16, 2^-8 bf16) per weight, as far off as the output's own rounding.
+// rescaled) only when a tile's exceeds it by more than 8, so most tiles need no exchange between lanes. P is taken as 2^7 times
+// the weight, 2^15 at most, and rounded to the inputs' type, half a step of it (2^-11 fp16, 2^-8 bf16) per weight, as far off as
+// the output's own rounding. The factor is in O and l alike; it keeps fp16 weights down to 2^-32 of the largest (2^-25 without),
+// of which a long context may have enough to count: 2^17 keys at 2^-25.5 are 2^-8.5 of the output.
 //
 // Bound, with many rows, by matrix and vector work (16 multiply-adds, 16 exponentials, 8 conversions and some 14 maxima beside 34
 // products per wave and tile of 32 rows, Dh 128) at the clock that power leaves: 2 x 4096 x 4096, 16 heads of 128, 295 us, 930 TFLOP/s;
@@ -49,7 +51,7 @@ struct CrossParams {
 };
 
 constexpr int XKT = 32;       // keys of a tile
-constexpr float XRESCALE = 8.f;
+constexpr float XRESCALE = 8.f, XLIFT = 7.f;  // log2: the maximum's slack, the weights' factor
 
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef short s4v __attribute__((ext_vector_type(4)));
@@ -216,7 +218,7 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_cross_attn(const Cross
     }
 
     floatx4 o[DH / 16][QB], l[QB];  // l: every register of a lane holds its row's sum (P^T times ones)
-    float m[QB], mn[QB];            // running maximum; its negative as subtracted (0 while the maximum is -inf)
+    float m[QB], mn[QB];            // running maximum; XLIFT minus it (0 while it is -inf)
 #pragma unroll
     for (int qb = 0; qb < QB; qb++) {
         m[qb] = -INFINITY;
@@ -289,7 +291,7 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_cross_attn(const Cross
             const float t = fmaxf(m[qb], quad_max(top[qb]));
             const float f = t > m[qb] ? __builtin_amdgcn_exp2f(m[qb] - t) : 1.f;
             m[qb] = t;
-            mn[qb] = t == -INFINITY ? 0.f : -t;
+            mn[qb] = t == -INFINITY ? 0.f : XLIFT - t;
             l[qb] *= f;
 #pragma unroll
             for (int db = 0; db < DH / 16; db++) o[db][qb] *= f;
@@ -594,6 +596,7 @@ static hipError_t cross_launch(CrossParams p, hipStream_t s) {
     p.rtiles = (p.rows + C::RT - 1) / C::RT;
     p.total = p.B * p.Hkv * p.ksplit * p.rtiles;
     p.per = (p.total + 7) / 8;
+    if (hipError_t e = grid_check((size_t)p.per * 8, C::THREADS)) return e;
     auto kern = p.kmask ? k_cross_attn<E, C, true> : k_cross_attn<E, C, false>;
     hipLaunchKernelGGL(kern, dim3(p.per * 8), dim3(C::THREADS), C::LDS, s, p);
     if (hipError_t e = hipGetLastError()) return e;

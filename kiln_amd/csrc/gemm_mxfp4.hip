@@ -249,6 +249,7 @@ static hipError_t mx_thin(MxGemmParams p, hipStream_t s) {
     p.tiles_n = (p.N + 16 * NB - 1) / (16 * NB);
     p.total = p.tiles_m * p.tiles_n;
     p.per = (p.total + 7) / 8;
+    if (hipError_t e = grid_check((size_t)p.per * 8, THIN_WAVES * 64)) return e;
     hipLaunchKernelGGL((k_mx_thin<EPI, NB, MB>), dim3(p.per * 8), dim3(THIN_WAVES * 64), THIN_WAVES * NB * MB * 1024, s, p);
     return hipGetLastError();
 }
@@ -477,6 +478,7 @@ static hipError_t mx_tiles(MxGemmParams p, hipStream_t s) {
     p.tiles_n = (p.N + C::BN - 1) / C::BN;
     p.total = p.tiles_m * p.tiles_n;
     p.per = (p.total + 7) / 8;
+    if (hipError_t e = grid_check((size_t)p.per * 8, C::THREADS)) return e;
     hipLaunchKernelGGL((k_mx_gemm<EPI, C>), dim3(p.per * 8), dim3(C::THREADS), C::LDS, s, p);
     return hipGetLastError();
 }
@@ -489,6 +491,7 @@ static hipError_t mx_few(const MxGemmParams& p, hipStream_t s) {
         if (mb == 2) return vec ? k_mx_few<E, EPI, 2, true> : k_mx_few<E, EPI, 2, false>;
         return vec ? k_mx_few<E, EPI, 4, true> : k_mx_few<E, EPI, 4, false>;
     };
+    if (hipError_t e = grid_check((p.N + 15) / 16, FEW_WAVES * 64)) return e;
     hipLaunchKernelGGL(pick(), dim3((p.N + 15) / 16), dim3(FEW_WAVES * 64), 0, s, p);
     return hipGetLastError();
 }

@@ -10,6 +10,10 @@ namespace kiln {
 enum class DT { F32 = 0, F16 = 1, BF16 = 2 };
 
 int cu_count();  // CUs of the current device (256 without one)
+// a grid of the section's kernels: the threads of a launch are counted in 32 bits
+inline hipError_t grid_check(size_t workgroups, int threads) {
+    return workgroups * threads < (size_t)1 << 32 ? hipSuccess : hipErrorInvalidConfiguration;
+}
 
 // One attention problem of a batched launch: queries q (rows [0, Tq), row stride ldq, head h at
 // column h*128) against the prepared K/V buffer kv (Tk real keys, npad analytic zero keys).

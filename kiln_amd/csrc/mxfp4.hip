@@ -165,8 +165,10 @@ static hipError_t dequantize_of(void* y, size_t ldy, const uint8_t* codes, const
 template <class E>
 static hipError_t quantize_pack_of(uint8_t* op, const void* x, size_t ldx, int rows, int cols, bool vec, hipStream_t s) {
     const int kbs = mx_kb(cols);
+    const size_t wgs = ((size_t)rows + 63) / 64 * kbs;
+    if (hipError_t e = grid_check(wgs, 256)) return e;
     auto kern = vec ? k_mx_quantize_pack<E, true> : k_mx_quantize_pack<E, false>;
-    hipLaunchKernelGGL(kern, dim3((unsigned)(((size_t)rows + 63) / 64 * kbs)), dim3(256), 0, s, op, op + mx_code_bytes(rows, cols),
+    hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(256), 0, s, op, op + mx_code_bytes(rows, cols),
                        static_cast<const E*>(x), ldx, rows, cols, kbs);
     return hipGetLastError();
 }
@@ -190,6 +192,7 @@ hipError_t launch_mx_dequantize(void* y, DT dt, size_t ldy, const uint8_t* codes
 }
 hipError_t launch_mx_pack(uint8_t* op, const uint8_t* codes, const uint8_t* scales, int rows, int cols, hipStream_t s) {
     const size_t units = (size_t)mx_rg(rows) * mx_kb(cols);
+    if (hipError_t e = grid_check((units + 3) / 4, 256)) return e;
     hipLaunchKernelGGL(k_mx_pack, dim3((unsigned)((units + 3) / 4)), dim3(256), 0, s, op, op + mx_code_bytes(rows, cols), codes, scales,
                        rows, cols, units);
     return hipGetLastError();

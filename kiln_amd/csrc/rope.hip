@@ -123,6 +123,7 @@ static hipError_t rope_of(RopeParams p, bool inter, bool aligned, hipStream_t s)
     p.inv_hu = ((1ull << 32) + p.hb * p.nu - 1) / (p.hb * p.nu);
     p.inv_u = ((1ull << 32) + p.nu - 1) / p.nu;
     const dim3 grid((p.T + p.tb - 1) / p.tb, (p.H + p.hb - 1) / p.hb);
+    if (hipError_t e = grid_check(grid.x, ROPE_THREADS)) return e;
     const size_t lds = (size_t)p.tb * (p.rot / 2) * sizeof(float2);
     auto kern = vec ? (inter ? k_rope<E, N, true> : k_rope<E, N, false>) : (inter ? k_rope<E, 1, true> : k_rope<E, 1, false>);
     hipLaunchKernelGGL(kern, grid, dim3(ROPE_THREADS), lds, s, p);

@@ -1,6 +1,8 @@
 """kiln_cross_attn against 64-bit attention: every form (rows per workgroup, keys split over waves and workgroups), shared key
 heads, lengths, masks, strides, values that move the maximum, and what masked states may hold."""
 
+import math
+
 import pytest
 import torch
 
@@ -44,7 +46,7 @@ def check(out, q, k, v, Hq, Hkv, keep=None, scale=None, what=""):
     rel = u + (Dh / 32 + 2) * 2.0 ** -22 * smag + (Tk / 4 + 64) * 2.0 ** -24 + 2.0 ** -21
     tol = rel * wmag
     if q.dtype == torch.float16:
-        tol = tol + 2.0 ** -25 * vsum  # weights below fp16's normal range, against a sum of 1 at least
+        tol = tol + 2.0 ** -32 * vsum  # weights below fp16's normal range (2^-25), against a largest of 2^7 at least
     tol = tol + u * (ref.abs() + tol) + torch.finfo(q.dtype).smallest_normal * u
     err = (out.double() - ref).abs()
     print(f"[cross_attn] {what}: worst error / tolerance {(err / tol).max():.3f}", flush=True)
@@ -171,6 +173,23 @@ def test_nonfinite_states_propagate(gpu):
     want[0, :, :2 * 64] = True
     want[1, :, 2 * 64 + 7] = want[1, :, 3 * 64 + 7] = True
     assert torch.equal(torch.isnan(out), want)
+
+
+@pytest.mark.parametrize("Tq", [1, 17])
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+def test_many_small_weights(gpu, dt, Tq):
+    """One state of weight 1 and value 0 ahead of 2^17 of weight 2^-25.5 and value 1: together 2^-8.5 of the output, though each
+    is less than fp16's least number. Without a workspace, so that they share a maximum."""
+    Tk, Dh = (1 << 17) + 1, 64
+    q, k, v = torch.zeros(1, Tq, Dh, device=DEV, dtype=dt), torch.zeros(1, Tk, Dh, device=DEV, dtype=dt), torch.ones(1, Tk, Dh, device=DEV, dtype=dt)
+    q[:, :, 0], k[:, 1:, 0], v[:, 0] = 1, -25.5, 0  # a score in log2 each
+    out = ka.cross_attn(torch.empty_like(q), q, k, v, 1, scale=math.log(2), workspace=torch.empty(16, dtype=torch.uint8, device=DEV))
+    tail = 2.0 ** (17 - 25.5)
+    # each weight 2^7 2^-25.5 to fp16's step of 2^-24, half of it (bf16: 2^-8 of it); 2^17 fp32 additions; the exponent's argument
+    # within 2^-21; the output's rounding
+    u = torch.finfo(dt).eps / 2
+    rel = (2.0 ** -25 / 2.0 ** -18.5 if dt == torch.float16 else u) + 2.0 ** -24 * (Tk / 4 + 64) + 2.0 ** -21 + u
+    assert ((out.double() - tail / (1 + tail)).abs() <= rel * tail).all()
 
 
 def test_strides_of_single_rows(gpu):

@@ -65,7 +65,7 @@ def test_rope_refusals(L):
     for kw in (dict(dt=3), dict(dt=-1), dict(T=-1), dict(H=0), dict(Dh=0), dict(rot=0), dict(rot=3), dict(rot=130), dict(y=None), dict(x=None),
                dict(freqs=None), dict(ldx=255), dict(ldy=255)):
         assert rope(L, **kw) == EINVAL, kw
-    for kw in (dict(Dh=2048, ldx=4096, ldy=4096), dict(H=65536, Dh=2, rot=2, ldx=1 << 18, ldy=1 << 18), dict(x=Q + 1), dict(dt=F32, y=P + 2),
+    for kw in (dict(Dh=2048, ldx=4096, ldy=4096), dict(H=65536, Dh=2, rot=2, ldx=1 << 18, ldy=1 << 18), dict(T=(1 << 30) + 1), dict(x=Q + 1), dict(dt=F32, y=P + 2),
                dict(freqs=R + 4), dict(pos=S + 2)):
         assert rope(L, **kw) == EUNSUP, kw
     # overlaps: shifted by a row, by some columns, with another stride; columns side by side are fine as far as the checks go
@@ -83,7 +83,8 @@ def cross(L, out=P, ldo=256, bso=1024, q=Q, ldq=256, bsq=1024, k=R, ldk=256, bsk
 def test_cross_attn_refusals(L):
     for kw in (dict(dt=F32), dict(dt=7), dict(B=-1), dict(Tq=-1), dict(Tk=-1), dict(Hq=0), dict(Hkv=0), dict(Hq=3), dict(scale=0.0),
                dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf), dict(out=None), dict(q=None), dict(k=None), dict(v=None),
-               dict(ldo=248), dict(ldq=0), dict(ldk=-256), dict(ldv=128), dict(bso=0), dict(bso=128)):
+               dict(ldo=248), dict(ldq=0), dict(ldk=-256), dict(ldv=128), dict(bso=0), dict(bso=128), dict(bso=256), dict(bso=768), dict(bso=-768),
+               dict(bso=256, ldo=504), dict(bso=128, Hq=1, Hkv=1, B=3, ldo=256)):
         assert cross(L, **kw) == EINVAL, kw
     for kw in (dict(Dh=96), dict(Dh=32), dict(out=P + 8), dict(q=Q + 2), dict(k=R + 8), dict(v=S + 4), dict(ldo=260), dict(ldk=257), dict(bsq=1028),
                dict(bsv=2049), dict(ldk=1 << 25), dict(klen=S + 2), dict(ws=S + 8, wsb=1 << 30), dict(Tk=(1 << 30) + 1), dict(Tq=1 << 30, Hq=4, ldo=512, ldq=512)):
