@@ -227,3 +227,20 @@ def test_python_checks(gpu):
         ka.cross_attn(o[:1].expand(2, -1, -1), q, k, v, 4, 2)
     with pytest.raises(ka.KilnError):
         ka.cross_attn(torch.empty(2, 4, 96, device=DEV).half(), torch.zeros(2, 4, 96, device=DEV).half(), *[torch.zeros(2, 8, 96, device=DEV).half()] * 2, 1)
+
+
+@pytest.mark.parametrize("B,Tq,Tk,Hq,Hkv,Dh", [(3, 40, 100, 4, 2, 64), (2, 1, 2000, 8, 2, 128), (2, 3, 50, 2, 2, 128), (2, 1500, 90, 16, 16, 128)])
+def test_items_side_by_side(gpu, B, Tq, Tk, Hq, Hkv, Dh):
+    """Tokens first, items second: the results of items one behind the other, bit for bit. A stride at which the items' outputs meet is refused."""
+    q, k, v = make(B, Tq, Tk, Hq, Hkv, Dh, torch.bfloat16)
+    klen = torch.arange(B, device=DEV, dtype=torch.int32) * 7 + 33
+    want = ka.cross_attn(torch.empty_like(q), q, k, v, Hq, Hkv, klen=klen)
+    tb = lambda t: t.transpose(0, 1).contiguous().transpose(0, 1)  # noqa: E731
+    out = tb(torch.empty_like(q))
+    ka.cross_attn(out, tb(q), tb(k), tb(v), Hq, Hkv, klen=klen)
+    assert torch.equal(out, want)
+    W = Hq * Dh
+    flat = torch.empty(B * Tq * W + W, device=DEV, dtype=q.dtype)
+    if Tq > 1:
+        with pytest.raises(ka.KilnError):
+            ka.cross_attn(flat.as_strided((B, Tq, W), (W, W, 1)), q, k, v, Hq, Hkv, klen=klen)

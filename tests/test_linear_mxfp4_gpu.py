@@ -174,3 +174,17 @@ def test_python_checks(gpu):
     with pytest.raises(ka.KilnError) as e:
         ka.linear_mxfp4(y, x, W, workspace=torch.empty(16, dtype=torch.uint8, device=DEV))
     assert e.value.status == ka.KILN_ENOMEM
+
+
+@pytest.mark.parametrize("T,N,bits,tile", [(20, 256, 27, 16), (100, 256, 25, 32), (1000, 1024, 22, 64), (1537, 2048, 21, 128), (4352, 8192, 19, 256)])
+@pytest.mark.parametrize("dt", [torch.float16, torch.float32])
+def test_rows_past_32_bits(gpu, T, N, bits, tile, dt):
+    """Rows of x and y so far apart that elements pass 2^31 and bytes 2^32: the results of dense rows, bit for bit."""
+    x, w = make(T, N, 128, dt)
+    W = ka.linear_mxfp4_weight(w)
+    assert ka.linear_mxfp4_tile(T, N, 128)[0] == tile
+    epi = EPI["f16" if dt == torch.float16 else "f32"]
+    far = torch.empty(T, (1 << bits) + 8, dtype=dt, device=DEV)
+    far[:, :128] = x
+    ka.linear_mxfp4(far[:, 128:128 + N], far[:, :128], W, epi=epi)
+    assert torch.equal(far[:, 128:128 + N], ka.linear_mxfp4(torch.empty(T, N, dtype=dt, device=DEV), x, W, epi=epi))

@@ -107,3 +107,26 @@ def test_python_checks(gpu):
     with pytest.raises(ka.KilnError):
         ka.mxfp4_quantize(torch.randn(4, 40, device=DEV), torch.empty(4, 20, dtype=torch.uint8, device=DEV),
                           torch.empty(4, 1, dtype=torch.uint8, device=DEV))
+
+
+def test_rows_past_32_bits(gpu):
+    """Rows so far apart that elements pass 2^31 and bytes 2^32."""
+    x = torch.randn(40, 96, device=DEV).half()
+    far = torch.empty(40, (1 << 26) + 8, dtype=torch.float16, device=DEV)
+    far[:, :96] = x
+    c, s = ka.mxfp4_quantize(far[:, :96])
+    c0, s0 = ka.mxfp4_quantize(x)
+    assert torch.equal(c, c0) and torch.equal(s, s0)
+    ka.mxfp4_dequantize(far[:, 96:192], c, s)
+    assert torch.equal(far[:, 96:192], ka.mxfp4_dequantize(torch.empty_like(x), c, s))
+
+
+def test_many_blocks(gpu):
+    """2^32 + 4096 values in one call, each pass of a thread through the loop: the last rows as by themselves."""
+    x = torch.empty((1 << 20) + 1, 4096, dtype=torch.float16, device=DEV)
+    x[:-5] = 1
+    x[-5:] = torch.randn(5, 4096, device=DEV)
+    c, s = ka.mxfp4_quantize(x)
+    c5, s5 = ka.mxfp4_quantize(x[-5:])
+    assert torch.equal(c[-5:], c5) and torch.equal(s[-5:], s5) and (s[:-5] == 125).all() and (c[:-5] == 0x66).all()
+    assert torch.equal(ka.mxfp4_dequantize(x.clone(), c, s)[-5:], ka.mxfp4_dequantize(torch.empty_like(x[-5:]), c5, s5))

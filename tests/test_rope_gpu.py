@@ -158,3 +158,17 @@ def test_batch_of_rows_is_each_row(gpu):
     y = ka.rope(torch.empty_like(x), x, H, Dh, f)
     for t in (0, 1, 1249, 2499):
         assert torch.equal(ka.rope(torch.empty_like(x[:1]), x[t:t + 1], H, Dh, f, pos0=t), y[t:t + 1])
+
+
+@pytest.mark.parametrize("inter", [False, True])
+def test_rows_past_32_bits(gpu, inter):
+    """Rows so far apart that elements pass 2^31 and bytes 2^32, into another part of themselves and in place."""
+    T, H, Dh = 40, 2, 64
+    f, _ = ka.rope_freqs(Dh, device=DEV)
+    x = torch.randn(T, H * Dh, device=DEV).half()
+    want = ka.rope(torch.empty_like(x), x, H, Dh, f, interleaved=inter)
+    far = torch.empty(T, (1 << 26) + 8, dtype=torch.float16, device=DEV)
+    far[:, :H * Dh] = x
+    ka.rope(far[:, H * Dh:2 * H * Dh], far[:, :H * Dh], H, Dh, f, interleaved=inter)
+    ka.rope(far[:, :H * Dh], far[:, :H * Dh], H, Dh, f, interleaved=inter)
+    assert torch.equal(far[:, H * Dh:2 * H * Dh], want) and torch.equal(far[:, :H * Dh], want)
