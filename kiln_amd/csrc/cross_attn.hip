@@ -13,10 +13,12 @@
 // never happens.
 //
 // Softmax in one pass: running maximum m and sum l per row in fp32, in units of log2. The maximum moves (and O and l are
-// rescaled) only when a tile's exceeds it by more than 8, so most tiles need no exchange between lanes. P is taken as 2^7 times
-// the weight, 2^15 at most, and rounded to the inputs' type, half a step of it (2^-11 fp16, 2^-8 bf16) per weight, as far off as
-// the output's own rounding. The factor is in O and l alike; it keeps fp16 weights down to 2^-32 of the largest (2^-25 without),
-// of which a long context may have enough to count: 2^17 keys at 2^-25.5 are 2^-8.5 of the output.
+// rescaled) only when a tile's exceeds it by more than 8, so most tiles need no exchange between lanes. P is taken as 2^lift times
+// the weight and rounded to the inputs' type, half a step of it (2^-11 fp16, 2^-8 bf16) per weight, as far off as the output's own
+// rounding. The factor is in O and l alike. In fp16 it is 2^7: P is 2^15 at most, and weights down to 2^-32 of the largest count
+// (2^-25 without), of which a long context may have enough: 2^17 keys at 2^-25.5 are 2^-8.5 of the output. bf16 has fp32's
+// exponents, for weights and for values: there P sums to less than 1 over all keys (lift = -9 - log2 Tk, rounded down), so that no
+// finite value overflows on its way; at the other end, products with values below 2^-117 Tk leave fp32's normal range.
 //
 // Bound, with many rows, by matrix and vector work (16 multiply-adds, 16 exponentials, 8 conversions and some 14 maxima beside 34
 // products per wave and tile of 32 rows, Dh 128) at the clock that power leaves: 2 x 4096 x 4096, 16 heads of 128, 295 us, 930 TFLOP/s;
@@ -43,7 +45,8 @@ struct CrossParams {
     const int* klen;
     const uint8_t* kmask;
     long long bsm;
-    float sc;  // scale log2(e)
+    float sc;                       // scale log2(e)
+    float lift;                     // log2 of the weights' factor
     int rows;                       // Tq G
     int rtiles, ksplit, ct;         // row tiles, key ranges of one (ct tiles each), ..
     int total, per;                 // .. work items, items per XCD
@@ -51,7 +54,7 @@ struct CrossParams {
 };
 
 constexpr int XKT = 32;       // keys of a tile
-constexpr float XRESCALE = 8.f, XLIFT = 7.f;  // log2: the maximum's slack, the weights' factor
+constexpr float XRESCALE = 8.f, XLIFT16 = 7.f;  // log2: the maximum's slack, the factor of fp16 weights
 
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef short s4v __attribute__((ext_vector_type(4)));
@@ -218,7 +221,8 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_cross_attn(const Cross
     }
 
     floatx4 o[DH / 16][QB], l[QB];  // l: every register of a lane holds its row's sum (P^T times ones)
-    float m[QB], mn[QB];            // running maximum; XLIFT minus it (0 while it is -inf)
+    const float lift = std::is_same<E, _Float16>::value ? XLIFT16 : p.lift;
+    float m[QB], mn[QB];            // running maximum; lift minus it (0 while it is -inf)
 #pragma unroll
     for (int qb = 0; qb < QB; qb++) {
         m[qb] = -INFINITY;
@@ -291,7 +295,7 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_cross_attn(const Cross
             const float t = fmaxf(m[qb], quad_max(top[qb]));
             const float f = t > m[qb] ? __builtin_amdgcn_exp2f(m[qb] - t) : 1.f;
             m[qb] = t;
-            mn[qb] = t == -INFINITY ? 0.f : XLIFT - t;
+            mn[qb] = t == -INFINITY ? 0.f : lift - t;
             l[qb] *= f;
 #pragma unroll
             for (int db = 0; db < DH / 16; db++) o[db][qb] *= f;
@@ -640,6 +644,11 @@ hipError_t launch_cross_attn(const CrossLaunch& c, hipStream_t s) {
     p.kmask = c.kmask;
     p.bsm = c.bsm;
     p.sc = c.scale * LOG2E;
+    p.lift = XLIFT16;
+    if (c.dt == DT::BF16) {
+        p.lift = -1.f - XRESCALE;
+        for (long n = 1; n < c.Tk; n *= 2) p.lift -= 1.f;
+    }
     p.rows = c.Tq * p.G;
     p.ksplit = f.ksplit;
     p.ct = f.ct;
