@@ -19,6 +19,9 @@
 // (2^-25 without), of which a long context may have enough: 2^17 keys at 2^-25.5 are 2^-8.5 of the output. bf16 has fp32's
 // exponents, for weights and for values: there P sums to less than 1 over all keys (lift = -9 - log2 Tk, rounded down), so that no
 // finite value overflows on its way; at the other end, products with values below 2^-117 Tk leave fp32's normal range.
+// The exponent is one fma, s sc + (lift - m): exact products against a rounded m, off by half a unit of m's last place for all
+// keys of a row alike. While |m| is at most 2^20 that is a factor of 2^(1/16), in O and l alike; beyond, where it would grow out of
+// the weights' range, products are rounded as m was before it is taken off (`far`: a branch that a wave takes or not).
 //
 // Bound, with many rows, by matrix and vector work (16 multiply-adds, 16 exponentials, 8 conversions and some 14 maxima beside 34
 // products per wave and tile of 32 rows, Dh 128) at the clock that power leaves: 2 x 4096 x 4096, 16 heads of 128, 295 us, 930 TFLOP/s;
@@ -55,6 +58,7 @@ struct CrossParams {
 
 constexpr int XKT = 32;       // keys of a tile
 constexpr float XRESCALE = 8.f, XLIFT16 = 7.f;  // log2: the maximum's slack, the factor of fp16 weights
+constexpr float XFAR = 1 << 20;                 // log2: a maximum from which scores are rounded on their own
 
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef short s4v __attribute__((ext_vector_type(4)));
@@ -222,11 +226,12 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_cross_attn(const Cross
 
     floatx4 o[DH / 16][QB], l[QB];  // l: every register of a lane holds its row's sum (P^T times ones)
     const float lift = std::is_same<E, _Float16>::value ? XLIFT16 : p.lift;
-    float m[QB], mn[QB];            // running maximum; lift minus it (0 while it is -inf)
+    float m[QB], mn[QB];            // running maximum; lift minus it (lift while it is -inf)
+    bool far = false;               // a row's maximum is far from zero: scores come to the weights less it, in log2
 #pragma unroll
     for (int qb = 0; qb < QB; qb++) {
         m[qb] = -INFINITY;
-        mn[qb] = 0.f;
+        mn[qb] = lift;
         l[qb] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int db = 0; db < DH / 16; db++) o[db][qb] = floatx4{0.f, 0.f, 0.f, 0.f};
@@ -285,29 +290,43 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_cross_attn(const Cross
             top[qb] = t * p.sc;
         }
     };
-    auto rescale = [&](const float (&top)[QB]) {
+    auto rescale = [&](const float (&top)[QB], floatx4 (&s)[2][QB]) {
+#pragma clang fp contract(off)  // tops are rounded products, and so are far scores, which are then at most 8 above m
         bool moves = false;
 #pragma unroll
-        for (int qb = 0; qb < QB; qb++) moves |= top[qb] > m[qb] + XRESCALE;  // from -inf: any score that is not
-        if (!__any(moves)) return;
+        for (int qb = 0; qb < QB; qb++) moves |= top[qb] - m[qb] > XRESCALE;  // from -inf: any score that is not
+        if (__any(moves)) {
+            bool big = false;
 #pragma unroll
-        for (int qb = 0; qb < QB; qb++) {
-            const float t = fmaxf(m[qb], quad_max(top[qb]));
-            const float f = t > m[qb] ? __builtin_amdgcn_exp2f(m[qb] - t) : 1.f;
-            m[qb] = t;
-            mn[qb] = t == -INFINITY ? 0.f : lift - t;
-            l[qb] *= f;
+            for (int qb = 0; qb < QB; qb++) {
+                const float t = fmaxf(m[qb], quad_max(top[qb]));
+                const float f = t > m[qb] ? __builtin_amdgcn_exp2f(m[qb] - t) : 1.f;
+                m[qb] = t;
+                big |= fabsf(t) > XFAR && t != -INFINITY;
+                l[qb] *= f;
 #pragma unroll
-            for (int db = 0; db < DH / 16; db++) o[db][qb] *= f;
+                for (int db = 0; db < DH / 16; db++) o[db][qb] *= f;
+            }
+            far = __any(big);
+#pragma unroll
+            for (int qb = 0; qb < QB; qb++) mn[qb] = far || m[qb] == -INFINITY ? lift : lift - m[qb];
+        }
+        if (far) {
+#pragma unroll
+            for (int qb = 0; qb < QB; qb++)
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    s[i / 4][qb][i % 4] = s[i / 4][qb][i % 4] * p.sc - (m[qb] == -INFINITY ? 0.f : m[qb]);
         }
     };
     auto weights = [&](const floatx4 (&s)[2][QB], u32x4 (&pf)[QB]) {
+        const float sc = far ? 1.f : p.sc;
 #pragma unroll
         for (int qb = 0; qb < QB; qb++)
 #pragma unroll
             for (int i = 0; i < 4; i++)
-                pf[qb][i] = M::pack(__builtin_amdgcn_exp2f(fmaf(s[i / 2][qb][2 * i % 4], p.sc, mn[qb])),
-                                    __builtin_amdgcn_exp2f(fmaf(s[i / 2][qb][2 * i % 4 + 1], p.sc, mn[qb])));
+                pf[qb][i] = M::pack(__builtin_amdgcn_exp2f(fmaf(s[i / 2][qb][2 * i % 4], sc, mn[qb])),
+                                    __builtin_amdgcn_exp2f(fmaf(s[i / 2][qb][2 * i % 4 + 1], sc, mn[qb])));
     };
 
     if constexpr (C::SHARED) {
@@ -346,7 +365,7 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_cross_attn(const Cross
             read_k((st + 1) % NS * C::STAGE, kf);
 #pragma unroll
             for (int db = 0; db < DH / 16; db++) vf[db] = read_v(st * C::STAGE, db);
-            rescale(top);
+            rescale(top, s[cur]);
             __builtin_amdgcn_sched_barrier(0);
             weights(s[cur], pf);
             scores(kf, s[cur ^ 1]);
@@ -403,7 +422,7 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_cross_attn(const Cross
             scores(kf, s);
             hide(j, s);
             largest(s, top);
-            rescale(top);
+            rescale(top, s);
             weights(s, pf);
 #pragma unroll
             for (int qb = 0; qb < QB; qb++) l[qb] = M::mul(ones, pf[qb], l[qb]);

@@ -55,3 +55,43 @@ def test_one_bf16_key(gpu):
     v = torch.full_like(k, 3e36)
     out = ka.cross_attn(torch.empty_like(q), q, k, v, 4)
     assert torch.equal(out, v.expand_as(out))
+
+
+@pytest.mark.parametrize("B,Tq,Tk,Hq,Hkv,Dh", SHAPES)
+@pytest.mark.parametrize("dt,e,sign", [(torch.float16, e, s) for e, s in ((10, 1), (17, 1), (20, -1), (26, 1), (26, -1), (30, 1), (30, -1))] +
+                         [(torch.bfloat16, e, s) for e, s in ((10, -1), (17, 1), (20, 1), (26, -1), (30, 1), (36, -1), (60, 1), (100, -1))])
+def test_scores_far_from_zero(gpu, B, Tq, Tk, Hq, Hkv, Dh, dt, e, sign):
+    """Scores of +-2^e and twelve steps beside it, which rise along the keys for even heads and fall for odd ones: steps of 1 up to
+    e = 20, where every key counts, of 2^(e - 22) from e = 26 on, where the keys of the largest score share the output."""
+    near = e <= 20
+    a = 0 if near else (e - 22) // 2
+    b = 0 if near else e - 22 - a
+    q, k, v = make(B, Tq, Tk, Hq, Hkv, Dh, dt)
+    q, k = torch.zeros_like(q), torch.zeros_like(k)
+    qv, kv = q.view(B, Tq, Hq, Dh), k.view(B, Tk, Hkv, Dh)
+    qv[..., 0], kv[..., 0] = 2.0 ** (e // 2), sign * 2.0 ** (e - e // 2)
+    qv[:, :, 0::2, 1], qv[:, :, 1::2, 1] = 2.0 ** a, -(2.0 ** a)
+    j = torch.arange(Tk, device=DEV) * 12 // Tk
+    kv[..., 1] = (j * 2.0 ** b)[None, :, None].to(dt)
+    step = 2.0 ** (a + b)
+    p = torch.softmax(torch.stack([j * step, -j * step]).double(), -1)[torch.arange(Hq, device=DEV) % 2]  # [Hq, Tk]
+    vv = v.double().view(B, Tk, Hkv, Dh).repeat_interleave(Hq // Hkv, 2)
+    over = lambda x: (p.t()[None, :, :, None] * x).sum(1).reshape(B, 1, Hq * Dh)  # noqa: E731
+    ref, mag = over(vv), over(vv.abs())
+    u = torch.finfo(dt).eps / 2
+    # P rounded to the type; sums; exp2, the rescales and the division. The scores are exact in fp32; times log2 e they are off by
+    # half a unit of 2^e's last place, d = 2^(e - 24), the key's and the maximum's: weights within 2^(2 d), their share within 2^(4 d).
+    # From e = 26 on a key of the next score has at most 2^(-1.44 2^(e - 22) + 2 d) <= 2^-15 of the weight of one of the largest,
+    # and there are at most as many of each score as one more than of another: twice 11 in all, and what they hold
+    rel = u + (Tk / 4 + 64) * 2.0 ** -24 + 2.0 ** -21
+    tol = (rel + (2.0 ** (4 * 2.0 ** (e - 24)) - 1 if near else 0)) * mag
+    if not near:
+        tol = tol + 44 * 2.0 ** -15 * vv.abs().amax(1).reshape(B, 1, Hq * Dh)
+    if dt == torch.float16:
+        tol = tol + 2.0 ** -32 * vv.abs().sum(1).reshape(B, 1, Hq * Dh)
+    tol = tol + u * (ref.abs() + tol) + torch.finfo(dt).smallest_normal * u
+    for out in both(q, k, v, Hq, Hkv, scale=1.0):
+        err = (out.double() - ref).abs()
+        print(f"[cross_attn] {B} {Tq} {Tk} {Hq} {Hkv} {Dh} {dt} 2^{e}: worst error / tolerance {(err / tol).max():.3f}", flush=True)
+        assert torch.isfinite(out).all()
+        assert (err <= tol).all()
