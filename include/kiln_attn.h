@@ -395,7 +395,7 @@ int kiln_rope(void* y, int ldy, const void* x, int ldx, int dtype, int T, int H,
               int pos0, const double* freqs, float mscale, kiln_stream_t stream);
 
 /* Attention of B items of Tq queries to Tk encoder states of another length, Hq query heads on Hkv key heads (query head h
- * reads key head h Hkv / Hq; Hq % Hkv == 0), Dh 64 or 128: out = softmax(scale Q K^T) V. q [Tq, ldq], k, v [Tk, ld*], out
+ * reads key head h Hkv / Hq; Hq % Hkv == 0), Dh 64 or 128: out = softmax(scale Q K^T) V, 0 < scale <= 2^127. q [Tq, ldq], k, v [Tk, ld*], out
  * [Tq, ldo] per item in dtype (F16 or BF16), items bs* elements apart (0: all items share it, inputs only; items' outputs
  * one behind the other, or side by side in rows of all of them, and apart from the inputs); 16-byte aligned
  * rows and item strides (KILN_EUNSUPPORTED otherwise), ld <= 2^24. Item b's keys are the states below klen[b] (device [B],

@@ -114,7 +114,8 @@ int kiln_cross_attn(void* out, int ldo, long long bso, const void* q, int ldq, l
     if (B < 0 || Tq < 0 || Tk < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv)
         return fail(KILN_EINVAL, "cross_attn: bad sizes B=%d Tq=%d Tk=%d Hq=%d Hkv=%d", B, Tq, Tk, Hq, Hkv);
     if (Dh != 64 && Dh != 128) return fail(KILN_EUNSUPPORTED, "cross_attn: head size %d (64 or 128)", Dh);
-    if (!(scale > 0.f) || !isfinite(scale)) return fail(KILN_EINVAL, "cross_attn: scale %g must be positive", (double)scale);
+    if (!(scale > 0.f) || !isfinite(scale * kiln::LOG2E))
+        return fail(KILN_EINVAL, "cross_attn: scale %g must be positive, and finite times log2(e)", (double)scale);
     if (!B || !Tq) return KILN_OK;
     if (!out || !q || (Tk && (!k || !v))) return fail(KILN_EINVAL, "cross_attn: null pointer");
     const long long G = Hq / Hkv, rows = Tq * G;
