@@ -363,7 +363,7 @@ int kiln_dit_cross_attn_x16(void* out, void* out_neg, int out_dtype, int ldo, co
  * The attention section over an encoder's states: rotary positions, cross-attention, MXFP4 linear layers. Activations
  * are [T, ld] rows as above, in KILN_F32, KILN_F16 or KILN_BF16 (cross-attention: the 16-bit types). Inference only, as
  * all of this library; calls are stream-ordered, allocate nothing, never synchronize, and may be captured into a graph.
- * Repeated calls give the same bits.
+ * Repeated calls give the same bits. A call's outputs and workspace are apart from its other buffers, unless it says otherwise.
  * ------------------------------------------------------------------------------------------ */
 
 /* How a model's rotary frequencies f_i = theta^(-2 i / rot), i < rot / 2, are stretched for contexts `factor` times the
@@ -425,7 +425,8 @@ int kiln_mxfp4_dequantize(void* y, int dtype, int ldy, const uint8_t* codes, con
 /* kiln_linear16's layer with an MXFP4 weight and the rows of x quantised to MXFP4 within the call: y = epilogue(Q(x) W^T), on
  * the scaled 4-bit matrix cores, products exact, sums fp32. x [T, cols] rows of ldx in dtype (F32, F16, BF16); epilogues as
  * kiln_linear16 (kiln_epi: fp32 or fp16 y, GELU, gated residual), any rows, T, ldy >= rows and alignment (y rows of 4 elements'
- * alignment are fastest), cols % 32 == 0. A LoRA pair is a kiln_linear16 call with KILN_EPI_F32, beta = 1 or KILN_EPI_RESID on
+ * alignment are fastest), cols % 32 == 0. x and y share no byte (KILN_EINVAL; columns side by side in rows of one stride are
+ * apart). A LoRA pair is a kiln_linear16 call with KILN_EPI_F32, beta = 1 or KILN_EPI_RESID on
  * the same y. wp: the weight's codes and scales in the product's layout, from kiln_linear_mxfp4_prepare_weight (which converts
  * plain codes and scales, e.g. a checkpoint's or kiln_mxfp4_quantize's; 16-byte aligned). workspace:
  * kiln_linear_mxfp4_workspace_bytes (the quantised rows; 0 for few rows), 16-byte aligned (KILN_ENOMEM if smaller). The order of

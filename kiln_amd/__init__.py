@@ -817,7 +817,7 @@ def linear_mxfp4_tile(T, rows, cols):
 
 def linear_mxfp4(y, x, w, epi=KILN_EPI_F32, gate=None, beta=0.0, workspace=None, stream=None):
     """linear16's layer with an MXFP4 weight (kiln_linear_mxfp4): y [T, rows] = epilogue(Q(x) w^T), x [T, cols] fp32, fp16 or
-    bf16, w an Mxfp4Weight, y fp32 (F32, RESID) or fp16 (F16, GELU16). workspace: linear_mxfp4_workspace_bytes; None takes
+    bf16, w an Mxfp4Weight, y fp32 (F32, RESID) or fp16 (F16, GELU16), apart from x. workspace: linear_mxfp4_workspace_bytes; None takes
     one for the call."""
     dev = _gpu(x, y, w.buf, gate, workspace)
     rows, cols = w.shape

@@ -23,17 +23,15 @@ bool aligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 bool ld_ok(int ld, long long cols, int T) { return T <= 1 || ld >= cols; }
 constexpr int MAX_ROWS = 1 << 30;
 
-// Two [T, W] windows of rows share no element, or are one and the same
-bool apart_or_same(const void* x, long long ldx, const void* y, long long ldy, size_t esz, int T, long long W) {
-    const long long bx = (long long)(intptr_t)x, by = (long long)(intptr_t)y, e = (long long)esz;
-    if (T == 1) ldx = ldy = W;
-    if (bx == by && ldx == ldy) return true;
-    const long long ex = bx + ((T - 1) * ldx + W) * e, ey = by + ((T - 1) * ldy + W) * e;
+// Windows of T rows of wx and wy bytes, lx and ly bytes apart, share none
+bool apart(const void* x, long long lx, long long wx, const void* y, long long ly, long long wy, int T) {
+    const long long bx = (long long)(intptr_t)x, by = (long long)(intptr_t)y;
+    const long long ex = bx + (T - 1) * lx + wx, ey = by + (T - 1) * ly + wy;
     if (ex <= by || ey <= bx) return true;
-    if (ldx != ldy) return false;
+    if (T == 1 || lx != ly) return false;
     // columns side by side in one row stride
-    const long long ld = ldx * e, d = ((by - bx) % ld + ld) % ld;
-    return d >= W * e && ld - d >= W * e;
+    const long long d = ((by - bx) % lx + lx) % lx;
+    return d >= wx && lx - d >= wy;
 }
 
 }  // namespace
@@ -88,7 +86,8 @@ int kiln_rope(void* y, int ldy, const void* x, int ldx, int dtype, int T, int H,
     if (!ld_ok(ldx, W, T) || !ld_ok(ldy, W, T)) return fail(KILN_EINVAL, "rope: row stride %d or %d below %lld", ldx, ldy, W);
     if (!aligned(x, esize(dtype)) || !aligned(y, esize(dtype)) || !aligned(freqs, 8) || !aligned(pos, 4))
         return fail(KILN_EUNSUPPORTED, "rope: a pointer is not aligned to its elements");
-    if (!apart_or_same(x, ldx, y, ldy, esize(dtype), T, W)) return fail(KILN_EINVAL, "rope: x and y overlap");
+    const long long e = (long long)esize(dtype);
+    if (!(x == y && (T == 1 || ldx == ldy)) && !apart(x, ldx * e, W * e, y, ldy * e, W * e, T)) return fail(KILN_EINVAL, "rope: x and y overlap");
     return hip_check(kiln::launch_rope(y, (size_t)(T == 1 ? W : ldy), x, (size_t)(T == 1 ? W : ldx), (DT)dtype, T, H, Dh, rot,
                                        interleaved != 0, pos, pos0, freqs, mscale, (hipStream_t)stream),
                      "rope launch");
@@ -238,6 +237,10 @@ int kiln_linear_mxfp4(void* y, int ldy, const void* x, int dtype, int ldx, int T
     const size_t ye = epi == KILN_EPI_F32 || epi == KILN_EPI_RESID ? 4 : 2;
     if (!aligned(wp, 16) || !aligned(x, esize(dtype)) || !aligned(y, ye) || !aligned(gate, 4) || !aligned(workspace, 16))
         return fail(KILN_EUNSUPPORTED, "linear_mxfp4: alignment");
+    // in place the few-row form would read what other workgroups have written
+    const long long xe = (long long)esize(dtype);
+    if (!apart(x, ldx * xe, cols * xe, y, ldy * (long long)ye, rows * (long long)ye, T))
+        return fail(KILN_EINVAL, "linear_mxfp4: x and y overlap");
     const size_t need = kiln::linear_mx_workspace(T, rows, cols);
     if (need && (!workspace || ws_bytes < need))
         return fail(KILN_ENOMEM, "linear_mxfp4: workspace %zu bytes < %zu needed", workspace ? ws_bytes : (size_t)0, need);
