@@ -665,12 +665,25 @@ def _nbytes(workspace, what):
     return workspace.numel() * workspace.element_size()
 
 
+_I32 = (1 << 31) - 1  # ctypes drops what an int argument holds beyond 32 bits
+
+
+def _fits(what, *values):
+    for v in values:
+        if not -_I32 - 1 <= v <= _I32:
+            raise ValueError(f"{what}: {v} does not fit 32 bits")
+
+
 def _rows(t, what):
     """Shape and row stride of a 2-D tensor whose rows are contiguous (the stride of one row is its columns)."""
     shape, st = t.shape, t.stride()
     if len(st) != 2 or (st[1] != 1 and shape[1] > 1):
         raise ValueError(f"{what}: expected a 2-D tensor with contiguous rows, got shape {tuple(shape)} strides {st}")
-    return shape, st[0] if shape[0] > 1 else shape[1]
+    rows, cols = shape
+    ld = st[0] if rows > 1 else cols
+    if rows > _I32 or cols > _I32 or ld > _I32:
+        raise ValueError(f"{what}: shape {tuple(shape)} strides {st} do not fit 32 bits")
+    return shape, ld
 
 
 def rope_freqs(rot, theta=10000.0, scaling="none", factor=1.0, trained=0.0, slow=1.0, fast=None, device=None):
@@ -680,6 +693,7 @@ def rope_freqs(rot, theta=10000.0, scaling="none", factor=1.0, trained=0.0, slow
     import torch
     if scaling not in ROPE_SCALINGS:
         raise ValueError(f"rope_freqs: scaling {scaling!r}, expected one of {sorted(ROPE_SCALINGS)}")
+    _fits("rope_freqs: rot", rot)
     fast = (4.0 if scaling == "bands" else 32.0) if fast is None else fast
     freqs, mscale = torch.empty(max(rot, 2) // 2, dtype=torch.float64), ctypes.c_float()
     _check(lib().kiln_rope_freqs(_ptr(freqs), ctypes.byref(mscale), rot, theta, ROPE_SCALINGS[scaling], factor, trained, slow, fast))
@@ -697,6 +711,8 @@ def rope(y, x, H, Dh, freqs, pos=None, pos0=0, interleaved=False, mscale=1.0, st
         raise ValueError(f"rope: x {tuple(x.shape)} {x.dtype}, y {tuple(y.shape)} {y.dtype} for {H} heads of {Dh}")
     if freqs.element_size() != 8 or not freqs.is_floating_point() or not freqs.is_contiguous():
         raise ValueError("rope: freqs must be a contiguous float64 tensor (rope_freqs)")
+    if not -_I32 - 1 <= pos0 <= _I32 or freqs.numel() > _I32 // 2:
+        raise ValueError(f"rope: pos0 {pos0} or {freqs.numel()} frequencies do not fit 32 bits")
     if pos is not None and (pos.element_size() != 4 or pos.is_floating_point() or pos.numel() != T or not pos.is_contiguous()):
         raise ValueError(f"rope: pos must be a contiguous int32 tensor of {T} positions")
     _launch((_LIB or lib()).kiln_rope, dev, stream, y.data_ptr(), ldy, x.data_ptr(), ldx, _dt3(x), T, H, Dh, 2 * freqs.numel(),
@@ -705,12 +721,14 @@ def rope(y, x, H, Dh, freqs, pos=None, pos0=0, interleaved=False, mscale=1.0, st
 
 
 def cross_attn_workspace_bytes(B, Tq, Tk, Hq, Hkv, Dh):
+    _fits("cross_attn_workspace_bytes", B, Tq, Tk, Hq, Hkv, Dh)
     return lib().kiln_cross_attn_workspace_bytes(B, Tq, Tk, Hq, Hkv, Dh)
 
 
 def cross_attn_form(B, Tq, Tk, Hq, Hkv, Dh):
     """The form that cross_attn runs these sizes on: query rows of a workgroup, its waves that split the keys, and whether
     the keys are split over workgroups."""
+    _fits("cross_attn_form", B, Tq, Tk, Hq, Hkv, Dh)
     f = lib().kiln_cross_attn_form(B, Tq, Tk, Hq, Hkv, Dh)
     return f >> 16, f >> 8 & 0xff, bool(f & 1)
 
@@ -733,6 +751,11 @@ def cross_attn(out, q, k, v, Hq, Hkv=None, scale=None, klen=None, kmask=None, wo
     Dh = W // Hq
     if out.shape != q.shape or k.shape != (B, Tk, Hkv * Dh) or v.shape != k.shape:
         raise ValueError(f"cross_attn: shapes out {tuple(out.shape)} q {tuple(q.shape)} k {tuple(k.shape)} v {tuple(v.shape)}")
+    # row strides (a single row's means nothing)
+    ldo, ldq = (so[1], sq[1]) if Tq > 1 else (W, W)
+    ldk, ldv = (sk[1], sv[1]) if Tk > 1 else (Hkv * Dh, Hkv * Dh)
+    if max(B, Tq, Tk, W, ldo, ldq, ldk, ldv) > _I32:
+        raise ValueError(f"cross_attn: sizes {B}, {Tq}, {Tk}, {W} or row strides {ldo}, {ldq}, {ldk}, {ldv} do not fit 32 bits")
     if klen is not None and (klen.element_size() != 4 or klen.is_floating_point() or klen.numel() != B or not klen.is_contiguous()):
         raise ValueError(f"cross_attn: klen must be a contiguous int32 tensor of {B} lengths")
     if kmask is not None:
@@ -744,8 +767,8 @@ def cross_attn(out, q, k, v, Hq, Hkv=None, scale=None, klen=None, kmask=None, wo
         n = L.kiln_cross_attn_workspace_bytes(B, Tq, Tk, Hq, Hkv, Dh)
         if n:
             workspace = _scratch(n, dev, stream)
-    _launch(L.kiln_cross_attn, dev, stream, out.data_ptr(), so[1], so[0], q.data_ptr(), sq[1], sq[0], k.data_ptr(), sk[1], sk[0],
-            v.data_ptr(), sv[1], sv[0], _dt3(q), B, Tq, Tk, Hq, Hkv, Dh, Dh ** -0.5 if scale is None else scale,
+    _launch(L.kiln_cross_attn, dev, stream, out.data_ptr(), ldo, so[0], q.data_ptr(), ldq, sq[0], k.data_ptr(), ldk, sk[0],
+            v.data_ptr(), ldv, sv[0], _dt3(q), B, Tq, Tk, Hq, Hkv, Dh, Dh ** -0.5 if scale is None else scale,
             klen.data_ptr() if klen is not None else None, kmask.data_ptr() if kmask is not None else None,
             sm[0] if kmask is not None else 0, workspace.data_ptr() if workspace is not None else None,
             _nbytes(workspace, "cross_attn"))
@@ -753,6 +776,7 @@ def cross_attn(out, q, k, v, Hq, Hkv=None, scale=None, klen=None, kmask=None, wo
 
 
 def _mx_plain(codes, scales, rows, cols, what):
+    _fits(what, rows, cols)
     if codes.shape != (rows, cols // 2) or scales.shape != (rows, cols // 32) or codes.element_size() != 1 or \
             scales.element_size() != 1 or not codes.is_contiguous() or not scales.is_contiguous():
         raise ValueError(f"{what}: codes and scales must be contiguous uint8 tensors {[rows, cols // 2]} and {[rows, cols // 32]}, got "
@@ -806,11 +830,13 @@ def linear_mxfp4_weight(w, scales=None, stream=None):
 
 
 def linear_mxfp4_workspace_bytes(T, rows, cols):
+    _fits("linear_mxfp4_workspace_bytes", T, rows, cols)
     return lib().kiln_linear_mxfp4_workspace_bytes(T, rows, cols)
 
 
 def linear_mxfp4_tile(T, rows, cols):
     """The tile (weight rows, rows of x) that linear_mxfp4 runs these sizes on; 16 weight rows: the form that quantises x itself."""
+    _fits("linear_mxfp4_tile", T, rows, cols)
     t = lib().kiln_linear_mxfp4_tile(T, rows, cols)
     return t >> 16, t & 0xffff
 
@@ -821,6 +847,7 @@ def linear_mxfp4(y, x, w, epi=KILN_EPI_F32, gate=None, beta=0.0, workspace=None,
     one for the call."""
     dev = _gpu(x, y, w.buf, gate, workspace)
     rows, cols = w.shape
+    _fits("linear_mxfp4: epi", epi)
     (T, width), ldx = _rows(x, "linear_mxfp4: x")
     shape_y, ldy = _rows(y, "linear_mxfp4: y")
     if width != cols or shape_y != (T, rows):

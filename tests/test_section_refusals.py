@@ -48,3 +48,61 @@ def test_linear_mxfp4_side_by_side(L):
     for kw in (dict(y=Q + 256, ldx=256, ldy=256), dict(y=Q - 256, ldx=256, ldy=256), dict(y=Q + 256, ldx=384, ldy=192, epi=ka.KILN_EPI_F32),
                dict(y=Q + 512, dt=F32, ldx=192, ldy=384), dict(y=Q + 200 * 256), dict(y=Q - 200 * 256), dict(y=Q + 199 * 256 + 256, ldy=999)):
         assert linear(L, **kw) == ENOMEM, kw
+
+
+def far_views(monkeypatch):
+    """The wrappers up to the launch, on tensors without memory: views whose strides and sizes pass 32 bits cost nothing."""
+    import torch
+    monkeypatch.setattr(ka, "_gpu", lambda *t: 0)
+
+    def launched(*a):
+        raise AssertionError("reached the launch")
+    monkeypatch.setattr(ka, "_launch", launched)
+    monkeypatch.setattr(ka, "_scratch", lambda n, dev, stream: torch.empty(n, dtype=torch.uint8, device="meta"))
+
+    def view(*shape, stride=None, dt=torch.float16):
+        t = torch.empty(1, dtype=dt, device="meta")
+        return torch.empty(shape, dtype=dt, device="meta") if stride is None else t.as_strided(shape, stride)
+    return torch, view
+
+
+BIG = 1 << 32
+
+
+def test_python_strides_past_32_bits(monkeypatch):
+    """A stride of 2^32 + W would arrive in the C ABI as W. (Of a single row it means nothing and passes.)"""
+    torch, view = far_views(monkeypatch)
+    f64 = view(64, dt=torch.float64)
+    for big in (BIG + 256, 1 << 31):
+        far, x = view(2, 256, stride=(big, 1)), view(2, 256)
+        w = ka.Mxfp4Weight(view(1 << 16, dt=torch.uint8), 256, 256)
+        codes, scales = view(2, 128, dt=torch.uint8), view(2, 8, dt=torch.uint8)
+        x3, far3 = view(2, 2, 256), view(2, 2, 256, stride=(512, big, 1))
+        calls = [lambda: ka.rope(far, x, 2, 128, f64), lambda: ka.rope(x, far, 2, 128, f64), lambda: ka.linear_mxfp4(far, x, w, epi=1),
+                 lambda: ka.linear_mxfp4(x, far, w, epi=1), lambda: ka.mxfp4_quantize(far, codes, scales), lambda: ka.mxfp4_dequantize(far, codes, scales)]
+        calls += [lambda i=i: ka.cross_attn(*[far3 if i == j else x3 for j in range(4)], 2) for i in range(4)]
+        for i, call in enumerate(calls):
+            with pytest.raises(ValueError, match="32 bits"):
+                call()
+    one, one3 = view(1, 256, stride=(BIG + 3, 1)), view(2, 1, 256, stride=(256, BIG + 8, 1))
+    for call in (lambda: ka.rope(one, one, 2, 128, f64), lambda: ka.cross_attn(one3, one3, one3, one3, 2)):
+        with pytest.raises(AssertionError, match="reached"):
+            call()
+
+
+def test_python_sizes_past_32_bits(monkeypatch):
+    torch, view = far_views(monkeypatch)
+    f64, u8, x = view(64, dt=torch.float64), torch.uint8, view(2, 256)
+    tall, wide = view(BIG + 2, 256), view(2, BIG + 256)
+    for call in (lambda: ka.rope(tall, tall, 2, 128, f64), lambda: ka.rope(x, x, 2, 128, f64, pos0=1 << 31), lambda: ka.rope(x, x, 2, 128, f64, pos0=-BIG),
+                 lambda: ka.rope(x, x, 2, 128, view((BIG + 64) // 2, dt=torch.float64)),
+                 lambda: ka.cross_attn(*[view(1, BIG + 2, 256)] * 2, *[view(1, 2, 256)] * 2, 2),
+                 lambda: ka.cross_attn(*[view(1, 2, 256)] * 2, *[view(1, BIG + 2, 256)] * 2, 2), lambda: ka.cross_attn(*[view(BIG + 2, 1, 256)] * 4, 2),
+                 lambda: ka.mxfp4_quantize(tall, view(BIG + 2, 128, dt=u8), view(BIG + 2, 8, dt=u8)),
+                 lambda: ka.mxfp4_dequantize(wide, view(2, BIG // 2 + 128, dt=u8), view(2, BIG // 32 + 8, dt=u8)),
+                 lambda: ka.linear_mxfp4_weight(view(BIG + 2, 128, dt=u8), view(BIG + 2, 8, dt=u8)), lambda: ka.rope_freqs(BIG + 64),
+                 lambda: ka.linear_mxfp4(x, x, ka.Mxfp4Weight(view(9, dt=u8), 256, 256), epi=BIG + 1),
+                 lambda: ka.cross_attn_workspace_bytes(1, 1, BIG + 8192, 16, 4, 128), lambda: ka.cross_attn_form(1, BIG + 1, 8, 1, 1, 64),
+                 lambda: ka.linear_mxfp4_workspace_bytes(BIG + 1000, 2048, 2048), lambda: ka.linear_mxfp4_tile(1, 64, BIG + 64)):
+        with pytest.raises(ValueError, match="32 bits"):
+            call()
