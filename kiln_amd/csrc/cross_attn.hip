@@ -639,7 +639,9 @@ static hipError_t cross_of(const CrossParams& p, XKind k, hipStream_t s) {
 }
 
 hipError_t launch_cross_attn(const CrossLaunch& c, hipStream_t s) {
-    const bool split = c.ws && c.ws_bytes >= cross_attn_workspace(c.B, c.Tq, c.Tk, c.Hq, c.Hkv, c.Dh);
+    // sizes that need no workspace run the same form with one and without
+    const size_t need = cross_attn_workspace(c.B, c.Tq, c.Tk, c.Hq, c.Hkv, c.Dh);
+    const bool split = need == 0 || (c.ws && c.ws_bytes >= need);
     const XForm f = cross_form(c.B, c.Tq, c.Tk, c.Hq, c.Hkv, c.Dh, split);
     CrossParams p{};
     p.q = c.q;

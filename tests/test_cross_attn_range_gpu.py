@@ -1,4 +1,4 @@
-"""kiln_cross_attn at the ends of its types' ranges: values up to the largest finite number, in every form."""
+"""kiln_cross_attn at the ends of its types' ranges: values up to the largest finite number, scores far from zero, in every form."""
 import pytest
 import torch
 
