@@ -224,8 +224,11 @@ inline void dit_cross_attention(uint16_t* out, uint16_t* out_neg, int ldo, const
 // Rotary frequencies and the factor on rotated values, on the host and on the device (kiln_rope_freqs).
 class RopeFreqs {
    public:
+    // fast left out: 4 turns over the trained length for the bands, 32 for the ramp
     explicit RopeFreqs(int rot, double theta = 10000.0, kiln_rope_scaling scaling = KILN_ROPE_NONE, double factor = 1.0,
-                       double trained = 0.0, double slow = 1.0, double fast = 32.0)
+                       double trained = 0.0, double slow = 1.0)
+        : RopeFreqs(rot, theta, scaling, factor, trained, slow, scaling == KILN_ROPE_BANDS ? 4.0 : 32.0) {}
+    RopeFreqs(int rot, double theta, kiln_rope_scaling scaling, double factor, double trained, double slow, double fast)
         : rot_(rot), host_(rot > 0 ? rot / 2 : 0) {
         check(kiln_rope_freqs(host_.data(), &mscale_, rot, theta, scaling, factor, trained, slow, fast), "rope_freqs");
         if (hipMalloc(&dev_, host_.size() * sizeof(double)) != hipSuccess) throw std::runtime_error("RopeFreqs: hipMalloc failed");
