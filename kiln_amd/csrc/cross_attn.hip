@@ -154,11 +154,13 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_cross_attn(const Cross
         uint8_t byte[8];  // all loads before the first is looked at
 #pragma unroll
         for (int i = 0; i < 8; i++) byte[i] = mask[min(key0 + 64 * i, (long long)L - 1)];
+        uint32_t word = 0;  // lane j < 16: the window's word j, stored as what tile_bits reads
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const unsigned long long m = __ballot((byte[i] != 0) & (key0 + 64 * i < L));
-            if (lane == i) *reinterpret_cast<unsigned long long*>(bits + (w & 1) * 16 + 2 * i) = m;
+            if (lane >> 1 == i) word = lane & 1 ? (uint32_t)(m >> 32) : (uint32_t)m;
         }
+        if (lane < 16) bits[(w & 1) * 16 + lane] = word;
         __builtin_amdgcn_wave_barrier();
     };
     auto tile_bits = [&](int j) -> uint32_t {
