@@ -23,10 +23,10 @@
 // keys of a row alike. While |m| is at most 2^20 that is a factor of 2^(1/16), in O and l alike; beyond, where it would grow out of
 // the weights' range, products are rounded as m was before it is taken off (`far`: a branch that a wave takes or not).
 //
-// Bound, with many rows, by matrix and vector work (16 multiply-adds, 16 exponentials, 8 conversions and some 14 maxima beside 34
-// products per wave and tile of 32 rows, Dh 128) at the clock that power leaves: 2 x 4096 x 4096, 16 heads of 128, 295 us, 930 TFLOP/s;
-// 2 x 4096 x 512 52 us, of which Q in and O out are ~15. With few rows by the keys' bytes: 8 x 1 x 8192, 16 heads on 4 of 128,
-// 134 MB in 25 us.
+// Bound, with many rows, by matrix and vector work in turn (16 multiply-adds, 16 exponentials, 8 conversions and some 14 maxima after
+// 16 and before 18 products per wave and tile of 32 rows, Dh 128): 2 x 4096 x 4096, 16 heads of 128, 277 us, 990 TFLOP/s, the matrix
+// cores busy 47% of the time; 2 x 4096 x 512 51 us, of which Q in and O out are ~15. With few rows by the keys' bytes: 8 x 1 x 8192,
+// 16 heads on 4 of 128, 134 MB in 25 us.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -332,9 +332,10 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_cross_attn(const Cross
     };
 
     if constexpr (C::SHARED) {
-        // The scores of tile j + 1 are computed between the exponentials of tile j, and its maxima between tile j's products
-        // with V, so that matrix and vector work overlap within a wave. K of tile j + 1 and V of tile j landed (past the last
-        // tile the copies go on with empty ranges, which keeps the count); every wave is done with K of tile j and V of tile
+        // A step computes the scores of tile j + 1 ahead of the weights and products of tile j. It would let the scores' products run
+        // beside the exponentials, but the branch around `hide` and the loop's break part them: as compiled, a wave's matrix and vector
+        // work follow each other, and overlap only with another wave's. K of tile j + 1 and V of tile j landed (past the
+        // last tile the copies go on with empty ranges, which keeps the count); every wave is done with K of tile j and V of tile
         // j - 1, whose places take K of tile j + NS and V of tile j + NS - 1. Stages are constants: the reads' offsets too.
         constexpr int NS = C::NS;
         static_assert(NS % 2 == 0, "the scores' two sets go with the stages");
@@ -587,7 +588,7 @@ static XForm cross_form(int B, int Tq, int Tk, int Hq, int Hkv, int Dh, bool spl
         return XForm{k, rt, (int)n, (int)(n == 1 ? tiles : ct)};
     };
     if (rows <= 16) {
-        // One row block, bound by the keys' bytes: single waves of 32 KB of LDS, five a CU, with ranges that fill the chip three
+        // One row block, bound by the keys' bytes: single waves of 32 KB of LDS and a mask's window, four a CU, with ranges that fill the chip three
         // times over (a shorter item's ranges past its length end at once), at least 4 tiles each. Few keys in four waves of
         // one workgroup need no merge. In us, four waves / ranges: 1 x 3000, 20 heads of 128 24.8 / 11.6; 1 x 2048, 16 of 64
         // 10.4 / 10.3; 4 x 512, 16 of 128 8.4 / 10.6; 64 x 100, 16 of 128 (1024 heads) 21.5 / 11.5 in one range.

@@ -259,13 +259,15 @@ static hipError_t mx_thin(MxGemmParams p, hipStream_t s) {
 // WN x WM waves of 16 NB x 16 MB blocks. A stage of the LDS ring holds one k block of 128: the tile's units of W and of x
 // (1 KB each) and their scales, all by LDS DMA in the operand layout, so that every operand read is 1 KB without conflicts.
 //
-// 256 x 256 (8 waves of 64 x 128): 8192^3 in 282 us with its quantise pass (25), 4.3 PFLOP/s; the matrix instructions alone, random operands
-// in registers, reach 6.9 on this chip (2.4 GHz gives way to 1.7 under the power limit, 9.3 on zeros), so that whatever else costs
-// energy costs time: three 1 KB operand reads per 8 products (four waves of 128 x 128 would need two, but their registers spill
-// into moves: 40% slower), the GELU, the stores. 6912 x 8192 x 2048 takes 76 us, with GELU 98. Two workgroups of 128 x 256 per CU
-// (one's epilogue beside the other's products, in step or staggered) measured the same.
-// 128 x 128 (4 waves of 64 x 64): bound by what a CU takes in, 57 GB/s while its lines come from beyond the L2, whatever the ring's
-// depth (4 to 9 stages) or the number of waves: 0.3 us for the 17 KB of a k block. 1537 x 2048 x 2048 in 10.4 us, fp32 out 12.3.
+// 256 x 256 (8 waves of 64 x 128): 8192^3 in 271 us with its quantise pass (36), 4.1 PFLOP/s, the matrix cores busy 64% of the product's
+// time at 1.74 GHz (alone, on random operands in registers, the matrix instructions reach 6.9 PFLOP/s on this chip at 1.7 GHz, on zeros
+// 9.2). Three 1 KB operand reads per 8 products; four waves of 128 x 128 would need two, but their registers spill into moves:
+// 40% slower. 6912 x 8192 x 2048 takes 75 us, with GELU 97, matrix cores busy 40% and 29%: 864 tiles in four rounds that would be
+// 3.4, and each round's start and epilogue. Two workgroups of 128 x 256 per CU (one's epilogue beside the other's products, in
+// step or staggered) measured the same.
+// 128 x 128 (4 waves of 64 x 64): 1537 x 2048 x 2048 in 10.4 us, fp32 out 12.7, about 0.3 us a k block of 17 KB whatever the ring's depth
+// (4 to 9 stages) or the number of waves. Two thirds of the requests hit the L2, next to nothing comes from HBM; what it waits
+// for is not known.
 template <int WN_, int WM_, int NB_, int MB_, int NST_, int WGS_>
 struct MxCfg {
     static constexpr int WN = WN_, WM = WM_, NB = NB_, MB = MB_, NST = NST_, WGS = WGS_, WAVES = WN * WM, THREADS = WAVES * 64;
