@@ -401,7 +401,7 @@ int kiln_rope(void* y, int ldy, const void* x, int ldx, int dtype, int T, int H,
  * rows and item strides (KILN_EUNSUPPORTED otherwise), ld <= 2^24. Item b's keys are the states below klen[b] (device [B],
  * clamped to 0 .. Tk; NULL: all) whose byte in kmask (device, [Tk] per item, bsm bytes apart; NULL: all) is not 0; what the
  * others hold does not matter, NaN included. A row without keys, or whose every score is -inf, gives zeros. Scores, maxima and
- * sums are fp32, the weights are rounded to dtype for the product with V. v may hold any finite value of dtype (bf16 values
+ * sums are fp32, in units of log2, the weights are rounded to dtype for the product with V. v may hold any finite value of dtype (bf16 values
  * below 2^-117 Tk lose accuracy). workspace: kiln_cross_attn_workspace_bytes, for
  * few rows against many keys, 16-byte aligned; NULL or a smaller one runs the call without splitting the keys over workgroups. */
 int kiln_cross_attn(void* out, int ldo, long long bso, const void* q, int ldq, long long bsq, const void* k, int ldk, long long bsk,

@@ -17,7 +17,7 @@
 // the weight and rounded to the inputs' type, half a step of it (2^-11 fp16, 2^-8 bf16) per weight, as far off as the output's own
 // rounding. The factor is in O and l alike. In fp16 it is 2^7: P is 2^15 at most, and weights down to 2^-32 of the largest count
 // (2^-25 without), of which a long context may have enough: 2^17 keys at 2^-25.5 are 2^-8.5 of the output. bf16 has fp32's
-// exponents, for weights and for values: there P sums to less than 1 over all keys (lift = -9 - log2 Tk, rounded down), so that no
+// exponents, for weights and for values: there P sums to less than 1 over all keys (lift = -9 - log2 Tk, to the integer below), so that no
 // finite value overflows on its way; at the other end, products with values below 2^-117 Tk leave fp32's normal range.
 // The exponent is one fma, s sc + (lift - m): exact products against a rounded m, off by half a unit of m's last place for all
 // keys of a row alike. While |m| is at most 2^20 that is a factor of 2^(1/16), in O and l alike; beyond, where it would grow out of
@@ -588,9 +588,9 @@ static XForm cross_form(int B, int Tq, int Tk, int Hq, int Hkv, int Dh, bool spl
         return XForm{k, rt, (int)n, (int)(n == 1 ? tiles : ct)};
     };
     if (rows <= 16) {
-        // One row block, bound by the keys' bytes: single waves of 32 KB of LDS and a mask's window, four a CU, with ranges that fill the chip three
-        // times over (a shorter item's ranges past its length end at once), at least 4 tiles each. Few keys in four waves of
-        // one workgroup need no merge. In us, four waves / ranges: 1 x 3000, 20 heads of 128 24.8 / 11.6; 1 x 2048, 16 of 64
+        // One row block, bound by the keys' bytes: single waves of 32 KB of LDS and a mask's windows, four a CU, with ranges that fill
+        // the chip three times over (a shorter item's ranges past its length end at once), at least 4 tiles each. Few keys in
+        // four waves of one workgroup need no merge. In us, four waves / ranges: 1 x 3000, 20 heads of 128 24.8 / 11.6; 1 x 2048, 16 of 64
         // 10.4 / 10.3; 4 x 512, 16 of 128 8.4 / 10.6; 64 x 100, 16 of 128 (1024 heads) 21.5 / 11.5 in one range.
         if (heads >= 2 * cus) return {X_ONE, 16, 1, (int)tiles};
         if (!split || (tiles <= 32 && heads <= cus)) return {X_FOUR, 16, 1, (int)tiles};
