@@ -70,7 +70,7 @@ int kiln_attn_workspace_release(void);
  * engine/src/kernels.cu:14-58, gpu.h:92-99). While enabled, every entry point records a hipEvent pair
  * on its stream under its category: attention (all attention entry points and the K/V prepare),
  * gemm_tc16 (linear16 and the projections of the fused DiT sections), gemm_fp32, matvec, norm,
- * layernorm, rope, nag, eltwise, w->f16, gemm_mxfp4, mxfp4. Not for use under HIP graph capture.
+ * layernorm, rope, nag, eltwise, w->f16, gemm_mxfp4, mxfp4, gemm_mxfp8, mxfp8. Not for use under HIP graph capture.
  * ------------------------------------------------------------------------------------------ */
 /* on != 0 starts a new profile (clears the previous one); 0 stops recording. */
 int kiln_prof_enable(int on);
@@ -439,6 +439,61 @@ size_t kiln_linear_mxfp4_workspace_bytes(int T, int rows, int cols);
 int kiln_linear_mxfp4_tile(int T, int rows, int cols);
 int kiln_linear_mxfp4(void* y, int ldy, const void* x, int dtype, int ldx, int T, const uint8_t* wp, int rows, int cols, int epi,
                       const float* gate, float beta, void* workspace, size_t ws_bytes, kiln_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
+ * A text encoder's layer: causal attention over packed prompts, the residual's addition with the RMS norm, linear layers of 8-bit rows.
+ * Conventions as in the section above: [T, ld] rows in KILN_F32, KILN_F16 or KILN_BF16 (attention: the 16-bit types), inference only,
+ * stream-ordered, nothing allocated, no synchronization, capture allowed, the same bits from repeated calls, outputs and workspace apart
+ * from the other buffers unless it says otherwise.
+ * ------------------------------------------------------------------------------------------ */
+
+/* Causal attention over B packed sequences, Hq query heads on Hkv key heads (query head h reads key head h Hkv / Hq; Hq % Hkv == 0), Dh 64
+ * or 128: out = softmax(scale Q K^T) V, 0 < scale <= 2^127. q [Tq, ldq], out [Tq, ldo], k, v [Tk, ld*] in dtype (F16 or BF16); 16-byte
+ * aligned rows (KILN_EUNSUPPORTED otherwise), ld <= 2^24.
+ * Sequence s holds the rows q_start[s] .. q_start[s + 1] - 1 of q and out (device [B + 1], ascending; NULL: one sequence of all rows, B = 1),
+ * nq of them, and the rows k_start[s] .. k_start[s] + k_len[s] - 1 of k and v (device [B] each; both NULL: the queries' own rows, Tk = Tq), nk
+ * of them. The queries are the last nq of the sequence's keys: query i sees its keys up to i + nk - nq. So whole prompts have nq = nk, a
+ * chunk behind cached keys nk > nq, single tokens nq = 1; places in a cache may be of any size and shared. Either may be 0.
+ * P keys of a prefix, pk, pv [P, ld*] (NULL with P = 0), stand in front of every sequence's own and are seen by all queries.
+ * A query without keys (nk < nq), or whose every score is -inf, gives zeros. What the keys hold that a query does not see does not matter to
+ * it, NaN included. Rows of out behind the last sequence (and before the first) are left as they are. Starts and lengths are read on the
+ * device and clamped to the tensors; rows that two sequences claim hold either's result.
+ * Scores, maxima and sums are fp32, in units of log2, the weights are rounded to dtype for the product with V. v may hold any finite value
+ * of dtype (bf16 values below 2^-117 (Tk + P) lose accuracy). workspace: kiln_prompt_attn_workspace_bytes, for few rows against many
+ * keys, 16-byte aligned; NULL or a smaller one runs the call without splitting the keys over workgroups. */
+int kiln_prompt_attn(void* out, int ldo, const void* q, int ldq, const void* k, int ldk, const void* v, int ldv, int dtype, int Tq, int Tk,
+                     int Hq, int Hkv, int Dh, float scale, int B, const int32_t* q_start, const int32_t* k_start, const int32_t* k_len,
+                     const void* pk, int ldpk, const void* pv, int ldpv, int P, void* workspace, size_t ws_bytes, kiln_stream_t stream);
+size_t kiln_prompt_attn_workspace_bytes(int B, int Tq, int Tk, int P, int Hq, int Hkv, int Dh);
+
+/* The residual's addition and the RMS norm: h = x + res, y = h / sqrt(mean(h^2) + eps) w per row of dim <= 32768 columns (w bf16 [dim], NULL = 1),
+ * in fp32 from the unrounded h; eps > 0. x [rows, ldx] in xdtype, res and h [rows, ld*] in rdtype (both NULL: y is the norm of x), y
+ * [rows, ldy] in ydtype, any alignment (rows of 16-byte multiples are fastest). h = res with ldh = ldr and y = x with the same type and
+ * stride are in place; other overlaps are refused. */
+int kiln_add_rmsnorm(void* y, int ydtype, int ldy, void* h, int ldh, const void* x, int xdtype, int ldx, const void* res, int rdtype, int ldr,
+                     const uint16_t* w_bf16, int rows, int dim, float eps, kiln_stream_t stream);
+/* The same with y as MXFP8 codes [rows, dim] and scales [rows, dim / 32] (below), the input of kiln_linear_mxfp8. dim % 32 == 0. */
+int kiln_add_rmsnorm_mxfp8(uint8_t* codes, uint8_t* scales, void* h, int ldh, const void* x, int xdtype, int ldx, const void* res, int rdtype,
+                           int ldr, const uint16_t* w_bf16, int rows, int dim, float eps, kiln_stream_t stream);
+
+/* MXFP8: the values of a row in blocks of 32 neighbours. A block's scale byte s stands for 2^(s - 127), the smallest power of two (not
+ * below 2^-127) of which the largest magnitude is at most 448 times; a value is an 8-bit code (e4m3: sign, 4 bits of exponent with bias 7,
+ * 3 of mantissa, no infinities, 0x7f and 0xff NaN), the one nearest to it over the scale (ties to the even code). A block with an
+ * infinity or a NaN has scale byte 255 and stands for NaNs. codes [rows, cols], scales [rows, cols / 32], both dense; codes 16-byte
+ * aligned. cols % 32 == 0 (KILN_EUNSUPPORTED otherwise). */
+int kiln_mxfp8_quantize(uint8_t* codes, uint8_t* scales, const void* x, int dtype, int ldx, int rows, int cols, kiln_stream_t stream);
+/* The values that codes and scales stand for (exact in F32 and, down to its subnormals, in BF16; rounded in F16 outside its range). */
+int kiln_mxfp8_dequantize(void* y, int dtype, int ldy, const uint8_t* codes, const uint8_t* scales, int rows, int cols,
+                          kiln_stream_t stream);
+
+/* kiln_linear_mxfp4's layer for rows that are MXFP8 already: y = epilogue(X W^T), on the scaled matrix cores, products exact, sums fp32.
+ * codes [T, cols] (16-byte aligned) and scales [T, cols / 32] dense, as kiln_add_rmsnorm_mxfp8 and kiln_mxfp8_quantize write them; wp as
+ * for kiln_linear_mxfp4; epilogues, y and its alignment as there, any rows and T, cols % 32 == 0, cols <= 2^22. y is apart from
+ * the codes and scales (KILN_EINVAL). No workspace. The order of a row's sum follows the sizes, as for kiln_linear16. */
+int kiln_linear_mxfp8(void* y, int ldy, const uint8_t* codes, const uint8_t* scales, int T, const uint8_t* wp, int rows, int cols, int epi,
+                      const float* gate, float beta, kiln_stream_t stream);
+/* Which tile a call runs on, for tests and profiles (weight rows << 16 | rows of X); 0 for sizes that the call refuses. */
+int kiln_linear_mxfp8_tile(int T, int rows, int cols, int epi);
 
 #ifdef __cplusplus
 }

@@ -110,6 +110,15 @@ _SIGS = {
     "kiln_linear_mxfp4_prepare_weight": (_i, [_vp, _vp, _vp, _i, _i, _vp]),
     "kiln_linear_mxfp4_workspace_bytes": (_sz, [_i, _i, _i]),
     "kiln_linear_mxfp4": (_i, [_vp, _i, _vp, _i, _i, _i, _vp, _i, _i, _i, _vp, _f, _vp, _sz, _vp]),
+    "kiln_prompt_attn": (_i, [_vp, _i, _vp, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _f, _i, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _vp, _sz,
+                              _vp]),
+    "kiln_prompt_attn_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i]),
+    "kiln_add_rmsnorm": (_i, [_vp, _i, _i, _vp, _i, _vp, _i, _i, _vp, _i, _i, _vp, _i, _i, _f, _vp]),
+    "kiln_add_rmsnorm_mxfp8": (_i, [_vp, _vp, _vp, _i, _vp, _i, _i, _vp, _i, _i, _vp, _i, _i, _f, _vp]),
+    "kiln_mxfp8_quantize": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _vp]),
+    "kiln_mxfp8_dequantize": (_i, [_vp, _i, _i, _vp, _vp, _i, _i, _vp]),
+    "kiln_linear_mxfp8": (_i, [_vp, _i, _vp, _vp, _i, _vp, _i, _i, _i, _vp, _f, _vp]),
+    "kiln_linear_mxfp8_tile": (_i, [_i, _i, _i, _i]),
 }
 
 _LIB = None
@@ -864,4 +873,159 @@ def linear_mxfp4(y, x, w, epi=KILN_EPI_F32, gate=None, beta=0.0, workspace=None,
     _launch(L.kiln_linear_mxfp4, dev, stream, y.data_ptr(), ldy, x.data_ptr(), _dt3(x), ldx, T, w.buf.data_ptr(), rows, cols, epi,
             gate.data_ptr() if gate is not None else None, beta, workspace.data_ptr() if workspace is not None else None,
             _nbytes(workspace, "linear_mxfp4"))
+    return y
+
+
+# ---------------------------------------------------------------------------------------------
+# a text encoder's layer (no counterpart in the reference's op layer)
+# ---------------------------------------------------------------------------------------------
+def prompt_attn_workspace_bytes(B, Tq, Tk, P, Hq, Hkv, Dh):
+    _fits("prompt_attn_workspace_bytes", B, Tq, Tk, P, Hq, Hkv, Dh)
+    return lib().kiln_prompt_attn_workspace_bytes(B, Tq, Tk, P, Hq, Hkv, Dh)
+
+
+def _ints(t, n, what):
+    if t.element_size() != 4 or t.is_floating_point() or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous int32 tensor of {n}")
+
+
+def prompt_attn(out, q, k, v, Hq, Hkv=None, q_start=None, k_start=None, k_len=None, prefix=None, scale=None, workspace=None, stream=None):
+    """Causal attention over packed sequences (kiln_prompt_attn): q, out [Tq, Hq*Dh], k, v [Tk, Hkv*Dh] rows, fp16 or bf16, Dh 64 or 128.
+    q_start: int32 [B + 1], where each sequence's queries begin (the last entry: where the last one's end), or None for one sequence of all
+    rows. k_start, k_len: int32 [B], each sequence's keys, the last of which are its queries' own; None: the queries' rows. prefix: (k, v)
+    [P, Hkv*Dh] that every query sees, or None. scale defaults to Dh^-0.5. workspace: prompt_attn_workspace_bytes; None takes one for the
+    call."""
+    pk, pv = (None, None) if prefix is None else prefix
+    dev = _gpu(q, out, k, v, q_start, k_start, k_len, pk, pv, workspace)
+    Hkv = Hq if Hkv is None else Hkv
+    (Tq, W), ldq = _rows(q, "prompt_attn: q")
+    shape_o, ldo = _rows(out, "prompt_attn: out")
+    (Tk, Wk), ldk = _rows(k, "prompt_attn: k")
+    shape_v, ldv = _rows(v, "prompt_attn: v")
+    if not out.dtype == q.dtype == k.dtype == v.dtype:
+        raise ValueError(f"prompt_attn: out is {out.dtype}, q {q.dtype}, k {k.dtype}, v {v.dtype}")
+    if Hq <= 0 or Hkv <= 0 or Hq % Hkv or W % Hq:
+        raise ValueError(f"prompt_attn: {W} columns, {Hq} query heads on {Hkv} key heads")
+    Dh = W // Hq
+    if shape_o != q.shape or Wk != Hkv * Dh or shape_v != k.shape:
+        raise ValueError(f"prompt_attn: shapes out {tuple(out.shape)} q {tuple(q.shape)} k {tuple(k.shape)} v {tuple(v.shape)}")
+    P = ldpk = ldpv = 0
+    if pk is not None:
+        (P, Wp), ldpk = _rows(pk, "prompt_attn: prefix k")
+        shape_pv, ldpv = _rows(pv, "prompt_attn: prefix v")
+        if Wp != Wk or shape_pv != pk.shape or not pk.dtype == pv.dtype == q.dtype:
+            raise ValueError(f"prompt_attn: prefix {tuple(pk.shape)} {pk.dtype} and {tuple(pv.shape)} {pv.dtype} for keys of {Wk} columns, {q.dtype}")
+    B = 1
+    if q_start is not None:
+        B = q_start.numel() - 1
+        if B < 0:
+            raise ValueError("prompt_attn: q_start needs an entry more than there are sequences")
+        _ints(q_start, B + 1, "prompt_attn: q_start")
+    if (k_start is None) != (k_len is None):
+        raise ValueError("prompt_attn: k_start and k_len go together")
+    if k_start is not None:
+        _ints(k_start, B, "prompt_attn: k_start")
+        _ints(k_len, B, "prompt_attn: k_len")
+    L = _LIB or lib()
+    if workspace is None:
+        n = L.kiln_prompt_attn_workspace_bytes(B, Tq, Tk, P, Hq, Hkv, Dh)
+        if n:
+            workspace = _scratch(n, dev, stream)
+    _launch(L.kiln_prompt_attn, dev, stream, out.data_ptr(), ldo, q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, _dt3(q), Tq, Tk, Hq,
+            Hkv, Dh, Dh ** -0.5 if scale is None else scale, B, q_start.data_ptr() if q_start is not None else None,
+            k_start.data_ptr() if k_start is not None else None, k_len.data_ptr() if k_len is not None else None,
+            pk.data_ptr() if P else None, ldpk, pv.data_ptr() if P else None, ldpv, P,
+            workspace.data_ptr() if workspace is not None else None, _nbytes(workspace, "prompt_attn"))
+    return out
+
+
+def add_rmsnorm(y, x, res=None, w=None, eps=1e-6, h=None, scales=None, stream=None):
+    """The residual's addition and the RMS norm (kiln_add_rmsnorm): h = x + res, y = h / sqrt(mean(h^2) + eps) * w per row; x, y [rows, dim]
+    fp32, fp16 or bf16, res and h of one of these types too, w bf16 [dim] or None. h None: the sum takes res's place. With scales (uint8
+    [rows, dim / 32]) y holds MXFP8 codes (uint8 [rows, dim], kiln_add_rmsnorm_mxfp8), the input of linear_mxfp8."""
+    h = res if h is None else h
+    if h is not None and res is None:
+        raise ValueError("add_rmsnorm: h without res")
+    dev = _gpu(x, y, res, h, w, scales)
+    shape, ldx = _rows(x, "add_rmsnorm: x")
+    rows, dim = shape
+    shape_y, ldy = _rows(y, "add_rmsnorm: y")
+    if shape_y != shape:
+        raise ValueError(f"add_rmsnorm: x {tuple(x.shape)}, y {tuple(y.shape)}")
+    ldr = ldh = rt = 0
+    if res is not None:
+        shape_r, ldr = _rows(res, "add_rmsnorm: res")
+        shape_h, ldh = _rows(h, "add_rmsnorm: h")
+        if shape_r != shape or shape_h != shape or res.dtype != h.dtype:
+            raise ValueError(f"add_rmsnorm: x {tuple(x.shape)}, res {tuple(res.shape)} {res.dtype}, h {tuple(h.shape)} {h.dtype}")
+        rt = _dt3(res)
+    if w is not None and (_dt3(w) != KILN_BF16 or w.numel() != dim or not w.is_contiguous()):
+        raise ValueError(f"add_rmsnorm: w must be a contiguous bfloat16 tensor of {dim}")
+    L = _LIB or lib()
+    hp, rp, wp = h.data_ptr() if h is not None else None, res.data_ptr() if res is not None else None, w.data_ptr() if w is not None else None
+    if scales is None:
+        _launch(L.kiln_add_rmsnorm, dev, stream, y.data_ptr(), _dt3(y), ldy, hp, ldh, x.data_ptr(), _dt3(x), ldx, rp, rt, ldr, wp, rows, dim, eps)
+    else:
+        _mx8_plain(y, scales, rows, dim, "add_rmsnorm")
+        _launch(L.kiln_add_rmsnorm_mxfp8, dev, stream, y.data_ptr(), scales.data_ptr(), hp, ldh, x.data_ptr(), _dt3(x), ldx, rp, rt, ldr, wp, rows,
+                dim, eps)
+    return y
+
+
+def _mx8_plain(codes, scales, rows, cols, what):
+    _fits(what, rows, cols)
+    if codes.shape != (rows, cols) or scales.shape != (rows, cols // 32) or codes.element_size() != 1 or scales.element_size() != 1 or \
+            not codes.is_contiguous() or not scales.is_contiguous():
+        raise ValueError(f"{what}: codes and scales must be contiguous uint8 tensors {[rows, cols]} and {[rows, cols // 32]}, got "
+                         f"{codes.dtype} {list(codes.shape)} and {scales.dtype} {list(scales.shape)}")
+
+
+def mxfp8_quantize(x, codes=None, scales=None, stream=None):
+    """x [rows, cols] (fp32, fp16 or bf16, cols % 32 == 0) to MXFP8 (kiln_mxfp8_quantize): uint8 codes [rows, cols] and scales
+    [rows, cols / 32]."""
+    dev, (rows, cols), ldx = _gpu(x, codes, scales), *_rows(x, "mxfp8_quantize: x")
+    if codes is None or scales is None:
+        if codes is not None or scales is not None:
+            raise ValueError("mxfp8_quantize: codes and scales go together")
+        import torch
+        with torch.cuda.stream(stream):
+            codes = torch.empty(rows, cols, dtype=torch.uint8, device=x.device)
+            scales = torch.empty(rows, cols // 32, dtype=torch.uint8, device=x.device)
+    _mx8_plain(codes, scales, rows, cols, "mxfp8_quantize")
+    _launch((_LIB or lib()).kiln_mxfp8_quantize, dev, stream, codes.data_ptr(), scales.data_ptr(), x.data_ptr(), _dt3(x), ldx, rows, cols)
+    return codes, scales
+
+
+def mxfp8_dequantize(y, codes, scales, stream=None):
+    """The values of MXFP8 codes and scales (kiln_mxfp8_dequantize) into y [rows, cols]."""
+    dev, (rows, cols), ldy = _gpu(y, codes, scales), *_rows(y, "mxfp8_dequantize: y")
+    _mx8_plain(codes, scales, rows, cols, "mxfp8_dequantize")
+    _launch((_LIB or lib()).kiln_mxfp8_dequantize, dev, stream, y.data_ptr(), _dt3(y), ldy, codes.data_ptr(), scales.data_ptr(), rows, cols)
+    return y
+
+
+def linear_mxfp8_tile(T, rows, cols, epi=KILN_EPI_F32):
+    """The tile (weight rows, rows of x) that linear_mxfp8 runs these sizes on."""
+    _fits("linear_mxfp8_tile", T, rows, cols, epi)
+    t = lib().kiln_linear_mxfp8_tile(T, rows, cols, epi)
+    return t >> 16, t & 0xffff
+
+
+def linear_mxfp8(y, codes, scales, w, epi=KILN_EPI_F32, gate=None, beta=0.0, stream=None):
+    """linear_mxfp4's layer for rows that are MXFP8 already (kiln_linear_mxfp8): y [T, rows] = epilogue(X w^T), X by its uint8 codes [T, cols]
+    and scales [T, cols / 32] (add_rmsnorm, mxfp8_quantize), w an Mxfp4Weight, y fp32 (F32, RESID) or fp16 (F16, GELU16)."""
+    dev = _gpu(codes, scales, y, w.buf, gate)
+    rows, cols = w.shape
+    _fits("linear_mxfp8: epi", epi)
+    shape_y, ldy = _rows(y, "linear_mxfp8: y")
+    T = shape_y[0]
+    if shape_y[1] != rows:
+        raise ValueError(f"linear_mxfp8: y {tuple(y.shape)} for a weight [{rows}, {cols}]")
+    _mx8_plain(codes, scales, T, cols, "linear_mxfp8")
+    if _dt3(y) != (KILN_F32 if epi in (KILN_EPI_F32, KILN_EPI_RESID) else KILN_F16):
+        raise ValueError(f"linear_mxfp8: y is {y.dtype} with epilogue {epi}")
+    if gate is not None and (_dt3(gate) != KILN_F32 or gate.numel() != rows or not gate.is_contiguous()):
+        raise ValueError(f"linear_mxfp8: gate must be a contiguous float32 tensor of {rows}")
+    _launch((_LIB or lib()).kiln_linear_mxfp8, dev, stream, y.data_ptr(), ldy, codes.data_ptr(), scales.data_ptr(), T, w.buf.data_ptr(), rows, cols,
+            epi, gate.data_ptr() if gate is not None else None, beta)
     return y

@@ -29,7 +29,7 @@ FLAGS = [
 ]
 # Sources whose results rest on NaN arithmetic: linear_f32.hip finds by a NaN sum the outputs that it recomputes; the
 # others pass NaNs and infinities on by their formulas
-NAN_SOURCES = {"linear_f32.hip", "rope.hip", "cross_attn.hip", "mxfp4.hip", "gemm_mxfp4.hip"}
+NAN_SOURCES = {"linear_f32.hip", "rope.hip", "cross_attn.hip", "mxfp4.hip", "gemm_mxfp4.hip", "prompt_attn.hip", "add_rmsnorm.hip", "mxfp8.hip"}
 
 
 def flags(src):

@@ -14,27 +14,12 @@
 using kiln::DT;
 using namespace kiln::capi;
 
-namespace {
-
-bool dtype_ok(int d) { return d == KILN_F32 || d == KILN_F16 || d == KILN_BF16; }
-size_t esize(int d) { return d == KILN_F32 ? 4 : 2; }
-bool aligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
-// a row stride holds the row's columns (one row needs none)
-bool ld_ok(int ld, long long cols, int T) { return T <= 1 || ld >= cols; }
-constexpr int MAX_ROWS = 1 << 30;
-
-// Windows of T rows of wx and wy bytes, lx and ly bytes apart, share none
-bool apart(const void* x, long long lx, long long wx, const void* y, long long ly, long long wy, int T) {
-    const long long bx = (long long)(intptr_t)x, by = (long long)(intptr_t)y;
-    const long long ex = bx + (T - 1) * lx + wx, ey = by + (T - 1) * ly + wy;
-    if (ex <= by || ey <= bx) return true;
-    if (T == 1 || lx != ly) return false;
-    // columns side by side in one row stride
-    const long long d = ((by - bx) % lx + lx) % lx;
-    return d >= wx && lx - d >= wy;
+int kiln::capi::mx_sizes(const char* what, int rows, int cols) {
+    if (rows < 0 || cols <= 0) return fail(KILN_EINVAL, "%s: bad sizes rows=%d cols=%d", what, rows, cols);
+    if (cols % kiln::MXB) return fail(KILN_EUNSUPPORTED, "%s: cols %d must be a multiple of 32", what, cols);
+    if (rows > MAX_ROWS || cols > MAX_ROWS) return fail(KILN_EUNSUPPORTED, "%s: more than 2^30 rows or columns", what);
+    return KILN_OK;
 }
-
-}  // namespace
 
 extern "C" {
 
@@ -87,7 +72,7 @@ int kiln_rope(void* y, int ldy, const void* x, int ldx, int dtype, int T, int H,
     if (!aligned(x, esize(dtype)) || !aligned(y, esize(dtype)) || !aligned(freqs, 8) || !aligned(pos, 4))
         return fail(KILN_EUNSUPPORTED, "rope: a pointer is not aligned to its elements");
     const long long e = (long long)esize(dtype);
-    if (!(x == y && (T == 1 || ldx == ldy)) && !apart(x, ldx * e, W * e, y, ldy * e, W * e, T)) return fail(KILN_EINVAL, "rope: x and y overlap");
+    if (!(x == y && (T == 1 || ldx == ldy)) && !apart(x, ldx * e, W * e, T, y, ldy * e, W * e, T)) return fail(KILN_EINVAL, "rope: x and y overlap");
     return hip_check(kiln::launch_rope(y, (size_t)(T == 1 ? W : ldy), x, (size_t)(T == 1 ? W : ldx), (DT)dtype, T, H, Dh, rot,
                                        interleaved != 0, pos, pos0, freqs, mscale, (hipStream_t)stream),
                      "rope launch");
@@ -166,14 +151,6 @@ int kiln_cross_attn(void* out, int ldo, long long bso, const void* q, int ldq, l
     return hip_check(kiln::launch_cross_attn(c, (hipStream_t)stream), "cross_attn launch");
 }
 
-// rows x cols of an MXFP4 matrix: KILN_OK, or the refusal
-static int mx_sizes(const char* what, int rows, int cols) {
-    if (rows < 0 || cols <= 0) return fail(KILN_EINVAL, "%s: bad sizes rows=%d cols=%d", what, rows, cols);
-    if (cols % kiln::MXB) return fail(KILN_EUNSUPPORTED, "%s: cols %d must be a multiple of 32", what, cols);
-    if (rows > MAX_ROWS || cols > MAX_ROWS) return fail(KILN_EUNSUPPORTED, "%s: more than 2^30 rows or columns", what);
-    return KILN_OK;
-}
-
 int kiln_mxfp4_quantize(uint8_t* codes, uint8_t* scales, const void* x, int dtype, int ldx, int rows, int cols, kiln_stream_t stream) {
     kiln::prof::Scope prof_("mxfp4", (hipStream_t)stream);
     if (!dtype_ok(dtype)) return fail(KILN_EINVAL, "mxfp4_quantize: dtype %d", dtype);
@@ -239,7 +216,7 @@ int kiln_linear_mxfp4(void* y, int ldy, const void* x, int dtype, int ldx, int T
         return fail(KILN_EUNSUPPORTED, "linear_mxfp4: alignment");
     // in place the few-row form would read what other workgroups have written
     const long long xe = (long long)esize(dtype);
-    if (!apart(x, ldx * xe, cols * xe, y, ldy * (long long)ye, rows * (long long)ye, T))
+    if (!apart(x, ldx * xe, cols * xe, T, y, ldy * (long long)ye, rows * (long long)ye, T))
         return fail(KILN_EINVAL, "linear_mxfp4: x and y overlap");
     const size_t need = kiln::linear_mx_workspace(T, rows, cols);
     if (need && (!workspace || ws_bytes < need))

@@ -5,6 +5,7 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "../../include/kiln_attn.h"
 #include "internal.hpp"
 
 namespace kiln::capi {
@@ -25,6 +26,27 @@ int flash_self(void* out, DT od, int ldo, long long bso, const void* q, int ldq,
                long long bsk, const void* v, int ldv, long long bsv, DT in, int B, int Tq, int Tk, int H, int npad,
                const uint16_t* qw, const uint16_t* kw, float eps, const float* rc, const float* rs, void* ws,
                size_t ws_bytes, hipStream_t stream);
+
+// ---- checks of the entry points that take fp32, fp16 and bf16 rows ----
+constexpr int MAX_ROWS = 1 << 30;
+inline bool dtype_ok(int d) { return d == KILN_F32 || d == KILN_F16 || d == KILN_BF16; }
+inline size_t esize(int d) { return d == KILN_F32 ? 4 : 2; }
+inline bool aligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+// a row stride holds the row's columns (one row needs none)
+inline bool ld_ok(int ld, long long cols, int T) { return T <= 1 || ld >= cols; }
+// Windows of Tx rows of wx bytes lx bytes apart, and of Ty rows of wy bytes ly apart, share no byte (rows of different strides: by the
+// bytes from the first to the last)
+inline bool apart(const void* x, long long lx, long long wx, int Tx, const void* y, long long ly, long long wy, int Ty) {
+    const long long bx = (long long)(intptr_t)x, by = (long long)(intptr_t)y;
+    const long long ex = bx + (Tx - 1) * lx + wx, ey = by + (Ty - 1) * ly + wy;
+    if (ex <= by || ey <= bx) return true;
+    if (Tx == 1 || Ty == 1 || lx != ly) return false;
+    // columns side by side in one row stride
+    const long long d = ((by - bx) % lx + lx) % lx;
+    return d >= wx && lx - d >= wy;
+}
+// rows x cols of a microscaled matrix (blocks of 32): KILN_OK, or the refusal
+int mx_sizes(const char* what, int rows, int cols);
 
 }  // namespace kiln::capi
 

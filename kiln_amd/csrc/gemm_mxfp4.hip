@@ -1,5 +1,6 @@
 // The MXFP4 linear layer (kiln_linear_mxfp4): y = epilogue(Q(x) Wq^T) with v_mfma_scale_f32_16x16x128_f8f6f4, both operands
-// 4-bit codes with a scale per 32 values (mxfp4.hpp). Products of codes and powers of two are exact; sums are fp32.
+// 4-bit codes with a scale per 32 values (mxfp4.hpp). Products of codes and powers of two are exact; sums are fp32. The layer of MXFP8 rows
+// (kiln_linear_mxfp8) is compiled with it: gemm_mxfp8.hpp, included at the end.
 #include <hip/hip_runtime.h>
 
 #include <math.h>
@@ -102,6 +103,69 @@ __device__ __forceinline__ void mx_store(const MxGemmParams& p, int m, int n, fl
         } else {
             static_cast<_Float16*>(p.y)[off + e] = (_Float16)v[e];
         }
+    }
+}
+
+// The tile of a wave: acc[nb][mb] holds columns n0 + 16 nb + 4 (lane / 16) .. + 3 of row m0 + 16 mb + lane % 16. WAVES waves share the LDS
+// bytes of the ring that the products are done with (this function waits for the others').
+template <int EPI, int NB, int MB, int WAVES, int LDS>
+__device__ __forceinline__ void mx_store_tile(const MxGemmParams& p, const floatx4 (&acc)[NB][MB], uint8_t* lds8, int wv, int lane, int m0,
+                                              int n0) {
+    const int g = lane >> 4, rl = lane & 15;
+    if (p.vec < 2) {
+#pragma unroll
+        for (int mb = 0; mb < MB; mb++)
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++) mx_store<EPI>(p, m0 + mb * 16 + rl, n0 + nb * 16 + 4 * g, acc[nb][mb]);
+        return;
+    }
+    // Aligned rows leave through LDS as whole rows of the wave's columns, 16 bytes a lane, instead of 8- or 16-byte pieces of
+    // 16 rows per store. The wave's region holds RB row blocks; 16-byte chunks lie permuted by the row (both sides conflict-free).
+    constexpr bool F32 = EPI == KILN_EPI_F32 || EPI == KILN_EPI_RESID;
+    constexpr int RB = F32 ? MB / 2 : MB, CH = NB * 16 * (F32 ? 4 : 2) / 16, PER = F32 ? 4 : 8;  // chunks of a row, values of a chunk
+    static_assert(RB * 16 * CH * 16 * WAVES <= LDS, "the waves' regions fit in the ring");
+    uint8_t* stg = lds8 + wv * (RB * 16 * CH * 16);
+    __builtin_amdgcn_s_waitcnt(0xC07F);
+    __builtin_amdgcn_s_barrier();  // every wave is done with the ring
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int h = 0; h < MB / RB; h++) {
+#pragma unroll
+        for (int r = 0; r < RB; r++)
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++) {
+                floatx4 v = acc[nb][h * RB + r];
+                if constexpr (EPI == KILN_EPI_GELU16)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) v[e] = mx_gelu(v[e]);
+                const int row = r * 16 + rl;
+                if constexpr (F32)
+                    *reinterpret_cast<floatx4*>(stg + row * CH * 16 + ((nb * 4 + g) ^ (row & (CH - 1))) * 16) = v;
+                else
+                    *reinterpret_cast<half4*>(stg + row * CH * 16 + ((nb * 2 + (g >> 1)) ^ (row & (CH - 1))) * 16 + (g & 1) * 8) =
+                        half4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+            }
+        __builtin_amdgcn_wave_barrier();  // a wave's LDS operations keep their order
+#pragma unroll 4
+        for (int i = 0; i < RB * 16 * CH / 64; i++) {
+            const int row = (i * 64 + lane) / CH, c = (i * 64 + lane) % CH;
+            const u32x4 v = *reinterpret_cast<const u32x4*>(stg + row * CH * 16 + (c ^ (row & (CH - 1))) * 16);
+            const int m = m0 + h * RB * 16 + row, n = n0 + c * PER;
+            if (m >= p.T || n >= p.N) continue;
+            const size_t off = (size_t)m * p.ldy + n;
+            if constexpr (F32) {
+                const floatx4 f = __builtin_bit_cast(floatx4, v);
+                mx_store<EPI>(p, m, n, f);
+            } else if (n + PER <= p.N) {
+                *reinterpret_cast<u32x4*>(static_cast<_Float16*>(p.y) + off) = v;
+            } else {
+                const half8 hv = __builtin_bit_cast(half8, v);
+#pragma unroll
+                for (int e = 0; e < PER; e++)
+                    if (n + e < p.N) static_cast<_Float16*>(p.y)[off + e] = hv[e];
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
     }
 }
 
@@ -411,63 +475,8 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES * C::WGS / 4) void k_mx_gemm(c
     }
     if (i < p.kbs) step(i, std::integral_constant<int, 0>{});
     wait_vmcnt<0>();  // no copy into LDS outlives the ring
-    const int g = lane >> 4, rl = lane & 15;
     const int m0 = tm * C::BM + wm * MB * 16, n0 = tn * C::BN + wn * NB * 16;
-    if (p.vec < 2) {
-#pragma unroll
-        for (int mb = 0; mb < MB; mb++)
-#pragma unroll
-            for (int nb = 0; nb < NB; nb++) mx_store<EPI>(p, m0 + mb * 16 + rl, n0 + nb * 16 + 4 * g, acc[nb][mb]);
-        return;
-    }
-    // Aligned rows leave through LDS as whole rows of the wave's columns, 16 bytes a lane, instead of 8- or 16-byte pieces of
-    // 16 rows per store. The wave's region holds RB row blocks; 16-byte chunks lie permuted by the row (both sides conflict-free).
-    constexpr bool F32 = EPI == KILN_EPI_F32 || EPI == KILN_EPI_RESID;
-    constexpr int RB = F32 ? MB / 2 : MB, CH = NB * 16 * (F32 ? 4 : 2) / 16, PER = F32 ? 4 : 8;  // chunks of a row, values of a chunk
-    static_assert(RB * 16 * CH * 16 * C::WAVES <= C::LDS, "the waves' regions fit in the ring");
-    uint8_t* stg = lds8 + wv * (RB * 16 * CH * 16);
-    __builtin_amdgcn_s_waitcnt(0xC07F);
-    __builtin_amdgcn_s_barrier();  // every wave is done with the ring
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int h = 0; h < MB / RB; h++) {
-#pragma unroll
-        for (int r = 0; r < RB; r++)
-#pragma unroll
-            for (int nb = 0; nb < NB; nb++) {
-                floatx4 v = acc[nb][h * RB + r];
-                if constexpr (EPI == KILN_EPI_GELU16)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) v[e] = mx_gelu(v[e]);
-                const int row = r * 16 + rl;
-                if constexpr (F32)
-                    *reinterpret_cast<floatx4*>(stg + row * CH * 16 + ((nb * 4 + g) ^ (row & (CH - 1))) * 16) = v;
-                else
-                    *reinterpret_cast<half4*>(stg + row * CH * 16 + ((nb * 2 + (g >> 1)) ^ (row & (CH - 1))) * 16 + (g & 1) * 8) =
-                        half4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
-            }
-        __builtin_amdgcn_wave_barrier();  // a wave's LDS operations keep their order
-#pragma unroll 4
-        for (int i = 0; i < RB * 16 * CH / 64; i++) {
-            const int row = (i * 64 + lane) / CH, c = (i * 64 + lane) % CH;
-            const u32x4 v = *reinterpret_cast<const u32x4*>(stg + row * CH * 16 + (c ^ (row & (CH - 1))) * 16);
-            const int m = m0 + h * RB * 16 + row, n = n0 + c * PER;
-            if (m >= p.T || n >= p.N) continue;
-            const size_t off = (size_t)m * p.ldy + n;
-            if constexpr (F32) {
-                const floatx4 f = __builtin_bit_cast(floatx4, v);
-                mx_store<EPI>(p, m, n, f);
-            } else if (n + PER <= p.N) {
-                *reinterpret_cast<u32x4*>(static_cast<_Float16*>(p.y) + off) = v;
-            } else {
-                const half8 hv = __builtin_bit_cast(half8, v);
-#pragma unroll
-                for (int e = 0; e < PER; e++)
-                    if (n + e < p.N) static_cast<_Float16*>(p.y)[off + e] = hv[e];
-            }
-        }
-        __builtin_amdgcn_wave_barrier();
-    }
+    mx_store_tile<EPI, NB, MB, C::WAVES, C::LDS>(p, acc, lds8, wv, lane, m0, n0);
 #endif
 }
 
@@ -582,3 +591,6 @@ hipError_t launch_linear_mx(void* y, size_t ldy, const void* x, DT dt, size_t ld
 }
 
 }  // namespace kiln
+
+// the layer of MXFP8 rows shares the epilogues above
+#include "gemm_mxfp8.hpp"

@@ -1,0 +1,411 @@
+// The linear layer of MXFP8 rows with an MXFP4 weight (kiln_linear_mxfp8): y = epilogue(X W^T) with v_mfma_scale_f32_16x16x128_f8f6f4, W's
+// operand 4-bit codes, X's 8-bit ones, a scale per 32 values of each (mxfp4.hpp, mxfp8.hpp). Products of codes and powers of two are exact;
+// sums are fp32. W lies in the operand layout of mxfp4.hpp; X is read as it is, codes [T, K] and scales [T, K / 32].
+//
+// X's operand, 16 rows x 128 columns: lane l holds of row l % 16 the bytes 16 (l / 16) .. + 15 and 64 + 16 (l / 16) .. + 15, and the scale
+// of the block of 32 that W's lane l holds, columns 32 (l / 16) .. + 31 (so the bytes of a block lie in two lanes, as measured with single
+// ones in either operand).
+#pragma once
+
+namespace kiln {
+
+// W's scale byte is selected from a register of four row blocks'; X's is the lowest byte
+template <int J>
+__device__ __forceinline__ floatx4 mx8_mfma(u32x4 w, uint32_t sw, i32x8 x, uint32_t sx, floatx4 c) {
+    const i32x8 A = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, x, c, 4, 0, J, (int)sw, 0, (int)sx);  // 4: E2M1, 0: E4M3
+}
+__device__ __forceinline__ floatx4 mx8_mfma_at(int j, u32x4 w, uint32_t sw, i32x8 x, uint32_t sx, floatx4 c) {
+    switch (j) {  // a constant once the loops around are unrolled
+        case 0: return mx8_mfma<0>(w, sw, x, sx, c);
+        case 1: return mx8_mfma<1>(w, sw, x, sx, c);
+        case 2: return mx8_mfma<2>(w, sw, x, sx, c);
+        default: return mx8_mfma<3>(w, sw, x, sx, c);
+    }
+}
+// The instruction adds the products of eight neighbouring columns with 13 bits below the largest one's exponent, cutting off what lies lower (as
+// measured with single values), and their sums in fp32. X's codes span 2^18, so a fp32 result would be off by some 7e-6 of its size: for
+// fp32 outputs X's codes go in two parts, those from 2^2 on and the rest (`mx8_parts`), of which each group's products are exact to 2^-17 of
+// the block's largest value. fp16 outputs, rounded by up to 2^-11 of their size, take one product: half the matrix work.
+__device__ __forceinline__ void mx8_parts(i32x8 x, i32x8& hi, i32x8& lo) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const uint32_t w = (uint32_t)x[i];
+        // bit 7 of a byte: magnitude 0x48 (2^2) or more; NaN codes are among them
+        const uint32_t big = ((w & 0x7f7f7f7fu) + 0x38383838u) >> 7 & 0x01010101u;
+        const uint32_t h = w & big * 255u;
+        hi[i] = (int)h;
+        lo[i] = (int)(w ^ h);
+    }
+}
+template <int EPI>
+constexpr bool MX8_EXACT = EPI == KILN_EPI_F32 || EPI == KILN_EPI_RESID;
+
+__device__ __forceinline__ i32x8 mx8_join(u32x4 a, u32x4 b) {
+    return __builtin_bit_cast(i32x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// ---- few rows and small products: operands straight into registers ----
+//
+// A workgroup takes 16 NB weight rows x 16 MB rows of X; its eight waves share out the k blocks, each reading whole 1 KB units of W and
+// 16-byte pieces of X two k blocks ahead of their products, and meet in LDS.
+constexpr int THIN8_WAVES = 8;
+template <int EPI, int NB, int MB>
+__global__ __launch_bounds__(THIN8_WAVES * 64, 2) void k_mx8_thin(const MxGemmParams p) {
+    extern __shared__ __attribute__((aligned(16))) floatx4 thin8_red[];  // [wave][block][lane]
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int ti = (int)(blockIdx.x & 7) * p.per + (int)(blockIdx.x >> 3);  // an XCD's range: the row tiles of a W tile together
+    if (ti >= p.total) return;
+    const int tm = ti % p.tiles_m, tn = ti / p.tiles_m, nb0 = tn * NB, mb0 = tm * MB;
+    const int g = lane >> 4;
+    const size_t wrg = mx_rg(p.N);
+    const uint8_t* wc = p.wc + (size_t)nb0 * MX_UNIT + lane * 16;
+    const uint8_t* wsc = p.ws + (size_t)(nb0 >> 2) * MX_SUNIT + lane * 4;
+    const int wsh = 8 * (nb0 & 3);  // the tile's first block's byte of a scale unit
+    const uint8_t* xc[MB];
+    const uint8_t* xs[MB];
+#pragma unroll
+    for (int i = 0; i < MB; i++) {  // rows past the last read it again; their results are not stored
+        const size_t m = min((mb0 + i) * 16 + (lane & 15), p.T - 1);
+        xc[i] = p.xc + m * p.K;
+        xs[i] = p.xs + m * (p.K / 32);
+    }
+    struct Ops {
+        u32x4 w[NB], x[MB][2];
+        uint32_t sw, sx[MB];
+    } ops[2];
+    auto load = [&](Ops& o, int kb) {
+        kb = min(kb, p.kbs - 1);
+        const int k0 = kb * 128 + 16 * g, kz = p.K;
+#pragma unroll
+        for (int i = 0; i < NB; i++) o.w[i] = *reinterpret_cast<const u32x4*>(wc + (kb * wrg * 4 + i) * MX_UNIT);
+        o.sw = *reinterpret_cast<const uint32_t*>(wsc + kb * wrg * MX_SUNIT);
+        const bool in0 = k0 < kz, in1 = k0 + 64 < kz, ins = kb * 128 + 32 * g < kz;  // columns past the last: zeros
+#pragma unroll
+        for (int i = 0; i < MB; i++) {
+            o.x[i][0] = *reinterpret_cast<const u32x4*>(xc[i] + (in0 ? k0 : 0));
+            o.x[i][1] = *reinterpret_cast<const u32x4*>(xc[i] + (in1 ? k0 + 64 : 0));
+            o.sx[i] = xs[i][ins ? kb * 4 + g : 0];
+        }
+        if (kb * 128 + 128 > kz) {
+#pragma unroll
+            for (int i = 0; i < MB; i++) {
+                if (!in0) o.x[i][0] = u32x4{0, 0, 0, 0};
+                if (!in1) o.x[i][1] = u32x4{0, 0, 0, 0};
+                if (!ins) o.sx[i] = 0;
+            }
+        }
+    };
+    floatx4 acc[NB][MB];
+#pragma unroll
+    for (int i = 0; i < NB; i++)
+#pragma unroll
+        for (int j = 0; j < MB; j++) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+    auto mul = [&](const Ops& o) {
+        const uint32_t sw = o.sw >> wsh;
+#pragma unroll
+        for (int j = 0; j < MB; j++) {
+            i32x8 x = mx8_join(o.x[j][0], o.x[j][1]);
+            if constexpr (MX8_EXACT<EPI>) {
+                i32x8 hi;
+                mx8_parts(x, hi, x);
+#pragma unroll
+                for (int i = 0; i < NB; i++) acc[i][j] = mx8_mfma_at(i, o.w[i], sw, hi, o.sx[j], acc[i][j]);
+            }
+#pragma unroll
+            for (int i = 0; i < NB; i++) acc[i][j] = mx8_mfma_at(i, o.w[i], sw, x, o.sx[j], acc[i][j]);
+        }
+    };
+    load(ops[0], wv);
+    load(ops[1], wv + THIN8_WAVES);
+    for (int kb = wv; kb < p.kbs; kb += 2 * THIN8_WAVES) {
+        mul(ops[0]);
+        load(ops[0], kb + 2 * THIN8_WAVES);
+        if (kb + THIN8_WAVES < p.kbs) mul(ops[1]);
+        load(ops[1], kb + 3 * THIN8_WAVES);
+    }
+#pragma unroll
+    for (int i = 0; i < NB; i++)
+#pragma unroll
+        for (int j = 0; j < MB; j++) thin8_red[(wv * NB * MB + i * MB + j) * 64 + lane] = acc[i][j];
+    __syncthreads();
+    for (int b = wv; b < NB * MB; b += THIN8_WAVES) {
+        floatx4 t = thin8_red[b * 64 + lane];
+#pragma unroll
+        for (int w = 1; w < THIN8_WAVES; w++) t += thin8_red[(w * NB * MB + b) * 64 + lane];
+        mx_store<EPI>(p, (mb0 + b % MB) * 16 + (lane & 15), (nb0 + b / MB) * 16 + 4 * g, t);
+    }
+}
+template <int EPI, int NB, int MB>
+static hipError_t mx8_thin(MxGemmParams p, hipStream_t s) {
+    p.tiles_m = (p.T + 16 * MB - 1) / (16 * MB);
+    p.tiles_n = (p.N + 16 * NB - 1) / (16 * NB);
+    p.total = p.tiles_m * p.tiles_n;
+    p.per = (p.total + 7) / 8;
+    if (hipError_t e = grid_check((size_t)p.per * 8, THIN8_WAVES * 64)) return e;
+    hipLaunchKernelGGL((k_mx8_thin<EPI, NB, MB>), dim3(p.per * 8), dim3(THIN8_WAVES * 64), THIN8_WAVES * NB * MB * 1024, s, p);
+    return hipGetLastError();
+}
+
+// ---- tiles ----
+//
+// WN x WM waves of 16 NB x 16 MB blocks. A stage of the LDS ring holds one k block of 128: the tile's units of W (1 KB each, operand order),
+// 128 bytes of each of its rows of X, and their scales, all by LDS DMA. The 16-byte chunks of X's rows lie permuted (chunk c of row r at
+// c ^ (r / 2 % 8)), so that 16 rows' chunks of an operand read lie in all banks. Rows past the last and columns past the last lie outside
+// the descriptor's range and arrive as zeros.
+template <int WN_, int WM_, int NB_, int MB_, int NST_, int WGS_, int SB_>
+struct Mx8Cfg {
+    static constexpr int WN = WN_, WM = WM_, NB = NB_, MB = MB_, NST = NST_, WGS = WGS_, SB = SB_, WAVES = WN * WM, THREADS = WAVES * 64;
+    static constexpr int BN = WN * NB * 16, BM = WM * MB * 16;
+    static constexpr int UN = BN / 16, XP = BM / 8;                        // 1 KB pieces of W and of X
+    static constexpr int SN = BN / 64, XSP = SB == 4 ? BM / 64 : BM / 16;  // 256-byte pieces of scales: of W; of X, by words of a row or by bytes
+    static constexpr int WD = UN / WAVES, XD = XP / WAVES, SD = SB == 4 ? 1 : 1 + XSP / WAVES, DPS = WD + XD + SD;
+    static constexpr int XO = UN * 1024, WSO = XO + BM * 128, XSO = WSO + SN * 256, STAGE = XSO + XSP * 256, LDS = NST * STAGE;
+    static_assert(UN % WAVES == 0 && XP % WAVES == 0 && NB % 4 == 0 && (SB == 4 ? SN + XSP == WAVES : WAVES % SN == 0 && XSP % WAVES == 0) && LDS * WGS <= 160 * 1024, "tile");
+};
+
+// SB 4: a row's scales of a k block by one aligned word (K % 128 == 0, aligned scales), 1: by bytes
+template <int EPI, class C>
+__global__ __launch_bounds__(C::THREADS, C::WAVES * C::WGS / 4) void k_mx8_gemm(const MxGemmParams p) {
+#ifdef __HIP_DEVICE_COMPILE__  // the host pass only needs the kernel's handle
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds8[];
+    constexpr int NB = C::NB, MB = C::MB;
+    // blocks go round the 8 XCDs: each takes a contiguous range of tiles, in groups of row tiles that share W in its L2
+    const int ti = (int)(blockIdx.x & 7) * p.per + (int)(blockIdx.x >> 3);
+    if (ti >= p.total) return;
+    int tm, tn;
+    raster_tile(ti, 4, p.tiles_m, p.tiles_n, tm, tn);
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wn = wv % C::WN, wm = wv / C::WN, g = lane >> 4, c16 = lane & 15;
+    const int wrg = mx_rg(p.N);
+    const int xrows = min(C::BM, p.T - tm * C::BM), K32 = p.K / 32;
+
+    // sources of the next k block to copy, and how far its bytes go
+    const uint8_t* wsrc = p.wc + (size_t)tn * C::UN * MX_UNIT;
+    const uint8_t* ssrc = p.ws + (size_t)tn * C::SN * MX_SUNIT;
+    const uint8_t* xsrc = p.xc + (size_t)tm * C::BM * p.K;
+    const uint8_t* tsrc = p.xs + (size_t)tm * C::BM * K32;
+    const int wbytes = min(C::UN, 4 * wrg - tn * C::UN) * MX_UNIT, sbytes = min(C::SN, wrg - tn * C::SN) * MX_SUNIT;
+    int kleft = p.K, xbytes = xrows * p.K, tbytes = xrows * K32;
+    // X piece i of a wave: rows 8 (wv + i WAVES) + lane / 8, 16 bytes of each lane
+    const int xchunk = (lane & 7) ^ ((4 * (wv & 1) + (lane >> 4)) & 7);
+    uint32_t xoff[C::XD];
+#pragma unroll
+    for (int i = 0; i < C::XD; i++) xoff[i] = (uint32_t)(8 * (wv + i * C::WAVES) + (lane >> 3)) * (uint32_t)p.K + xchunk * 16;
+    constexpr uint32_t FAR = 0x7ffffff0u;  // outside every range
+    typedef __attribute__((address_space(3))) void* lds_p;
+    auto rsrc = [](const uint8_t* at, int bytes) {
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(at), (short)0, bytes, 0x00020000 /* raw */);
+    };
+    // piece i of the k block
+    auto dma_piece = [&](int i, uint8_t* base) {
+        if (i < C::WD) {
+            const int u = wv + i * C::WAVES;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc(wsrc, kleft > 0 ? wbytes : 0), (lds_p)(base + u * 1024), 16, u * 1024 + lane * 16, 0, 0, 0);
+        } else if (i < C::WD + C::XD) {
+            const int j = i - C::WD;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc(xsrc, kleft > 0 ? xbytes : 0), (lds_p)(base + C::XO + (wv + j * C::WAVES) * 1024), 16,
+                                                     xchunk * 16 < kleft ? xoff[j] : FAR, 0, 0, 0);
+        } else if (i < C::DPS) {
+            const int n = i - C::WD - C::XD;
+            if constexpr (C::SB == 4) {  // one piece a wave, of W's or of X's: a selection, not a branch (which would part the products)
+                const bool of_w = wv < C::SN;
+                const int u = of_w ? wv : wv - C::SN;
+                const uint32_t off = of_w ? u * 256 + lane * 4 : (uint32_t)(u * 64 + lane) * (uint32_t)K32;
+                const uint8_t *ws = ssrc, *xs = tsrc;  // (values: a selection of the variables themselves would put them into memory)
+                const int wn_ = sbytes, xn = tbytes;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc(of_w ? ws : xs, kleft > 0 ? of_w ? wn_ : xn : 0),
+                                                         (lds_p)(base + (of_w ? C::WSO : C::XSO) + u * 256), 4, off, 0, 0, 0);
+            } else if (n == 0) {
+                const int u = wv % C::SN;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc(ssrc, kleft > 0 ? sbytes : 0), (lds_p)(base + C::WSO + u * 256), 4,
+                                                         u * 256 + lane * 4, 0, 0, 0);
+            } else {
+                const int u = wv + (n - 1) * C::WAVES;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                    rsrc(tsrc, kleft > 0 ? tbytes : 0), (lds_p)(base + C::XSO + u * 256), 1,
+                    (lane & 3) * 32 < kleft ? (uint32_t)(u * 16 + (lane >> 2)) * (uint32_t)K32 + (lane & 3) : FAR, 0, 0, 0);
+            }
+        }
+    };
+    auto next_block = [&]() {
+        kleft -= 128;  // past the end the ranges are empty, wherever the sources are
+        wsrc += (size_t)4 * MX_UNIT * wrg;
+        ssrc += (size_t)MX_SUNIT * wrg;
+        xsrc += 128;
+        tsrc += 4;
+        xbytes -= 128;
+        tbytes -= 4;
+    };
+    auto dma = [&](int stage) {
+#pragma unroll
+        for (int i = 0; i < C::DPS; i++) dma_piece(i, lds8 + stage * C::STAGE);
+        next_block();
+    };
+
+    const uint32_t lds_base = (uint32_t)(size_t)(__attribute__((address_space(3))) uint8_t*)lds8;
+    floatx4 acc[NB][MB];
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+        for (int mb = 0; mb < MB; mb++) acc[nb][mb] = floatx4{0.f, 0.f, 0.f, 0.f};
+
+    u32x4 fw[NB];
+    i32x8 fx[2][MB];
+    uint32_t sw[2][NB / 4], sx[2][MB];
+    const uint32_t wa = lds_base + wn * NB * 1024 + lane * 16;
+    const uint32_t xa = lds_base + C::XO + (wm * MB * 16 + c16) * 128 + (g ^ (c16 >> 1 & 7)) * 16, xb = xa ^ 64;
+    const uint32_t swa = lds_base + C::WSO + wn * NB / 4 * 256 + lane * 4;
+    const uint32_t sxa = lds_base + C::XSO + (wm * MB * 16 + c16) * (C::SB == 4 ? 4 : 16) + g * (C::SB == 4 ? 1 : 4);
+    typedef __attribute__((address_space(3))) uint8_t lds_u8;
+    auto read_w = [&](int nb, uint32_t st) { fw[nb] = *reinterpret_cast<const lds_u32x4*>((size_t)(wa + st + nb * 1024)); };
+    auto read_x = [&](int b, int mb, uint32_t st) {
+        fx[b][mb] = mx8_join(*reinterpret_cast<const lds_u32x4*>((size_t)(xa + st + mb * 2048)),
+                             *reinterpret_cast<const lds_u32x4*>((size_t)(xb + st + mb * 2048)));
+    };
+    auto read_s = [&](int b, uint32_t st) {
+#pragma unroll
+        for (int i = 0; i < NB / 4; i++) sw[b][i] = *reinterpret_cast<const lds_u32*>((size_t)(swa + st + i * 256));
+#pragma unroll
+        for (int i = 0; i < MB; i++) sx[b][i] = *reinterpret_cast<const lds_u8*>((size_t)(sxa + st + i * (C::SB == 4 ? 64 : 256)));
+    };
+
+#pragma unroll
+    for (int s = 0; s < C::NST - 1; s++) dma(s);
+    wait_vmcnt<(C::NST - 2) * C::DPS>();
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++) read_w(nb, 0);
+#pragma unroll
+    for (int mb = 0; mb < MB; mb++) read_x(0, mb, 0);
+    read_s(0, 0);
+    int next = 1;  // the stage of step i + 1
+    // Step i: its operands are in registers. Those of step i + 1 landed in every wave; the stage of step i - 1, whose reads every wave
+    // finished before its products of i - 1, is refilled. The operands of i + 1 are read between the products of i.
+    auto step = [&](auto tag) {
+        constexpr int cur = decltype(tag)::value;
+        wait_vmcnt<(C::NST - 3) * C::DPS>();
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        const int ds = next >= 2 ? next - 2 : next - 2 + C::NST;
+        const uint32_t st = next * C::STAGE;
+        read_s(cur ^ 1, st);
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++) {
+#pragma unroll
+            for (int mb = 0; mb < MB; mb++) {
+                i32x8 x = fx[cur][mb];
+                if constexpr (MX8_EXACT<EPI>) {
+                    i32x8 hi;
+                    mx8_parts(x, hi, x);
+                    acc[nb][mb] = mx8_mfma_at(nb & 3, fw[nb], sw[cur][nb / 4], hi, sx[cur][mb], acc[nb][mb]);
+                }
+                acc[nb][mb] = mx8_mfma_at(nb & 3, fw[nb], sw[cur][nb / 4], x, sx[cur][mb], acc[nb][mb]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            read_w(nb, st);
+            if (nb % (NB / MB) == 0) read_x(cur ^ 1, nb / (NB / MB), st);
+#pragma unroll
+            for (int n = 0; n < (C::DPS + NB - 1) / NB; n++) dma_piece(nb * ((C::DPS + NB - 1) / NB) + n, lds8 + ds * C::STAGE);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        next_block();
+        next = next == C::NST - 1 ? 0 : next + 1;
+    };
+    int i = 0;
+    for (; i + 2 <= p.kbs; i += 2) {
+        step(std::integral_constant<int, 0>{});
+        step(std::integral_constant<int, 1>{});
+    }
+    if (i < p.kbs) step(std::integral_constant<int, 0>{});
+    wait_vmcnt<0>();  // no copy into LDS outlives the ring
+    mx_store_tile<EPI, NB, MB, C::WAVES, C::LDS>(p, acc, lds8, wv, lane, tm * C::BM + wm * MB * 16, tn * C::BN + wn * NB * 16);
+#endif
+}
+
+template <int SB>
+using Mx8Big = Mx8Cfg<2, 4, 8, 4, 3, 1, SB>;  // 256 x 256 (n x m), 8 waves
+template <int SB>
+using Mx8Mid = Mx8Cfg<2, 2, 4, 4, 3, 2, SB>;  // 128 x 128, 4 waves
+
+template <int EPI, class C>
+static hipError_t mx8_tiles(MxGemmParams p, hipStream_t s) {
+    p.tiles_m = (p.T + C::BM - 1) / C::BM;
+    p.tiles_n = (p.N + C::BN - 1) / C::BN;
+    p.total = p.tiles_m * p.tiles_n;
+    p.per = (p.total + 7) / 8;
+    if (hipError_t e = grid_check((size_t)p.per * 8, C::THREADS)) return e;
+    hipLaunchKernelGGL((k_mx8_gemm<EPI, C>), dim3(p.per * 8), dim3(C::THREADS), C::LDS, s, p);
+    return hipGetLastError();
+}
+
+// The form of a product.
+enum Mx8Kind { M8_11, M8_12, M8_14, M8_22, M8_44, M8_MID, M8_BIG };
+static Mx8Kind mx8_choose(int T, int N, int K, bool exact) {
+    if (T <= 16) return M8_11;
+    if (T <= 32) return M8_12;
+    const double cus = cu_count(), kb = mx_kb(K);
+    auto tiles = [&](int bn, int bm) { return (double)((N + bn - 1) / bn) * ((T + bm - 1) / bm); };
+    const double t22 = tiles(32, 32), t44 = tiles(64, 64), tm = tiles(128, 128), tb = tiles(256, 256);
+    const double cost[4] = {0.8 + 0.01 * kb + (0.25 + 0.05 * kb) * t22 / cus,
+                            ceil(t44 / cus) * (1.2 + 0.045 * kb) + 0.125 * kb * t44 / cus,
+                            1.9 * std::max(1.0, tm / cus) + kb * (0.155 + 0.22 * tm / cus),
+                            ceil(tb / cus) * (5.0 + 0.55 * kb) + 0.35 * kb * tb / cus};
+    return (Mx8Kind)(M8_22 + (std::min_element(cost, cost + (exact ? 3 : 4)) - cost));  // (both parts of X and 256 x 256: too many registers)
+}
+int linear_mx8_tile(int T, int rows, int cols, int epi) {
+    switch (mx8_choose(T, rows, cols, epi == KILN_EPI_F32 || epi == KILN_EPI_RESID)) {
+        case M8_11: return 16 << 16 | 16;
+        case M8_12: return 16 << 16 | 32;
+        case M8_14: return 16 << 16 | 64;
+        case M8_22: return 32 << 16 | 32;
+        case M8_44: return 64 << 16 | 64;
+        case M8_MID: return 128 << 16 | 128;
+        default: return 256 << 16 | 256;
+    }
+}
+
+template <int EPI>
+static hipError_t linear_mx8_epi(const MxGemmParams& p, hipStream_t s) {
+    const bool words = p.K % 128 == 0 && ((uintptr_t)p.xs & 3) == 0;
+    switch (mx8_choose(p.T, p.N, p.K, MX8_EXACT<EPI>)) {
+        case M8_11: return mx8_thin<EPI, 1, 1>(p, s);
+        case M8_12: return mx8_thin<EPI, 1, 2>(p, s);
+        case M8_14: return mx8_thin<EPI, 1, 4>(p, s);
+        case M8_22: return mx8_thin<EPI, 2, 2>(p, s);
+        case M8_44: return mx8_thin<EPI, 4, 4>(p, s);
+        case M8_MID: return words ? mx8_tiles<EPI, Mx8Mid<4>>(p, s) : mx8_tiles<EPI, Mx8Mid<1>>(p, s);
+        default:
+            if constexpr (MX8_EXACT<EPI>) return hipErrorInvalidValue;
+            else return words ? mx8_tiles<EPI, Mx8Big<4>>(p, s) : mx8_tiles<EPI, Mx8Big<1>>(p, s);
+    }
+}
+
+hipError_t launch_linear_mx8(void* y, size_t ldy, const uint8_t* codes, const uint8_t* scales, int T, const uint8_t* wp, int rows, int cols,
+                             int epi, const float* gate, float beta, hipStream_t s) {
+    MxGemmParams p{};
+    p.xc = codes;
+    p.xs = scales;
+    p.wc = wp;
+    p.ws = wp + mx_code_bytes(rows, cols);
+    p.T = T;
+    p.N = rows;
+    p.K = cols;
+    p.kbs = mx_kb(cols);
+    p.y = y;
+    p.ldy = ldy;
+    p.gate = gate;
+    p.beta = beta;
+    const int e4 = epi == KILN_EPI_F32 || epi == KILN_EPI_RESID ? 16 : 8;
+    p.vec = ((uintptr_t)y & (e4 - 1)) == 0 && (T == 1 || ldy % 4 == 0);
+    if (p.vec && ((uintptr_t)y & 15) == 0 && (T == 1 || ldy * e4 / 4 % 16 == 0)) p.vec = 2;
+    switch (epi) {
+        case KILN_EPI_F32: return linear_mx8_epi<KILN_EPI_F32>(p, s);
+        case KILN_EPI_F16: return linear_mx8_epi<KILN_EPI_F16>(p, s);
+        case KILN_EPI_GELU16: return linear_mx8_epi<KILN_EPI_GELU16>(p, s);
+        default: return linear_mx8_epi<KILN_EPI_RESID>(p, s);
+    }
+}
+
+}  // namespace kiln

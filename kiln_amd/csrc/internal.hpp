@@ -181,6 +181,51 @@ size_t cross_attn_workspace(int B, int Tq, int Tk, int Hq, int Hkv, int Dh);
 int cross_attn_form(int B, int Tq, int Tk, int Hq, int Hkv, int Dh);  // rows << 16 | waves along the keys << 8 | split
 hipError_t launch_cross_attn(const CrossLaunch& c, hipStream_t s);
 
+// causal attention over packed sequences (prompt_attn.hip); strides in elements, F16 or BF16; ws smaller than
+// prompt_attn_workspace (or null): the keys are not split over workgroups
+struct PromptLaunch {
+    void* out;
+    const void* q;
+    const void* k;
+    const void* v;
+    const void* pk;  // prefix [P, ld], or null
+    const void* pv;
+    size_t ldo, ldq, ldk, ldv, ldpk, ldpv;
+    DT dt;
+    int B, Tq, Tk, P, Hq, Hkv, Dh;
+    float scale;
+    const int* q_start;  // [B + 1] on the device, or null (B = 1)
+    const int* k_start;  // [B], k_len [B], or null: the queries' own rows
+    const int* k_len;
+    void* ws;
+    size_t ws_bytes;
+};
+size_t prompt_attn_workspace(int B, int Tq, int Tk, int P, int Hq, int Hkv, int Dh);
+hipError_t launch_prompt_attn(const PromptLaunch& c, hipStream_t s);
+
+// h = x + res (res, h null: x alone), y = h / rms(h) w (add_rmsnorm.hip): y in ydt, or MXFP8 codes when scales is not null
+struct RmsLaunch {
+    void* y;
+    uint8_t* scales;
+    void* h;
+    const void* x;
+    const void* res;
+    const uint16_t* w;
+    DT ydt, xdt, rdt;
+    size_t ldy, ldh, ldx, ldr;
+    int rows, dim;
+    float eps;
+};
+hipError_t launch_add_rmsnorm(const RmsLaunch& c, hipStream_t s);
+
+// MXFP8 (mxfp8.hip): cols % 32 == 0
+hipError_t launch_mx8_quantize(uint8_t* codes, uint8_t* scales, const void* x, DT dt, size_t ldx, int rows, int cols, hipStream_t s);
+hipError_t launch_mx8_dequantize(void* y, DT dt, size_t ldy, const uint8_t* codes, const uint8_t* scales, int rows, int cols, hipStream_t s);
+// the linear layer of MXFP8 rows with an MXFP4 weight (gemm_mxfp8.hpp)
+int linear_mx8_tile(int T, int rows, int cols, int epi);  // weight rows << 16 | rows of x
+hipError_t launch_linear_mx8(void* y, size_t ldy, const uint8_t* codes, const uint8_t* scales, int T, const uint8_t* wp, int rows, int cols,
+                             int epi, const float* gate, float beta, hipStream_t s);
+
 // torch.manual_seed(seed); torch.randn(n) on the host (host_rng.cpp); false if n < 16
 bool host_torch_randn(float* out, uint64_t seed, size_t n);
 

@@ -9,20 +9,6 @@
 
 namespace kiln {
 
-__device__ __forceinline__ uint32_t quad_umax(uint32_t v) {  // over the four lanes of a quad
-    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, false));
-    return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, false));
-}
-
-// Eight neighbours are a unit: n = rows * cols / 8 of them, row by row. The place of unit i in rows of stride ld: dense rows need no
-// row number, others a 32-bit division (64-bit ones took a third of the kernels' time)
-template <bool DENSE>
-__device__ __forceinline__ size_t mx_place(size_t i, size_t n, uint32_t per_row, size_t ld) {
-    if constexpr (DENSE) return i * 8;
-    const size_t r = n >> 32 ? i / per_row : (uint32_t)i / per_row;
-    return r * ld + (i - r * per_row) * 8;
-}
-
 // x [rows, cols] to codes [rows, cols / 2] (even column in the low half) and scales [rows, cols / 32]. Four lanes take a
 // block of 32, eight values each: loads of 16 or 32 contiguous bytes per lane, 4-byte stores of codes.
 template <class E, bool VEC, bool DENSE>
@@ -141,15 +127,13 @@ __global__ __launch_bounds__(256) void k_mx_quantize_pack(uint8_t* oc, uint8_t* 
     if (j == 0) *reinterpret_cast<uint32_t*>(os + (kb * rgs + rg) * MX_SUNIT + lane * 4) = *reinterpret_cast<const uint32_t*>(ls[lane]);
 }
 
-static unsigned grid_of(size_t n) { return (unsigned)std::min<size_t>((n + 255) / 256, (size_t)cu_count() * 32); }
-
 template <class E>
 static hipError_t quantize_of(uint8_t* codes, uint8_t* scales, const void* x, size_t ldx, int rows, int cols, bool vec, hipStream_t s) {
     const size_t n = (size_t)rows * (cols / 8);
     const bool dense = rows == 1 || ldx == (size_t)cols;
     auto kern = vec ? (dense ? k_mx_quantize<E, true, true> : k_mx_quantize<E, true, false>)
                     : (dense ? k_mx_quantize<E, false, true> : k_mx_quantize<E, false, false>);
-    hipLaunchKernelGGL(kern, dim3(grid_of(n)), dim3(256), 0, s, codes, scales, static_cast<const E*>(x), ldx, n, (uint32_t)(cols / 8));
+    hipLaunchKernelGGL(kern, dim3(mx_grid(n)), dim3(256), 0, s, codes, scales, static_cast<const E*>(x), ldx, n, (uint32_t)(cols / 8));
     return hipGetLastError();
 }
 template <class E>
@@ -159,7 +143,7 @@ static hipError_t dequantize_of(void* y, size_t ldy, const uint8_t* codes, const
     const bool dense = rows == 1 || ldy == (size_t)cols;
     auto kern = vec ? (dense ? k_mx_dequantize<E, true, true> : k_mx_dequantize<E, true, false>)
                     : (dense ? k_mx_dequantize<E, false, true> : k_mx_dequantize<E, false, false>);
-    hipLaunchKernelGGL(kern, dim3(grid_of(n)), dim3(256), 0, s, static_cast<E*>(y), ldy, codes, scales, n, (uint32_t)(cols / 8));
+    hipLaunchKernelGGL(kern, dim3(mx_grid(n)), dim3(256), 0, s, static_cast<E*>(y), ldy, codes, scales, n, (uint32_t)(cols / 8));
     return hipGetLastError();
 }
 template <class E>
@@ -172,11 +156,6 @@ static hipError_t quantize_pack_of(uint8_t* op, const void* x, size_t ldx, int r
                        static_cast<const E*>(x), ldx, rows, cols, kbs);
     return hipGetLastError();
 }
-// 16-byte loads of the rows
-static bool rows16(const void* p, size_t ld, DT dt, int rows) {
-    return ((uintptr_t)p & 15) == 0 && (rows == 1 || ld * (dt == DT::F32 ? 4 : 2) % 16 == 0);
-}
-
 hipError_t launch_mx_quantize(uint8_t* codes, uint8_t* scales, const void* x, DT dt, size_t ldx, int rows, int cols, hipStream_t s) {
     const bool vec = rows16(x, ldx, dt, rows);
     if (dt == DT::F32) return quantize_of<float>(codes, scales, x, ldx, rows, cols, vec, s);

@@ -9,6 +9,8 @@
 // first: workgroups of a product are at about the same k block, and its row blocks side by side lie in all of an L2's channels
 // (with the row block first they were KB kilobytes apart, often in the same few).
 #pragma once
+#include <algorithm>
+
 #include "common.hpp"
 #include "internal.hpp"
 
@@ -116,6 +118,26 @@ struct MxVals<__bf16, N> : MxVals16<__bf16, N> {
         return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, this->template pair<bf2v>(i, 3), s, 3);
     }
 };
+
+__device__ __forceinline__ uint32_t quad_umax(uint32_t v) {  // over the four lanes of a quad
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, false));
+    return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, false));
+}
+
+// Eight neighbours are a unit: n = rows * cols / 8 of them, row by row. The place of unit i in rows of stride ld: dense rows need no
+// row number, others a 32-bit division (64-bit ones took a third of the kernels' time)
+template <bool DENSE>
+__device__ __forceinline__ size_t mx_place(size_t i, size_t n, uint32_t per_row, size_t ld) {
+    if constexpr (DENSE) return i * 8;
+    const size_t r = n >> 32 ? i / per_row : (uint32_t)i / per_row;
+    return r * ld + (i - r * per_row) * 8;
+}
+// workgroups of 256 for n units, one each
+inline unsigned mx_grid(size_t n) { return (unsigned)std::min<size_t>((n + 255) / 256, (size_t)cu_count() * 32); }
+// 16-byte loads of the rows
+inline bool rows16(const void* p, size_t ld, DT dt, int rows) {
+    return ((uintptr_t)p & 15) == 0 && (rows == 1 || ld * (dt == DT::F32 ? 4 : 2) % 16 == 0);
+}
 
 // the 32 codes of a whole block in one lane, and its scale byte
 template <class E>
