@@ -34,7 +34,17 @@ struct PromptParams {
     const int* k_len;
     float sc;            // scale log2(e)
     float lift;          // log2 of the weights' factor
+    int nw;              // keys shared out: workgroups per key head
+    size_t rows_part;    // .. partial results by row in front of those by workgroup
+    float* part;         // .. partial results [.][DH], then [.](m, l)
+    float* part_ml;
 };
+
+// How the keys go over the workgroups. WHOLE: a workgroup per key head and row tile. SPLIT: every key head's tiles of keys, row tile by row tile,
+// are one line that its nw workgroups share out in equal parts; a row tile that is cut leaves partial results, joined by k_prompt_merge.
+// PACK: as SPLIT, but the prefix's keys come first and once for all sequences' rows, whose own keys follow without it.
+enum PromptMode { PM_WHOLE, PM_SPLIT, PM_PACK };
+constexpr int PROMPT_LEAST = 4;  // tiles of a workgroup's part
 
 // A sequence's rows: queries q0 .. q0 + nq - 1, keys k0 .. k0 + nk - 1, inside the tensors whatever the lengths on the device say
 struct PromptSeq {
@@ -55,6 +65,16 @@ __device__ __forceinline__ PromptSeq prompt_seq(const PromptParams& p, int s) {
     return r;
 }
 
+// Keys that the last row of a sequence's row tile `place` sees, and its tiles (one at least: a row without keys is zeros) behind np of the prefix
+template <int RT>
+__device__ __forceinline__ int prompt_keys(const PromptParams& p, const PromptSeq& q, int place) {
+    const int rows = q.nq * p.G;
+    return max(0, min(q.nk, (min(rows, (place + 1) * RT) - 1) / p.G + q.nk - q.nq + 1));
+}
+template <int RT>
+__device__ __forceinline__ int prompt_tiles(const PromptParams& p, const PromptSeq& q, int place, int np) {
+    return max(1, np + (prompt_keys<RT>(p, q, place) + XKT - 1) / XKT);
+}
 // the sum over a wave's lanes, in all of them
 __device__ __forceinline__ int wave_sum(int v) {
     v += __builtin_amdgcn_update_dpp(0, v, 0x121, 0xF, 0xF, false);  // row_ror 1, 2, 4, 8
@@ -66,6 +86,64 @@ __device__ __forceinline__ int wave_sum(int v) {
     r = __builtin_amdgcn_permlane32_swap((unsigned)v, (unsigned)v, false, false);
     return __builtin_amdgcn_readfirstlane((int)(r[0] + r[1]));
 }
+
+// the sum over the lanes up to a lane's own
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast 15 to rows 1 and 3, 31 to rows 2 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+    return v;
+}
+
+// A key head's line of tiles: `ahead` of the prefix over all rows (PACK), then each sequence's; `each` tiles to a workgroup
+template <int RT, PromptMode MODE>
+struct PromptLine {
+    int lane, np, ahead, total, each, first;  // first: the tiles of sequence `lane`
+    __device__ __forceinline__ int of(const PromptParams& p, int s) const {
+        if (s >= p.B) return 0;
+        const PromptSeq q = prompt_seq(p, s);
+        int n = 0;
+        for (int i = 0; i * RT < q.nq * p.G; i++) n += prompt_tiles<RT>(p, q, i, MODE == PM_PACK ? 0 : np);
+        return n;
+    }
+    __device__ __forceinline__ explicit PromptLine(const PromptParams& p) {
+        lane = threadIdx.x & 63;
+        np = (p.P + XKT - 1) / XKT;
+        ahead = MODE == PM_PACK ? (p.Tq * p.G + RT - 1) / RT * np : 0;
+        first = of(p, lane);
+        int n = first;
+        for (int s = 64; s < p.B; s += 64) n += of(p, s + lane);
+        total = ahead + wave_sum(n);
+        each = max(PROMPT_LEAST, (total + p.nw - 1) / p.nw);
+    }
+    // the sequence that holds place `at` of the line (>= ahead), or -1; at: counted from the sequence's first tile
+    __device__ __forceinline__ int find(const PromptParams& p, int& at) const {
+        at -= ahead;
+        for (int s0 = 0; s0 < p.B; s0 += 64) {
+            const int n = s0 ? of(p, s0 + lane) : first, up = wave_scan(n);
+            const unsigned long long past = __ballot(up > at);
+            if (past) {
+                const int i = __ffsll(past) - 1;
+                at -= __builtin_amdgcn_readlane(up - n, i);
+                return s0 + i;
+            }
+            at -= __builtin_amdgcn_readlane(up, 63);
+        }
+        return -1;
+    }
+    // the place of sequence s's first tile
+    __device__ __forceinline__ int start(const PromptParams& p, int s) const {
+        int at = ahead;
+        for (int s0 = 0; s0 < s; s0 += 64) {
+            const int n = s0 ? of(p, s0 + lane) : first;
+            at += wave_sum(s0 + lane < s ? n : 0);
+        }
+        return at;
+    }
+};
 
 // Row tile number `rank` of all sequences' tiles of RT rows, in the order of falling place in their sequence (the longest ranges of keys
 // first): its sequence and place, or -1 past the last. With F(n) the number of tiles at place n or later, F(n + 1) <= rank < F(n).
@@ -120,28 +198,51 @@ __device__ __forceinline__ int prompt_find(const PromptParams& p, int rank, int&
     return -1;
 }
 
-template <class E, class C>
+template <class E, class C, PromptMode MODE>
 __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_prompt_attn(const PromptParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)  // the host pass drops a kernel template whose target builtins it cannot check
     using M = XMma<E>;
     constexpr int DH = C::DH, QB = C::QB;
-    static_assert(C::SHARED, "the waves share the keys");
+    static_assert(C::SHARED || C::NW == 1, "waves share the keys, or one has them to itself");
     extern __shared__ __attribute__((aligned(16))) uint8_t xlds[];
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, c16 = lane & 15;
     // key heads side by side: blocks go round the 8 XCDs, so that a head's row tiles share the L2s of few, and every XCD has long and
     // short ones
-    const int hk = (int)(blockIdx.x % p.Hkv);
-    int jt;
-    const int s = prompt_find<C::RT>(p, (int)(blockIdx.x / p.Hkv), jt);
-    if (s < 0) return;
-    const PromptSeq sq = prompt_seq(p, s);
+    const int hk = (int)(blockIdx.x % p.Hkv), bx = (int)(blockIdx.x / p.Hkv);
+    // a row tile: sequence (-1: the prefix's pass over all rows), place in it, its tiles t0 .. t1 - 1 of kt
+    int s = 0, jt = 0, t0 = 0, t1, kt, left_u = 0;
+    PromptSeq sq;
+    if constexpr (MODE == PM_WHOLE) {
+        s = prompt_find<C::RT>(p, bx, jt);
+        if (s < 0) return;
+        sq = prompt_seq(p, s);
+    } else {
+        const PromptLine<C::RT, MODE> line(p);
+        int u = bx * line.each;
+        left_u = min(line.total - u, line.each);
+        if (left_u <= 0) return;
+        if (u < line.ahead) {
+            s = -1;
+            jt = u / line.np;
+            t0 = u % line.np;
+        } else {
+            s = line.find(p, u);
+            sq = prompt_seq(p, s);
+            for (int n; u >= (n = prompt_tiles<C::RT>(p, sq, jt, MODE == PM_PACK ? 0 : line.np)); jt++) u -= n;
+            t0 = u;
+        }
+    }
+    for (;;) {
+    const bool ahead = MODE == PM_PACK && s < 0;
+    if (ahead) sq = PromptSeq{0, p.Tq, 0, 0};
     const int rows = sq.nq * p.G, diff = sq.nk - sq.nq;
-    const int np = (p.P + XKT - 1) / XKT;
-    const int row0 = jt * C::RT + wv * C::RW;
-    // keys of the tile's last row: the row tile's own keys
-    const int L = max(0, min(sq.nk, (min(rows, (jt + 1) * C::RT) - 1) / p.G + diff + 1));
-    const int t0 = 0, t1 = np + (L + XKT - 1) / XKT;
+    const int np = MODE == PM_PACK && !ahead ? 0 : (p.P + XKT - 1) / XKT;
+    const int row0 = jt * C::RT + (C::SHARED ? wv * C::RW : 0);
+    // the row tile's own keys
+    const int L = ahead ? 0 : prompt_keys<C::RT>(p, sq, jt);
+    kt = max(1, np + (L + XKT - 1) / XKT);
+    t1 = MODE == PM_WHOLE ? kt : min(kt, t0 + left_u);
 
     uint8_t* ring = xlds;
     const uint32_t lds_base = (uint32_t)(size_t)(__attribute__((address_space(3))) uint8_t*)ring;
@@ -160,7 +261,7 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_prompt_attn(const Prom
         kst.ld2 = ld2;
 #pragma unroll
         for (int i = 0; i < C::DMA; i++) {
-            const int pc = i * C::RTHREADS + (int)threadIdx.x, r = pc / C::PC, c = pc % C::PC;
+            const int pc = i * C::RTHREADS + (C::SHARED ? (int)threadIdx.x : lane), r = pc / C::PC, c = pc % C::PC;
             kst.off[i] = r * ld2 + k_swz<DH>(c, r) * 16;
         }
     };
@@ -168,7 +269,7 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_prompt_attn(const Prom
         vst.ld2 = ld2;
 #pragma unroll
         for (int i = 0; i < C::DMA; i++) {
-            const int pc = i * C::RTHREADS + (int)threadIdx.x, r = pc / C::PC, c = pc % C::PC;
+            const int pc = i * C::RTHREADS + (C::SHARED ? (int)threadIdx.x : lane), r = pc / C::PC, c = pc % C::PC;
             vst.off[i] = r * ld2 + v_swz<DH>(c, r) * 16;
         }
     };
@@ -189,7 +290,7 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_prompt_attn(const Prom
         const int left = t.j < t1 ? min(XKT, left_of(t.j)) : 0;
         const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
             const_cast<uint8_t*>(t.src), (short)0, left > 0 ? (int)((left - 1) * t.ld2 + DH * 2) : 0, 0x00020000 /* raw */);
-        uint8_t* dst = ring + at + wv * 1024;
+        uint8_t* dst = ring + at + (C::SHARED ? wv * 1024 : 0);
 #pragma unroll
         for (int i = 0; i < C::DMA; i++)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(dst + i * C::RTHREADS * 16), 16, t.off[i], 0, 0, 0);
@@ -224,7 +325,7 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_prompt_attn(const Prom
         lim[qb] = t + diff + 1;
     }
     // of the wave's first and last row
-    const int lim0 = min(row0, rows - 1) / p.G + diff + 1, lim1 = min(row0 + C::RW, rows) - 1 < 0 ? lim0 : max(lim0, (min(row0 + C::RW, rows) - 1) / p.G + diff + 1);
+    const int lim0 = min(row0, rows - 1) / p.G + diff + 1, lim1 = min(row0 + C::RW - 1, rows - 1) / p.G + diff + 1;
 
     floatx4 o[DH / 16][QB], l[QB];  // l: every register of a lane holds its row's sum (P^T times ones)
     const float lift = std::is_same<E, _Float16>::value ? XLIFT16 : p.lift;
@@ -381,68 +482,132 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_prompt_attn(const Prom
         }
     };
 
-    // A step computes the scores of tile j + 1 ahead of the weights and products of tile j. K of tile j + 1 and V of tile j landed (past
-    // the last tile the copies go on with empty ranges, which keeps the count); every wave is done with K of tile j and V of tile
-    // j - 1, whose places take K of tile j + NS and V of tile j + NS - 1.
-    constexpr int NS = C::NS;
-    static_assert(NS % 2 == 0, "the scores' two sets go with the stages");
-    floatx4 sc[2][2][QB];
-    float top[QB];
-    u32x4 kf[2][DH / 32], vf[DH / 16], pf[QB];
-    copy_k(0);
+    auto apart = [&](int j) { return j >= np && lim0 < lim1 && lim0 - (j - np) * XKT < XKT; };
+    if constexpr (C::SHARED) {
+        // A step computes the scores of tile j + 1 ahead of the weights and products of tile j. K of tile j + 1 and V of tile j landed (past
+        // the last tile the copies go on with empty ranges, which keeps the count); every wave is done with K of tile j and V of tile
+        // j - 1, whose places take K of tile j + NS and V of tile j + NS - 1.
+        constexpr int NS = C::NS;
+        static_assert(NS % 2 == 0, "the scores' two sets go with the stages");
+        floatx4 sc[2][2][QB];
+        float top[QB];
+        u32x4 kf[2][DH / 32], vf[DH / 16], pf[QB];
+        copy_k(0);
 #pragma unroll
-    for (int i = 1; i < NS; i++) {
-        copy_k(i);
-        copy_v(i - 1);
-    }
-    x_wait_vmcnt<2 * (NS - 1) * C::DMA>();
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_sched_barrier(0);
-    if (t0 < t1) {
+        for (int i = 1; i < NS; i++) {
+            copy_k(i);
+            copy_v(i - 1);
+        }
+        x_wait_vmcnt<2 * (NS - 1) * C::DMA>();
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
         read_k(0, kf);
         scores(kf, sc[0]);
         hide(t0, sc[0]);
         largest(sc[0], top);
-    }
-    auto step = [&](int j, auto parity, auto st) {  // st: the stage of tile j, a constant or not
-        constexpr int cur = decltype(parity)::value;
-        x_wait_vmcnt<2 * (NS - 2) * C::DMA>();
-        __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
-        __builtin_amdgcn_s_barrier();
-        __builtin_amdgcn_sched_barrier(0);
-        copy_k(st);
-        copy_v((st + NS - 1) % NS);
-        read_k((st + 1) % NS * C::STAGE, kf);
+        auto step = [&](int j, auto parity, auto st) {  // st: the stage of tile j, a constant or not
+            constexpr int cur = decltype(parity)::value;
+            x_wait_vmcnt<2 * (NS - 2) * C::DMA>();
+            __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+            copy_k(st);
+            copy_v((st + NS - 1) % NS);
+            read_k((st + 1) % NS * C::STAGE, kf);
 #pragma unroll
-        for (int db = 0; db < DH / 16; db++) vf[db] = read_v(st * C::STAGE, db);
-        rescale(top, sc[cur]);
-        __builtin_amdgcn_sched_barrier(0);
-        weights(sc[cur], pf);
-        scores(kf, sc[cur ^ 1]);
-        __builtin_amdgcn_sched_barrier(0);
-        if (j >= np && lim0 < lim1 && lim0 - (j - np) * XKT < XKT) keep_apart(j, st * C::STAGE, vf, pf);
-        if (j + 1 < t1) hide(j + 1, sc[cur ^ 1]);
+            for (int db = 0; db < DH / 16; db++) vf[db] = read_v(st * C::STAGE, db);
+            rescale(top, sc[cur]);
+            __builtin_amdgcn_sched_barrier(0);
+            weights(sc[cur], pf);
+            scores(kf, sc[cur ^ 1]);
+            __builtin_amdgcn_sched_barrier(0);
+            if (apart(j)) keep_apart(j, st * C::STAGE, vf, pf);
+            if (j + 1 < t1) hide(j + 1, sc[cur ^ 1]);
 #pragma unroll
-        for (int qb = 0; qb < QB; qb++) l[qb] = M::mul(ones, pf[qb], l[qb]);
+            for (int qb = 0; qb < QB; qb++) l[qb] = M::mul(ones, pf[qb], l[qb]);
 #pragma unroll
-        for (int db = 0; db < DH / 16; db++)
+            for (int db = 0; db < DH / 16; db++)
 #pragma unroll
-            for (int qb = 0; qb < QB; qb++) o[db][qb] = M::mul(vf[db], pf[qb], o[db][qb]);
-        largest(sc[cur ^ 1], top);
-    };
-    using P0 = std::integral_constant<int, 0>;
-    using P1 = std::integral_constant<int, 1>;
-    for (int j = t0, st = 0; j < t1; j += 2, st = (st + 2) % NS) {
-        step(j, P0{}, st);
-        if (j + 1 >= t1) break;
-        step(j + 1, P1{}, st + 1);
+                for (int qb = 0; qb < QB; qb++) o[db][qb] = M::mul(vf[db], pf[qb], o[db][qb]);
+            largest(sc[cur ^ 1], top);
+        };
+        using P0 = std::integral_constant<int, 0>;
+        using P1 = std::integral_constant<int, 1>;
+        if constexpr (QB == 1) {
+            for (int j = t0, st = 0; j < t1; j += 2, st = (st + 2) % NS) {
+                step(j, P0{}, st);
+                if (j + 1 >= t1) break;
+                step(j + 1, P1{}, st + 1);
+            }
+        } else {
+            static_assert(NS == 4, "the loop names its stages");
+            for (int j = t0; j < t1; j += 4) {
+                step(j, P0{}, P0{});
+                if (j + 1 >= t1) break;
+                step(j + 1, P1{}, P1{});
+                if (j + 2 >= t1) break;
+                step(j + 2, P0{}, std::integral_constant<int, 2>{});
+                if (j + 3 >= t1) break;
+                step(j + 3, P1{}, std::integral_constant<int, 3>{});
+            }
+        }
+    } else {
+        int stage = 0;
+#pragma unroll
+        for (int i = 0; i < C::NS - 1; i++) {
+            copy_k(i);
+            copy_v(i);
+        }
+        for (int j = t0; j < t1; j++) {
+            x_wait_vmcnt<(C::NS - 2) * 2 * C::DMA>();
+            __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): this wave is done with tile j - 1, whose stage is refilled
+            __builtin_amdgcn_sched_barrier(0);
+            const int into = stage == 0 ? C::NS - 1 : stage - 1;
+            copy_k(into);
+            copy_v(into);
+            const uint32_t st = stage * C::STAGE;
+            floatx4 sc[2][QB];
+            float top[QB];
+            u32x4 kf[2][DH / 32], vf[DH / 16], pf[QB];
+            read_k(st, kf);
+            scores(kf, sc);
+            hide(j, sc);
+            largest(sc, top);
+            rescale(top, sc);
+            weights(sc, pf);
+#pragma unroll
+            for (int db = 0; db < DH / 16; db++) vf[db] = read_v(st, db);
+            if (apart(j)) keep_apart(j, st, vf, pf);
+#pragma unroll
+            for (int qb = 0; qb < QB; qb++) l[qb] = M::mul(ones, pf[qb], l[qb]);
+#pragma unroll
+            for (int db = 0; db < DH / 16; db++)
+#pragma unroll
+                for (int qb = 0; qb < QB; qb++) o[db][qb] = M::mul(vf[db], pf[qb], o[db][qb]);
+            stage = stage == C::NS - 1 ? 0 : stage + 1;
+        }
     }
     x_wait_vmcnt<0>();  // no copy into LDS outlives its ring
 
+    const bool whole = MODE == PM_WHOLE || (t0 == 0 && t1 == kt);
+    if (MODE != PM_WHOLE && (MODE == PM_PACK || !whole)) {
+        // partial results: of a whole row tile by row (PACK), else by workgroup: one that begins before it, one that ends behind it
+        size_t base = p.rows_part + (((size_t)hk * p.nw + bx) * 2 + (t0 > 0 ? 0 : 1)) * C::RT + (C::SHARED ? wv * C::RW : 0);
+        if (MODE == PM_PACK && whole) base = ((size_t)(ahead ? p.Hkv : 0) + hk) * p.Tq * p.G + (size_t)sq.q0 * p.G + row0;
+#pragma unroll
+        for (int qb = 0; qb < QB; qb++) {
+            if (row0 + 16 * qb + c16 >= rows) continue;
+            const size_t at = base + 16 * qb + c16;
+#pragma unroll
+            for (int db = 0; db < DH / 16; db++) *reinterpret_cast<floatx4*>(p.part + at * DH + 16 * db + 4 * g) = o[db][qb];
+            if (g == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(m[qb], l[qb][0]);
+        }
+        if constexpr (C::SHARED) __builtin_amdgcn_s_barrier();  // every wave is done with the ring
+    } else {
     // rows leave through LDS, whole and 16 bytes a lane; a row's chunks lie permuted by its number
     static_assert(C::RW * DH * 2 * C::NW <= C::RINGS, "the waves' rows fit in the rings");
     uint8_t* stg = xlds + wv * C::RW * DH * 2;
-    __builtin_amdgcn_s_barrier();  // every wave is done with the ring, and its copies landed
+    if constexpr (C::SHARED) __builtin_amdgcn_s_barrier();  // every wave is done with the ring, and its copies landed
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int qb = 0; qb < QB; qb++) {
@@ -462,22 +627,157 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_prompt_attn(const Prom
         const int t = r / p.G, h = hk * p.G + r % p.G;
         *reinterpret_cast<u32x4*>(static_cast<uint8_t*>(p.o) + ((long long)(sq.q0 + t) * p.ldo + (long long)h * DH + c * 8) * 2) = v;
     }
+    if (MODE != PM_WHOLE && C::SHARED) {
+        __builtin_amdgcn_s_waitcnt(0xC07F);
+        __builtin_amdgcn_s_barrier();  // every wave's rows are out of LDS
+    }
+    }
+    if constexpr (MODE == PM_WHOLE) return;
+    // the next row tile of the line
+    left_u -= t1 - t0;
+    if (left_u <= 0) return;
+    __builtin_amdgcn_s_waitcnt(0xC07F);
+    __builtin_amdgcn_sched_barrier(0);
+    t0 = 0;
+    if (++jt * C::RT >= rows) {
+        jt = 0;
+        do {
+            if (++s >= p.B) return;
+            sq = prompt_seq(p, s);
+        } while (sq.nq == 0);
+    }
+    }
 #endif
 }
 
-size_t prompt_attn_workspace(int B, int Tq, int Tk, int P, int Hq, int Hkv, int Dh) { return 0; }
+// The partial results of a row joined, in the line's order: a wave per row
+template <class E, int DH, int RT, PromptMode MODE>
+__global__ __launch_bounds__(256) void k_prompt_merge(const PromptParams p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const int lane = threadIdx.x & 63, hk = (int)(blockIdx.x % p.Hkv);
+    const long long R = (long long)(blockIdx.x / p.Hkv) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (R >= (long long)p.Tq * p.G) return;
+    const int t = (int)(R / p.G);
+    // the row's sequence: the last that claims it
+    int s = -1;
+    for (int s0 = 0; s0 < p.B; s0 += 64) {
+        bool in = false;
+        if (s0 + lane < p.B) {
+            const PromptSeq q = prompt_seq(p, s0 + lane);
+            in = t >= q.q0 && t - q.q0 < q.nq;
+        }
+        const unsigned long long has = __ballot(in);
+        if (has) s = s0 + 63 - __clzll(has);
+    }
+    if (s < 0) return;
+    const PromptLine<RT, MODE> line(p);
+    const PromptSeq sq = prompt_seq(p, s);
+    const int r = (int)(R - (long long)sq.q0 * p.G), place = r / RT;
+    // the row tile's stretches of the line: workgroups w .. w + n - 1 hold parts of it
+    int at = line.start(p, s);
+    for (int i = 0; i < place; i++) at += prompt_tiles<RT>(p, sq, i, MODE == PM_PACK ? 0 : line.np);
+    const int kt = prompt_tiles<RT>(p, sq, place, MODE == PM_PACK ? 0 : line.np);
+    const int w = at / line.each, n = (at + kt - 1) / line.each - w + 1;
+    if (MODE == PM_SPLIT && n == 1) return;  // written by its workgroup
+    int w2 = 0, n2 = 0;
+    if (MODE == PM_PACK) {
+        const int at2 = (int)(R / RT) * line.np;
+        w2 = at2 / line.each;
+        n2 = (at2 + line.np - 1) / line.each - w2 + 1;
+    }
+    const size_t all = (size_t)p.Tq * p.G;
+    auto index = [&](int i) -> size_t {  // of the row's partial result i
+        const bool own = MODE == PM_SPLIT || i < n;
+        const int k = own ? i : i - n, cut = own ? n : n2;
+        if (cut == 1) return ((size_t)(own ? 0 : p.Hkv) + hk) * all + R;
+        return p.rows_part + (((size_t)hk * p.nw + (own ? w : w2) + k) * 2 + (k == 0 ? 1 : 0)) * RT + (own ? r % RT : (int)(R % RT));
+    };
+    const int parts = n + n2;
+    float mm = -INFINITY;
+    for (int i = lane; i < parts; i += 64) mm = fmaxf(mm, p.part_ml[index(i) * 2]);
+#pragma unroll
+    for (int i = 32; i; i >>= 1) mm = fmaxf(mm, __shfl_xor(mm, i, 64));
+    const float me = mm == -INFINITY ? 0.f : mm;
+    constexpr int PER = DH / 64;
+    typedef float vec __attribute__((ext_vector_type(PER)));
+    vec acc = 0.f;
+    float ll = 0.f;
+    for (int i0 = 0; i0 < parts; i0 += 64) {
+        float f = 0.f;
+        if (i0 + lane < parts) {
+            const float2 e = *reinterpret_cast<const float2*>(p.part_ml + index(i0 + lane) * 2);
+            f = __builtin_amdgcn_exp2f(e.x - me);
+            ll += f * e.y;
+        }
+        const int end = min(64, parts - i0);
+        for (int i = 0; i < end; i += 4) {  // four in flight; past the last the factor is 0
+            vec v[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) v[k] = *reinterpret_cast<const vec*>(p.part + index(i0 + min(i + k, end - 1)) * DH + PER * lane);
+#pragma unroll
+            for (int k = 0; k < 4; k++) acc += __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), i + k)) * v[k];
+        }
+    }
+#pragma unroll
+    for (int i = 32; i; i >>= 1) ll += __shfl_xor(ll, i, 64);
+    const float inv = ll > 0.f || ll != ll ? 1.f / ll : 0.f;
+    uint8_t* dst = static_cast<uint8_t*>(p.o) + ((long long)t * p.ldo + (long long)(hk * p.G + (int)(R % p.G)) * DH + PER * lane) * 2;
+    if constexpr (PER == 2) *reinterpret_cast<uint32_t*>(dst) = XMma<E>::pack(acc[0] * inv, acc[1] * inv);
+    else *reinterpret_cast<uint16_t*>(dst) = __builtin_bit_cast(uint16_t, (E)(acc[0] * inv));
+#endif
+}
+
+// The form of a call. Rows, keys and work are guesses from the tensors' sizes: lengths are on the device.
+struct PromptForm {
+    PromptMode mode;
+    bool one;   // single waves of 16 rows (else four that share the keys)
+    int rt;     // rows of a workgroup
+    int nw;     // keys shared out: workgroups per key head
+};
+static PromptForm prompt_form(int B, int Tq, int Tk, int P, int Hq, int Hkv, int Dh, bool split) {
+    const long G = Hq / Hkv, cus = cu_count(), rows = std::max<long>(1, (long)Tq * G / B), keys = Tk / B + P;
+    const long tiles = std::max<long>(B, (long)Tq * G / 64) * Hkv;
+    // the line's places are counted in 32 bits, whatever the lengths
+    const bool fits = ((long)Tq * G / 16 + B) * ((Tk + (long)P) / XKT + 2) < 1 << 29;
+    if (!split || !fits || keys <= 16 * XKT || (rows > 16 && tiles >= 2 * cus)) {
+        const long tiles128 = std::max<long>(B, (long)Tq * G / 128) * Hkv;
+        return {PM_WHOLE, false, tiles128 >= 2 * cus ? 128 : 64, 0};
+    }
+    const bool pack = P >= 2 * XKT && B > 1 && rows <= 32;
+    const long slots = rows <= 16 ? 4 * cus : 2 * cus;
+    return {pack ? PM_PACK : PM_SPLIT, rows <= 16, rows <= 16 ? 16 : 64, (int)std::max<long>(1, slots / Hkv)};
+}
+static size_t prompt_rows_part(const PromptForm& f, int Tq, int Hq) { return f.mode == PM_PACK ? (size_t)2 * Tq * Hq : 0; }
+static size_t prompt_parts(const PromptForm& f, int Tq, int Hq, int Hkv) {
+    return f.mode == PM_WHOLE ? 0 : prompt_rows_part(f, Tq, Hq) + (size_t)Hkv * f.nw * 2 * f.rt;
+}
+size_t prompt_attn_workspace(int B, int Tq, int Tk, int P, int Hq, int Hkv, int Dh) {
+    return prompt_parts(prompt_form(B, Tq, Tk, P, Hq, Hkv, Dh, true), Tq, Hq, Hkv) * (Dh + 2) * sizeof(float);
+}
 
 template <class E, class C>
-static hipError_t prompt_launch(const PromptParams& p, hipStream_t s) {
+static hipError_t prompt_whole(const PromptParams& p, hipStream_t s) {
     // every sequence rounds its rows up to whole tiles
     const size_t tiles = ((size_t)p.Tq * p.G) / C::RT + p.B;
     if (hipError_t e = grid_check(tiles * p.Hkv, C::THREADS)) return e;
-    hipLaunchKernelGGL((k_prompt_attn<E, C>), dim3((unsigned)(tiles * p.Hkv)), dim3(C::THREADS), C::LDS, s, p);
+    hipLaunchKernelGGL((k_prompt_attn<E, C, PM_WHOLE>), dim3((unsigned)(tiles * p.Hkv)), dim3(C::THREADS), C::LDS, s, p);
+    return hipGetLastError();
+}
+template <class E, class C, PromptMode MODE>
+static hipError_t prompt_split(const PromptParams& p, hipStream_t s) {
+    const size_t merges = ((size_t)p.Tq * p.G + 3) / 4 * p.Hkv;
+    if (hipError_t e = grid_check(merges, 256)) return e;
+    hipLaunchKernelGGL((k_prompt_attn<E, C, MODE>), dim3(p.nw * p.Hkv), dim3(C::THREADS), C::LDS, s, p);
+    if (hipError_t e = hipGetLastError()) return e;
+    hipLaunchKernelGGL((k_prompt_merge<E, C::DH, C::RT, MODE>), dim3((unsigned)merges), dim3(256), 0, s, p);
     return hipGetLastError();
 }
 template <class E, int DH>
-static hipError_t prompt_of(const PromptParams& p, hipStream_t s) {
-    return prompt_launch<E, XCfg<DH, 1, 4, true, 4>>(p, s);
+static hipError_t prompt_of(const PromptParams& p, const PromptForm& f, hipStream_t s) {
+    if (f.mode == PM_WHOLE) return f.rt == 128 ? prompt_whole<E, XCfg<DH, 2, 4, true, 4>>(p, s) : prompt_whole<E, XCfg<DH, 1, 4, true, 4>>(p, s);
+    if (f.mode == PM_SPLIT)
+        return f.one ? prompt_split<E, XCfg<DH, 1, 1, false, 2>, PM_SPLIT>(p, s) : prompt_split<E, XCfg<DH, 1, 4, true, 4>, PM_SPLIT>(p, s);
+    return f.one ? prompt_split<E, XCfg<DH, 1, 1, false, 2>, PM_PACK>(p, s) : prompt_split<E, XCfg<DH, 1, 4, true, 4>, PM_PACK>(p, s);
 }
 
 hipError_t launch_prompt_attn(const PromptLaunch& c, hipStream_t s) {
@@ -506,8 +806,15 @@ hipError_t launch_prompt_attn(const PromptLaunch& c, hipStream_t s) {
     p.sc = c.scale * LOG2E;
     p.lift = -1.f - XRESCALE;  // bf16: the weights of all keys sum to less than 1
     for (long n = 1; n < (long)c.Tk + c.P; n *= 2) p.lift -= 1.f;
-    if (c.dt == DT::F16) return c.Dh == 64 ? prompt_of<_Float16, 64>(p, s) : prompt_of<_Float16, 128>(p, s);
-    return c.Dh == 64 ? prompt_of<__bf16, 64>(p, s) : prompt_of<__bf16, 128>(p, s);
+    // sizes that need no workspace run the same form with one and without
+    const size_t need = prompt_attn_workspace(c.B, c.Tq, c.Tk, c.P, c.Hq, c.Hkv, c.Dh);
+    const PromptForm f = prompt_form(c.B, c.Tq, c.Tk, c.P, c.Hq, c.Hkv, c.Dh, need == 0 || (c.ws && c.ws_bytes >= need));
+    p.nw = f.nw;
+    p.rows_part = prompt_rows_part(f, c.Tq, c.Hq);
+    p.part = static_cast<float*>(c.ws);
+    p.part_ml = p.part + prompt_parts(f, c.Tq, c.Hq, c.Hkv) * c.Dh;
+    if (c.dt == DT::F16) return c.Dh == 64 ? prompt_of<_Float16, 64>(p, f, s) : prompt_of<_Float16, 128>(p, f, s);
+    return c.Dh == 64 ? prompt_of<__bf16, 64>(p, f, s) : prompt_of<__bf16, 128>(p, f, s);
 }
 
 }  // namespace kiln
