@@ -38,6 +38,7 @@ struct PromptParams {
     size_t rows_part;    // .. partial results by row in front of those by workgroup
     float* part;         // .. partial results [.][DH], then [.](m, l)
     float* part_ml;
+    uint32_t* cuts;      // .. of each row: its first workgroup, and << 16 their number; then the tiles of a workgroup's part
 };
 
 // How the keys go over the workgroups. WHOLE: a workgroup per key head and row tile. SPLIT: every key head's tiles of keys, row tile by row tile,
@@ -134,15 +135,6 @@ struct PromptLine {
         }
         return -1;
     }
-    // the place of sequence s's first tile
-    __device__ __forceinline__ int start(const PromptParams& p, int s) const {
-        int at = ahead;
-        for (int s0 = 0; s0 < s; s0 += 64) {
-            const int n = s0 ? of(p, s0 + lane) : first;
-            at += wave_sum(s0 + lane < s ? n : 0);
-        }
-        return at;
-    }
 };
 
 // Row tile number `rank` of all sequences' tiles of RT rows, in the order of falling place in their sequence (the longest ranges of keys
@@ -211,7 +203,7 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_prompt_attn(const Prom
     // short ones
     const int hk = (int)(blockIdx.x % p.Hkv), bx = (int)(blockIdx.x / p.Hkv);
     // a row tile: sequence (-1: the prefix's pass over all rows), place in it, its tiles t0 .. t1 - 1 of kt
-    int s = 0, jt = 0, t0 = 0, t1, kt, left_u = 0;
+    int s = 0, jt = 0, t0 = 0, t1, kt, left_u = 0, each = 0;
     PromptSeq sq;
     if constexpr (MODE == PM_WHOLE) {
         s = prompt_find<C::RT>(p, bx, jt);
@@ -219,8 +211,10 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_prompt_attn(const Prom
         sq = prompt_seq(p, s);
     } else {
         const PromptLine<C::RT, MODE> line(p);
-        int u = bx * line.each;
-        left_u = min(line.total - u, line.each);
+        each = line.each;
+        if (bx == 0 && hk == 0 && threadIdx.x == 0) p.cuts[(size_t)p.Tq * p.G] = each;
+        int u = bx * each;
+        left_u = min(line.total - u, each);
         if (left_u <= 0) return;
         if (u < line.ahead) {
             s = -1;
@@ -590,6 +584,10 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_prompt_attn(const Prom
     x_wait_vmcnt<0>();  // no copy into LDS outlives its ring
 
     const bool whole = MODE == PM_WHOLE || (t0 == 0 && t1 == kt);
+    if (MODE != PM_WHOLE && hk == 0 && !ahead && t0 == 0) {  // where the merge finds these rows' parts (the same for every key head)
+        const uint32_t n = kt <= left_u ? 1 : 1 + (kt - left_u + each - 1) / each;
+        for (int i = threadIdx.x; i < C::RT && jt * C::RT + i < rows; i += C::THREADS) p.cuts[(size_t)sq.q0 * p.G + jt * C::RT + i] = (uint32_t)bx | n << 16;
+    }
     if (MODE != PM_WHOLE && (MODE == PM_PACK || !whole)) {
         // partial results: of a whole row tile by row (PACK), else by workgroup: one that begins before it, one that ends behind it
         size_t base = p.rows_part + (((size_t)hk * p.nw + bx) * 2 + (t0 > 0 ? 0 : 1)) * C::RT + (C::SHARED ? wv * C::RW : 0);
@@ -670,26 +668,20 @@ __global__ __launch_bounds__(256) void k_prompt_merge(const PromptParams p) {
         if (has) s = s0 + 63 - __clzll(has);
     }
     if (s < 0) return;
-    const PromptLine<RT, MODE> line(p);
-    const PromptSeq sq = prompt_seq(p, s);
-    const int r = (int)(R - (long long)sq.q0 * p.G), place = r / RT;
-    // the row tile's stretches of the line: workgroups w .. w + n - 1 hold parts of it
-    int at = line.start(p, s);
-    for (int i = 0; i < place; i++) at += prompt_tiles<RT>(p, sq, i, MODE == PM_PACK ? 0 : line.np);
-    const int kt = prompt_tiles<RT>(p, sq, place, MODE == PM_PACK ? 0 : line.np);
-    const int w = at / line.each, n = (at + kt - 1) / line.each - w + 1;
+    const uint32_t cut = p.cuts[R];
+    const int r = (int)(R - (long long)prompt_seq(p, s).q0 * p.G), w = cut & 0xffff, n = cut >> 16;
     if (MODE == PM_SPLIT && n == 1) return;  // written by its workgroup
     int w2 = 0, n2 = 0;
     if (MODE == PM_PACK) {
-        const int at2 = (int)(R / RT) * line.np;
-        w2 = at2 / line.each;
-        n2 = (at2 + line.np - 1) / line.each - w2 + 1;
+        const int np = (p.P + XKT - 1) / XKT, each = (int)p.cuts[(size_t)p.Tq * p.G], at = (int)(R / RT) * np;
+        w2 = at / each;
+        n2 = (at + np - 1) / each - w2 + 1;
     }
     const size_t all = (size_t)p.Tq * p.G;
     auto index = [&](int i) -> size_t {  // of the row's partial result i
         const bool own = MODE == PM_SPLIT || i < n;
-        const int k = own ? i : i - n, cut = own ? n : n2;
-        if (cut == 1) return ((size_t)(own ? 0 : p.Hkv) + hk) * all + R;
+        const int k = own ? i : i - n;
+        if ((own ? n : n2) == 1) return ((size_t)(own ? 0 : p.Hkv) + hk) * all + R;
         return p.rows_part + (((size_t)hk * p.nw + (own ? w : w2) + k) * 2 + (k == 0 ? 1 : 0)) * RT + (own ? r % RT : (int)(R % RT));
     };
     const int parts = n + n2;
@@ -745,14 +737,16 @@ static PromptForm prompt_form(int B, int Tq, int Tk, int P, int Hq, int Hkv, int
     }
     const bool pack = P >= 2 * XKT && B > 1 && rows <= 32;
     const long slots = rows <= 16 ? 4 * cus : 2 * cus;
-    return {pack ? PM_PACK : PM_SPLIT, rows <= 16, rows <= 16 ? 16 : 64, (int)std::max<long>(1, slots / Hkv)};
+    const int rt = rows <= 16 ? 16 : pack || rows < 128 ? 64 : 128;
+    return {pack ? PM_PACK : PM_SPLIT, rows <= 16, rt, (int)std::min<long>(0xffff, std::max<long>(1, slots / Hkv))};
 }
 static size_t prompt_rows_part(const PromptForm& f, int Tq, int Hq) { return f.mode == PM_PACK ? (size_t)2 * Tq * Hq : 0; }
 static size_t prompt_parts(const PromptForm& f, int Tq, int Hq, int Hkv) {
     return f.mode == PM_WHOLE ? 0 : prompt_rows_part(f, Tq, Hq) + (size_t)Hkv * f.nw * 2 * f.rt;
 }
 size_t prompt_attn_workspace(int B, int Tq, int Tk, int P, int Hq, int Hkv, int Dh) {
-    return prompt_parts(prompt_form(B, Tq, Tk, P, Hq, Hkv, Dh, true), Tq, Hq, Hkv) * (Dh + 2) * sizeof(float);
+    const size_t parts = prompt_parts(prompt_form(B, Tq, Tk, P, Hq, Hkv, Dh, true), Tq, Hq, Hkv);
+    return parts ? parts * (Dh + 2) * sizeof(float) + ((size_t)Tq * (Hq / Hkv) + 1) * sizeof(uint32_t) : 0;
 }
 
 template <class E, class C>
@@ -776,7 +770,9 @@ template <class E, int DH>
 static hipError_t prompt_of(const PromptParams& p, const PromptForm& f, hipStream_t s) {
     if (f.mode == PM_WHOLE) return f.rt == 128 ? prompt_whole<E, XCfg<DH, 2, 4, true, 4>>(p, s) : prompt_whole<E, XCfg<DH, 1, 4, true, 4>>(p, s);
     if (f.mode == PM_SPLIT)
-        return f.one ? prompt_split<E, XCfg<DH, 1, 1, false, 2>, PM_SPLIT>(p, s) : prompt_split<E, XCfg<DH, 1, 4, true, 4>, PM_SPLIT>(p, s);
+        return f.one         ? prompt_split<E, XCfg<DH, 1, 1, false, 2>, PM_SPLIT>(p, s)
+               : f.rt == 128 ? prompt_split<E, XCfg<DH, 2, 4, true, 4>, PM_SPLIT>(p, s)
+                             : prompt_split<E, XCfg<DH, 1, 4, true, 4>, PM_SPLIT>(p, s);
     return f.one ? prompt_split<E, XCfg<DH, 1, 1, false, 2>, PM_PACK>(p, s) : prompt_split<E, XCfg<DH, 1, 4, true, 4>, PM_PACK>(p, s);
 }
 
@@ -812,7 +808,9 @@ hipError_t launch_prompt_attn(const PromptLaunch& c, hipStream_t s) {
     p.nw = f.nw;
     p.rows_part = prompt_rows_part(f, c.Tq, c.Hq);
     p.part = static_cast<float*>(c.ws);
-    p.part_ml = p.part + prompt_parts(f, c.Tq, c.Hq, c.Hkv) * c.Dh;
+    const size_t parts = prompt_parts(f, c.Tq, c.Hq, c.Hkv);
+    p.part_ml = p.part + parts * c.Dh;
+    p.cuts = reinterpret_cast<uint32_t*>(p.part_ml + parts * 2);
     if (c.dt == DT::F16) return c.Dh == 64 ? prompt_of<_Float16, 64>(p, f, s) : prompt_of<_Float16, 128>(p, f, s);
     return c.Dh == 64 ? prompt_of<__bf16, 64>(p, f, s) : prompt_of<__bf16, 128>(p, f, s);
 }
