@@ -465,6 +465,9 @@ int kiln_prompt_attn(void* out, int ldo, const void* q, int ldq, const void* k, 
                      int Hq, int Hkv, int Dh, float scale, int B, const int32_t* q_start, const int32_t* k_start, const int32_t* k_len,
                      const void* pk, int ldpk, const void* pv, int ldpv, int P, void* workspace, size_t ws_bytes, kiln_stream_t stream);
 size_t kiln_prompt_attn_workspace_bytes(int B, int Tq, int Tk, int P, int Hq, int Hkv, int Dh);
+/* Which form a call with that workspace runs, for tests and profiles: query rows (tokens Hq / Hkv) of a workgroup << 16 | 1 where the keys are
+ * shared out over workgroups, 2 where the prefix's are taken once for all rows besides; 0 for sizes that the call refuses. */
+int kiln_prompt_attn_form(int B, int Tq, int Tk, int P, int Hq, int Hkv, int Dh);
 
 /* The residual's addition and the RMS norm: h = x + res, y = h / sqrt(mean(h^2) + eps) w per row of dim <= 32768 columns (w bf16 [dim], NULL = 1),
  * in fp32 from the unrounded h; eps > 0. x [rows, ldx] in xdtype, res and h [rows, ld*] in rdtype (both NULL: y is the norm of x), y

@@ -113,6 +113,7 @@ _SIGS = {
     "kiln_prompt_attn": (_i, [_vp, _i, _vp, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _f, _i, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _vp, _sz,
                               _vp]),
     "kiln_prompt_attn_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i]),
+    "kiln_prompt_attn_form": (_i, [_i, _i, _i, _i, _i, _i, _i]),
     "kiln_add_rmsnorm": (_i, [_vp, _i, _i, _vp, _i, _vp, _i, _i, _vp, _i, _i, _vp, _i, _i, _f, _vp]),
     "kiln_add_rmsnorm_mxfp8": (_i, [_vp, _vp, _vp, _i, _vp, _i, _i, _vp, _i, _i, _vp, _i, _i, _f, _vp]),
     "kiln_mxfp8_quantize": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _vp]),
@@ -882,6 +883,14 @@ def linear_mxfp4(y, x, w, epi=KILN_EPI_F32, gate=None, beta=0.0, workspace=None,
 def prompt_attn_workspace_bytes(B, Tq, Tk, P, Hq, Hkv, Dh):
     _fits("prompt_attn_workspace_bytes", B, Tq, Tk, P, Hq, Hkv, Dh)
     return lib().kiln_prompt_attn_workspace_bytes(B, Tq, Tk, P, Hq, Hkv, Dh)
+
+
+def prompt_attn_form(B, Tq, Tk, P, Hq, Hkv, Dh):
+    """The form that prompt_attn runs these sizes on: query rows of a workgroup, and 0, 1 (keys shared out over workgroups) or 2 (the prefix's
+    once for all rows besides)."""
+    _fits("prompt_attn_form", B, Tq, Tk, P, Hq, Hkv, Dh)
+    f = lib().kiln_prompt_attn_form(B, Tq, Tk, P, Hq, Hkv, Dh)
+    return f >> 16, f & 0xffff
 
 
 def _ints(t, n, what):

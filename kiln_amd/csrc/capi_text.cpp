@@ -13,10 +13,19 @@ using namespace kiln::capi;
 
 extern "C" {
 
+// sizes that kiln_prompt_attn takes
+static bool prompt_sizes(int B, int Tq, int Tk, int P, int Hq, int Hkv, int Dh) {
+    if (B <= 0 || Tq <= 0 || Tk < 0 || P < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || (Dh != 64 && Dh != 128)) return false;
+    const long long rows = (long long)Tq * (Hq / Hkv);
+    return rows <= MAX_ROWS && Tk <= MAX_ROWS && P <= MAX_ROWS && (rows / 16 + B) * Hkv < 1 << 24;
+}
+
 size_t kiln_prompt_attn_workspace_bytes(int B, int Tq, int Tk, int P, int Hq, int Hkv, int Dh) {
-    if (B <= 0 || Tq <= 0 || Tk < 0 || P < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || (Dh != 64 && Dh != 128)) return 0;
-    if (Tk > MAX_ROWS || P > MAX_ROWS || (long long)Tq * (Hq / Hkv) > MAX_ROWS) return 0;
-    return kiln::prompt_attn_workspace(B, Tq, Tk, P, Hq, Hkv, Dh);
+    return prompt_sizes(B, Tq, Tk, P, Hq, Hkv, Dh) ? kiln::prompt_attn_workspace(B, Tq, Tk, P, Hq, Hkv, Dh) : 0;
+}
+
+int kiln_prompt_attn_form(int B, int Tq, int Tk, int P, int Hq, int Hkv, int Dh) {
+    return prompt_sizes(B, Tq, Tk, P, Hq, Hkv, Dh) ? kiln::prompt_attn_form(B, Tq, Tk, P, Hq, Hkv, Dh) : 0;
 }
 
 int kiln_prompt_attn(void* out, int ldo, const void* q, int ldq, const void* k, int ldk, const void* v, int ldv, int dtype, int Tq, int Tk,
@@ -34,8 +43,7 @@ int kiln_prompt_attn(void* out, int ldo, const void* q, int ldq, const void* k, 
     if (!q_start && B != 1) return fail(KILN_EINVAL, "prompt_attn: %d sequences without q_start", B);
     if (!k_start && Tk != Tq) return fail(KILN_EINVAL, "prompt_attn: keys of the queries' own rows, but Tq=%d, Tk=%d", Tq, Tk);
     if (!out || !q || (Tk && (!k || !v)) || (P && (!pk || !pv))) return fail(KILN_EINVAL, "prompt_attn: null pointer");
-    const long long G = Hq / Hkv, rows = Tq * G;
-    if (rows > MAX_ROWS || Tk > MAX_ROWS || P > MAX_ROWS || (rows / 16 + B) * Hkv >= 1 << 24)
+    if (!prompt_sizes(B, Tq, Tk, P, Hq, Hkv, Dh))
         return fail(KILN_EUNSUPPORTED, "prompt_attn: too many rows, keys or sequences (B=%d Tq=%d Tk=%d P=%d)", B, Tq, Tk, P);
     const struct {
         const char* name;

@@ -201,6 +201,7 @@ struct PromptLaunch {
     size_t ws_bytes;
 };
 size_t prompt_attn_workspace(int B, int Tq, int Tk, int P, int Hq, int Hkv, int Dh);
+int prompt_attn_form(int B, int Tq, int Tk, int P, int Hq, int Hkv, int Dh);  // rows << 16 | how keys are shared out
 hipError_t launch_prompt_attn(const PromptLaunch& c, hipStream_t s);
 
 // h = x + res (res, h null: x alone), y = h / rms(h) w (add_rmsnorm.hip): y in ydt, or MXFP8 codes when scales is not null

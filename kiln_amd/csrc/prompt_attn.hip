@@ -29,21 +29,23 @@ struct PromptParams {
     void* o;
     size_t ldq, ldk, ldv, ldo, ldpk, ldpv;
     int B, Tq, Tk, P, Hkv, G;
+    uint32_t g_mul;      // r / G = r g_mul >> g_shift, exactly for r < 2^31
+    int g_shift;
     const int* q_start;  // [B + 1], or null: one sequence of all rows
     const int* k_start;  // [B], k_len [B], or null: the queries' own rows
     const int* k_len;
     float sc;            // scale log2(e)
     float lift;          // log2 of the weights' factor
-    int nw;              // keys shared out: workgroups per key head
-    size_t rows_part;    // .. partial results by row in front of those by workgroup
-    float* part;         // .. partial results [.][DH], then [.](m, l)
+    int nw;              // keys shared out: parts per key head that are aimed at
+    int items;           // .. the most that can come of it
+    float* part;         // .. partial results [key head][item][row of the tile][DH], then [.](m, l)
     float* part_ml;
-    uint32_t* cuts;      // .. of each row: its first workgroup, and << 16 their number; then the tiles of a workgroup's part
+    uint32_t* cuts;      // .. of each row: its first item, their number; then the tiles of an item
 };
 
-// How the keys go over the workgroups. WHOLE: a workgroup per key head and row tile. SPLIT: every key head's tiles of keys, row tile by row tile,
-// are one line that its nw workgroups share out in equal parts; a row tile that is cut leaves partial results, joined by k_prompt_merge.
-// PACK: as SPLIT, but the prefix's keys come first and once for all sequences' rows, whose own keys follow without it.
+// How the keys go over the workgroups. WHOLE: a workgroup per key head and row tile. SPLIT: row tiles are cut into items of about equal numbers
+// of key tiles, as many over all sequences as fill the chip, a workgroup each; the partial results of a row are joined by
+// k_prompt_merge. PACK: as SPLIT, but the prefix's keys are taken once for all sequences' rows, whose own keys follow without it.
 enum PromptMode { PM_WHOLE, PM_SPLIT, PM_PACK };
 constexpr int PROMPT_LEAST = 4;  // tiles of a workgroup's part
 
@@ -66,15 +68,30 @@ __device__ __forceinline__ PromptSeq prompt_seq(const PromptParams& p, int s) {
     return r;
 }
 
-// Keys that the last row of a sequence's row tile `place` sees, and its tiles (one at least: a row without keys is zeros) behind np of the prefix
+__device__ __forceinline__ int prompt_token(const PromptParams& p, int r) { return (int)((uint64_t)(uint32_t)r * p.g_mul >> p.g_shift); }  // r / G
+// the sequences, the first 64 of them a lane each
+struct PromptSeqs {
+    PromptSeq mine;  // of sequence `lane` (none: no rows)
+    __device__ __forceinline__ explicit PromptSeqs(const PromptParams& p) : mine{0, 0, 0, 0} {
+        const int lane = threadIdx.x & 63;
+        if (lane < p.B) mine = prompt_seq(p, lane);
+    }
+    __device__ __forceinline__ PromptSeq lane_of(const PromptParams& p, int s0) const {  // sequence s0 + lane
+        if (s0 == 0) return mine;
+        const int s = s0 + (int)(threadIdx.x & 63);
+        return s < p.B ? prompt_seq(p, s) : PromptSeq{0, 0, 0, 0};
+    }
+    __device__ __forceinline__ PromptSeq get(const PromptParams& p, int s) const {  // s the same in all lanes
+        if (s >= 64) return prompt_seq(p, s);
+        return {__builtin_amdgcn_readlane(mine.q0, s), __builtin_amdgcn_readlane(mine.nq, s), __builtin_amdgcn_readlane(mine.k0, s),
+                __builtin_amdgcn_readlane(mine.nk, s)};
+    }
+};
+
+// Keys that the last row of a sequence's row tile `place` sees
 template <int RT>
 __device__ __forceinline__ int prompt_keys(const PromptParams& p, const PromptSeq& q, int place) {
-    const int rows = q.nq * p.G;
-    return max(0, min(q.nk, (min(rows, (place + 1) * RT) - 1) / p.G + q.nk - q.nq + 1));
-}
-template <int RT>
-__device__ __forceinline__ int prompt_tiles(const PromptParams& p, const PromptSeq& q, int place, int np) {
-    return max(1, np + (prompt_keys<RT>(p, q, place) + XKT - 1) / XKT);
+    return max(0, min(q.nk, min(q.nq - 1, prompt_token(p, (place + 1) * RT - 1)) + q.nk - q.nq + 1));
 }
 // the sum over a wave's lanes, in all of them
 __device__ __forceinline__ int wave_sum(int v) {
@@ -99,32 +116,33 @@ __device__ __forceinline__ int wave_scan(int v) {
     return v;
 }
 
-// A key head's line of tiles: `ahead` of the prefix over all rows (PACK), then each sequence's; `each` tiles to a workgroup
+// A key head's items: `ahead` of the prefix over all rows (PACK; each row tile `per` of them), then each sequence's. A sequence's row tiles are all
+// cut into as many as its longest needs to have at most `each` key tiles in one (early ones of a causal prompt have fewer, or none).
 template <int RT, PromptMode MODE>
-struct PromptLine {
-    int lane, np, ahead, total, each, first;  // first: the tiles of sequence `lane`
-    __device__ __forceinline__ int of(const PromptParams& p, int s) const {
-        if (s >= p.B) return 0;
-        const PromptSeq q = prompt_seq(p, s);
-        int n = 0;
-        for (int i = 0; i * RT < q.nq * p.G; i++) n += prompt_tiles<RT>(p, q, i, MODE == PM_PACK ? 0 : np);
-        return n;
-    }
-    __device__ __forceinline__ explicit PromptLine(const PromptParams& p) {
-        lane = threadIdx.x & 63;
+struct PromptItems {
+    int np, each, per, ahead;
+    __device__ __forceinline__ static int row_tiles(const PromptParams& p, const PromptSeq& q) { return (q.nq * p.G + RT - 1) / RT; }
+    __device__ __forceinline__ int key_tiles(const PromptSeq& q) const { return max(1, (MODE == PM_PACK ? 0 : np) + (q.nk + XKT - 1) / XKT); }
+    __device__ __forceinline__ int cuts(const PromptSeq& q) const { return (key_tiles(q) + each - 1) / each; }
+    __device__ __forceinline__ PromptItems(const PromptParams& p, const PromptSeqs& seqs) {
         np = (p.P + XKT - 1) / XKT;
-        ahead = MODE == PM_PACK ? (p.Tq * p.G + RT - 1) / RT * np : 0;
-        first = of(p, lane);
-        int n = first;
-        for (int s = 64; s < p.B; s += 64) n += of(p, s + lane);
-        total = ahead + wave_sum(n);
+        const int all = (p.Tq * p.G + RT - 1) / RT;  // row tiles of all rows
+        int n = 0;
+        for (int s0 = 0; s0 < p.B; s0 += 64) {
+            const PromptSeq q = seqs.lane_of(p, s0);
+            n += row_tiles(p, q) * key_tiles(q);
+        }
+        const int total = wave_sum(n) + (MODE == PM_PACK ? all * np : 0);
         each = max(PROMPT_LEAST, (total + p.nw - 1) / p.nw);
+        per = (np + each - 1) / each;
+        ahead = MODE == PM_PACK ? all * per : 0;
     }
-    // the sequence that holds place `at` of the line (>= ahead), or -1; at: counted from the sequence's first tile
-    __device__ __forceinline__ int find(const PromptParams& p, int& at) const {
+    // the sequence that holds item `at` >= ahead, or -1; at: counted from the sequence's first
+    __device__ __forceinline__ int find(const PromptParams& p, const PromptSeqs& seqs, int& at) const {
         at -= ahead;
         for (int s0 = 0; s0 < p.B; s0 += 64) {
-            const int n = s0 ? of(p, s0 + lane) : first, up = wave_scan(n);
+            const PromptSeq q = seqs.lane_of(p, s0);
+            const int n = row_tiles(p, q) * cuts(q), up = wave_scan(n);
             const unsigned long long past = __ballot(up > at);
             if (past) {
                 const int i = __ffsll(past) - 1;
@@ -140,35 +158,22 @@ struct PromptLine {
 // Row tile number `rank` of all sequences' tiles of RT rows, in the order of falling place in their sequence (the longest ranges of keys
 // first): its sequence and place, or -1 past the last. With F(n) the number of tiles at place n or later, F(n + 1) <= rank < F(n).
 template <int RT>
-__device__ __forceinline__ int prompt_find(const PromptParams& p, int rank, int& place) {
+__device__ __forceinline__ int prompt_find(const PromptParams& p, const PromptSeqs& seqs, int rank, int& place) {
     const int lane = threadIdx.x & 63;
-    auto tiles = [&](int s) {
-        if (s >= p.B) return 0;
-        const PromptSeq q = prompt_seq(p, s);
-        return (q.nq * p.G + RT - 1) / RT;
-    };
+    auto tiles = [&](int s0) { return (seqs.lane_of(p, s0).nq * p.G + RT - 1) / RT; };
+    const int own = tiles(0);
     if (p.B == 1) {
-        place = __builtin_amdgcn_readfirstlane(tiles(0)) - 1 - rank;
+        place = __builtin_amdgcn_readfirstlane(own) - 1 - rank;
         return place >= 0 ? 0 : -1;
     }
-    int own[4], most = 0;  // of the first 256 sequences; more are read again
-#pragma unroll
-    for (int c = 0; c < 4; c++) {
-        own[c] = c * 64 < p.B ? tiles(c * 64 + lane) : 0;
-        most = max(most, own[c]);
-    }
-    for (int s = 256; s < p.B; s += 64) most = max(most, tiles(s + lane));
     auto from = [&](int n) {  // F(n)
-        int sum = 0;
-#pragma unroll
-        for (int c = 0; c < 4; c++) sum += max(0, own[c] - n);
-        for (int s = 256; s < p.B; s += 64) sum += max(0, tiles(s + lane) - n);
+        int sum = max(0, own - n);
+        for (int s0 = 64; s0 < p.B; s0 += 64) sum += max(0, tiles(s0) - n);
         return wave_sum(sum);
     };
     if (rank >= from(0)) return -1;
-#pragma unroll
-    for (int i = 32; i; i >>= 1) most = max(most, __shfl_xor(most, i, 64));
-    int lo = 0, hi = __builtin_amdgcn_readfirstlane(most), fhi = 0;  // F(lo) > rank >= F(hi) = fhi
+    int lo = 0, hi = 1, fhi;  // F(lo) > rank >= F(hi) = fhi
+    while ((fhi = from(hi)) > rank) lo = hi, hi *= 2;
     while (hi - lo > 1) {
         const int mid = (lo + hi) / 2, f = from(mid);
         if (f > rank) lo = mid;
@@ -178,7 +183,7 @@ __device__ __forceinline__ int prompt_find(const PromptParams& p, int rank, int&
     // the sequences with a tile at this place, in their order
     int want = rank - fhi;
     for (int s0 = 0; s0 < p.B; s0 += 64) {
-        const unsigned long long has = __ballot(tiles(s0 + lane) > lo);
+        const unsigned long long has = __ballot((s0 ? tiles(s0) : own) > lo);
         const int n = __popcll(has);
         if (want < n) {
             // lane i counts the set bits below it
@@ -190,121 +195,113 @@ __device__ __forceinline__ int prompt_find(const PromptParams& p, int rank, int&
     return -1;
 }
 
+// A workgroup's geometry: RV waves of 16 QB rows, KG times: key groups that take every KG-th tile, each with a ring of NS tiles that its
+// waves share, and join their results in LDS. One wave alone: a ring of its own.
+template <int DH_, int QB_, int RV_, int KG_, int NS_>
+struct PCfg {
+    static constexpr int DH = DH_, QB = QB_, RV = RV_, KG = KG_, NS = NS_, NW = RV * KG;
+    static constexpr bool SHARED = NW > 1;
+    static constexpr int THREADS = 64 * NW, GTHREADS = 64 * RV, RW = 16 * QB, RT = RW * RV;  // threads of a key group, rows of a wave, of the workgroup
+    static constexpr int PC = DH / 8;                                  // 16-byte chunks of a row
+    static constexpr int TILE = XKT * DH * 2, STAGE = 2 * TILE;        // K tile, V tile
+    static constexpr int DMA = XKT * PC / GTHREADS;                    // 16-byte pieces per thread, for K and for V each
+    static constexpr int RING = NS * STAGE;
+    static constexpr int JOIN = (KG - 1) * RT * (DH + 8) * 4;          // a lane's accumulators, and m and l of its rows
+    static constexpr int LDS = RING * KG > JOIN ? RING * KG : JOIN;
+    static constexpr int WAVES = 2;                                    // per SIMD that registers have to allow
+};
+
 template <class E, class C, PromptMode MODE>
 __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_prompt_attn(const PromptParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)  // the host pass drops a kernel template whose target builtins it cannot check
     using M = XMma<E>;
     constexpr int DH = C::DH, QB = C::QB;
-    static_assert(C::SHARED || C::NW == 1, "waves share the keys, or one has them to itself");
     extern __shared__ __attribute__((aligned(16))) uint8_t xlds[];
-    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int kg = wave / C::RV, wv = wave % C::RV;  // key group, rows' wave
     const int g = lane >> 4, c16 = lane & 15;
     // key heads side by side: blocks go round the 8 XCDs, so that a head's row tiles share the L2s of few, and every XCD has long and
     // short ones
     const int hk = (int)(blockIdx.x % p.Hkv), bx = (int)(blockIdx.x / p.Hkv);
-    // a row tile: sequence (-1: the prefix's pass over all rows), place in it, its tiles t0 .. t1 - 1 of kt
-    int s = 0, jt = 0, t0 = 0, t1, kt, left_u = 0, each = 0;
-    PromptSeq sq;
+    // a row tile: its sequence and place there; all its tiles, or (part) item `cut` of `cuts`
+    int s = 0, jt = 0, cut = 0, cuts = 1;
+    bool ahead = false;  // the prefix's pass over all rows
+    const PromptSeqs seqs(p);
     if constexpr (MODE == PM_WHOLE) {
-        s = prompt_find<C::RT>(p, bx, jt);
+        s = prompt_find<C::RT>(p, seqs, bx, jt);
         if (s < 0) return;
-        sq = prompt_seq(p, s);
     } else {
-        const PromptLine<C::RT, MODE> line(p);
-        each = line.each;
-        if (bx == 0 && hk == 0 && threadIdx.x == 0) p.cuts[(size_t)p.Tq * p.G] = each;
-        int u = bx * each;
-        left_u = min(line.total - u, each);
-        if (left_u <= 0) return;
-        if (u < line.ahead) {
-            s = -1;
-            jt = u / line.np;
-            t0 = u % line.np;
+        const PromptItems<C::RT, MODE> items(p, seqs);
+        if (bx == 0 && hk == 0 && threadIdx.x == 0) p.cuts[(size_t)p.Tq * p.G * 2] = items.each;
+        ahead = bx < items.ahead;
+        int at = bx;
+        if (ahead) {
+            cuts = items.per;
         } else {
-            s = line.find(p, u);
-            sq = prompt_seq(p, s);
-            for (int n; u >= (n = prompt_tiles<C::RT>(p, sq, jt, MODE == PM_PACK ? 0 : line.np)); jt++) u -= n;
-            t0 = u;
+            s = items.find(p, seqs, at);
+            if (s < 0) return;
+            cuts = items.cuts(seqs.get(p, s));
         }
+        jt = at / cuts;
+        cut = at % cuts;
     }
-    for (;;) {
-    const bool ahead = MODE == PM_PACK && s < 0;
-    if (ahead) sq = PromptSeq{0, p.Tq, 0, 0};
+    const PromptSeq sq = ahead ? PromptSeq{0, p.Tq, 0, 0} : seqs.get(p, s);
     const int rows = sq.nq * p.G, diff = sq.nk - sq.nq;
-    const int np = MODE == PM_PACK && !ahead ? 0 : (p.P + XKT - 1) / XKT;
-    const int row0 = jt * C::RT + (C::SHARED ? wv * C::RW : 0);
-    // the row tile's own keys
+    const int P = MODE == PM_PACK && !ahead ? 0 : p.P;
+    const int row0 = jt * C::RT + wv * C::RW;
+    // the row tile's own keys; its tiles: the prefix's whole ones, the own keys', the prefix's end (order is nothing to a softmax, and so those
+    // with keys to hide come last)
     const int L = ahead ? 0 : prompt_keys<C::RT>(p, sq, jt);
-    kt = max(1, np + (L + XKT - 1) / XKT);
-    t1 = MODE == PM_WHOLE ? kt : min(kt, t0 + left_u);
+    const int fp = P / XKT, own_end = fp + (L + XKT - 1) / XKT, kt = max(1, own_end + (P % XKT ? 1 : 0));
+    const int t0 = MODE == PM_WHOLE ? 0 : (int)((long long)kt * cut / cuts), t1 = MODE == PM_WHOLE ? kt : (int)((long long)kt * (cut + 1) / cuts);
+    if (MODE != PM_WHOLE && hk == 0 && !ahead && cut == 0)  // where the merge finds these rows' parts (the same for every key head)
+        for (int i = threadIdx.x; i < C::RT && jt * C::RT + i < rows; i += C::THREADS)
+            *reinterpret_cast<uint2*>(p.cuts + ((size_t)sq.q0 * p.G + jt * C::RT + i) * 2) = make_uint2(bx, cuts);
 
-    uint8_t* ring = xlds;
+    uint8_t* ring = xlds + kg * C::RING;
     const uint32_t lds_base = (uint32_t)(size_t)(__attribute__((address_space(3))) uint8_t*)ring;
 
-    // DMA of the tiles' K and V in turn: a thread's pieces are chunks of fixed rows of a tile; the descriptor's range ends with
-    // the last row (empty past the last tile)
+    // DMA of this key group's tiles t0 + kg, t0 + kg + KG, .., K and V in turn: a thread's pieces are chunks of fixed rows of a tile; the
+    // descriptor's range ends with the last row of the prefix or of the own keys, and is empty from tile t1 on
     struct Stream {
-        const uint8_t* src;     // the next tile to copy
-        uint32_t ld2;           // bytes from row to row
-        int j;                  // its index
+        const uint8_t* src;  // the next tile to copy
+        uint32_t ld2;        // bytes from row to row
+        int left;            // rows from its first on
+        int j, end;          // its number, and where the rows' stretch ends
         uint32_t off[C::DMA];
     } kst, vst;
-    const uint8_t* own_k = static_cast<const uint8_t*>(p.k) + ((long long)sq.k0 * p.ldk + (long long)hk * DH) * 2;
-    const uint8_t* own_v = static_cast<const uint8_t*>(p.v) + ((long long)sq.k0 * p.ldv + (long long)hk * DH) * 2;
-    auto place_k = [&](uint32_t ld2) {
-        kst.ld2 = ld2;
+    auto place = [&](Stream& t, const void* pre, size_t ld_pre, const void* own, size_t ld_own, auto is_k) {  // the stretch of tile t.j
+        const bool mine = t.j >= fp && t.j < own_end;
+        const size_t ld = mine ? ld_own : ld_pre;
+        const uint32_t ld2 = t.ld2 = (uint32_t)ld * 2;
+        const int tile = t.j < fp ? t.j : mine ? t.j - fp : fp;  // its place in the stretch's rows
+        const int rows = t.j >= t1 ? 0 : mine ? min(L, (t1 - fp) * XKT) : min(P, t1 * XKT);
+        t.end = t.j < fp ? fp : mine ? own_end : 0x7fffffff;
+        t.src = static_cast<const uint8_t*>(mine ? own : pre) + ((mine ? (long long)sq.k0 * ld : 0) + (long long)hk * DH) * 2 + (long long)tile * XKT * ld2;
+        t.left = rows - tile * XKT;
 #pragma unroll
         for (int i = 0; i < C::DMA; i++) {
-            const int pc = i * C::RTHREADS + (C::SHARED ? (int)threadIdx.x : lane), r = pc / C::PC, c = pc % C::PC;
-            kst.off[i] = r * ld2 + k_swz<DH>(c, r) * 16;
+            const int pc = i * C::GTHREADS + wv * 64 + lane, r = pc / C::PC, c = pc % C::PC;
+            t.off[i] = r * ld2 + (decltype(is_k)::value ? k_swz<DH>(c, r) : v_swz<DH>(c, r)) * 16;
         }
     };
-    auto place_v = [&](uint32_t ld2) {
-        vst.ld2 = ld2;
-#pragma unroll
-        for (int i = 0; i < C::DMA; i++) {
-            const int pc = i * C::RTHREADS + (C::SHARED ? (int)threadIdx.x : lane), r = pc / C::PC, c = pc % C::PC;
-            vst.off[i] = r * ld2 + v_swz<DH>(c, r) * 16;
-        }
-    };
-    kst.j = vst.j = t0;
-    if (t0 < np) {
-        place_k((uint32_t)p.ldpk * 2);
-        place_v((uint32_t)p.ldpv * 2);
-        kst.src = static_cast<const uint8_t*>(p.pk) + (long long)hk * DH * 2 + (long long)t0 * XKT * kst.ld2;
-        vst.src = static_cast<const uint8_t*>(p.pv) + (long long)hk * DH * 2 + (long long)t0 * XKT * vst.ld2;
-    } else {
-        place_k((uint32_t)p.ldk * 2);
-        place_v((uint32_t)p.ldv * 2);
-        kst.src = own_k + (long long)(t0 - np) * XKT * kst.ld2;
-        vst.src = own_v + (long long)(t0 - np) * XKT * vst.ld2;
-    }
-    auto left_of = [&](int j) { return j < np ? p.P - j * XKT : L - (j - np) * XKT; };  // keys from tile j's first on
-    auto copy = [&](Stream& t, uint32_t at) {
-        const int left = t.j < t1 ? min(XKT, left_of(t.j)) : 0;
+    auto copy = [&](Stream& t, uint32_t at, const void* pre, size_t ld_pre, const void* own, size_t ld_own, auto is_k) {
+        if (t.j >= t.end) place(t, pre, ld_pre, own, ld_own, is_k);
         const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
-            const_cast<uint8_t*>(t.src), (short)0, left > 0 ? (int)((left - 1) * t.ld2 + DH * 2) : 0, 0x00020000 /* raw */);
-        uint8_t* dst = ring + at + (C::SHARED ? wv * 1024 : 0);
+            const_cast<uint8_t*>(t.src), (short)0, t.left > 0 ? (int)((min(t.left, XKT) - 1) * t.ld2 + DH * 2) : 0, 0x00020000 /* raw */);
+        uint8_t* dst = ring + at + wv * 1024;
 #pragma unroll
         for (int i = 0; i < C::DMA; i++)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(dst + i * C::RTHREADS * 16), 16, t.off[i], 0, 0, 0);
-        if (t.j + 1 < t1) t.src += (size_t)XKT * t.ld2;
-        t.j++;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(dst + i * C::GTHREADS * 16), 16, t.off[i], 0, 0, 0);
+        t.src += (size_t)C::KG * XKT * t.ld2;
+        t.left -= C::KG * XKT;
+        t.j += C::KG;
     };
-    auto copy_k = [&](int stage) {
-        copy(kst, stage * C::STAGE);
-        if (kst.j == np && np < t1) {  // from the prefix to the sequence's own keys
-            place_k((uint32_t)p.ldk * 2);
-            kst.src = own_k;
-        }
-    };
-    auto copy_v = [&](int stage) {
-        copy(vst, stage * C::STAGE + C::TILE);
-        if (vst.j == np && np < t1) {
-            place_v((uint32_t)p.ldv * 2);
-            vst.src = own_v;
-        }
-    };
+    kst.j = vst.j = t0 + kg;
+    place(kst, p.pk, p.ldpk, p.k, p.ldk, std::true_type{});
+    place(vst, p.pv, p.ldpv, p.v, p.ldv, std::false_type{});
+    auto copy_k = [&](int stage) { copy(kst, stage * C::STAGE, p.pk, p.ldpk, p.k, p.ldk, std::true_type{}); };
+    auto copy_v = [&](int stage) { copy(vst, stage * C::STAGE + C::TILE, p.pv, p.ldpv, p.v, p.ldv, std::false_type{}); };
 
     // Q: the B operands of S^T, lane (row c16, chunk 4 cc + g); rows past the last read the last and are not stored. lim: the own keys
     // that a row sees
@@ -312,14 +309,14 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_prompt_attn(const Prom
     int lim[QB];
 #pragma unroll
     for (int qb = 0; qb < QB; qb++) {
-        const int r = min(row0 + 16 * qb + c16, rows - 1), t = r / p.G, h = hk * p.G + r % p.G;
+        const int r = min(row0 + 16 * qb + c16, rows - 1), t = prompt_token(p, r), h = hk * p.G + r - t * p.G;
         const uint8_t* src = static_cast<const uint8_t*>(p.q) + ((long long)(sq.q0 + t) * p.ldq + (long long)h * DH + 8 * g) * 2;
 #pragma unroll
         for (int cc = 0; cc < DH / 32; cc++) qf[qb][cc] = *reinterpret_cast<const u32x4*>(src + 64 * cc);
         lim[qb] = t + diff + 1;
     }
     // of the wave's first and last row
-    const int lim0 = min(row0, rows - 1) / p.G + diff + 1, lim1 = min(row0 + C::RW - 1, rows - 1) / p.G + diff + 1;
+    const int lim0 = prompt_token(p, min(row0, rows - 1)) + diff + 1, lim1 = prompt_token(p, min(row0 + C::RW - 1, rows - 1)) + diff + 1;
 
     floatx4 o[DH / 16][QB], l[QB];  // l: every register of a lane holds its row's sum (P^T times ones)
     const float lift = std::is_same<E, _Float16>::value ? XLIFT16 : p.lift;
@@ -367,14 +364,16 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_prompt_attn(const Prom
                 for (int qb = 0; qb < QB; qb++)
                     s[kk][qb] = M::mul(kf[kk][cc], qf[qb][cc], cc == 0 ? floatx4{0.f, 0.f, 0.f, 0.f} : s[kk][qb]);
     };
-    // tile j's keys that a row sees: the first lim - (its first own key), or all up to the prefix's end
+    // The first tile with keys that some row of the wave does not see (the prefix's end, at last); in own ones from `from_apart` on rows see
+    // different keys.
+    const int from_hide = min(C::KG > 1 ? min(t1, own_end) : own_end, fp + max(lim0, 0) / XKT);
+    const int from_apart = lim0 < lim1 ? fp + max(lim0, 0) / XKT : 0x7fffffff;
+    // a row sees the first lim - (its first own key) of tile j's keys, or all up to the prefix's end; none of a tile past the last
     auto hide = [&](int j, floatx4 (&s)[2][QB]) {
-        const bool pre = j < np;
-        const int key0 = (j - np) * XKT;
-        if ((pre ? p.P - j * XKT : lim0 - key0) >= XKT) return;
+        if (j < from_hide) return;
 #pragma unroll
         for (int qb = 0; qb < QB; qb++) {
-            const int seen = (pre ? p.P - j * XKT : lim[qb] - key0) - 4 * g;
+            const int seen = (C::KG > 1 && j >= t1 ? 0 : j < own_end ? lim[qb] - (j - fp) * XKT : P % XKT) - 4 * g;
 #pragma unroll
             for (int kk = 0; kk < 2; kk++)
 #pragma unroll
@@ -432,10 +431,11 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_prompt_attn(const Prom
     // Tile j, that rows of this wave see different parts of: infinities and NaNs of V leave the operands; the rows that see them take
     // their products here. V's rows are read from the stage itself, four dimensions of a key a lane, as the accumulators lie.
     auto keep_apart = [&](int j, uint32_t st, u32x4 (&vf)[DH / 16], const u32x4 (&pf)[QB]) __attribute__((always_inline)) {
-        floatx4 z = {0.f, 0.f, 0.f, 0.f};
+        floatx4 z[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-        for (int db = 0; db < DH / 16; db++) z = M::mul(vf[db], u32x4{0, 0, 0, 0}, z);
-        const float zs = (z[0] + z[1]) + (z[2] + z[3]);
+        for (int db = 0; db < DH / 16; db++) z[db & 1] = M::mul(vf[db], u32x4{0, 0, 0, 0}, z[db & 1]);
+        z[0] += z[1];
+        const float zs = (z[0][0] + z[0][1]) + (z[0][2] + z[0][3]);
         if (!__any(zs != 0.f)) return;  // 0, or NaN
         constexpr uint32_t EXP = std::is_same<E, _Float16>::value ? 0x7c00u : 0x7f80u;
 #pragma unroll
@@ -463,7 +463,7 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_prompt_attn(const Prom
                 const uint32_t word = w == 0 ? pf[qb][0] : w == 1 ? pf[qb][1] : w == 2 ? pf[qb][2] : pf[qb][3];
                 const uint16_t pb = (uint16_t)(__shfl(word, 16 * (key >> 2 & 3) + c16, 64) >> (16 * (key & 1)));
                 const float pw = (float)__builtin_bit_cast(E, pb);
-                const bool sees = (j - np) * XKT + key < lim[qb];
+                const bool sees = (j - fp) * XKT + key < lim[qb];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const uint16_t vb = (uint16_t)(v4[i / 2] >> (16 * (i & 1)));
@@ -476,12 +476,11 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_prompt_attn(const Prom
         }
     };
 
-    auto apart = [&](int j) { return j >= np && lim0 < lim1 && lim0 - (j - np) * XKT < XKT; };
     if constexpr (C::SHARED) {
         // A step computes the scores of tile j + 1 ahead of the weights and products of tile j. K of tile j + 1 and V of tile j landed (past
         // the last tile the copies go on with empty ranges, which keeps the count); every wave is done with K of tile j and V of tile
         // j - 1, whose places take K of tile j + NS and V of tile j + NS - 1.
-        constexpr int NS = C::NS;
+        constexpr int NS = C::NS, KG = C::KG;
         static_assert(NS % 2 == 0, "the scores' two sets go with the stages");
         floatx4 sc[2][2][QB];
         float top[QB];
@@ -497,54 +496,75 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_prompt_attn(const Prom
         __builtin_amdgcn_sched_barrier(0);
         read_k(0, kf);
         scores(kf, sc[0]);
-        hide(t0, sc[0]);
+        hide(t0 + kg, sc[0]);
         largest(sc[0], top);
-        auto step = [&](int j, auto parity, auto st) {  // st: the stage of tile j, a constant or not
-            constexpr int cur = decltype(parity)::value;
+        auto begin = [&](auto st) {
             x_wait_vmcnt<2 * (NS - 2) * C::DMA>();
             __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
             __builtin_amdgcn_s_barrier();
             __builtin_amdgcn_sched_barrier(0);
+        };
+        // (behind the reads of V: the compiler has each wait for all copies that are under way)
+        auto copies = [&](auto st) {
+            __builtin_amdgcn_sched_barrier(0);
             copy_k(st);
             copy_v((st + NS - 1) % NS);
-            read_k((st + 1) % NS * C::STAGE, kf);
-#pragma unroll
-            for (int db = 0; db < DH / 16; db++) vf[db] = read_v(st * C::STAGE, db);
-            rescale(top, sc[cur]);
             __builtin_amdgcn_sched_barrier(0);
-            weights(sc[cur], pf);
-            scores(kf, sc[cur ^ 1]);
-            __builtin_amdgcn_sched_barrier(0);
-            if (apart(j)) keep_apart(j, st * C::STAGE, vf, pf);
-            if (j + 1 < t1) hide(j + 1, sc[cur ^ 1]);
+        };
+        auto products = [&]() {
 #pragma unroll
             for (int qb = 0; qb < QB; qb++) l[qb] = M::mul(ones, pf[qb], l[qb]);
 #pragma unroll
             for (int db = 0; db < DH / 16; db++)
 #pragma unroll
                 for (int qb = 0; qb < QB; qb++) o[db][qb] = M::mul(vf[db], pf[qb], o[db][qb]);
+        };
+        auto step = [&](auto parity, auto st) {  // a tile with nothing to hide, nor the next, at a stage that is a constant
+            constexpr int cur = decltype(parity)::value;
+            begin(st);
+            read_k((st + 1) % NS * C::STAGE, kf);
+#pragma unroll
+            for (int db = 0; db < DH / 16; db++) vf[db] = read_v(st * C::STAGE, db);
+            copies(st);
+            rescale(top, sc[cur]);
+            __builtin_amdgcn_sched_barrier(0);
+            weights(sc[cur], pf);
+            scores(kf, sc[cur ^ 1]);
+            __builtin_amdgcn_sched_barrier(0);
+            products();
             largest(sc[cur ^ 1], top);
+        };
+        auto step_any = [&](int j, int st) {  // any tile, any stage
+            begin(st);
+            read_k((st + 1) % NS * C::STAGE, kf);
+#pragma unroll
+            for (int db = 0; db < DH / 16; db++) vf[db] = read_v(st * C::STAGE, db);
+            copies(st);
+            rescale(top, sc[0]);
+            __builtin_amdgcn_sched_barrier(0);
+            weights(sc[0], pf);
+            scores(kf, sc[0]);
+            __builtin_amdgcn_sched_barrier(0);
+            if (j >= from_apart && j < own_end) keep_apart(j, st * C::STAGE, vf, pf);
+            products();
+            hide(j + KG, sc[0]);
+            largest(sc[0], top);
         };
         using P0 = std::integral_constant<int, 0>;
         using P1 = std::integral_constant<int, 1>;
-        if constexpr (QB == 1) {
-            for (int j = t0, st = 0; j < t1; j += 2, st = (st + 2) % NS) {
-                step(j, P0{}, st);
-                if (j + 1 >= t1) break;
-                step(j + 1, P1{}, st + 1);
-            }
-        } else {
-            static_assert(NS == 4, "the loop names its stages");
-            for (int j = t0; j < t1; j += 4) {
-                step(j, P0{}, P0{});
-                if (j + 1 >= t1) break;
-                step(j + 1, P1{}, P1{});
-                if (j + 2 >= t1) break;
-                step(j + 2, P0{}, std::integral_constant<int, 2>{});
-                if (j + 3 >= t1) break;
-                step(j + 3, P1{}, std::integral_constant<int, 3>{});
+        // First the tiles with nothing to hide in any wave, two steps at a time, their stages constants; then the others one by one. (The
+        // groups take the same number of steps: the second's last tile may lie past the end.)
+        const int special = min(t1, min(own_end, fp + max(prompt_token(p, min(jt * C::RT, rows - 1)) + diff + 1, 0) / XKT));
+        int j = t0 + kg, st = 0;
+        for (; j - kg + NS * KG + KG - 1 < special; j += NS * KG) {
+            step(P0{}, P0{});
+            step(P1{}, P1{});
+            if constexpr (NS == 4) {
+                step(P0{}, std::integral_constant<int, 2>{});
+                step(P1{}, std::integral_constant<int, 3>{});
             }
         }
+        for (; j - kg < t1; j += KG, st = (st + 1) % NS) step_any(j, st);
     } else {
         int stage = 0;
 #pragma unroll
@@ -571,7 +591,7 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_prompt_attn(const Prom
             weights(sc, pf);
 #pragma unroll
             for (int db = 0; db < DH / 16; db++) vf[db] = read_v(st, db);
-            if (apart(j)) keep_apart(j, st, vf, pf);
+            if (j >= from_apart && j < own_end) keep_apart(j, st, vf, pf);
 #pragma unroll
             for (int qb = 0; qb < QB; qb++) l[qb] = M::mul(ones, pf[qb], l[qb]);
 #pragma unroll
@@ -582,16 +602,40 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_prompt_attn(const Prom
         }
     }
     x_wait_vmcnt<0>();  // no copy into LDS outlives its ring
-
-    const bool whole = MODE == PM_WHOLE || (t0 == 0 && t1 == kt);
-    if (MODE != PM_WHOLE && hk == 0 && !ahead && t0 == 0) {  // where the merge finds these rows' parts (the same for every key head)
-        const uint32_t n = kt <= left_u ? 1 : 1 + (kt - left_u + each - 1) / each;
-        for (int i = threadIdx.x; i < C::RT && jt * C::RT + i < rows; i += C::THREADS) p.cuts[(size_t)sq.q0 * p.G + jt * C::RT + i] = (uint32_t)bx | n << 16;
+    if constexpr (C::KG > 1) {
+        // the second group's results go to the first's lanes, which hold the same rows and dimensions
+        static_assert(C::KG == 2, "two groups");
+        floatx4* jo = reinterpret_cast<floatx4*>(xlds) + wv * (DH / 16 * QB + QB) * 64 + lane;
+        __builtin_amdgcn_s_waitcnt(0xC07F);
+        __builtin_amdgcn_s_barrier();  // every wave is done with the rings, and its copies landed
+        __builtin_amdgcn_sched_barrier(0);
+        if (kg == 1) {
+#pragma unroll
+            for (int qb = 0; qb < QB; qb++) {
+#pragma unroll
+                for (int db = 0; db < DH / 16; db++) jo[(qb * (DH / 16) + db) * 64] = o[db][qb];
+                jo[(QB * (DH / 16) + qb) * 64] = floatx4{m[qb], l[qb][0], 0.f, 0.f};
+            }
+        }
+        __syncthreads();
+        if (kg == 0) {
+#pragma unroll
+            for (int qb = 0; qb < QB; qb++) {
+                const floatx4 e = jo[(QB * (DH / 16) + qb) * 64];
+                const float t = fmaxf(m[qb], e[0]), te = t == -INFINITY ? 0.f : t;
+                const float f0 = __builtin_amdgcn_exp2f(m[qb] - te), f1 = __builtin_amdgcn_exp2f(e[0] - te);
+                m[qb] = t;
+                l[qb][0] = f0 * l[qb][0] + f1 * e[1];
+#pragma unroll
+                for (int db = 0; db < DH / 16; db++) o[db][qb] = f0 * o[db][qb] + f1 * jo[(qb * (DH / 16) + db) * 64];
+            }
+        }
+        __syncthreads();
     }
-    if (MODE != PM_WHOLE && (MODE == PM_PACK || !whole)) {
-        // partial results: of a whole row tile by row (PACK), else by workgroup: one that begins before it, one that ends behind it
-        size_t base = p.rows_part + (((size_t)hk * p.nw + bx) * 2 + (t0 > 0 ? 0 : 1)) * C::RT + (C::SHARED ? wv * C::RW : 0);
-        if (MODE == PM_PACK && whole) base = ((size_t)(ahead ? p.Hkv : 0) + hk) * p.Tq * p.G + (size_t)sq.q0 * p.G + row0;
+
+    if (kg != 0) return;
+    if (MODE == PM_PACK || (MODE == PM_SPLIT && cuts > 1)) {
+        const size_t base = ((size_t)hk * p.items + bx) * C::RT + wv * C::RW;
 #pragma unroll
         for (int qb = 0; qb < QB; qb++) {
             if (row0 + 16 * qb + c16 >= rows) continue;
@@ -600,12 +644,12 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_prompt_attn(const Prom
             for (int db = 0; db < DH / 16; db++) *reinterpret_cast<floatx4*>(p.part + at * DH + 16 * db + 4 * g) = o[db][qb];
             if (g == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(m[qb], l[qb][0]);
         }
-        if constexpr (C::SHARED) __builtin_amdgcn_s_barrier();  // every wave is done with the ring
-    } else {
+        return;
+    }
     // rows leave through LDS, whole and 16 bytes a lane; a row's chunks lie permuted by its number
-    static_assert(C::RW * DH * 2 * C::NW <= C::RINGS, "the waves' rows fit in the rings");
+    static_assert(C::RT * DH * 2 <= C::LDS, "the waves' rows fit in the rings");
     uint8_t* stg = xlds + wv * C::RW * DH * 2;
-    if constexpr (C::SHARED) __builtin_amdgcn_s_barrier();  // every wave is done with the ring, and its copies landed
+    if constexpr (C::SHARED && C::KG == 1) __builtin_amdgcn_s_barrier();  // every wave is done with the ring, and its copies landed
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int qb = 0; qb < QB; qb++) {
@@ -622,28 +666,8 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_prompt_attn(const Prom
         const int rl = (i * 64 + lane) / C::PC, c = lane % C::PC, r = row0 + rl;
         const u32x4 v = *reinterpret_cast<const u32x4*>(stg + rl * DH * 2 + (c ^ (rl & (C::PC - 1))) * 16);
         if (r >= rows) continue;
-        const int t = r / p.G, h = hk * p.G + r % p.G;
+        const int t = prompt_token(p, r), h = hk * p.G + r - t * p.G;
         *reinterpret_cast<u32x4*>(static_cast<uint8_t*>(p.o) + ((long long)(sq.q0 + t) * p.ldo + (long long)h * DH + c * 8) * 2) = v;
-    }
-    if (MODE != PM_WHOLE && C::SHARED) {
-        __builtin_amdgcn_s_waitcnt(0xC07F);
-        __builtin_amdgcn_s_barrier();  // every wave's rows are out of LDS
-    }
-    }
-    if constexpr (MODE == PM_WHOLE) return;
-    // the next row tile of the line
-    left_u -= t1 - t0;
-    if (left_u <= 0) return;
-    __builtin_amdgcn_s_waitcnt(0xC07F);
-    __builtin_amdgcn_sched_barrier(0);
-    t0 = 0;
-    if (++jt * C::RT >= rows) {
-        jt = 0;
-        do {
-            if (++s >= p.B) return;
-            sq = prompt_seq(p, s);
-        } while (sq.nq == 0);
-    }
     }
 #endif
 }
@@ -668,21 +692,18 @@ __global__ __launch_bounds__(256) void k_prompt_merge(const PromptParams p) {
         if (has) s = s0 + 63 - __clzll(has);
     }
     if (s < 0) return;
-    const uint32_t cut = p.cuts[R];
-    const int r = (int)(R - (long long)prompt_seq(p, s).q0 * p.G), w = cut & 0xffff, n = cut >> 16;
+    const uint2 cut = *reinterpret_cast<const uint2*>(p.cuts + R * 2);
+    const int r = (int)(R - (long long)prompt_seq(p, s).q0 * p.G), w = (int)cut.x, n = (int)cut.y;
+    if (cut.x >= (uint32_t)p.items || cut.y > (uint32_t)p.items - cut.x) return;  // (starts that do not ascend: a tile too many, never begun)
     if (MODE == PM_SPLIT && n == 1) return;  // written by its workgroup
-    int w2 = 0, n2 = 0;
+    int n2 = 0;
     if (MODE == PM_PACK) {
-        const int np = (p.P + XKT - 1) / XKT, each = (int)p.cuts[(size_t)p.Tq * p.G], at = (int)(R / RT) * np;
-        w2 = at / each;
-        n2 = (at + np - 1) / each - w2 + 1;
+        const int np = (p.P + XKT - 1) / XKT, each = (int)p.cuts[(size_t)p.Tq * p.G * 2];
+        n2 = (np + each - 1) / each;
     }
-    const size_t all = (size_t)p.Tq * p.G;
     auto index = [&](int i) -> size_t {  // of the row's partial result i
         const bool own = MODE == PM_SPLIT || i < n;
-        const int k = own ? i : i - n;
-        if ((own ? n : n2) == 1) return ((size_t)(own ? 0 : p.Hkv) + hk) * all + R;
-        return p.rows_part + (((size_t)hk * p.nw + (own ? w : w2) + k) * 2 + (k == 0 ? 1 : 0)) * RT + (own ? r % RT : (int)(R % RT));
+        return ((size_t)hk * p.items + (own ? w + i : (int)(R / RT) * n2 + i - n)) * RT + (own ? r % RT : (int)(R % RT));
     };
     const int parts = n + n2;
     float mm = -INFINITY;
@@ -722,31 +743,47 @@ __global__ __launch_bounds__(256) void k_prompt_merge(const PromptParams p) {
 // The form of a call. Rows, keys and work are guesses from the tensors' sizes: lengths are on the device.
 struct PromptForm {
     PromptMode mode;
-    bool one;   // single waves of 16 rows (else four that share the keys)
-    int rt;     // rows of a workgroup
+    int rt;     // rows of a workgroup: 16 (a wave alone), 64 (two row waves by two key groups), 128 (four row waves)
     int nw;     // keys shared out: workgroups per key head
 };
+//
+// The times of both ways are modelled in us. WHOLE: a workgroup's start and its longest range of keys, once per round of workgroups. Shared
+// out: the merge and two starts, then all tiles over the whole chip. Per 32 keys of a 64-row tile 0.4 us (heads of 64: 0.22). Fitted to, WHOLE / shared
+// out, 16 heads on 8 of 128: 3 x 100 rows after 4000 keys (32 on 4 of 64) 37.3 / 20.7; 300 after 8000 106 / 40; 8 x 100 after 1000 20.5 / 23.1; 40 after
+// 1000 18.9 / 12.5; single tokens, 16 after 8191 175 / 81; 2 after 600 12.5 / 9.7; 64 after 600 22.3 / 23.8; 32 after 200 8.7 / 9.9. A prefix once for
+// all (16-row tiles): 64 tokens behind 8192 140 / 30, 8 x 8 behind 4000 51 / 15.
+// 128 rows share a tile's way from LDS among more, but have to fill the chip some rounds over, or have few keys each: 64 / 128 rows, 24 prompts
+// of up to 2000 400 / 290, one of 8192 287 / 254, of 4096 80 / 95, of 3000 49 / 68; 8 of up to 500 22.4 / 19.2.
 static PromptForm prompt_form(int B, int Tq, int Tk, int P, int Hq, int Hkv, int Dh, bool split) {
-    const long G = Hq / Hkv, cus = cu_count(), rows = std::max<long>(1, (long)Tq * G / B), keys = Tk / B + P;
-    const long tiles = std::max<long>(B, (long)Tq * G / 64) * Hkv;
-    // the line's places are counted in 32 bits, whatever the lengths
-    const bool fits = ((long)Tq * G / 16 + B) * ((Tk + (long)P) / XKT + 2) < 1 << 29;
-    if (!split || !fits || keys <= 16 * XKT || (rows > 16 && tiles >= 2 * cus)) {
-        const long tiles128 = std::max<long>(B, (long)Tq * G / 128) * Hkv;
-        return {PM_WHOLE, false, tiles128 >= 2 * cus ? 128 : 64, 0};
-    }
+    const long G = Hq / Hkv, cus = cu_count(), rows = std::max<long>(1, (long)Tq * G / B);
+    const double tile = Dh == 64 ? 0.22 : 0.4, own = tile * Tk / B / XKT, pre = tile * P / XKT;
+    auto tiles = [&](long rt) { return std::max<long>(B, (long)Tq * G / rt) * Hkv; };
+    const double fill = tiles(64) / (2.0 * cus), least = 0.05;  // of a round
     const bool pack = P >= 2 * XKT && B > 1 && rows <= 32;
-    const long slots = rows <= 16 ? 4 * cus : 2 * cus;
-    const int rt = rows <= 16 ? 16 : pack || rows < 128 ? 64 : 128;
-    return {pack ? PM_PACK : PM_SPLIT, rows <= 16, rt, (int)std::min<long>(0xffff, std::max<long>(1, slots / Hkv))};
+    const double whole = 5 + (own + pre) * std::max(1.0, fill);
+    const double pre_fill = pack ? ((double)Tq * G / 64 + 1) * Hkv / (2.0 * cus) : fill;
+    const double shared = (rows <= 16 ? 9 : 15) + 1.5 * (own * std::max(fill, least) + pre * std::max(pre_fill, least));
+    // items are counted in 32 bits, whatever the lengths
+    const bool fits = ((long)Tq * G / 16 + B) * ((Tk + (long)P) / XKT + 2) < 1 << 29;
+    if (!split || !fits || whole <= shared) return {PM_WHOLE, tiles(128) >= 4 * cus || (own + pre <= 16 * tile && fill > 1) ? 128 : 64, 0};
+    const int rt = rows <= 16 ? 16 : 64;
+    // one round of workgroups: four single waves a CU, or two of 64 rows, less what the row tiles' rounding adds
+    const long slots = (rt == 16 ? 4 : 2) * cus / Hkv, over = (long)Tq * G / rt + B;
+    return {pack ? PM_PACK : PM_SPLIT, rt, (int)std::max<long>(std::max<long>(1, slots / 2), slots - over)};
 }
-static size_t prompt_rows_part(const PromptForm& f, int Tq, int Hq) { return f.mode == PM_PACK ? (size_t)2 * Tq * Hq : 0; }
-static size_t prompt_parts(const PromptForm& f, int Tq, int Hq, int Hkv) {
-    return f.mode == PM_WHOLE ? 0 : prompt_rows_part(f, Tq, Hq) + (size_t)Hkv * f.nw * 2 * f.rt;
+// items per key head at most: every row tile rounds its parts up
+static size_t prompt_items(const PromptForm& f, int B, int Tq, int G) {
+    return f.mode == PM_WHOLE ? 0 : f.nw + (size_t)Tq * G / f.rt + B + (f.mode == PM_PACK ? (size_t)Tq * G / f.rt + 1 : 0);
 }
 size_t prompt_attn_workspace(int B, int Tq, int Tk, int P, int Hq, int Hkv, int Dh) {
-    const size_t parts = prompt_parts(prompt_form(B, Tq, Tk, P, Hq, Hkv, Dh, true), Tq, Hq, Hkv);
-    return parts ? parts * (Dh + 2) * sizeof(float) + ((size_t)Tq * (Hq / Hkv) + 1) * sizeof(uint32_t) : 0;
+    const PromptForm f = prompt_form(B, Tq, Tk, P, Hq, Hkv, Dh, true);
+    const size_t rows = prompt_items(f, B, Tq, Hq / Hkv) * Hkv * f.rt;
+    return rows ? rows * (Dh + 2) * sizeof(float) + ((size_t)Tq * (Hq / Hkv) * 2 + 2) * sizeof(uint32_t) : 0;
+}
+
+int prompt_attn_form(int B, int Tq, int Tk, int P, int Hq, int Hkv, int Dh) {
+    const PromptForm f = prompt_form(B, Tq, Tk, P, Hq, Hkv, Dh, true);
+    return f.rt << 16 | (int)f.mode;
 }
 
 template <class E, class C>
@@ -761,19 +798,20 @@ template <class E, class C, PromptMode MODE>
 static hipError_t prompt_split(const PromptParams& p, hipStream_t s) {
     const size_t merges = ((size_t)p.Tq * p.G + 3) / 4 * p.Hkv;
     if (hipError_t e = grid_check(merges, 256)) return e;
-    hipLaunchKernelGGL((k_prompt_attn<E, C, MODE>), dim3(p.nw * p.Hkv), dim3(C::THREADS), C::LDS, s, p);
+    if (hipError_t e = grid_check((size_t)p.items * p.Hkv, C::THREADS)) return e;
+    hipLaunchKernelGGL((k_prompt_attn<E, C, MODE>), dim3((unsigned)((size_t)p.items * p.Hkv)), dim3(C::THREADS), C::LDS, s, p);
     if (hipError_t e = hipGetLastError()) return e;
     hipLaunchKernelGGL((k_prompt_merge<E, C::DH, C::RT, MODE>), dim3((unsigned)merges), dim3(256), 0, s, p);
     return hipGetLastError();
 }
 template <class E, int DH>
 static hipError_t prompt_of(const PromptParams& p, const PromptForm& f, hipStream_t s) {
-    if (f.mode == PM_WHOLE) return f.rt == 128 ? prompt_whole<E, XCfg<DH, 2, 4, true, 4>>(p, s) : prompt_whole<E, XCfg<DH, 1, 4, true, 4>>(p, s);
-    if (f.mode == PM_SPLIT)
-        return f.one         ? prompt_split<E, XCfg<DH, 1, 1, false, 2>, PM_SPLIT>(p, s)
-               : f.rt == 128 ? prompt_split<E, XCfg<DH, 2, 4, true, 4>, PM_SPLIT>(p, s)
-                             : prompt_split<E, XCfg<DH, 1, 4, true, 4>, PM_SPLIT>(p, s);
-    return f.one ? prompt_split<E, XCfg<DH, 1, 1, false, 2>, PM_PACK>(p, s) : prompt_split<E, XCfg<DH, 1, 4, true, 4>, PM_PACK>(p, s);
+    using One = PCfg<DH, 1, 1, 1, 2>;
+    using R64 = PCfg<DH, 2, 2, 2, 2>;
+    using R128 = PCfg<DH, 2, 4, 1, 4>;
+    if (f.mode == PM_WHOLE) return f.rt == 128 ? prompt_whole<E, R128>(p, s) : prompt_whole<E, R64>(p, s);
+    if (f.mode == PM_PACK) return f.rt == 16 ? prompt_split<E, One, PM_PACK>(p, s) : prompt_split<E, R64, PM_PACK>(p, s);
+    return f.rt == 16 ? prompt_split<E, One, PM_SPLIT>(p, s) : prompt_split<E, R64, PM_SPLIT>(p, s);
 }
 
 hipError_t launch_prompt_attn(const PromptLaunch& c, hipStream_t s) {
@@ -796,6 +834,9 @@ hipError_t launch_prompt_attn(const PromptLaunch& c, hipStream_t s) {
     p.P = c.P;
     p.Hkv = c.Hkv;
     p.G = c.Hq / c.Hkv;
+    p.g_shift = 31;
+    while ((1 << (p.g_shift - 31)) < p.G) p.g_shift++;
+    p.g_mul = (uint32_t)(((1ull << p.g_shift) + p.G - 1) / p.G);
     p.q_start = c.q_start;
     p.k_start = c.k_start;
     p.k_len = c.k_len;
@@ -806,11 +847,11 @@ hipError_t launch_prompt_attn(const PromptLaunch& c, hipStream_t s) {
     const size_t need = prompt_attn_workspace(c.B, c.Tq, c.Tk, c.P, c.Hq, c.Hkv, c.Dh);
     const PromptForm f = prompt_form(c.B, c.Tq, c.Tk, c.P, c.Hq, c.Hkv, c.Dh, need == 0 || (c.ws && c.ws_bytes >= need));
     p.nw = f.nw;
-    p.rows_part = prompt_rows_part(f, c.Tq, c.Hq);
+    p.items = (int)prompt_items(f, c.B, c.Tq, p.G);
+    const size_t rows = (size_t)p.items * c.Hkv * f.rt;
     p.part = static_cast<float*>(c.ws);
-    const size_t parts = prompt_parts(f, c.Tq, c.Hq, c.Hkv);
-    p.part_ml = p.part + parts * c.Dh;
-    p.cuts = reinterpret_cast<uint32_t*>(p.part_ml + parts * 2);
+    p.part_ml = p.part + rows * c.Dh;
+    p.cuts = reinterpret_cast<uint32_t*>(p.part_ml + rows * 2);
     if (c.dt == DT::F16) return c.Dh == 64 ? prompt_of<_Float16, 64>(p, f, s) : prompt_of<_Float16, 128>(p, f, s);
     return c.Dh == 64 ? prompt_of<__bf16, 64>(p, f, s) : prompt_of<__bf16, 128>(p, f, s);
 }

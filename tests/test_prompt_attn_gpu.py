@@ -122,11 +122,26 @@ def test_sequences(gpu, name, P, Hq, Hkv, Dh, dt):
     c.check(f"{name} P={P} {Hq}/{Hkv} of {Dh} {dt}")
 
 
-@pytest.mark.parametrize("lens,Hq,Hkv,Dh,P", [
+MANY = [
     ([(1500, 1500)], 4, 2, 128, 0), ([(2049, 2049)], 2, 2, 64, 0), ([(700, 700), (1, 1), (1200, 1200), (5, 5)], 16, 8, 128, 0), ([(900, 3000)], 2, 1, 128, 0),
     ([(1, 20000)], 2, 1, 128, 0), ([(1, 9001), (1, 4)], 16, 2, 64, 0), ([(40, 6000), (7, 100)], 8, 8, 128, 0), ([(1, 300)] * 40, 16, 8, 128, 2500),
     ([(1, 1)] * 70, 4, 1, 64, 5000), ([(300, 300)] * 3, 16, 8, 128, 1000), ([(2, 2)], 1, 1, 128, 9000), ([(1, 12)] * 300, 4, 2, 128, 70),
-    ([(i % 7, i % 7 + i % 41) for i in range(600)], 2, 1, 64, 0)])
+    ([(i % 7, i % 7 + i % 41) for i in range(600)], 2, 1, 64, 0), ([(200, 200)] * 40, 16, 8, 128, 0), ([(150, 150)] * 90, 8, 8, 64, 33),
+    ([(70, 70)] * 5, 4, 4, 64, 0), ([(20, 220)] * 6, 8, 8, 64, 3001), ([(30, 30), (25, 400)] * 4, 2, 2, 128, 4000), ([(33, 9000)], 4, 4, 64, 0)]
+
+
+def form_of(lens, Hq, Hkv, Dh, P):
+    Tq, own = sum(nq for nq, _ in lens) + 1, all(nq == nk for nq, nk in lens)
+    return Dh, ka.prompt_attn_form(len(lens), Tq, Tq if own else sum(nk + 3 for _, nk in lens) + 2, P, Hq, Hkv, Dh)
+
+
+def test_cases_reach_every_form(gpu):
+    """A workgroup per row tile of 64 or 128 rows; keys shared out over single waves of 16 rows and workgroups of 64; a prefix once for all rows."""
+    forms = {form_of(*c) for c in MANY}
+    assert forms == {(d, f) for d in (64, 128) for f in ((64, 0), (128, 0), (16, 1), (64, 1), (16, 2), (64, 2))}
+
+
+@pytest.mark.parametrize("lens,Hq,Hkv,Dh,P", MANY)
 @pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
 def test_long_and_many(gpu, lens, Hq, Hkv, Dh, P, dt):
     c = Case(lens, Hq, Hkv, Dh, dt, P=P, seed=len(lens), pad=1)
