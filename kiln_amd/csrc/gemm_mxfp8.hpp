@@ -75,7 +75,7 @@ __global__ __launch_bounds__(THIN8_WAVES * 64, 2) void k_mx8_thin(const MxGemmPa
         uint32_t sw, sx[MB];
     } ops[2];
     auto load = [&](Ops& o, int kb) {
-        kb = min(kb, p.kbs - 1);
+        if (kb >= p.kbs) return;  // (a wave's: loads past the end took as long as others, half of all at K = 2048)
         const int k0 = kb * 128 + 16 * g, kz = p.K;
 #pragma unroll
         for (int i = 0; i < NB; i++) o.w[i] = *reinterpret_cast<const u32x4*>(wc + (kb * wrg * 4 + i) * MX_UNIT);
@@ -121,7 +121,8 @@ __global__ __launch_bounds__(THIN8_WAVES * 64, 2) void k_mx8_thin(const MxGemmPa
     for (int kb = wv; kb < p.kbs; kb += 2 * THIN8_WAVES) {
         mul(ops[0]);
         load(ops[0], kb + 2 * THIN8_WAVES);
-        if (kb + THIN8_WAVES < p.kbs) mul(ops[1]);
+        if (kb + THIN8_WAVES >= p.kbs) break;
+        mul(ops[1]);
         load(ops[1], kb + 3 * THIN8_WAVES);
     }
 #pragma unroll
@@ -340,27 +341,25 @@ static hipError_t mx8_tiles(MxGemmParams p, hipStream_t s) {
     return hipGetLastError();
 }
 
-// The form of a product.
-enum Mx8Kind { M8_11, M8_12, M8_14, M8_22, M8_44, M8_MID, M8_BIG };
+// The form of a product: modelled times of the forms in us, fitted to T = 1 .. 6912 x {1024 x 1024, 2048 x 2048, 8192 x 2048, 2048 x 8192}.
+// The few-row forms: a start, and per 256 workgroups a time per k block. Tiles: the chain of a tile's k blocks, which takes its time however few
+// tiles there are, and what they take from each other. fp32 outputs (both parts of X) have no 256 x 256 form: their registers would spill.
+// Where forms meet they measured, fp16 out: 2048 x 2048, T = 32 16 x 16 4.2, 32 x 32 5.6, T = 120 8.7 and 5.7, T = 400 32 x 32 16.6, 128 x 128
+// 11.4; 8192 x 2048, T = 800 128 x 128 19.2, 256 x 256 26.5, T = 1537 35.3 and 29.1.
+enum Mx8Kind { M8_11, M8_22, M8_MID, M8_BIG };
 static Mx8Kind mx8_choose(int T, int N, int K, bool exact) {
-    if (T <= 16) return M8_11;
-    if (T <= 32) return M8_12;
-    const double cus = cu_count(), kb = mx_kb(K);
-    auto tiles = [&](int bn, int bm) { return (double)((N + bn - 1) / bn) * ((T + bm - 1) / bm); };
-    const double t22 = tiles(32, 32), t44 = tiles(64, 64), tm = tiles(128, 128), tb = tiles(256, 256);
-    const double cost[4] = {0.8 + 0.01 * kb + (0.25 + 0.05 * kb) * t22 / cus,
-                            ceil(t44 / cus) * (1.2 + 0.045 * kb) + 0.125 * kb * t44 / cus,
-                            1.9 * std::max(1.0, tm / cus) + kb * (0.155 + 0.22 * tm / cus),
-                            ceil(tb / cus) * (5.0 + 0.55 * kb) + 0.35 * kb * tb / cus};
-    return (Mx8Kind)(M8_22 + (std::min_element(cost, cost + (exact ? 3 : 4)) - cost));  // (both parts of X and 256 x 256: too many registers)
+    const double kb = mx_kb(K), cus = cu_count();
+    auto fill = [&](int bn, int bm) { return (double)((N + bn - 1) / bn) * ((T + bm - 1) / bm) / cus; };
+    const double mid = fill(128, 128);
+    const double cost[4] = {2.6 + std::max(1.0, fill(16, 16)) * 0.092 * kb, 2.8 + ceil(fill(32, 32)) * 0.18 * kb,
+                            exact ? 3 + 1.15 * kb * std::max(1.0, 0.55 + 0.8 * mid) : 3 + 0.46 * kb * std::max(1.0, 0.3 + 1.12 * mid),
+                            ceil(fill(256, 256)) * (5.8 + 1.36 * kb)};
+    return (Mx8Kind)(std::min_element(cost, cost + (exact ? 3 : 4)) - cost);
 }
 int linear_mx8_tile(int T, int rows, int cols, int epi) {
     switch (mx8_choose(T, rows, cols, epi == KILN_EPI_F32 || epi == KILN_EPI_RESID)) {
         case M8_11: return 16 << 16 | 16;
-        case M8_12: return 16 << 16 | 32;
-        case M8_14: return 16 << 16 | 64;
         case M8_22: return 32 << 16 | 32;
-        case M8_44: return 64 << 16 | 64;
         case M8_MID: return 128 << 16 | 128;
         default: return 256 << 16 | 256;
     }
@@ -371,10 +370,7 @@ static hipError_t linear_mx8_epi(const MxGemmParams& p, hipStream_t s) {
     const bool words = p.K % 128 == 0 && ((uintptr_t)p.xs & 3) == 0;
     switch (mx8_choose(p.T, p.N, p.K, MX8_EXACT<EPI>)) {
         case M8_11: return mx8_thin<EPI, 1, 1>(p, s);
-        case M8_12: return mx8_thin<EPI, 1, 2>(p, s);
-        case M8_14: return mx8_thin<EPI, 1, 4>(p, s);
         case M8_22: return mx8_thin<EPI, 2, 2>(p, s);
-        case M8_44: return mx8_thin<EPI, 4, 4>(p, s);
         case M8_MID: return words ? mx8_tiles<EPI, Mx8Mid<4>>(p, s) : mx8_tiles<EPI, Mx8Mid<1>>(p, s);
         default:
             if constexpr (MX8_EXACT<EPI>) return hipErrorInvalidValue;

@@ -55,7 +55,7 @@ def check(y, before, xv, wv, epi, gate, beta, what):
 
 SIZES = [(1, 1, 32), (1, 2048, 2048), (3, 33, 96), (16, 100, 1024), (17, 64, 160), (33, 47, 2080), (64, 2048, 8192), (65, 130, 64), (120, 2048, 2048),
          (200, 2048, 1056), (129, 255, 128), (500, 1024, 2048), (1537, 2048, 2048), (1000, 1500, 224), (2000, 4096, 1024), (2049, 4111, 992), (3, 70000, 64),
-         (100000, 7, 64), (300, 300, 20000), (3333, 8200, 544)]
+         (100000, 7, 64), (300, 300, 20000), (1500, 8190, 2048), (6700, 2040, 2080)]
 
 
 def test_sizes_reach_every_tile(gpu):
@@ -74,7 +74,7 @@ def test_sizes(gpu, T, N, K):
         check(y, before, xv, wv, epi, gate, 0.5, f"{T}x{N}x{K} epilogue {epi} tile {ka.linear_mxfp8_tile(T, N, K, epi)}")
 
 
-@pytest.mark.parametrize("T,N,K", [(5, 70, 96), (40, 200, 128), (130, 300, 256), (700, 1030, 160), (2100, 2052, 128)])
+@pytest.mark.parametrize("T,N,K", [(5, 70, 96), (40, 200, 128), (130, 300, 256), (700, 1030, 160), (2100, 2052, 128), (1530, 8190, 2080)])
 @pytest.mark.parametrize("extra,off", [(3, 1), (4, 0), (8, 4)])
 def test_strides(gpu, T, N, K, extra, off):
     """Rows of y of any stride and alignment; what lies between them stays."""
@@ -104,7 +104,7 @@ def test_unaligned_scales(gpu, T):
         check(y, y, xv, wv, 0, None, 0.0, f"scales from byte {off}, T {T}")
 
 
-@pytest.mark.parametrize("T,N,K", [(4, 64, 128), (40, 64, 256), (300, 600, 416), (2100, 2100, 512)])
+@pytest.mark.parametrize("T,N,K", [(4, 64, 128), (40, 64, 256), (300, 600, 416), (2100, 2100, 512), (1530, 8190, 2080)])
 def test_nan_blocks(gpu, T, N, K):
     """A NaN block of X makes its row NaN, one of W its column, and nothing else."""
     codes, scales, w, xv, wv = make(T, N, K, seed=3)
