@@ -31,9 +31,9 @@ __device__ __forceinline__ void mx8_parts(i32x8 x, i32x8& hi, i32x8& lo) {
 #pragma unroll
     for (int i = 0; i < 8; i++) {
         const uint32_t w = (uint32_t)x[i];
-        // bit 7 of a byte: magnitude 0x48 (2^2) or more; NaN codes are among them
-        const uint32_t big = ((w & 0x7f7f7f7fu) + 0x38383838u) >> 7 & 0x01010101u;
-        const uint32_t h = w & big * 255u;
+        // bit 7 of a byte: magnitude 0x48 (2^2) or more, NaN codes among them; then all its bits, each from its byte's top one
+        const uint32_t t = (w & 0x7f7f7f7fu) + 0x38383838u;
+        const uint32_t h = w & __builtin_amdgcn_perm(t, t << 8, 0x0b090a08u);
         hi[i] = (int)h;
         lo[i] = (int)(w ^ h);
     }
@@ -160,9 +160,9 @@ struct Mx8Cfg {
     static constexpr int BN = WN * NB * 16, BM = WM * MB * 16;
     static constexpr int UN = BN / 16, XP = BM / 8;                        // 1 KB pieces of W and of X
     static constexpr int SN = BN / 64, XSP = SB == 4 ? BM / 64 : BM / 16;  // 256-byte pieces of scales: of W; of X, by words of a row or by bytes
-    static constexpr int WD = UN / WAVES, XD = XP / WAVES, SD = SB == 4 ? 1 : 1 + XSP / WAVES, DPS = WD + XD + SD;
+    static constexpr int WD = UN / WAVES, XD = XP / WAVES, SD = SB == 4 ? (SN + XSP + WAVES - 1) / WAVES : 1 + XSP / WAVES, DPS = WD + XD + SD;
     static constexpr int XO = UN * 1024, WSO = XO + BM * 128, XSO = WSO + SN * 256, STAGE = XSO + XSP * 256, LDS = NST * STAGE;
-    static_assert(UN % WAVES == 0 && XP % WAVES == 0 && NB % 4 == 0 && (SB == 4 ? SN + XSP == WAVES : WAVES % SN == 0 && XSP % WAVES == 0) && LDS * WGS <= 160 * 1024, "tile");
+    static_assert(UN % WAVES == 0 && XP % WAVES == 0 && NB % 4 == 0 && (SB == 4 || (WAVES % SN == 0 && XSP % WAVES == 0)) && LDS * WGS <= 160 * 1024, "tile");
 };
 
 // SB 4: a row's scales of a k block by one aligned word (K % 128 == 0, aligned scales), 1: by bytes
@@ -209,9 +209,10 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES * C::WGS / 4) void k_mx8_gemm(
                                                      xchunk * 16 < kleft ? xoff[j] : FAR, 0, 0, 0);
         } else if (i < C::DPS) {
             const int n = i - C::WD - C::XD;
-            if constexpr (C::SB == 4) {  // one piece a wave, of W's or of X's: a selection, not a branch (which would part the products)
-                const bool of_w = wv < C::SN;
-                const int u = of_w ? wv : wv - C::SN;
+            if constexpr (C::SB == 4) {  // pieces of W's or of X's: a selection, not a branch (which would part the products)
+                const int piece = (wv + n * C::WAVES) % (C::SN + C::XSP);  // a wave without one copies another's again
+                const bool of_w = piece < C::SN;
+                const int u = of_w ? piece : piece - C::SN;
                 const uint32_t off = of_w ? u * 256 + lane * 4 : (uint32_t)(u * 64 + lane) * (uint32_t)K32;
                 const uint8_t *ws = ssrc, *xs = tsrc;  // (values: a selection of the variables themselves would put them into memory)
                 const int wn_ = sbytes, xn = tbytes;
@@ -272,8 +273,8 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES * C::WGS / 4) void k_mx8_gemm(
     };
 
 #pragma unroll
-    for (int s = 0; s < C::NST - 1; s++) dma(s);
-    wait_vmcnt<(C::NST - 2) * C::DPS>();
+    for (int s = 0; s < C::NST; s++) dma(s);
+    wait_vmcnt<(C::NST - 1) * C::DPS>();
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -281,15 +282,15 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES * C::WGS / 4) void k_mx8_gemm(
 #pragma unroll
     for (int mb = 0; mb < MB; mb++) read_x(0, mb, 0);
     read_s(0, 0);
-    int next = 1;  // the stage of step i + 1
-    // Step i: its operands are in registers. Those of step i + 1 landed in every wave; the stage of step i - 1, whose reads every wave
-    // finished before its products of i - 1, is refilled. The operands of i + 1 are read between the products of i.
+    int now = 0, next = 1;  // the stages of steps i and i + 1
+    // Step i: its operands are in registers, in every wave (which is waited for), so that its stage is refilled with block i + NST. Those of
+    // step i + 1 landed in every wave, and are read between the products of i.
     auto step = [&](auto tag) {
         constexpr int cur = decltype(tag)::value;
-        wait_vmcnt<(C::NST - 3) * C::DPS>();
+        wait_vmcnt<(C::NST - 2) * C::DPS>();
+        __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
-        const int ds = next >= 2 ? next - 2 : next - 2 + C::NST;
         const uint32_t st = next * C::STAGE;
         read_s(cur ^ 1, st);
 #pragma unroll
@@ -308,10 +309,11 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES * C::WGS / 4) void k_mx8_gemm(
             read_w(nb, st);
             if (nb % (NB / MB) == 0) read_x(cur ^ 1, nb / (NB / MB), st);
 #pragma unroll
-            for (int n = 0; n < (C::DPS + NB - 1) / NB; n++) dma_piece(nb * ((C::DPS + NB - 1) / NB) + n, lds8 + ds * C::STAGE);
+            for (int n = 0; n < (C::DPS + NB - 1) / NB; n++) dma_piece(nb * ((C::DPS + NB - 1) / NB) + n, lds8 + now * C::STAGE);
             __builtin_amdgcn_sched_barrier(0);
         }
         next_block();
+        now = next;
         next = next == C::NST - 1 ? 0 : next + 1;
     };
     int i = 0;
@@ -326,9 +328,9 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES * C::WGS / 4) void k_mx8_gemm(
 }
 
 template <int SB>
-using Mx8Big = Mx8Cfg<2, 4, 8, 4, 3, 1, SB>;  // 256 x 256 (n x m), 8 waves
+using Mx8Mid = Mx8Cfg<2, 2, 4, 4, 3, 2, SB>;  // 128 x 128 (n x m), 4 waves
 template <int SB>
-using Mx8Mid = Mx8Cfg<2, 2, 4, 4, 3, 2, SB>;  // 128 x 128, 4 waves
+using Mx8Big = Mx8Cfg<2, 2, 8, 4, 2, 2, SB>;  // 256 x 128, 4 waves
 
 template <int EPI, class C>
 static hipError_t mx8_tiles(MxGemmParams p, hipStream_t s) {
@@ -341,19 +343,19 @@ static hipError_t mx8_tiles(MxGemmParams p, hipStream_t s) {
     return hipGetLastError();
 }
 
-// The form of a product: modelled times of the forms in us, fitted to T = 1 .. 6912 x {1024 x 1024, 2048 x 2048, 8192 x 2048, 2048 x 8192}.
-// The few-row forms: a start, and per 256 workgroups a time per k block. Tiles: the chain of a tile's k blocks, which takes its time however few
-// tiles there are, and what they take from each other. fp32 outputs (both parts of X) have no 256 x 256 form: their registers would spill.
-// Where forms meet they measured, fp16 out: 2048 x 2048, T = 32 16 x 16 4.2, 32 x 32 5.6, T = 120 8.7 and 5.7, T = 400 32 x 32 16.6, 128 x 128
-// 11.4; 8192 x 2048, T = 800 128 x 128 19.2, 256 x 256 26.5, T = 1537 35.3 and 29.1.
+// The form of a product: modelled times of the forms in us, fitted to T = 1 .. 6912 x {1024 x 1024, 2048 x 2048, 8192 x 2048, 2048 x 8192}: a start,
+// and per round of 256 workgroups (half ones for the largest) a time per k block. Both parts of X (fp32 outputs) and 256 rows of W: registers
+// would spill. Where forms meet they measured, fp16 out: 2048 x 2048, T = 32 16 x 16 4.2 and 32 x 32 5.6, T = 120 8.7 and 5.8, T = 200 32 x 32 9.5 and
+// 128 x 128 10.2, T = 400 16.8 and 10.4; 8192 x 2048, T = 800 128 x 128 18.0 and 256 x 128 18.4, T = 1537 31.2 and 27.0.
 enum Mx8Kind { M8_11, M8_22, M8_MID, M8_BIG };
 static Mx8Kind mx8_choose(int T, int N, int K, bool exact) {
     const double kb = mx_kb(K), cus = cu_count();
-    auto fill = [&](int bn, int bm) { return (double)((N + bn - 1) / bn) * ((T + bm - 1) / bm) / cus; };
-    const double mid = fill(128, 128);
-    const double cost[4] = {2.6 + std::max(1.0, fill(16, 16)) * 0.092 * kb, 2.8 + ceil(fill(32, 32)) * 0.18 * kb,
-                            exact ? 3 + 1.15 * kb * std::max(1.0, 0.55 + 0.8 * mid) : 3 + 0.46 * kb * std::max(1.0, 0.3 + 1.12 * mid),
-                            ceil(fill(256, 256)) * (5.8 + 1.36 * kb)};
+    auto rounds = [&](int bn, int bm, int parts) {
+        return std::max(1.0, ceil(parts * (double)((N + bn - 1) / bn) * ((T + bm - 1) / bm) / cus) / parts);
+    };
+    const double cost[4] = {2.6 + rounds(16, 16, 1) * 0.09 * kb, 2 + rounds(32, 32, 1) * ((exact ? 1.1 : 0.7) + 0.182 * kb),
+                            exact ? 2.5 + 0.3 * kb + rounds(128, 128, 1) * 0.78 * kb : 3.4 + rounds(128, 128, 1) * 0.43 * kb,
+                            3 + rounds(256, 128, 2) * 0.78 * kb};
     return (Mx8Kind)(std::min_element(cost, cost + (exact ? 3 : 4)) - cost);
 }
 int linear_mx8_tile(int T, int rows, int cols, int epi) {
@@ -361,7 +363,7 @@ int linear_mx8_tile(int T, int rows, int cols, int epi) {
         case M8_11: return 16 << 16 | 16;
         case M8_22: return 32 << 16 | 32;
         case M8_MID: return 128 << 16 | 128;
-        default: return 256 << 16 | 256;
+        default: return 256 << 16 | 128;
     }
 }
 
