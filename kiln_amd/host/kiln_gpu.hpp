@@ -307,4 +307,52 @@ inline void linear_mxfp4(void* y, int ldy, const void* x, int dtype, int ldx, in
           "linear_mxfp4");
 }
 
+// ---- a text encoder's layer: causal attention over packed prompts, the residual's addition with the RMS norm, MXFP8 rows ----
+
+// B packed sequences (kiln_prompt_attn): q, out [Tq, ld], k, v [Tk, ld]; q_start [B + 1], k_start and k_len [B] on the device, or null: the
+// queries' own rows.
+struct PromptBatch {
+    int B, Tq, Tk;
+    const int32_t* q_start;
+    const int32_t* k_start = nullptr;
+    const int32_t* k_len = nullptr;
+    // keys in front of every sequence's own
+    const void* pk = nullptr;
+    int ldpk = 0;
+    const void* pv = nullptr;
+    int ldpv = 0;
+    int P = 0;
+};
+inline void prompt_attn(void* out, int ldo, const void* q, int ldq, const void* k, int ldk, const void* v, int ldv, int dtype,
+                        const PromptBatch& b, int Hq, int Hkv, int Dh, float scale, void* workspace = nullptr, size_t ws_bytes = 0) {
+    check(kiln_prompt_attn(out, ldo, q, ldq, k, ldk, v, ldv, dtype, b.Tq, b.Tk, Hq, Hkv, Dh, scale, b.B, b.q_start, b.k_start, b.k_len, b.pk,
+                           b.ldpk, b.pv, b.ldpv, b.P, workspace, ws_bytes, (kiln_stream_t)stream_ref()),
+          "prompt_attn");
+}
+
+// h = x + res, y = rms(h) w (kiln_add_rmsnorm); dense rows, h = res is in place, res = h = null: y = rms(x) w.
+inline void add_rmsnorm(void* y, int ydtype, void* h, const void* x, int xdtype, const void* res, int rdtype, const uint16_t* w_bf16,
+                        int rows, int dim, float eps) {
+    check(kiln_add_rmsnorm(y, ydtype, dim, h, dim, x, xdtype, dim, res, rdtype, dim, w_bf16, rows, dim, eps, (kiln_stream_t)stream_ref()),
+          "add_rmsnorm");
+}
+inline void add_rmsnorm_mxfp8(uint8_t* codes, uint8_t* scales, void* h, const void* x, int xdtype, const void* res, int rdtype,
+                              const uint16_t* w_bf16, int rows, int dim, float eps) {
+    check(kiln_add_rmsnorm_mxfp8(codes, scales, h, dim, x, xdtype, dim, res, rdtype, dim, w_bf16, rows, dim, eps, (kiln_stream_t)stream_ref()),
+          "add_rmsnorm_mxfp8");
+}
+
+inline void mxfp8_quantize(uint8_t* codes, uint8_t* scales, const void* x, int dtype, int ldx, int rows, int cols) {
+    check(kiln_mxfp8_quantize(codes, scales, x, dtype, ldx, rows, cols, (kiln_stream_t)stream_ref()), "mxfp8_quantize");
+}
+inline void mxfp8_dequantize(void* y, int dtype, int ldy, const uint8_t* codes, const uint8_t* scales, int rows, int cols) {
+    check(kiln_mxfp8_dequantize(y, dtype, ldy, codes, scales, rows, cols, (kiln_stream_t)stream_ref()), "mxfp8_dequantize");
+}
+// y [T, ldy] (fp32 for F32/Resid, fp16 for F16/Gelu16) from T MXFP8 rows of W.cols().
+inline void linear_mxfp8(void* y, int ldy, const uint8_t* codes, const uint8_t* scales, int T, const Mxfp4Weight& W, Epi16 epi,
+                         const float* gate = nullptr, float beta = 0.f) {
+    check(kiln_linear_mxfp8(y, ldy, codes, scales, T, W.data(), W.rows(), W.cols(), (int)epi, gate, beta, (kiln_stream_t)stream_ref()),
+          "linear_mxfp8");
+}
+
 }  // namespace kiln

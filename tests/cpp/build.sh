@@ -11,3 +11,5 @@ ROOT=$(cd "$HERE/../.." && pwd)
   -L"$ROOT/kiln_amd" -lkiln_attn -Wl,-rpath,"\$ORIGIN/../../kiln_amd"
 /opt/rocm/bin/hipcc -O2 -std=c++17 --offload-arch=gfx950 "$HERE/rope_freqs_test.cpp" -o "$HERE/rope_freqs_test" \
   -L"$ROOT/kiln_amd" -lkiln_attn -Wl,-rpath,"\$ORIGIN/../../kiln_amd"
+/opt/rocm/bin/hipcc -O2 -std=c++17 --offload-arch=gfx950 "$HERE/text_layer_test.cpp" -o "$HERE/text_layer_test" \
+  -L"$ROOT/kiln_amd" -lkiln_attn -Wl,-rpath,"\$ORIGIN/../../kiln_amd"
