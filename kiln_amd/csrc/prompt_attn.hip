@@ -155,11 +155,11 @@ struct PromptItems {
     }
 };
 
-// Row tile number `rank` of all sequences' tiles of RT rows, in the order of falling place in their sequence (the longest ranges of keys
-// first): its sequence and place, or -1 past the last. With F(n) the number of tiles at place n or later, F(n + 1) <= rank < F(n).
+// Row tile number `rank` of all sequences' tiles of RT rows: its sequence and place there, or -1 past the last. The order goes by bands of places,
+// 2^n to 2^(n+1) - 1, the highest first, so that the longest ranges of keys do not begin last; in a band sequence by sequence, so that the tiles
+// that run at one time share their keys in the L2s. F(n): the number of tiles at place n or later.
 template <int RT>
 __device__ __forceinline__ int prompt_find(const PromptParams& p, const PromptSeqs& seqs, int rank, int& place) {
-    const int lane = threadIdx.x & 63;
     auto tiles = [&](int s0) { return (seqs.lane_of(p, s0).nq * p.G + RT - 1) / RT; };
     const int own = tiles(0);
     if (p.B == 1) {
@@ -174,23 +174,16 @@ __device__ __forceinline__ int prompt_find(const PromptParams& p, const PromptSe
     if (rank >= from(0)) return -1;
     int lo = 0, hi = 1, fhi;  // F(lo) > rank >= F(hi) = fhi
     while ((fhi = from(hi)) > rank) lo = hi, hi *= 2;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2, f = from(mid);
-        if (f > rank) lo = mid;
-        else hi = mid, fhi = f;
-    }
-    place = lo;
-    // the sequences with a tile at this place, in their order
-    int want = rank - fhi;
+    rank -= fhi;
     for (int s0 = 0; s0 < p.B; s0 += 64) {
-        const unsigned long long has = __ballot((s0 ? tiles(s0) : own) > lo);
-        const int n = __popcll(has);
-        if (want < n) {
-            // lane i counts the set bits below it
-            const int below = __popcll(has & ((1ull << lane) - 1));
-            return s0 + __ffsll((unsigned long long)__ballot((has >> lane & 1) && below == want)) - 1;
+        const int n = max(0, min(s0 ? tiles(s0) : own, hi) - lo), up = wave_scan(n);  // tiles in the band
+        const unsigned long long past = __ballot(up > rank);
+        if (past) {
+            const int i = __ffsll(past) - 1;
+            place = lo + __builtin_amdgcn_readlane(up, i) - 1 - rank;
+            return s0 + i;
         }
-        want -= n;
+        rank -= __builtin_amdgcn_readlane(up, 63);
     }
     return -1;
 }
