@@ -112,17 +112,17 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void k_add_rmsnorm(c
     };
     ss = all(ss, 0);
     float rs = 1.f / sqrtf(ss / (float)p.dim + p.eps);
-    if (!(ss < INFINITY)) {  // squares beyond fp32: the sum of (2^-70 h)^2 (rows with infinities and NaNs come here too, and keep them)
+    if (!(ss < INFINITY)) {  // squares beyond fp32: the row times 2^-80 (rows with infinities and NaNs come here too, and keep them)
         float s2 = 0.f;
 #pragma unroll
         for (int c = 0; c < CH; c++)
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const float t = f[c][i] * 0x1p-70f;
-                s2 = fmaf(t, t, s2);
+                f[c][i] *= 0x1p-80f;
+                s2 = fmaf(f[c][i], f[c][i], s2);
             }
         s2 = all(s2, 1);
-        rs = 0x1p-70f / sqrtf(s2 / (float)p.dim);
+        rs = 1.f / sqrtf(s2 / (float)p.dim);
     }
 #pragma unroll
     for (int c = 0; c < CH; c++) {

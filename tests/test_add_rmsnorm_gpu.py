@@ -231,3 +231,22 @@ def test_capture(gpu):
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, eager[0]) and torch.equal(h, eager[1])
+
+
+@pytest.mark.parametrize("dim", [96, 2048, 32768])
+def test_rows_of_the_largest_values(gpu, dim):
+    """Sums of squares beyond fp32, up to full rows of fp32's largest values: h / rms(h) is then 1, off by the roundings of a sum, a division, a root
+    and two products."""
+    top = torch.finfo(torch.float32).max
+    x = torch.full((3, dim), top, device=DEV)
+    x[1] *= -1
+    x[2, 1:] = 2.0 ** 60
+    y = torch.empty_like(x)
+    ka.add_rmsnorm(y, x)
+    want = torch.ones_like(x, dtype=torch.float64)
+    want[1] = -1
+    want[2] = 2.0 ** 60 / (top / dim ** 0.5)
+    want[2, 0] = dim ** 0.5
+    # a sum of dim terms over 64 lanes at least: dim / 64 + 10 roundings and as many of the squares
+    tol = (dim / 64 + 20) * 2.0 ** -24
+    assert ((y.double() - want).abs() <= tol * want.abs()).all()
