@@ -457,7 +457,7 @@ int kiln_linear_mxfp4(void* y, int ldy, const void* x, int dtype, int ldx, int T
  * P keys of a prefix, pk, pv [P, ld*] (NULL with P = 0), stand in front of every sequence's own and are seen by all queries.
  * A query without keys (nk < nq), or whose every score is -inf, gives zeros. What the keys hold that a query does not see does not matter to
  * it, NaN included. Rows of out behind the last sequence (and before the first) are left as they are. Starts and lengths are read on the
- * device and clamped to the tensors; rows that two sequences claim hold either's result.
+ * device and clamped to the tensors; where starts do not ascend, rows of out may hold anything. B <= 16384 (KILN_EUNSUPPORTED).
  * Scores, maxima and sums are fp32, in units of log2, the weights are rounded to dtype for the product with V. v may hold any finite value
  * of dtype (bf16 values below 2^-117 (Tk + P) lose accuracy). workspace: kiln_prompt_attn_workspace_bytes, for few rows against many
  * keys, 16-byte aligned; NULL or a smaller one runs the call without splitting the keys over workgroups. */
@@ -489,7 +489,9 @@ int kiln_mxfp8_quantize(uint8_t* codes, uint8_t* scales, const void* x, int dtyp
 int kiln_mxfp8_dequantize(void* y, int dtype, int ldy, const uint8_t* codes, const uint8_t* scales, int rows, int cols,
                           kiln_stream_t stream);
 
-/* kiln_linear_mxfp4's layer for rows that are MXFP8 already: y = epilogue(X W^T), on the scaled matrix cores, products exact, sums fp32.
+/* kiln_linear_mxfp4's layer for rows that are MXFP8 already: y = epilogue(X W^T), on the scaled matrix cores. Products are exact; of
+ * eight neighbours each is added to the largest with 13 bits below that one's exponent (F32 and RESID: X's codes in two parts by size, so
+ * that this is some 2^-17 of the largest product at most), and those sums in fp32.
  * codes [T, cols] (16-byte aligned) and scales [T, cols / 32] dense, as kiln_add_rmsnorm_mxfp8 and kiln_mxfp8_quantize write them; wp as
  * for kiln_linear_mxfp4; epilogues, y and its alignment as there, any rows and T, cols % 32 == 0, cols <= 2^22. y is apart from
  * the codes and scales (KILN_EINVAL). No workspace. The order of a row's sum follows the sizes, as for kiln_linear16. */

@@ -13,9 +13,11 @@ using namespace kiln::capi;
 
 extern "C" {
 
+constexpr int MAX_SEQS = 1 << 14;  // each workgroup goes over all of them for its place
+
 // sizes that kiln_prompt_attn takes
 static bool prompt_sizes(int B, int Tq, int Tk, int P, int Hq, int Hkv, int Dh) {
-    if (B <= 0 || Tq <= 0 || Tk < 0 || P < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || (Dh != 64 && Dh != 128)) return false;
+    if (B <= 0 || B > MAX_SEQS || Tq <= 0 || Tk < 0 || P < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || (Dh != 64 && Dh != 128)) return false;
     const long long rows = (long long)Tq * (Hq / Hkv);
     return rows <= MAX_ROWS && Tk <= MAX_ROWS && P <= MAX_ROWS && (rows / 16 + B) * Hkv < 1 << 24;
 }

@@ -127,13 +127,14 @@ struct PromptItems {
     __device__ __forceinline__ PromptItems(const PromptParams& p, const PromptSeqs& seqs) {
         np = (p.P + XKT - 1) / XKT;
         const int all = (p.Tq * p.G + RT - 1) / RT;  // row tiles of all rows
-        int n = 0;
+        uint32_t n = 0;
         for (int s0 = 0; s0 < p.B; s0 += 64) {
             const PromptSeq q = seqs.lane_of(p, s0);
-            n += row_tiles(p, q) * key_tiles(q);
+            n += (uint32_t)(row_tiles(p, q) * key_tiles(q));
         }
-        const int total = wave_sum(n) + (MODE == PM_PACK ? all * np : 0);
-        each = max(PROMPT_LEAST, (total + p.nw - 1) / p.nw);
+        // below 2^29 where the starts ascend; where they do not, n may be anything, and the prefix's items still stay below their number
+        const int pre = MODE == PM_PACK ? all * np : 0, total = (int)((uint32_t)wave_sum((int)n) + (uint32_t)(pre + p.nw - 1));
+        each = max(PROMPT_LEAST, max(total / p.nw, (pre + p.nw - 1) / p.nw));
         per = (np + each - 1) / each;
         ahead = MODE == PM_PACK ? all * per : 0;
     }
@@ -166,9 +167,10 @@ __device__ __forceinline__ int prompt_find(const PromptParams& p, const PromptSe
         place = __builtin_amdgcn_readfirstlane(own) - 1 - rank;
         return place >= 0 ? 0 : -1;
     }
-    auto from = [&](int n) {  // F(n)
+    // F(n); less than 2^24 where the starts ascend, and no overflow where they do not
+    auto from = [&](int n) {
         int sum = max(0, own - n);
-        for (int s0 = 64; s0 < p.B; s0 += 64) sum += max(0, tiles(s0) - n);
+        for (int s0 = 64; s0 < p.B; s0 += 64) sum = min(sum + max(0, tiles(s0) - n), 1 << 24);
         return wave_sum(sum);
     };
     if (rank >= from(0)) return -1;

@@ -266,6 +266,25 @@ def test_starts_that_are_wrong(gpu):
         assert (c.out[free] == 7).all()
 
 
+def test_many_sequences(gpu):
+    """The most sequences there may be, single tokens with a key each (out = v), and all of them claiming all rows (nothing else
+    is touched)."""
+    B, H, Dh = 1 << 14, 2, 64
+    q, k, v = (torch.randn(B, H * Dh, device=DEV).half() for _ in range(3))
+    out, starts = torch.empty_like(q), torch.arange(B + 1, dtype=torch.int32, device=DEV)
+    ka.prompt_attn(out, q, k, v, H, H, q_start=starts)
+    assert torch.equal(out, v)
+    with pytest.raises(ka.KilnError):
+        ka.prompt_attn(out, q, k, v, H, H, q_start=torch.arange(B + 2, dtype=torch.int32, device=DEV))
+    for rows in (40, 2000):
+        starts = (torch.arange(B + 1, device=DEV) % 2 * rows).to(torch.int32)
+        for P in (0, 100):
+            out.fill_(7.0)
+            pre = (k[:P], v[:P]) if P else None
+            ka.prompt_attn(out[:rows], q[:rows], k[:rows], v[:rows], H, H, q_start=starts, prefix=pre)
+            assert (out[rows:] == 7).all()
+
+
 def test_shared_cache_places(gpu):
     """Sequences may read the same keys: three streams that continue one prompt."""
     c = Case([(1, 90)] * 3, 4, 2, 128, torch.float16, cached=True)

@@ -31,7 +31,7 @@ def attn(L, out=A[0], ldo=512, q=A[1], ldq=512, k=A[2], ldk=256, v=A[3], ldv=256
     (EUNSUP, dict(qs=A[4] + 2)), (EUNSUP, dict(ks=A[5] + 1, kl=A[6])), (EUNSUP, dict(ws=A[8] + 8, wsb=1 << 20)),
     (EINVAL, dict(out=A[1])), (EINVAL, dict(out=A[1] + 1024)), (EINVAL, dict(out=A[2] + 16)), (EINVAL, dict(out=A[3])),
     (EINVAL, dict(P=4, pk=A[0] + 64, pv=A[7], ldpk=256, ldpv=256)), (EINVAL, dict(P=4, pk=A[6], pv=A[0], ldpk=256, ldpv=256)),
-    (EUNSUP, dict(B=1 << 24)), (EUNSUP, dict(Tq=1 << 30, Tk=1 << 30, q=1 << 50, k=1 << 52, v=1 << 53, out=1 << 54)),
+    (EUNSUP, dict(B=1 << 24)), (EUNSUP, dict(B=(1 << 14) + 1)), (EUNSUP, dict(Tq=1 << 30, Tk=1 << 30, q=1 << 50, k=1 << 52, v=1 << 53, out=1 << 54)),
 ])
 def test_prompt_attn(L, want, kw):
     assert attn(L, **kw) == want, ka.lib().kiln_attn_last_error()
