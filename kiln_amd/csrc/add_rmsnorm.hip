@@ -3,7 +3,9 @@
 // squares and its use; the norm takes the sum before it is rounded to the residual's type.
 //
 // A row to a wave up to 2048 columns, to 4, 8 or 16 waves beyond: eight neighbours a lane and chunk, at most four chunks a lane, all loads
-// under way before the first is used. Bound by memory.
+// under way before the first is used. Bound by memory: 6912 x 2048, bf16 x on a fp32 residual to MXFP8, 25.1 us (6.2 TB/s of what is read and
+// written); 4096 columns, all bf16, 33.4 (6.8); 2000 x 32768, sixteen waves a row that meet at two barriers, 101 (5.2). One row of 2048: 3.3, a
+// launch and one round trip.
 #include <hip/hip_runtime.h>
 
 #include "mxfp8.hpp"

