@@ -754,7 +754,10 @@ struct PromptForm {
 // out: the merge and two starts, then all tiles over the whole chip. Per 32 keys of a 64-row tile 0.4 us (heads of 64: 0.22). Fitted to, WHOLE / shared
 // out, 16 heads on 8 of 128: 3 x 100 rows after 4000 keys (32 on 4 of 64) 37.3 / 20.7; 300 after 8000 106 / 40; 8 x 100 after 1000 20.5 / 23.1; 40 after
 // 1000 18.9 / 12.5; single tokens, 16 after 8191 175 / 81; 2 after 600 12.5 / 9.7; 64 after 600 22.3 / 23.8; 32 after 200 8.7 / 9.9. A prefix once for
-// all (16-row tiles): 64 tokens behind 8192 140 / 30, 8 x 8 behind 4000 51 / 15.
+// all: 64 tokens behind 8192 140 / 30, 8 x 8 behind 4000 51 / 15.
+// Up to 16 rows a sequence take 16-row tiles, but 64-row ones where a prefix before many sequences passes through LDS too often. Fitted to, 16 / 64
+// rows, tokens with 200 keys of their own behind a prefix: 32 behind 1000 13.6 / 17.0, behind 4096 18.0 / 20.5; 64 behind 1000 20.4 / 24.9, behind 8192 37.9 /
+// 29.2, behind 4096 (32 heads on 4 of 64) 21.4 / 17.3; 128 with 100 behind 4096 35.1 / 33.7; 8 x 8 behind 4000 17.2 / 19.1.
 // 128 rows share a tile's way from LDS among more, but have to fill the chip some rounds over, or have few keys each: 64 / 128 rows, 24 prompts
 // of up to 2000 400 / 290, one of 8192 287 / 254, of 4096 80 / 95, of 3000 49 / 68; 8 of up to 500 22.4 / 19.2.
 static PromptForm prompt_form(int B, int Tq, int Tk, int P, int Hq, int Hkv, int Dh, bool split) {
@@ -769,7 +772,9 @@ static PromptForm prompt_form(int B, int Tq, int Tk, int P, int Hq, int Hkv, int
     // items are counted in 32 bits, whatever the lengths
     const bool fits = ((long)Tq * G / 16 + B) * ((Tk + (long)P) / XKT + 2) < 1 << 29;
     if (!split || !fits || whole <= shared) return {PM_WHOLE, tiles(128) >= 4 * cus || (own + pre <= 16 * tile && fill > 1) ? 128 : 64, 0};
-    const int rt = rows <= 16 ? 16 : 64;
+    const double unit = (Dh == 64 ? 0.55 : 1) * Hkv * 32 / cus, own_tiles = (double)Tk / XKT + B;  // of a 16-row tile by 32 keys of 8 heads of 128
+    auto units = [&](long rt) { return unit * (((double)Tq * G / rt + 1) * P / XKT + own_tiles); };
+    const int rt = rows > 16 || (pack && 15 + 0.0165 * units(64) < 8 + 0.0115 * units(16)) ? 64 : 16;
     // one round of workgroups: four single waves a CU, or two of 64 rows, less what the row tiles' rounding adds
     const long slots = (rt == 16 ? 4 : 2) * cus / Hkv, over = (long)Tq * G / rt + B;
     return {pack ? PM_PACK : PM_SPLIT, rt, (int)std::max<long>(std::max<long>(1, slots / 2), slots - over)};

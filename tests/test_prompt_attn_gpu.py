@@ -154,6 +154,16 @@ def test_long_and_many(gpu, lens, Hq, Hkv, Dh, P, dt):
     assert torch.equal(c.out, split)  # the same bits again
 
 
+@pytest.mark.parametrize("Hq,Hkv,Dh,P", [(32, 4, 64, 4001), (4, 2, 128, 12000)])
+def test_many_tokens_behind_a_long_prefix(gpu, Hq, Hkv, Dh, P):
+    """Single tokens whose prefix is taken by workgroups of 64 rows, each sequence's own keys too."""
+    lens = [(1, 1 + 13 * i % 90) for i in range(150)]
+    assert form_of(lens, Hq, Hkv, Dh, P) == (Dh, (64, 2))
+    c = Case(lens, Hq, Hkv, Dh, torch.float16, P=P, seed=9, pad=1)
+    c.run()
+    c.check(f"150 tokens behind {P}")
+
+
 def test_one_sequence_without_starts(gpu):
     c = Case([(77, 77)], 4, 2, 64, torch.float16)
     ka.prompt_attn(c.out, c.q, c.k, c.v, 4, 2)
