@@ -16,7 +16,7 @@
 // hides a part: finding its tile 1.0, the first keys' and Q's way 2.4, the first scores 0.7, the tiles one by one (12% slower than two or four in
 // a row), the rows' way out 1.2. 4 x 120 tokens 8.3, one such chain. Single tokens after 16 x 8191 keys: memory, 408 MB in 76 us, 5.4 TB/s, then the merge
 // (4.8). 3 x 100 rows after 4000 keys (32 heads on 4 of 64): 15.6, one round of 256 workgroups with 16 tiles at least, and the merge 4.9.
-// A prefix of 4096 keys before 32 single tokens with 300 of their own: 12.4 and 5.4; without sharing 570 MB would be read, with it 41.
+// A prefix of 4096 keys before 32 single tokens with 300 of their own: 12.4 and the merge, 17.1 together; without sharing 570 MB would be read, with it 41.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -675,7 +675,8 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_prompt_attn(const Prom
 #endif
 }
 
-// The partial results of a row joined, in the line's order: a wave per row
+// The partial results of a row joined, in the line's order: a wave per row. Loads in flight are what it waits for: 16 where there are many (a token
+// after 8191 keys 17.8 -> 14.8 us, of 64 parts; 32 tokens behind a prefix of 4096 19.5 -> 18.7, of 21), 4 where a few are left.
 template <class E, int DH, int RT, PromptMode MODE>
 __global__ __launch_bounds__(256) void k_prompt_merge(const PromptParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -726,13 +727,17 @@ __global__ __launch_bounds__(256) void k_prompt_merge(const PromptParams p) {
             ll += f * e.y;
         }
         const int end = min(64, parts - i0);
-        for (int i = 0; i < end; i += 4) {  // four in flight; past the last the factor is 0
-            vec v[4];
+        auto take = [&](int i, auto n) {  // n at once
+            constexpr int N = decltype(n)::value;
+            vec v[N];
 #pragma unroll
-            for (int k = 0; k < 4; k++) v[k] = *reinterpret_cast<const vec*>(p.part + index(i0 + min(i + k, end - 1)) * DH + PER * lane);
+            for (int k = 0; k < N; k++) v[k] = *reinterpret_cast<const vec*>(p.part + index(i0 + min(i + k, end - 1)) * DH + PER * lane);
 #pragma unroll
-            for (int k = 0; k < 4; k++) acc += __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), i + k)) * v[k];
-        }
+            for (int k = 0; k < N; k++) acc += __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), i + k)) * (i + k < end ? v[k] : vec(0.f));
+        };
+        int i = 0;
+        for (; i + 8 < end; i += 16) take(i, std::integral_constant<int, 16>{});
+        for (; i < end; i += 4) take(i, std::integral_constant<int, 4>{});
     }
 #pragma unroll
     for (int i = 32; i; i >>= 1) ll += __shfl_xor(ll, i, 64);
