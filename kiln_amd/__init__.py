@@ -893,6 +893,13 @@ def prompt_attn_form(B, Tq, Tk, P, Hq, Hkv, Dh):
     return f >> 16, f & 0xffff
 
 
+def _ld_as(t, shape, what):
+    """The row stride of t, or None if it is not of this 2-D shape, whose sizes fit 32 bits."""
+    if t.shape != shape:
+        return None
+    return shape[1] if t.is_contiguous() else _rows(t, what)[1]
+
+
 def _ints(t, n, what):
     if t.element_size() != 4 or t.is_floating_point() or t.numel() != n or not t.is_contiguous():
         raise ValueError(f"{what} must be a contiguous int32 tensor of {n}")
@@ -908,21 +915,21 @@ def prompt_attn(out, q, k, v, Hq, Hkv=None, q_start=None, k_start=None, k_len=No
     dev = _gpu(q, out, k, v, q_start, k_start, k_len, pk, pv, workspace)
     Hkv = Hq if Hkv is None else Hkv
     (Tq, W), ldq = _rows(q, "prompt_attn: q")
-    shape_o, ldo = _rows(out, "prompt_attn: out")
+    ldo = _ld_as(out, q.shape, "prompt_attn: out")
     (Tk, Wk), ldk = _rows(k, "prompt_attn: k")
-    shape_v, ldv = _rows(v, "prompt_attn: v")
+    ldv = _ld_as(v, k.shape, "prompt_attn: v")
     if not out.dtype == q.dtype == k.dtype == v.dtype:
         raise ValueError(f"prompt_attn: out is {out.dtype}, q {q.dtype}, k {k.dtype}, v {v.dtype}")
     if Hq <= 0 or Hkv <= 0 or Hq % Hkv or W % Hq:
         raise ValueError(f"prompt_attn: {W} columns, {Hq} query heads on {Hkv} key heads")
     Dh = W // Hq
-    if shape_o != q.shape or Wk != Hkv * Dh or shape_v != k.shape:
+    if ldo is None or ldv is None or Wk != Hkv * Dh:
         raise ValueError(f"prompt_attn: shapes out {tuple(out.shape)} q {tuple(q.shape)} k {tuple(k.shape)} v {tuple(v.shape)}")
     P = ldpk = ldpv = 0
     if pk is not None:
         (P, Wp), ldpk = _rows(pk, "prompt_attn: prefix k")
-        shape_pv, ldpv = _rows(pv, "prompt_attn: prefix v")
-        if Wp != Wk or shape_pv != pk.shape or not pk.dtype == pv.dtype == q.dtype:
+        ldpv = _ld_as(pv, pk.shape, "prompt_attn: prefix v")
+        if Wp != Wk or ldpv is None or not pk.dtype == pv.dtype == q.dtype:
             raise ValueError(f"prompt_attn: prefix {tuple(pk.shape)} {pk.dtype} and {tuple(pv.shape)} {pv.dtype} for keys of {Wk} columns, {q.dtype}")
     B = 1
     if q_start is not None:
@@ -958,14 +965,14 @@ def add_rmsnorm(y, x, res=None, w=None, eps=1e-6, h=None, scales=None, stream=No
     dev = _gpu(x, y, res, h, w, scales)
     shape, ldx = _rows(x, "add_rmsnorm: x")
     rows, dim = shape
-    shape_y, ldy = _rows(y, "add_rmsnorm: y")
-    if shape_y != shape:
+    ldy = _ld_as(y, shape, "add_rmsnorm: y")
+    if ldy is None:
         raise ValueError(f"add_rmsnorm: x {tuple(x.shape)}, y {tuple(y.shape)}")
     ldr = ldh = rt = 0
     if res is not None:
-        shape_r, ldr = _rows(res, "add_rmsnorm: res")
-        shape_h, ldh = _rows(h, "add_rmsnorm: h")
-        if shape_r != shape or shape_h != shape or res.dtype != h.dtype:
+        ldr = _ld_as(res, shape, "add_rmsnorm: res")
+        ldh = ldr if h is res else _ld_as(h, shape, "add_rmsnorm: h")
+        if ldr is None or ldh is None or res.dtype != h.dtype:
             raise ValueError(f"add_rmsnorm: x {tuple(x.shape)}, res {tuple(res.shape)} {res.dtype}, h {tuple(h.shape)} {h.dtype}")
         rt = _dt3(res)
     if w is not None and (_dt3(w) != KILN_BF16 or w.numel() != dim or not w.is_contiguous()):
@@ -982,7 +989,6 @@ def add_rmsnorm(y, x, res=None, w=None, eps=1e-6, h=None, scales=None, stream=No
 
 
 def _mx8_plain(codes, scales, rows, cols, what):
-    _fits(what, rows, cols)
     if codes.shape != (rows, cols) or scales.shape != (rows, cols // 32) or codes.element_size() != 1 or scales.element_size() != 1 or \
             not codes.is_contiguous() or not scales.is_contiguous():
         raise ValueError(f"{what}: codes and scales must be contiguous uint8 tensors {[rows, cols]} and {[rows, cols // 32]}, got "
