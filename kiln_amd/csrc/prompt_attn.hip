@@ -318,8 +318,7 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_prompt_attn(const Prom
         for (int cc = 0; cc < DH / 32; cc++) qf[qb][cc] = *reinterpret_cast<const u32x4*>(src + 64 * cc);
         lim[qb] = t + diff + 1;
     }
-    // of the wave's first and last row
-    const int lim0 = prompt_token(p, min(row0, rows - 1)) + diff + 1, lim1 = prompt_token(p, min(row0 + C::RW - 1, rows - 1)) + diff + 1;
+    const int lim0 = prompt_token(p, min(row0, rows - 1)) + diff + 1;  // of the wave's first row
 
     floatx4 o[DH / 16][QB], l[QB];  // l: every register of a lane holds its row's sum (P^T times ones)
     const float lift = std::is_same<E, _Float16>::value ? XLIFT16 : p.lift;
@@ -367,10 +366,10 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_prompt_attn(const Prom
                 for (int qb = 0; qb < QB; qb++)
                     s[kk][qb] = M::mul(kf[kk][cc], qf[qb][cc], cc == 0 ? floatx4{0.f, 0.f, 0.f, 0.f} : s[kk][qb]);
     };
-    // The first tile with keys that some row of the wave does not see (the prefix's end, at last); in own ones from `from_apart` on rows see
-    // different keys.
+    // The first tile with keys that some row of the wave does not see (the prefix's end, at last); own ones from `from_apart` on hold keys that
+    // some row of the workgroup sees, up to L, but the wave's first does not (with 32 or more query heads on a key head none of the wave's may).
     const int from_hide = min(C::KG > 1 ? min(t1, own_end) : own_end, fp + max(lim0, 0) / XKT);
-    const int from_apart = lim0 < lim1 ? fp + max(lim0, 0) / XKT : 0x7fffffff;
+    const int from_apart = lim0 < L ? fp + max(lim0, 0) / XKT : 0x7fffffff;
     // a row sees the first lim - (its first own key) of tile j's keys, or all up to the prefix's end; none of a tile past the last
     auto hide = [&](int j, floatx4 (&s)[2][QB]) {
         if (j < from_hide) return;
@@ -431,7 +430,7 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_prompt_attn(const Prom
                 pf[qb][i] = M::pack(__builtin_amdgcn_exp2f(fmaf(s[i / 2][qb][2 * i % 4], sc, mn[qb])),
                                     __builtin_amdgcn_exp2f(fmaf(s[i / 2][qb][2 * i % 4 + 1], sc, mn[qb])));
     };
-    // Tile j, that rows of this wave see different parts of: infinities and NaNs of V leave the operands; the rows that see them take
+    // Tile j, with keys that not all rows of this wave see: infinities and NaNs of V leave the operands; the rows that see them take
     // their products here. V's rows are read from the stage itself, four dimensions of a key a lane, as the accumulators lie.
     auto keep_apart = [&](int j, uint32_t st, u32x4 (&vf)[DH / 16], const u32x4 (&pf)[QB]) __attribute__((always_inline)) {
         floatx4 z[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
