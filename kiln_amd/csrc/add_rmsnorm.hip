@@ -109,6 +109,8 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void k_add_rmsnorm(c
             v = red[at][0];
 #pragma unroll
             for (int i = 1; i < WAVES; i++) v += red[at][i];
+        } else {  // the lanes add in different orders: one's sum for all, which then take the same branches
+            v = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v)));
         }
         return v;
     };

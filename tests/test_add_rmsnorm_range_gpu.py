@@ -1,0 +1,23 @@
+"""kiln_add_rmsnorm at the borders of fp32's range: sums of squares next to the largest value."""
+
+import pytest
+import torch
+
+import kiln_amd as ka
+from test_add_rmsnorm_gpu import DEV, norm_rel, reference
+
+pytestmark = pytest.mark.gpu
+DIMS = [64, 500, 1024, 2048, 4096, 20000]
+
+
+@pytest.mark.parametrize("dim", DIMS)
+@pytest.mark.parametrize("off", [0.0, 2.0 ** -23, -2.0 ** -23])
+def test_sums_of_squares_next_to_the_largest(gpu, dim, off):
+    """Rows of unequal values whose squares sum to fp32's largest value, give or take its last places."""
+    g = torch.Generator(device=DEV).manual_seed(dim)
+    x = torch.randn(500, dim, generator=g, device=DEV, dtype=torch.float64)
+    x = (x * ((1 + off) * torch.finfo(torch.float32).max / (x * x).sum(-1, keepdim=True)).sqrt()).float()
+    y = torch.empty_like(x)
+    ka.add_rmsnorm(y, x)
+    ref = reference(x, None, None)[1]
+    assert ((y.double() - ref).abs() <= norm_rel(dim) * ref.abs() + 2.0 ** -149).all()
