@@ -116,17 +116,23 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void k_add_rmsnorm(c
     };
     ss = all(ss, 0);
     float rs = 1.f / sqrtf(ss / (float)p.dim + p.eps);
-    if (!(ss < INFINITY)) {  // squares beyond fp32: the row times 2^-80 (rows with infinities and NaNs come here too, and keep them)
+    if (!(ss < INFINITY)) {  // squares beyond fp32: of the row times 2^-80 (rows with infinities and NaNs come here too, and keep them)
         float s2 = 0.f;
 #pragma unroll
         for (int c = 0; c < CH; c++)
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                f[c][i] *= 0x1p-80f;
-                s2 = fmaf(f[c][i], f[c][i], s2);
+                const float v = f[c][i] * 0x1p-80f;
+                s2 = fmaf(v, v, s2);
             }
         s2 = all(s2, 1);
         rs = 1.f / sqrtf(s2 / (float)p.dim);
+        // in this order small values do not pass through subnormal ones
+#pragma unroll
+        for (int c = 0; c < CH; c++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) f[c][i] = f[c][i] * rs * 0x1p-80f;
+        rs = 1.f;
     }
 #pragma unroll
     for (int c = 0; c < CH; c++) {

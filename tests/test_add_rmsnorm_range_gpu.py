@@ -1,4 +1,4 @@
-"""kiln_add_rmsnorm at the borders of fp32's range: sums of squares next to the largest value."""
+"""kiln_add_rmsnorm at the borders of fp32's range: sums of squares next to the largest value, small values beside ones whose squares overflow."""
 
 import pytest
 import torch
@@ -17,6 +17,18 @@ def test_sums_of_squares_next_to_the_largest(gpu, dim, off):
     g = torch.Generator(device=DEV).manual_seed(dim)
     x = torch.randn(500, dim, generator=g, device=DEV, dtype=torch.float64)
     x = (x * ((1 + off) * torch.finfo(torch.float32).max / (x * x).sum(-1, keepdim=True)).sqrt()).float()
+    y = torch.empty_like(x)
+    ka.add_rmsnorm(y, x)
+    ref = reference(x, None, None)[1]
+    assert ((y.double() - ref).abs() <= norm_rel(dim) * ref.abs() + 2.0 ** -149).all()
+
+
+@pytest.mark.parametrize("dim", DIMS)
+def test_small_values_beside_the_largest(gpu, dim):
+    """Values down to where their result leaves fp32's normal range keep their relative accuracy."""
+    g = torch.Generator(device=DEV).manual_seed(dim)
+    x = torch.randn(40, dim, generator=g, device=DEV) * torch.exp2(torch.randint(-64, 1, (40, dim), generator=g, device=DEV).float())
+    x[:, 3] = 2.0 ** torch.linspace(64, 127, 40, device=DEV)
     y = torch.empty_like(x)
     ka.add_rmsnorm(y, x)
     ref = reference(x, None, None)[1]
