@@ -116,22 +116,28 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void k_add_rmsnorm(c
     };
     ss = all(ss, 0);
     float rs = 1.f / sqrtf(ss / (float)p.dim + p.eps);
-    if (!(ss < INFINITY)) {  // squares beyond fp32: of the row times 2^-80 (rows with infinities and NaNs come here too, and keep them)
+    // Squares beyond fp32, or below its normal range where eps does not exceed them: of the row times a power of two (rows with infinities and
+    // NaNs come here too, and keep them)
+    constexpr float LITTLE = 0x1p-100f;
+    if (!(ss < INFINITY) || (p.eps < LITTLE && ss < LITTLE)) {
+        const bool big = !(ss < LITTLE);
+        const float k = big ? 0x1p-80f : 0x1p80f;
         float s2 = 0.f;
 #pragma unroll
         for (int c = 0; c < CH; c++)
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const float v = f[c][i] * 0x1p-80f;
+                const float v = f[c][i] * k;
                 s2 = fmaf(v, v, s2);
             }
         s2 = all(s2, 1);
-        rs = 1.f / sqrtf(s2 / (float)p.dim);
+        rs = 1.f / sqrtf(s2 / (float)p.dim + p.eps * k * k);
         // in this order small values do not pass through subnormal ones
+        const float a = big ? rs : k, b = big ? k : rs;
 #pragma unroll
         for (int c = 0; c < CH; c++)
 #pragma unroll
-            for (int i = 0; i < 8; i++) f[c][i] = f[c][i] * rs * 0x1p-80f;
+            for (int i = 0; i < 8; i++) f[c][i] = f[c][i] * a * b;
         rs = 1.f;
     }
 #pragma unroll

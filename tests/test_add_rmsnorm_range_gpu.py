@@ -1,4 +1,5 @@
-"""kiln_add_rmsnorm at the borders of fp32's range: sums of squares next to the largest value, small values beside ones whose squares overflow."""
+"""kiln_add_rmsnorm at the borders of fp32's range: sums of squares next to the largest value, small values beside ones whose squares overflow,
+and the smallest eps."""
 
 import pytest
 import torch
@@ -33,3 +34,17 @@ def test_small_values_beside_the_largest(gpu, dim):
     ka.add_rmsnorm(y, x)
     ref = reference(x, None, None)[1]
     assert ((y.double() - ref).abs() <= norm_rel(dim) * ref.abs() + 2.0 ** -149).all()
+
+
+@pytest.mark.parametrize("dim", DIMS)
+def test_small_eps(gpu, dim):
+    """Squares below fp32's normal range count where eps does not exceed them; with an eps of 0.5 to 2 times their mean; rows of zeros."""
+    g = torch.Generator(device=DEV).manual_seed(dim)
+    for e in (-149, -148, -140, -130, -126, -110, -101, -99):
+        eps = 2.0 ** e
+        x = torch.randn(4, dim, generator=g, device=DEV, dtype=torch.float64) * 2.0 ** (e / 2)
+        x = (x * torch.tensor([[0.7], [1.4], [0.0], [2.0 ** 60]], dtype=torch.float64, device=DEV)).float()
+        y = torch.empty_like(x)
+        ka.add_rmsnorm(y, x, eps=eps)
+        ref = reference(x, None, None, eps)[1]
+        assert ((y.double() - ref).abs() <= norm_rel(dim) * ref.abs() + 2.0 ** -149).all(), e
