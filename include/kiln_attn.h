@@ -472,7 +472,7 @@ int kiln_prompt_attn_form(int B, int Tq, int Tk, int P, int Hq, int Hkv, int Dh)
 /* The residual's addition and the RMS norm: h = x + res, y = h / sqrt(mean(h^2) + eps) w per row of dim <= 32768 columns (w bf16 [dim], NULL = 1),
  * in fp32 from the unrounded h; eps > 0. x [rows, ldx] in xdtype, res and h [rows, ld*] in rdtype (both NULL: y is the norm of x), y
  * [rows, ldy] in ydtype, any alignment (rows of 16-byte multiples are fastest). h = res with ldh = ldr and y = x with the same type and
- * stride are in place; other overlaps are refused. */
+ * stride are in place; other overlaps of y, the scales or h with any buffer are refused. */
 int kiln_add_rmsnorm(void* y, int ydtype, int ldy, void* h, int ldh, const void* x, int xdtype, int ldx, const void* res, int rdtype, int ldr,
                      const uint16_t* w_bf16, int rows, int dim, float eps, kiln_stream_t stream);
 /* The same with y as MXFP8 codes [rows, dim] and scales [rows, dim / 32] (below), the input of kiln_linear_mxfp8. dim % 32 == 0. */

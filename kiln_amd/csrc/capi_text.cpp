@@ -119,6 +119,21 @@ static int add_rmsnorm(const char* what, void* y, int ydt, int ldy, uint8_t* sca
         if (!apart(y, ly * ye, dim * ye, rows, res, ldr * re, dim * re, rows) || !apart(y, ly * ye, dim * ye, rows, h, ldh * re, dim * re, rows))
             return fail(KILN_EINVAL, "%s: y overlaps the residual or the sum", what);
     }
+    const struct {
+        const char* name;
+        const void* p;
+        long long ld, width;
+        int T;
+        bool written;
+    } buf[] = {{"y", y, ly * ye, dim * ye, rows, true}, {"the sum", h, ldh * re, dim * re, rows, true}, {"x", x, ldx * xe, dim * xe, rows, false},
+               {"the residual", res, ldr * re, dim * re, rows, false}, {"the weight", w, dim * 2LL, dim * 2LL, 1, false}};
+    const long long sw = (long long)rows * (dim / 32);
+    for (const auto& b : buf) {
+        if (!b.p) continue;
+        if (scales && !apart(scales, sw, sw, 1, b.p, b.ld, b.width, b.T)) return fail(KILN_EINVAL, "%s: the scales and %s overlap", what, b.name);
+        if (w && b.written && !apart(w, dim * 2LL, dim * 2LL, 1, b.p, b.ld, b.width, b.T))
+            return fail(KILN_EINVAL, "%s: the weight and %s overlap", what, b.name);
+    }
     kiln::RmsLaunch c{};
     c.y = y;
     c.scales = scales;

@@ -34,16 +34,17 @@ inline size_t esize(int d) { return d == KILN_F32 ? 4 : 2; }
 inline bool aligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 // a row stride holds the row's columns (one row needs none)
 inline bool ld_ok(int ld, long long cols, int T) { return T <= 1 || ld >= cols; }
-// Windows of Tx rows of wx bytes lx bytes apart, and of Ty rows of wy bytes ly apart, share no byte (rows of different strides: by the
-// bytes from the first to the last)
+// Windows of Tx rows of wx bytes lx bytes apart, and of Ty rows of wy bytes ly apart, share no byte (rows of different strides, neither
+// dense: by the bytes from the first to the last)
 inline bool apart(const void* x, long long lx, long long wx, int Tx, const void* y, long long ly, long long wy, int Ty) {
     const long long bx = (long long)(intptr_t)x, by = (long long)(intptr_t)y;
     const long long ex = bx + (Tx - 1) * lx + wx, ey = by + (Ty - 1) * ly + wy;
     if (ex <= by || ey <= bx) return true;
-    if (Tx == 1 || Ty == 1 || lx != ly) return false;
-    // columns side by side in one row stride
-    const long long d = ((by - bx) % lx + lx) % lx;
-    return d >= wx && lx - d >= wy;
+    const bool one_x = Tx == 1 || lx == wx, one_y = Ty == 1 || ly == wy;  // without gaps
+    if ((one_x && one_y) || (!one_x && !one_y && lx != ly)) return false;
+    // columns side by side in one row stride, or one window in a gap of the other's rows
+    const long long l = one_x ? ly : lx, d = ((by - bx) % l + l) % l;
+    return d >= (one_x ? ex - bx : wx) && l - d >= (one_y ? ey - by : wy);
 }
 // rows x cols of a microscaled matrix (blocks of 32): KILN_OK, or the refusal
 int mx_sizes(const char* what, int rows, int cols);
