@@ -48,3 +48,15 @@ def test_small_eps(gpu, dim):
         ka.add_rmsnorm(y, x, eps=eps)
         ref = reference(x, None, None, eps)[1]
         assert ((y.double() - ref).abs() <= norm_rel(dim) * ref.abs() + 2.0 ** -149).all(), e
+
+
+@pytest.mark.parametrize("dim", DIMS)
+def test_large_eps(gpu, dim):
+    """An eps next to the mean of squares that overflow in the sum."""
+    g = torch.Generator(device=DEV).manual_seed(dim)
+    x = (torch.randn(6, dim, generator=g, device=DEV, dtype=torch.float64) * (2.0 ** torch.linspace(126, 140, 6, device=DEV)[:, None].double()).sqrt()).float()
+    y = torch.empty_like(x)
+    for eps in (1e30, 1e37, 1e38, 3e38):
+        ka.add_rmsnorm(y, x, eps=eps)
+        ref = reference(x, None, None, eps)[1]
+        assert ((y.double() - ref).abs() <= norm_rel(dim) * ref.abs() + 2.0 ** -149).all(), eps
