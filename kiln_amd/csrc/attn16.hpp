@@ -1,5 +1,5 @@
 // Pieces shared by the attention kernels that read K and V where they lie (cross_attn.hip, prompt_attn.hip): the matrix products of both
-// 16-bit types, the permutation of a key tile's rows in LDS, a workgroup's geometry.
+// 16-bit types, the permutation of a key tile's rows in LDS, the softmax's constants.
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -54,23 +54,5 @@ template <int DH>
 __device__ __forceinline__ int v_swz(int c, int r) {
     return DH == 128 ? c ^ ((r & 7) << 1) : c ^ (((r >> 1) & 3) << 1);
 }
-
-// A workgroup's geometry: NW waves of 16 QB rows. SHARED: the waves have rows of their own and share a ring of NS tiles.
-// Otherwise every wave has the same rows, a ring and a share of the keys of its own; the results of four meet in LDS.
-template <int DH_, int QB_, int NW_, bool SHARED_, int NS_>
-struct XCfg {
-    static constexpr int DH = DH_, QB = QB_, NW = NW_, NS = NS_;
-    static constexpr bool SHARED = SHARED_;
-    static constexpr int THREADS = 64 * NW, RW = 16 * QB, RT = SHARED ? RW * NW : RW;  // rows of a wave, of the workgroup
-    static constexpr int PC = DH / 8;                                  // 16-byte chunks of a row
-    static constexpr int TILE = XKT * DH * 2, STAGE = 2 * TILE;        // K tile, V tile
-    static constexpr int RTHREADS = SHARED ? THREADS : 64;             // threads that fill a ring
-    static constexpr int DMA = XKT * PC / RTHREADS;                    // 16-byte pieces per thread, for K and for V each
-    static constexpr int RING = NS * STAGE, RINGS = SHARED ? RING : RING * NW;
-    static constexpr int BITS = NW * 32 * 4;                           // each wave's mask windows: 2 x 16 words
-    static constexpr int MERGE = !SHARED && NW > 1 ? NW * RW * (DH + 2) * 4 : 0;
-    static constexpr int LDS = (RINGS > MERGE ? RINGS : MERGE) + BITS;
-    static constexpr int WAVES = QB == 1 && NW > 1 && LDS <= 40 * 1024 ? 4 : LDS <= 80 * 1024 || NW == 1 || NW == 8 ? 2 : 1;  // per SIMD that registers have to allow
-};
 
 }  // namespace kiln

@@ -57,6 +57,24 @@ struct CrossParams {
     float* part;                    // ksplit > 1: partial results [item][row of the tile][DH], then [item][row](m, l)
 };
 
+// A workgroup's geometry: NW waves of 16 QB rows. SHARED: the waves have rows of their own and share a ring of NS tiles.
+// Otherwise every wave has the same rows, a ring and a share of the keys of its own; the results of four meet in LDS.
+template <int DH_, int QB_, int NW_, bool SHARED_, int NS_>
+struct XCfg {
+    static constexpr int DH = DH_, QB = QB_, NW = NW_, NS = NS_;
+    static constexpr bool SHARED = SHARED_;
+    static constexpr int THREADS = 64 * NW, RW = 16 * QB, RT = SHARED ? RW * NW : RW;  // rows of a wave, of the workgroup
+    static constexpr int PC = DH / 8;                                  // 16-byte chunks of a row
+    static constexpr int TILE = XKT * DH * 2, STAGE = 2 * TILE;        // K tile, V tile
+    static constexpr int RTHREADS = SHARED ? THREADS : 64;             // threads that fill a ring
+    static constexpr int DMA = XKT * PC / RTHREADS;                    // 16-byte pieces per thread, for K and for V each
+    static constexpr int RING = NS * STAGE, RINGS = SHARED ? RING : RING * NW;
+    static constexpr int BITS = NW * 32 * 4;                           // each wave's mask windows: 2 x 16 words
+    static constexpr int MERGE = !SHARED && NW > 1 ? NW * RW * (DH + 2) * 4 : 0;
+    static constexpr int LDS = (RINGS > MERGE ? RINGS : MERGE) + BITS;
+    static constexpr int WAVES = QB == 1 && NW > 1 && LDS <= 40 * 1024 ? 4 : LDS <= 80 * 1024 || NW == 1 || NW == 8 ? 2 : 1;  // per SIMD that registers have to allow
+};
+
 template <class E, class C, bool MASK>
 __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_cross_attn(const CrossParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)  // the host pass drops a kernel template whose target builtins it cannot check

@@ -10,13 +10,15 @@
 // must not see it: in tiles where that can be, a product of V with zeros finds them (8 matrix instructions), and they go to the rows
 // that see them one by one (`keep_apart`), the others' operand holding zeros in their place.
 //
-// What bounds it (16 heads on 8 of 128 where nothing else is said, two workgroups or eight single waves a CU). Whole prompts: the matrix cores and
+// What bounds it (16 heads on 8 of 128 where nothing else is said, two workgroups or four single waves a CU; a single wave's
+// ring is 32 KB of LDS, of which five would fit, and half of that for heads of 64). Whole prompts: the matrix cores and
 // the vector work of the softmax, which in one wave follow each other and beside another wave's overlap: 8192 tokens 241 to 260 us, 1.06 to 1.14
 // PFLOP/s. 24 prompts of 2048 446, 0.92 PFLOP/s: of a workgroup's 37 us some 8 are its start and end, of which another workgroup of the CU
 // hides a part: finding its tile 1.0, the first keys' and Q's way 2.4, the first scores 0.7, the tiles one by one (12% slower than two or four in
 // a row), the rows' way out 1.2. 4 x 120 tokens 8.3, one such chain. Single tokens after 16 x 8191 keys: memory, 408 MB in 76 us, 5.4 TB/s, then the merge
-// (4.8). 3 x 100 rows after 4000 keys (32 heads on 4 of 64): 15.6, one round of 256 workgroups with 16 tiles at least, and the merge 4.9.
-// A prefix of 4096 keys before 32 single tokens with 300 of their own: 12.4 and the merge, 17.1 together; without sharing 570 MB would be read, with it 41.
+// (4.6). 3 x 100 rows after 4000 keys (32 heads on 4 of 64): 20.6, of it one round of 256 workgroups with 16 tiles at least (16.8 in a trace) and the
+// merge (5.0). A prefix of 4096 keys before 32 single tokens with 300 of their own: 17.1 (12.0 and 4.4); without sharing 570 MB would be read, with it
+// 41. Every workgroup looks through all sequences for its place: 512 single tokens after 50 keys 80 us, 1024 208, 4096 2137.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -675,7 +677,7 @@ __global__ __launch_bounds__(C::THREADS, C::WAVES) void k_prompt_attn(const Prom
 }
 
 // The partial results of a row joined, in the line's order: a wave per row. Loads in flight are what it waits for: 16 where there are many (a token
-// after 8191 keys 17.8 -> 14.8 us, of 64 parts; 32 tokens behind a prefix of 4096 19.5 -> 18.7, of 21), 4 where a few are left.
+// after 8191 keys 17.8 -> 14.8 us, of 64 parts; 32 tokens behind a prefix of 4096 17.9 -> 17.1, of 21), 4 where a few are left.
 template <class E, int DH, int RT, PromptMode MODE>
 __global__ __launch_bounds__(256) void k_prompt_merge(const PromptParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -747,7 +749,9 @@ __global__ __launch_bounds__(256) void k_prompt_merge(const PromptParams p) {
 #endif
 }
 
-// The form of a call. Rows, keys and work are guesses from the tensors' sizes: lengths are on the device.
+// The form of a call. Rows, keys and work are guesses from the tensors' sizes, the same for every sequence: lengths are on the device. Where one has
+// most of the keys, or many read the same ones, WHOLE may be taken for long ranges: a token after 8191 keys among 63 after 50 112 us (alone, shared
+// out, 14.8), 32 tokens that all read one place of 8192 keys 110.
 struct PromptForm {
     PromptMode mode;
     int rt;     // rows of a workgroup: 16 (a wave alone), 64 (two row waves by two key groups), 128 (four row waves)
