@@ -158,7 +158,8 @@ static hipError_t mx8_thin(MxGemmParams p, hipStream_t s) {
 //
 // 256 x 128 with fp16 outputs: 6912 x 8192 x 2048 94 us (2.5 PFLOP/s), with GELU 102 to 108; 6912 x 2048 x 2048 28. Two workgroups a CU, so that one's
 // epilogue and fills go beside the other's products; one of 256 x 256 was slower. 128 x 128: 1537 x 2048 x 2048 11.7. In two parts (fp32 outputs)
-// 6912 x 8192 x 2048 201, 6912 x 2048 x 8192 209 (1.1 PFLOP/s of the product, 2.2 of what the matrix cores do); the parts beside the products of
+// 6912 x 8192 x 2048 201 to 214, 6912 x 2048 x 8192 onto the residual 209 to 232 (1.0 to 1.1 PFLOP/s of the product, twice that of what the matrix cores
+// do; linear16 with fp16 rows and weights 185 to 194); the parts beside the products of
 // the row block before, instead of once ahead of them, took the same.
 template <int WN_, int WM_, int NB_, int MB_, int NST_, int WGS_, int SB_>
 struct Mx8Cfg {
